@@ -18,7 +18,11 @@ PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 BUILD = PKG / "build"
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
-CUDA_SOURCES = ["elementwise.cu", "suffix_scan.cu", "interface_jac.cu", "gated_norm.cu", "siso_prep.cu", "mamba_small.cu", "gemm_tcgen05.cu", "attn_pullback.cu", "attn_fwd.cu", "ssd.cu", "peer.cu", "noalloc.cu"]
+CUDA_SOURCES = ["elementwise.cu", "suffix_scan.cu", "interface_jac.cu", "gated_norm.cu", "siso_prep.cu", "mamba_small.cu", "gemm_tcgen05.cu", "attn_pullback.cu", "attn_fwd.cu", "ssd.cu", "peer.cu", "noalloc.cu",
+                "paged_kv.cu", "paged_attn.cu", "logits.cu"]
+BINDINGS = ["binding.cpp", "binding_paged.cpp"]
+# sources that divide and round as IEEE says (quantisation, penalties); the others trade that for speed
+PRECISE_SOURCES = {"paged_kv.cu", "paged_attn.cu", "logits.cu"}
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "--use_fast_math",
     "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",
@@ -57,9 +61,9 @@ def build(force: bool = False, verbose_ptxas: bool = False, bounds_check: bool =
     BUILD.mkdir(exist_ok=True)
     sources = [CSRC / s for s in CUDA_SOURCES if (CSRC / s).exists()]
     headers = list(CSRC.glob("*.h")) + list(CSRC.glob("*.cuh"))
-    binding = CSRC / "binding.cpp"
+    bindings = [CSRC / s for s in BINDINGS]
     stamp = BUILD / "stamp.txt"
-    digest = _digest([*sources, *headers, binding]) + torch.__version__
+    digest = _digest([*sources, *headers, *bindings]) + torch.__version__
     out = _ext_path(name)
     if not force and out.exists() and stamp.exists() and stamp.read_text() == digest:
         return out
@@ -71,15 +75,16 @@ def build(force: bool = False, verbose_ptxas: bool = False, bounds_check: bool =
     for src in sources:
         obj = BUILD / (src.stem + ".o")
         objects.append(obj)
-        flags = list(NVCC_FLAGS) + extra + (["-Xptxas", "-v"] if verbose_ptxas else [])
+        flags = [f for f in NVCC_FLAGS if f != "--use_fast_math" or src.name not in PRECISE_SOURCES] + extra + (["-Xptxas", "-v"] if verbose_ptxas else [])
         jobs.append([NVCC, *flags, f"-I{CSRC}", "-I/usr/local/cuda/include", "-c", str(src), "-o", str(obj)])
-    bind_obj = BUILD / "binding.o"
-    objects.append(bind_obj)
     cxx11_abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
-    jobs.append([
-        "g++", "-O2", "-std=c++17", "-fPIC", f"-DTORCH_EXTENSION_NAME={name}", "-DTORCH_API_INCLUDE_EXTENSION_H", *extra,
-        f"-D_GLIBCXX_USE_CXX11_ABI={cxx11_abi}", *inc, "-c", str(binding), "-o", str(bind_obj),
-    ])
+    for src in bindings:
+        obj = BUILD / (src.stem + ".o")
+        objects.append(obj)
+        jobs.append([
+            "g++", "-O2", "-std=c++17", "-fPIC", f"-DTORCH_EXTENSION_NAME={name}", "-DTORCH_API_INCLUDE_EXTENSION_H", *extra,
+            f"-D_GLIBCXX_USE_CXX11_ABI={cxx11_abi}", *inc, "-c", str(src), "-o", str(obj),
+        ])
     with ThreadPoolExecutor(max_workers=min(8, len(jobs))) as pool:
         list(pool.map(_run, jobs))
     lib_dirs = cpp_extension.library_paths(device_type="cuda")

@@ -8,6 +8,15 @@
 #include "api_ssd.h"
 #include "api_gemm.h"
 #include "api_peer.h"
+#include "binding.h"
+
+// One word per device and thread that the kernels record wait time-outs and bad indices in.
+torch::Tensor status_word(const torch::Tensor& like) {
+  static thread_local std::vector<torch::Tensor> words(16);
+  int dev = like.get_device();
+  if (!words[dev].defined()) words[dev] = torch::zeros({1}, like.options().dtype(at::kInt));
+  return words[dev];
+}
 
 namespace {
 
@@ -22,13 +31,6 @@ void check(int rc, const char* what) {
 #define CHECK_BF16(x) TORCH_CHECK((x).is_cuda() && (x).scalar_type() == at::kBFloat16 && (x).is_contiguous(), #x " must be a contiguous CUDA bf16 tensor")
 #define CHECK_LP16(x) TORCH_CHECK((x).is_cuda() && ((x).scalar_type() == at::kBFloat16 || (x).scalar_type() == at::kHalf) && (x).is_contiguous(), #x " must be a contiguous CUDA bf16 / fp16 tensor")
 #define CHECK_F32(x) TORCH_CHECK((x).is_cuda() && (x).scalar_type() == at::kFloat && (x).is_contiguous(), #x " must be a contiguous CUDA fp32 tensor")
-
-Tensor status_word(const Tensor& like) {
-  static thread_local std::vector<Tensor> words(16);
-  int dev = like.get_device();
-  if (!words[dev].defined()) words[dev] = torch::zeros({1}, like.options().dtype(at::kInt));
-  return words[dev];
-}
 
 std::tuple<Tensor, Tensor, Tensor> add_rmsnorm_fwd(const Tensor& branch, const c10::optional<Tensor>& stream_in,
                                                    const Tensor& weight, double eps) {
@@ -1237,6 +1239,7 @@ int64_t kernel_status(const Tensor& like) {
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+  bind_paged(m);
   m.def("add_rmsnorm_fwd", &add_rmsnorm_fwd);
   m.def("rmsnorm_bwd", &rmsnorm_bwd);
   m.def("rmsnorm_bwd_lowp", &rmsnorm_bwd_lowp);

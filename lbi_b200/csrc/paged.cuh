@@ -1,0 +1,103 @@
+// Device helpers shared by the operators over a paged key / value cache: element types, the batch's geometry, page lookup.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <stdint.h>
+
+#include "api_paged.h"
+#include "common.cuh"
+
+namespace lbi {
+namespace paged {
+
+template <int TYPE> struct Elem;
+template <> struct Elem<LBI_F32> { using T = float; };
+template <> struct Elem<LBI_BF16> { using T = __nv_bfloat16; };
+template <> struct Elem<LBI_F16> { using T = __half; };
+template <> struct Elem<LBI_E4M3> { using T = __nv_fp8_storage_t; };
+
+template <typename T> __device__ __forceinline__ float to_f(T x);
+template <> __device__ __forceinline__ float to_f(float x) { return x; }
+template <> __device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <> __device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
+template <> __device__ __forceinline__ float to_f(__nv_fp8_storage_t x) { return __half2float(__half(__nv_cvt_fp8_to_halfraw(x, __NV_E4M3))); }
+
+template <typename T> __device__ __forceinline__ T from_f(float x);
+template <> __device__ __forceinline__ float from_f(float x) { return x; }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f(float x) { return __float2bfloat16_rn(x); }
+template <> __device__ __forceinline__ __half from_f(float x) { return __float2half_rn(x); }
+
+// N elements of T (N * sizeof(T) a multiple of 4) as fp32, loaded and stored in the widest words that fit.
+template <typename T, int N>
+struct alignas(sizeof(T) * N >= 16 ? 16 : sizeof(T) * N) Vec {
+  T v[N];
+};
+template <typename T, int N>
+__device__ __forceinline__ void load_f(const T* p, float* f) {
+  Vec<T, N> x = *reinterpret_cast<const Vec<T, N>*>(p);
+#pragma unroll
+  for (int i = 0; i < N; ++i) f[i] = to_f<T>(x.v[i]);
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_f(T* p, const float* f) {
+  Vec<T, N> x;
+#pragma unroll
+  for (int i = 0; i < N; ++i) x.v[i] = from_f<T>(f[i]);
+  *reinterpret_cast<Vec<T, N>*>(p) = x;
+}
+
+// max that keeps a NaN (fmaxf drops it): a row with a NaN gets a NaN scale, as the plain form's amax gives
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// [first, last) rows of the new tokens of sequence b.  Offsets are clamped to the rows that exist: a wrong one can leave tokens
+// out but never reach outside q.
+__device__ __forceinline__ int2 seq_rows(const lbi_paged_batch& p, int b) {
+  if (!p.cu) {
+    const int each = p.rows / p.batch;
+    return make_int2(b * each, (b + 1) * each);
+  }
+  const int lo = min(max(__ldg(p.cu + b), 0), p.rows);
+  return make_int2(lo, min(max(__ldg(p.cu + b + 1), lo), p.rows));
+}
+
+// Sequence that row `row` belongs to (the last b with cu[b] <= row), or batch when the row lies behind the last sequence.
+__device__ __forceinline__ int seq_of_row(const lbi_paged_batch& p, int row) {
+  if (!p.cu) return row / (p.rows / p.batch);
+  int lo = 0, hi = p.batch;   // cu[lo] <= row < cu[hi + 1]
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (__ldg(p.cu + mid) <= row) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+__device__ __forceinline__ int last_row(const lbi_paged_batch& p) {
+  return p.cu ? min(max(__ldg(p.cu + p.batch), 0), p.rows) : p.rows;
+}
+
+// Page of position pos of sequence b, or -1 (recorded as status 84) where the table or the pool ends.
+__device__ __forceinline__ int page_of(const lbi_paged_batch& p, int b, int pos, int page_shift) {
+  const int i = pos >> page_shift;
+  int page = -1;
+  if (i < p.table_width) page = __ldg(p.table + (int64_t)b * p.table_stride + i);
+  if (page < 0 || page >= p.num_pages) {
+    if (p.status) atomicCAS(p.status, 0, 84);
+    return -1;
+  }
+  return page;
+}
+
+__host__ __device__ __forceinline__ int shift_of(int page_size) {
+  int s = 0;
+  while ((1 << s) < page_size) ++s;
+  return s;
+}
+
+}  // namespace paged
+}  // namespace lbi

@@ -1,0 +1,187 @@
+// Writing the paged key / value cache (rotary turn and 8-bit quantisation included) and reading it back.
+//
+// append:  row = (q | k | v).  (a, b) -> (a cos - b sin, a sin + b cos) on the heads of q and k, in fp32; k and v rows go to
+//          slot position % page_size of page table[position / page_size].  e4m3: scale = max |x| / 448 of the head row (the largest
+//          e4m3 value), code = round(x / scale); a row of zeros has scale 0 and codes 0.
+// gather:  out[b, h, j] = code * scale (or the stored value), 0 behind the context.
+//
+// Both are bound by memory: a head row of head_dim elements belongs to head_dim / 16 threads of 16 elements each.  In append a
+// thread's 16 elements are 8 of each half of the head (the two partners of 8 turns) or 16 neighbours when the pairs are
+// interleaved, so a turn needs no exchange between threads; a block owns one token, so a thread loads its 8 cosines and sines once
+// for all heads.
+#include "paged.cuh"
+
+namespace lbi {
+namespace paged {
+
+constexpr int APPEND_THREADS = 128;
+
+struct AppendArgs {
+  lbi_paged_batch b;
+  const void* qkv;
+  int64_t qkv_stride;
+  void* q_out;
+  int heads, interleaved, zero_tail, page_shift, group_shift;   // 1 << group_shift threads serve one head row
+  const float* cos_tab;
+  const float* sin_tab;
+  int64_t rope_rows;
+};
+
+template <int TYPE, bool E4M3>
+__global__ void __launch_bounds__(APPEND_THREADS) append_kernel(const AppendArgs a) {
+  using T = typename Elem<TYPE>::T;
+  using C = typename Elem<E4M3 ? LBI_E4M3 : TYPE>::T;
+  const lbi_paged_batch& p = a.b;
+  const int row = blockIdx.x, dim = p.head_dim, half = dim >> 1;
+  const int group = 1 << a.group_shift, lane = threadIdx.x & (group - 1);
+  const int d0 = a.interleaved ? lane * 16 : lane * 8, d1 = a.interleaved ? d0 + 8 : d0 + half;   // two runs of 8 elements
+  const bool active = lane * 16 < dim;
+  const int total = a.heads + 2 * p.kv_heads;
+  T* q_out = (T*)a.q_out + (int64_t)row * a.heads * dim;
+
+  const bool owned = row < last_row(p);
+  int pos = -1, page = -1;
+  bool turn_ok = true;
+  if (owned) {
+    const int b = seq_of_row(p, row);
+    const int2 r = seq_rows(p, b);
+    pos = __ldg(p.context + b) - (r.y - r.x) + (row - r.x);
+    if (pos >= 0) page = page_of(p, b, pos, a.page_shift);
+    if (a.cos_tab && pos >= a.rope_rows) {
+      turn_ok = false;
+      if (threadIdx.x == 0 && p.status) atomicCAS(p.status, 0, 83);
+    }
+  }
+  if (!owned && !a.zero_tail) return;
+  const bool dead = pos < 0 || !turn_ok;   // no position: q is zero, nothing is written
+  float cs[8], sn[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) cs[i] = 1.f, sn[i] = 0.f;
+  if (a.cos_tab && !dead && active) {
+    load_f<float, 8>(a.cos_tab + (int64_t)pos * half + lane * 8, cs);
+    load_f<float, 8>(a.sin_tab + (int64_t)pos * half + lane * 8, sn);
+  }
+  const T* src = (const T*)a.qkv + (int64_t)row * a.qkv_stride;
+  for (int h0 = 0; h0 < total; h0 += APPEND_THREADS >> a.group_shift) {
+    const int h = h0 + (threadIdx.x >> a.group_shift);
+    float x[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = 0.f;
+    if (h < total && active && !dead) {
+      load_f<T, 8>(src + (int64_t)h * dim + d0, x);
+      load_f<T, 8>(src + (int64_t)h * dim + d1, x + 8);
+      if (a.cos_tab && h < a.heads + p.kv_heads) {
+        // separate roundings (no fused multiply-add), so that the values that get quantised do not depend on contraction
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int ia = a.interleaved ? 2 * i : i, ib = a.interleaved ? 2 * i + 1 : 8 + i;
+          const float u = x[ia], w = x[ib];
+          x[ia] = __fsub_rn(__fmul_rn(u, cs[i]), __fmul_rn(w, sn[i]));
+          x[ib] = __fadd_rn(__fmul_rn(u, sn[i]), __fmul_rn(w, cs[i]));
+        }
+      }
+    }
+    float top = 0.f;
+    if (E4M3) {   // every thread of the warp takes part in the exchange
+#pragma unroll
+      for (int i = 0; i < 16; ++i) top = max_nan(top, fabsf(x[i]));
+      for (int o = 1; o < group; o <<= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+    }
+    if (h >= total || !active) continue;
+    if (h < a.heads) {
+      store_f<T, 8>(q_out + (int64_t)h * dim + d0, x);
+      store_f<T, 8>(q_out + (int64_t)h * dim + d1, x + 8);
+      continue;
+    }
+    if (dead || page < 0) continue;
+    const int kh = h - a.heads < p.kv_heads ? h - a.heads : h - a.heads - p.kv_heads;
+    const bool is_k = h - a.heads < p.kv_heads;
+    const int64_t slot = ((int64_t)page * p.kv_heads + kh) * p.page_size + (pos & (p.page_size - 1));
+    C* dst = (C*)(is_k ? p.k : p.v) + slot * dim;
+    if (E4M3) {
+      const float scale = __fdiv_rn(top, 448.f);
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t lo = 0, hi = 0;
+        if (top != 0.f) {
+          lo = __nv_cvt_float2_to_fp8x2(make_float2(__fdiv_rn(x[4 * i], scale), __fdiv_rn(x[4 * i + 1], scale)), __NV_SATFINITE, __NV_E4M3);
+          hi = __nv_cvt_float2_to_fp8x2(make_float2(__fdiv_rn(x[4 * i + 2], scale), __fdiv_rn(x[4 * i + 3], scale)), __NV_SATFINITE, __NV_E4M3);
+        }
+        w[i] = lo | hi << 16;
+      }
+      *reinterpret_cast<uint2*>(dst + d0) = make_uint2(w[0], w[1]);
+      *reinterpret_cast<uint2*>(dst + d1) = make_uint2(w[2], w[3]);
+      if (lane == 0) (is_k ? p.k_scale : p.v_scale)[slot] = scale;
+    } else {
+      store_f<T, 8>((T*)dst + d0, x);
+      store_f<T, 8>((T*)dst + d1, x + 8);
+    }
+  }
+}
+
+template <int TYPE, bool E4M3>
+__global__ void __launch_bounds__(256) gather_kernel(const lbi_paged_batch p, void* k_out, void* v_out, int64_t max_len, int page_shift) {
+  using T = typename Elem<TYPE>::T;
+  using C = typename Elem<E4M3 ? LBI_E4M3 : TYPE>::T;
+  const int dim = p.head_dim, parts = dim >> 4;   // 16 elements per thread
+  const int b = blockIdx.y / p.kv_heads, h = blockIdx.y % p.kv_heads;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t pos = i / parts;
+  if (pos >= max_len) return;
+  const int d = (int)(i % parts) * 16;
+  float x[16];
+#pragma unroll
+  for (int e = 0; e < 16; ++e) x[e] = 0.f;
+  const bool is_k = blockIdx.z == 0;
+  if (pos < __ldg(p.context + b)) {
+    const int page = page_of(p, b, (int)pos, page_shift);
+    if (page >= 0) {
+      const int64_t slot = ((int64_t)page * p.kv_heads + h) * p.page_size + (pos & (p.page_size - 1));
+      load_f<C, 16>((const C*)(is_k ? p.k : p.v) + slot * dim + d, x);
+      if (E4M3) {
+        const float scale = __ldg((is_k ? p.k_scale : p.v_scale) + slot);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[e] *= scale;
+      }
+    }
+  }
+  T* out = (T*)(is_k ? k_out : v_out) + ((int64_t)blockIdx.y * max_len + pos) * dim + d;
+  store_f<T, 16>(out, x);
+}
+
+}  // namespace paged
+}  // namespace lbi
+
+#define LBI_BY_TYPE(type, e4m3, CALL)                                              \
+  do {                                                                             \
+    if ((type) == LBI_F32) { if (e4m3) CALL(LBI_F32, true); else CALL(LBI_F32, false); }      \
+    else if ((type) == LBI_BF16) { if (e4m3) CALL(LBI_BF16, true); else CALL(LBI_BF16, false); } \
+    else { if (e4m3) CALL(LBI_F16, true); else CALL(LBI_F16, false); }             \
+  } while (0)
+
+extern "C" int lbi_kv_append(const lbi_paged_batch* p, const void* qkv, int64_t qkv_stride, void* q_out, int type, int heads,
+                             const float* cos_tab, const float* sin_tab, int64_t rope_rows, int interleaved, int zero_tail, cudaStream_t st) {
+  using namespace lbi::paged;
+  if (p->head_dim % 16 != 0 || p->head_dim > 256 || p->rows < 0 || type < 0 || type > LBI_F16) return (int)cudaErrorInvalidValue;
+  if (p->rows == 0) return 0;
+  AppendArgs a{*p, qkv, qkv_stride, q_out, heads, interleaved, zero_tail, shift_of(p->page_size), shift_of(p->head_dim / 16), cos_tab, sin_tab, rope_rows};
+#define LBI_APPEND(T, E) append_kernel<T, E><<<p->rows, APPEND_THREADS, 0, st>>>(a)
+  LBI_BY_TYPE(type, p->cache_type == LBI_E4M3, LBI_APPEND);
+#undef LBI_APPEND
+  return (int)cudaGetLastError();
+}
+
+extern "C" int lbi_kv_gather(const lbi_paged_batch* p, void* k_out, void* v_out, int64_t max_len, int type, cudaStream_t st) {
+  using namespace lbi::paged;
+  if (p->head_dim % 16 != 0 || p->head_dim > 256 || type < 0 || type > LBI_F16) return (int)cudaErrorInvalidValue;
+  if (max_len <= 0 || p->batch == 0) return 0;
+  const int64_t blocks = (max_len * (p->head_dim / 16) + 255) / 256;
+  if (blocks >= (1ll << 31) || (int64_t)p->batch * p->kv_heads > 65535) return (int)cudaErrorInvalidValue;
+  dim3 grid((unsigned)blocks, p->batch * p->kv_heads, 2);
+  const int shift = shift_of(p->page_size);
+#define LBI_GATHER(T, E) gather_kernel<T, E><<<grid, 256, 0, st>>>(*p, k_out, v_out, max_len, shift)
+  LBI_BY_TYPE(type, p->cache_type == LBI_E4M3, LBI_GATHER);
+#undef LBI_GATHER
+  return (int)cudaGetLastError();
+}

@@ -45,5 +45,14 @@ from .dispatch import (  # noqa: E402
     swiglu_fwd,
     transpose_2d,
 )
+from .paged import (  # noqa: E402
+    KVPages,
+    adjust_logits,
+    kv_append,
+    kv_gather,
+    kv_pages,
+    pack_token_mask,
+    paged_attention,
+)
 
 __all__ = [name for name in dir() if not name.startswith("_")]

@@ -278,3 +278,130 @@ def adamw_step(param, grad, exp_avg, exp_avg_sq, lr, beta1, beta2, eps, weight_d
     if shadow is not None:
         shadow.copy_(param)
     return param
+
+
+# ---------------------------------------------------------------- paged key / value cache
+def _sequences(rows, context_lens, cu_seqlens):
+    """(sequence, first row, number of new tokens, context length) of every sequence, offsets clamped to the rows that exist."""
+    ctx = context_lens.tolist()
+    if cu_seqlens is None:
+        each = rows // len(ctx) if ctx else 0
+        starts = [i * each for i in range(len(ctx) + 1)]
+    else:
+        starts = [min(max(s, 0), rows) for s in cu_seqlens.tolist()]
+    return [(b, starts[b], max(0, starts[b + 1] - starts[b]), c) for b, c in enumerate(ctx)]
+
+
+def _slots(pages, page_table, b, pos):
+    """(page, slot, whether there is such a page) of the positions ``pos`` of sequence b."""
+    page_size = pages.k.shape[2]
+    column = pos // page_size
+    inside = (pos >= 0) & (column < page_table.shape[1])
+    if page_table.shape[1] == 0:
+        return torch.zeros_like(pos), pos % page_size, torch.zeros_like(inside)
+    page = page_table[b].long()[torch.where(inside, column, 0)]
+    inside &= (page >= 0) & (page < pages.k.shape[0])
+    return torch.where(inside, page, 0), pos % page_size, inside
+
+
+def _read_pages(pages, page_table, b, length):
+    """fp32 k and v [kv_heads, length, head_dim] of sequence b (zeros where there is no page) and whether each position has one."""
+    page, slot, inside = _slots(pages, page_table, b, torch.arange(length, device=page_table.device))
+    out = []
+    for x, scale in ((pages.k, pages.k_scale), (pages.v, pages.v_scale)):
+        raw = x.view(torch.uint8)[page, :, slot].view(x.dtype) if scale is not None else x[page, :, slot]
+        val = raw.float() if scale is None else raw.float() * scale[page, :, slot].unsqueeze(-1)
+        out.append(torch.where(inside[:, None, None], val, 0.0).transpose(0, 1))
+    return out[0], out[1], inside
+
+
+def quantize_e4m3(x):
+    """(codes, scales) of the rows of fp32 ``x`` along its last dimension: scale = max |x| / 448, code = round(x / scale)."""
+    scale = x.abs().amax(dim=-1) / 448.0
+    code = torch.where(scale.unsqueeze(-1) == 0, 0.0, x / scale.unsqueeze(-1))
+    return code.to(torch.float8_e4m3fn), scale
+
+
+def kv_append(qkv, pages, page_table, context_lens, n_heads, cu_seqlens=None, rope=None, out=None):
+    kv_heads, head_dim = pages.k.shape[1], pages.k.shape[3]
+    rows = qkv.shape[0]
+    out = qkv.new_zeros(rows, n_heads, head_dim) if out is None else out
+    for b, start, new, ctx in _sequences(rows, context_lens, cu_seqlens):
+        pos = torch.arange(ctx - new, ctx, device=qkv.device)
+        x = qkv[start : start + new].float().view(new, n_heads + 2 * kv_heads, head_dim)
+        alive = pos >= 0
+        if rope is not None:
+            cos, sin, interleaved = rope
+            alive &= pos < cos.shape[0]
+            if cos.shape[0] > 0:
+                at = torch.where(alive, pos, 0)
+                c, s = cos[at].unsqueeze(1), sin[at].unsqueeze(1)
+                turn = x[:, : n_heads + kv_heads]
+                if interleaved:
+                    a, d = turn[..., 0::2], turn[..., 1::2]
+                    turned = torch.stack((a * c - d * s, a * s + d * c), dim=-1).flatten(-2)
+                else:
+                    a, d = turn.chunk(2, dim=-1)
+                    turned = torch.cat((a * c - d * s, a * s + d * c), dim=-1)
+                x = torch.cat((turned, x[:, n_heads + kv_heads :]), dim=1)
+        out[start : start + new] = torch.where(alive[:, None, None], x[:, :n_heads], 0.0).to(out.dtype)
+        page, slot, inside = _slots(pages, page_table, b, pos)
+        write = inside & alive
+        page, slot, x = page[write], slot[write], x[write]
+        for dst, scales, val in ((pages.k, pages.k_scale, x[:, n_heads : n_heads + kv_heads]), (pages.v, pages.v_scale, x[:, n_heads + kv_heads :])):
+            if scales is None:
+                dst[page, :, slot] = val.to(dst.dtype)
+            else:
+                code, scale = quantize_e4m3(val)
+                dst.view(torch.uint8)[page, :, slot] = code.view(torch.uint8)
+                scales[page, :, slot] = scale
+    return out
+
+
+def kv_gather(pages, page_table, context_lens, max_len, dtype):
+    batch, kv_heads, head_dim = context_lens.shape[0], pages.k.shape[1], pages.k.shape[3]
+    k_out, v_out = (torch.zeros(batch, kv_heads, max_len, head_dim, dtype=dtype, device=pages.k.device) for _ in range(2))
+    for b, n in enumerate(context_lens.tolist()):
+        n = min(max(n, 0), max_len)
+        k, v, _ = _read_pages(pages, page_table, b, n)
+        k_out[b, :, :n], v_out[b, :, :n] = k.to(dtype), v.to(dtype)
+    return k_out, v_out
+
+
+def paged_attention(q, pages, page_table, context_lens, scale, cu_seqlens=None, out=None):
+    rows, heads, head_dim = q.shape
+    group = heads // pages.k.shape[1]
+    out = torch.zeros_like(q, memory_format=torch.contiguous_format) if out is None else out
+    for b, start, new, ctx in _sequences(rows, context_lens, cu_seqlens):
+        if new == 0:
+            continue
+        k, v, inside = _read_pages(pages, page_table, b, max(ctx, 0))
+        x = q[start : start + new].float().transpose(0, 1)
+        score = x @ k.repeat_interleave(group, dim=0).transpose(-1, -2) * scale
+        last = torch.arange(ctx - new, ctx, device=q.device)
+        visible = (torch.arange(max(ctx, 0), device=q.device) <= last[:, None]) & inside
+        prob = torch.softmax(score.masked_fill(~visible, float("-inf")), dim=-1)
+        prob = torch.where(visible.any(dim=-1)[:, None], prob, 0.0)
+        out[start : start + new] = (prob @ v.repeat_interleave(group, dim=0)).transpose(0, 1).to(out.dtype)
+    return out
+
+
+def adjust_logits(logits, tokens, lengths, prompt_lengths, repetition, presence, frequency, bias, allowed, out=None):
+    batch, vocab = logits.shape
+    x = logits.float()
+    at = torch.arange(tokens.shape[1], device=x.device)
+    counted = (at < lengths[:, None]) if lengths is not None else torch.ones_like(tokens, dtype=torch.bool)
+    counted = counted & (tokens >= 0) & (tokens < vocab)
+    behind = counted if prompt_lengths is None else counted & (at >= prompt_lengths[:, None])
+    ids = torch.where(counted, tokens, 0)
+    seen = torch.zeros(batch, vocab, device=x.device).scatter_add_(1, ids, counted.float())
+    made = torch.zeros(batch, vocab, device=x.device).scatter_add_(1, ids, behind.float())
+    r, p, f = (v[:, None] if torch.is_tensor(v) else v for v in (repetition, presence, frequency))
+    x = torch.where(seen > 0, torch.where(x > 0, x / r, x * r), x)
+    x = torch.where(made > 0, x - p - f * made, x)
+    if bias is not None:
+        x = x + bias
+    if allowed is not None:
+        token = torch.arange(vocab, device=x.device)
+        x = x.masked_fill((allowed[..., token // 32] >> (token % 32)) & 1 == 0, float("-inf"))
+    return x if out is None else out.copy_(x)
