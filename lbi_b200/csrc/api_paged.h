@@ -39,9 +39,16 @@ int lbi_kv_append(const lbi_paged_batch* p, const void* qkv, int64_t qkv_stride,
 // k_out, v_out [batch, kv_heads, max_len, head_dim] of `type`: positions below the context length, zeros behind it.
 int lbi_kv_gather(const lbi_paged_batch* p, void* k_out, void* v_out, int64_t max_len, int type, cudaStream_t stream);
 
+// How a long context is cut: `splits` parts of `split_keys` keys (the last takes what is left).  With more than one part the caller
+// supplies part_o fp32 [rows * heads, splits, head_dim] and part_lse fp32 [rows * heads, splits].
+typedef struct {
+  int splits, split_keys;
+} lbi_attention_plan;
+lbi_attention_plan lbi_paged_attention_plan(const lbi_paged_batch* p, int type, int heads, int64_t max_context, int sm_count);
+
 // out [rows, heads * head_dim] = causal attention of the new tokens q (row stride q_stride elements) over the sequences' pages.
-int lbi_paged_attention(const lbi_paged_batch* p, const void* q, int64_t q_stride, void* out, int type, int heads, float scale,
-                        int zero_tail, cudaStream_t stream);
+int lbi_paged_attention(const lbi_paged_batch* p, const void* q, int64_t q_stride, void* out, float* part_o, float* part_lse,
+                        lbi_attention_plan plan, int type, int heads, float scale, int zero_tail, cudaStream_t stream);
 
 // out fp32 [batch, vocab] from logits [batch, vocab] (row stride, type), the rules of logits.cu.  Null pointers: the scalar is used.
 typedef struct {

@@ -94,8 +94,8 @@ Tensor aligned_rows(const Tensor& x) {
   return x.clone(at::MemoryFormat::Contiguous);
 }
 
-Tensor output(const OptTensor& out, at::IntArrayRef sizes, const Tensor& like, at::ScalarType type) {
-  if (!given(out)) return torch::empty(sizes, like.options().dtype(type));
+Tensor output(const OptTensor& out, at::IntArrayRef sizes, const Tensor& like, at::ScalarType type, bool nobody = false) {
+  if (!given(out)) return nobody ? torch::zeros(sizes, like.options().dtype(type)) : torch::empty(sizes, like.options().dtype(type));
   TORCH_CHECK_VALUE(out->sizes() == sizes && out->scalar_type() == type && out->device() == like.device() && out->is_contiguous() &&
                         (uintptr_t)out->data_ptr() % 16 == 0,
                     "out must be a contiguous tensor of the result's shape and type on its device");
@@ -151,6 +151,7 @@ std::tuple<Tensor, Tensor> kv_gather(const Tensor& k, const Tensor& v, const Opt
 
 Tensor paged_attention(const Tensor& q_in, const Tensor& k, const Tensor& v, const OptTensor& k_scale, const OptTensor& v_scale, const Tensor& table,
                        const Tensor& context, double scale, const OptTensor& cu, int64_t max_context, const OptTensor& out) {
+  TORCH_CHECK_VALUE(max_context >= 0, "max_context must not be negative");
   TORCH_CHECK_VALUE(q_in.is_cuda() && q_in.dim() == 3, "q must be a CUDA tensor [rows, heads, head_dim]");
   check_cache_type(q_in, k);
   c10::cuda::CUDAGuard guard(k.device());
@@ -160,9 +161,15 @@ Tensor paged_attention(const Tensor& q_in, const Tensor& k, const Tensor& v, con
                     p.kv_heads, " of ", p.head_dim);
   const bool packed = q_in.stride(2) == 1 && (heads == 1 || q_in.stride(1) == p.head_dim);
   const Tensor q = aligned_rows(packed ? q_in : q_in.contiguous());
-  Tensor o = output(out, q.sizes(), q, q.scalar_type());
-  check(lbi_paged_attention(&p, q.data_ptr(), q.size(0) > 1 ? q.stride(0) : heads * p.head_dim, o.data_ptr(), type_of(q, "q"), (int)heads, (float)scale,
-                            given(out) ? 0 : 1, cur_stream()),
+  Tensor o = output(out, q.sizes(), q, q.scalar_type(), p.batch == 0);
+  const int type = type_of(q, "q");
+  const lbi_attention_plan plan = lbi_paged_attention_plan(&p, type, (int)heads, max_context, at::cuda::getCurrentDeviceProperties()->multiProcessorCount);
+  Tensor parts;   // results of the parts of a long context, then the logarithms of their sums
+  const int64_t part_rows = q.size(0) * heads * plan.splits;
+  if (plan.splits > 1) parts = torch::empty({part_rows * (p.head_dim + 1)}, q.options().dtype(at::kFloat));
+  float* part_o = plan.splits > 1 ? parts.data_ptr<float>() : nullptr;
+  check(lbi_paged_attention(&p, q.data_ptr(), q.size(0) > 1 ? q.stride(0) : heads * p.head_dim, o.data_ptr(), part_o,
+                            part_o ? part_o + part_rows * p.head_dim : nullptr, plan, type, (int)heads, (float)scale, given(out) ? 0 : 1, cur_stream()),
         "paged_attention");
   return o;
 }

@@ -93,6 +93,69 @@ __device__ __forceinline__ int page_of(const lbi_paged_batch& p, int b, int pos,
   return page;
 }
 
+// Work is cut into tiles of `per_tile` rows (row r of a sequence's tile space = token * group + head of the group); sequence b owns
+// the tiles from cu[b] * group / per_tile + b on, which is never less than the tiles of the sequences before it need, so a tile finds
+// its sequence without a prefix sum over the batch and the host needs only rows and batch to size the grid.
+__device__ __forceinline__ int64_t first_tile(const lbi_paged_batch& p, int b, int group, int per_tile) {
+  const int64_t start = p.cu ? min(max(__ldg(p.cu + b), 0), p.rows) : (int64_t)b * (p.rows / p.batch);
+  return start * group / per_tile + b;
+}
+inline int64_t tile_bound(const lbi_paged_batch& p, int group, int per_tile) { return (int64_t)p.rows * group / per_tile + p.batch; }
+
+// Sequence of tile `tile` (the last b with first_tile(b) <= tile); a full warp calls, 32 candidates are read at a time.
+__device__ __forceinline__ int seq_of_tile(const lbi_paged_batch& p, int64_t tile, int group, int per_tile) {
+  int lo = 0, n = p.batch;
+  const int lane = threadIdx.x & 31;
+  while (n > 1) {
+    const int step = (n + 31) >> 5;
+    const int b = lo + lane * step;
+    const bool below = lane * step < n && first_tile(p, b, group, per_tile) <= tile;
+    const int hit = max(__popc(__ballot_sync(0xffffffffu, below)) - 1, 0);
+    n = min(step, n - hit * step);
+    lo += hit * step;
+  }
+  return lo;
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float lg2(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Two fp32 values as one 32-bit word of a 16-bit type (a in the low half).
+template <int TYPE>
+__device__ __forceinline__ uint32_t pack16(float a, float b) {
+  uint32_t d;
+  if (TYPE == LBI_F16) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(b), "f"(a));
+  else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(b), "f"(a));
+  return d;
+}
+
+// Four e4m3 codes -> two words of a 16-bit type, exactly.  fp16 has the conversion; for bf16 sign, exponent and mantissa are moved to
+// their places (which divides the value by 2^120, codes below the normal range included) and multiplied by 2^120.  A NaN code comes
+// out as 480 there: rows with a NaN are written with a NaN scale.
+template <int TYPE>
+__device__ __forceinline__ void codes_to_16(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if (TYPE == LBI_F16) {
+    asm("{\n.reg .b16 a, b;\nmov.b32 {a, b}, %2;\ncvt.rn.f16x2.e4m3x2 %0, a;\ncvt.rn.f16x2.e4m3x2 %1, b;\n}" : "=r"(lo), "=r"(hi) : "r"(w));
+  } else {
+    const uint32_t a = __byte_perm(w, 0, 0x1404), b = __byte_perm(w, 0, 0x3424);
+    const uint32_t x = ((a >> 4) & 0x07f007f0u) | (a & 0x80008000u), y = ((b >> 4) & 0x07f007f0u) | (b & 0x80008000u);
+    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(lo) : "r"(x), "r"(0x7b807b80u));
+    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(hi) : "r"(y), "r"(0x7b807b80u));
+  }
+}
+
+// Scale of a value row: a row of zeros has scale 0, which has no logarithm and no reciprocal; its codes are 0, so any positive
+// scale serves.  A NaN stays.
+__device__ __forceinline__ float positive_scale(float s) { return s < 1e-30f ? 1e-30f : s; }
+
 __host__ __device__ __forceinline__ int shift_of(int page_size) {
   int s = 0;
   while ((1 << s) < page_size) ++s;
