@@ -19,10 +19,10 @@ CSRC = PKG / "csrc"
 BUILD = PKG / "build"
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 CUDA_SOURCES = ["elementwise.cu", "suffix_scan.cu", "interface_jac.cu", "gated_norm.cu", "siso_prep.cu", "mamba_small.cu", "gemm_tcgen05.cu", "attn_pullback.cu", "attn_fwd.cu", "ssd.cu", "peer.cu", "noalloc.cu",
-                "paged_kv.cu", "paged_attn.cu", "logits.cu"]
+                "paged_kv.cu", "paged_attn.cu", "paged_attn_tc.cu", "logits.cu"]
 BINDINGS = ["binding.cpp", "binding_paged.cpp"]
 # sources that divide and round as IEEE says (quantisation, penalties); the others trade that for speed
-PRECISE_SOURCES = {"paged_kv.cu", "paged_attn.cu", "logits.cu"}
+PRECISE_SOURCES = {"paged_kv.cu", "paged_attn.cu", "paged_attn_tc.cu", "logits.cu"}
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "--use_fast_math",
     "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",

@@ -42,9 +42,10 @@ int lbi_kv_gather(const lbi_paged_batch* p, void* k_out, void* v_out, int64_t ma
 // How a long context is cut: `splits` parts of `split_keys` keys (the last takes what is left).  With more than one part the caller
 // supplies part_o fp32 [rows * heads, splits, head_dim] and part_lse fp32 [rows * heads, splits].
 typedef struct {
+  int kernel;   // 0 one warp per row, 1 tiles of 16 rows, 2 tiles of 256 rows
   int splits, split_keys;
 } lbi_attention_plan;
-lbi_attention_plan lbi_paged_attention_plan(const lbi_paged_batch* p, int type, int heads, int64_t max_context, int sm_count);
+lbi_attention_plan lbi_paged_attention_plan(const lbi_paged_batch* p, int type, int heads, float scale, int64_t max_context, int sm_count);
 
 // out [rows, heads * head_dim] = causal attention of the new tokens q (row stride q_stride elements) over the sequences' pages.
 int lbi_paged_attention(const lbi_paged_batch* p, const void* q, int64_t q_stride, void* out, float* part_o, float* part_lse,

@@ -163,7 +163,7 @@ Tensor paged_attention(const Tensor& q_in, const Tensor& k, const Tensor& v, con
   const Tensor q = aligned_rows(packed ? q_in : q_in.contiguous());
   Tensor o = output(out, q.sizes(), q, q.scalar_type(), p.batch == 0);
   const int type = type_of(q, "q");
-  const lbi_attention_plan plan = lbi_paged_attention_plan(&p, type, (int)heads, max_context, at::cuda::getCurrentDeviceProperties()->multiProcessorCount);
+  const lbi_attention_plan plan = lbi_paged_attention_plan(&p, type, (int)heads, (float)scale, max_context, at::cuda::getCurrentDeviceProperties()->multiProcessorCount);
   Tensor parts;   // results of the parts of a long context, then the logarithms of their sums
   const int64_t part_rows = q.size(0) * heads * plan.splits;
   if (plan.splits > 1) parts = torch::empty({part_rows * (p.head_dim + 1)}, q.options().dtype(at::kFloat));

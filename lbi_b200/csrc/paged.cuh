@@ -11,6 +11,19 @@
 namespace lbi {
 namespace paged {
 
+struct AttnArgs {
+  lbi_paged_batch b;
+  const void* q;
+  int64_t q_stride;
+  void* out;
+  float* part_o;      // [rows * heads, splits, head_dim] results of the parts, null when there is one
+  float* part_lse;    // [rows * heads, splits] base-2 logarithm of the sum of exponentials
+  int heads, group, zero_tail, page_shift, splits, split_keys;
+  float scale_log2;
+};
+
+int launch_attn_tiles(const AttnArgs& a, int type, cudaStream_t st);   // paged_attn_tc.cu
+
 template <int TYPE> struct Elem;
 template <> struct Elem<LBI_F32> { using T = float; };
 template <> struct Elem<LBI_BF16> { using T = __nv_bfloat16; };

@@ -4,6 +4,7 @@
 //
 // Three kernels:
 //   attn_rows_kernel   16 query rows at a time (tokens x heads of a group) for 16-bit queries: decoding, a few new tokens.
+//   attn_tiles_kernel  256 rows at a time on tcgen05 (paged_attn_tc.cu): chunks of a prompt.
 //   attn_row_kernel    one warp per (token, head): fp32 queries and head sizes that the tiles do not cover.
 //   combine_kernel     joins the parts of a long context.
 #include <algorithm>
@@ -12,17 +13,6 @@
 
 namespace lbi {
 namespace paged {
-
-struct AttnArgs {
-  lbi_paged_batch b;
-  const void* q;
-  int64_t q_stride;
-  void* out;
-  float* part_o;      // [rows * heads, splits, head_dim] results of the parts, null when there is one
-  float* part_lse;    // [rows * heads, splits] base-2 logarithm of the sum of exponentials
-  int heads, group, zero_tail, page_shift, splits, split_keys;
-  float scale_log2;
-};
 
 // ------------------------------------------------------------------------------------------------ 16-row tiles
 // Bound by reading the cache once: 2 head_dim sizeof(code) bytes per key and kv head.  All query heads of a group (and several new
@@ -490,28 +480,38 @@ int launch_row(const AttnArgs& a, cudaStream_t st) {
 }  // namespace paged
 }  // namespace lbi
 
-namespace {
-
-bool rows_tile_covers(const lbi_paged_batch* p, int type) {
-  return type != LBI_F32 && (p->head_dim == 32 || p->head_dim == 64 || p->head_dim == 128);
-}
-
-}  // namespace
-
-extern "C" lbi_attention_plan lbi_paged_attention_plan(const lbi_paged_batch* p, int type, int heads, int64_t max_context, int sm_count) {
+extern "C" lbi_attention_plan lbi_paged_attention_plan(const lbi_paged_batch* p, int type, int heads, float scale, int64_t max_context, int sm_count) {
   using namespace lbi::paged;
-  lbi_attention_plan plan{1, 1 << 30};
-  if (!rows_tile_covers(p, type) || p->rows == 0) return plan;
+  lbi_attention_plan plan{0, 1, 1 << 30};
+  if (type == LBI_F32 || p->rows == 0 || p->batch == 0 || !(p->head_dim == 32 || p->head_dim == 64 || p->head_dim == 128)) return plan;
+  const int group = heads / p->kv_heads;
   const int64_t capacity = (int64_t)p->table_width * p->page_size;
   const int64_t longest = max_context > 0 ? std::min(max_context, capacity) : capacity;
-  // Parts of equal length, so that a batch of uneven contexts is balanced by the order in which blocks finish: as long as two blocks
-  // per SM are there, at most 2048 keys (the partial results are under 2 % of the bytes read), and not below 256.
-  const int64_t units = tile_bound(*p, heads / p->kv_heads, ROW_TILE) * p->kv_heads;
-  const int64_t wanted = std::max<int64_t>(1, 2 * sm_count / units);
-  int64_t keys = (longest + wanted - 1) / wanted;
-  keys = std::min<int64_t>(2048, std::max<int64_t>(256, (keys + 63) / 64 * 64));
-  plan.splits = (int)std::max<int64_t>(1, (longest + keys - 1) / keys);
-  plan.split_keys = (int)keys;
+  // the tcgen05 kernel takes its row maximum before the scale, so it needs a positive one
+  plan.kernel = p->head_dim >= 64 && (int64_t)p->rows * group >= 64ll * p->batch && scale > 0.f ? 2 : 1;
+  if (plan.kernel == 2) {
+    // One block per SM.  Parts of a context pay where whole units leave the last round of blocks half empty: the number of parts (of
+    // 512 keys at least) with the fewest key tiles per SM, 4 % added per part for the partial results and the block's own start.
+    const int64_t units = tile_bound(*p, group, 256) * p->kv_heads;
+    double best = 0;
+    for (int splits = 1; splits <= 16 && (splits == 1 || longest / splits >= 512); ++splits) {
+      const double cost = (double)((units * splits + sm_count - 1) / sm_count) / splits * (1 + 0.04 * (splits - 1));
+      if (splits == 1 || cost < 0.95 * best) {
+        best = cost;
+        plan.splits = splits;
+      }
+    }
+    plan.split_keys = (int)std::max<int64_t>(128, ((longest + plan.splits - 1) / plan.splits + 127) / 128 * 128);
+  } else {
+    // Parts of equal length, so that a batch of uneven contexts is balanced by the order in which blocks finish: as long as two
+    // blocks per SM are there, at most 2048 keys (the partial results are under 2 % of the bytes read), and not below 256.
+    const int64_t units = tile_bound(*p, group, ROW_TILE) * p->kv_heads;
+    const int64_t wanted = std::max<int64_t>(1, 2 * sm_count / units);
+    int64_t keys = (longest + wanted - 1) / wanted;
+    keys = std::min<int64_t>(2048, std::max<int64_t>(256, (keys + 63) / 64 * 64));
+    plan.splits = (int)std::max<int64_t>(1, (longest + keys - 1) / keys);
+    plan.split_keys = (int)keys;
+  }
   return plan;
 }
 
@@ -520,12 +520,12 @@ extern "C" int lbi_paged_attention(const lbi_paged_batch* p, const void* q, int6
   using namespace lbi::paged;
   if (p->head_dim % 16 != 0 || p->head_dim > 256 || type < 0 || type > LBI_F16 || heads % p->kv_heads != 0) return (int)cudaErrorInvalidValue;
   if (p->rows == 0 || p->batch == 0) return 0;
+  if ((plan.splits > 1) != (part_o != nullptr)) return (int)cudaErrorInvalidValue;
   AttnArgs a{*p, q, q_stride, out, part_o, part_lse, heads, heads / p->kv_heads, zero_tail, shift_of(p->page_size), plan.splits, plan.split_keys,
              scale * 1.4426950408889634f};
-  if (!rows_tile_covers(p, type))
+  if (plan.kernel == 0)
     return type == LBI_F32 ? launch_row<LBI_F32>(a, st) : type == LBI_BF16 ? launch_row<LBI_BF16>(a, st) : launch_row<LBI_F16>(a, st);
-  if ((plan.splits > 1) != (part_o != nullptr)) return (int)cudaErrorInvalidValue;
-  const int rc = type == LBI_BF16 ? launch_rows<LBI_BF16>(a, st) : launch_rows<LBI_F16>(a, st);
+  const int rc = plan.kernel == 2 ? launch_attn_tiles(a, type, st) : type == LBI_BF16 ? launch_rows<LBI_BF16>(a, st) : launch_rows<LBI_F16>(a, st);
   if (rc != 0 || plan.splits == 1) return rc;
   const int64_t blocks = ((int64_t)p->rows * heads + 3) / 4;
   if (blocks >= (1ll << 31)) return (int)cudaErrorInvalidValue;

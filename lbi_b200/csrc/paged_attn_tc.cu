@@ -1,0 +1,521 @@
+// Causal attention of a chunk of new tokens over a paged cache, on tcgen05 / TMEM / TMA: 16-bit queries, head_dim 64 or 128.
+//
+// A block owns 256 rows (token x head of a group, heads fastest, so that a key is loaded once for all heads of its group): two tiles
+// of 128 rows, each with a softmax warpgroup of its own (one thread per row), and walks the keys 128 at a time:
+//     S_g = Q_g K_j^T        M 128 x N 128, TMEM columns [128 g, 128 g + 128)
+//     P_g = 2^(S_g - m)      rounded to the queries' type and stored over S_g in TMEM (columns [128 g, 128 g + 64)): the second
+//                            product takes its left operand from there, so P never passes through shared memory
+//     O_g += P_g V_j         M 128 x N head_dim, accumulated in TMEM columns [256 + head_dim g, ..)
+// Products of a thread run in the order in which they are issued, so S_g of the next tile may be issued right behind the product that
+// still reads P_g, and the barrier that announces S_g(j + 1) also says that O_g holds tile j.  The running maximum follows the row only
+// when it has grown by more than 2^8: P stays in (0, 2^8], and O is rescaled (a read and a write of TMEM) in the first tiles only.
+// While one warpgroup computes exponentials the tensor core works for the other.
+//
+// Bound by the exponentials (16 per clock and SM: 1024 cycles per 128 x 128 tile) and, at head_dim 128, equally by the products.
+//
+// Keys and values: 16-bit pages come by TMA, one box of page_size rows per page and 64 columns (128-byte swizzle), the ids of a
+// tile's pages read one tile ahead, a lane per page.  Slots behind the context and pages that do not exist are masked out of S, and
+// their rows of V are cleared before the product (0 * NaN would reach every row).  e4m3 pages are read by a converting warpgroup, which
+// stores the codes as 16-bit values (exact) and prepares the scales: with u_j = scale s_j k_scale_j + log2 v_scale_j the weights
+// 2^(u_j - m) carry the value's scale, and the sum of exponentials takes 2^(u_j - m) / v_scale_j.
+// Every wait is bounded (tcgen05.cuh).
+#include <algorithm>
+#include <mutex>
+
+#include "paged.cuh"
+#include "tcgen05.cuh"
+
+namespace lbi {
+namespace paged {
+
+using namespace tc;
+
+constexpr int TC_TILE = 128;
+constexpr int TC_PANEL = TC_TILE * 128;    // 128 rows x 64 16-bit columns
+
+struct alignas(16) KeyMeta {
+  uint32_t there[4];                       // which of the tile's 128 keys exist
+  float ks[TC_TILE], lv[TC_TILE], iv[TC_TILE];   // e4m3: scale * log2(e) * k_scale, log2 v_scale, 1 / v_scale
+};
+
+template <bool E4M3, int DH>
+struct TcSmem {
+  static constexpr int SLOTS = DH == 128 ? 4 : 8;   // K_0, V_0, K_1, V_1, ...
+  // Masks and scales of a key tile: K_j is stored when S_(j - SLOTS / 2) is complete, which follows the softmax of the tile before
+  // that one, so SLOTS / 2 + 2 entries never meet one that is still read.
+  static constexpr int META = SLOTS / 2 + 2;
+  alignas(1024) uint8_t q[2][TC_TILE * DH * 2];
+  alignas(1024) uint8_t kv[SLOTS][TC_TILE * DH * 2];
+  KeyMeta meta[META];
+  int slot_of[2][TC_TILE];                 // e4m3: where the keys of a tile are
+  uint64_t bar_q;
+  uint64_t bar_full[SLOTS];
+  uint64_t bar_empty[SLOTS];
+  uint64_t bar_s[2];
+  uint64_t bar_p[2];
+  uint64_t bar_o[2];
+  uint32_t tmem_base;
+  volatile int abort_flag;
+};
+
+// D[tmem] (+)= A[tmem] * B[smem]
+__device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      "setp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
+      "}\n" ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// 32 lanes x 16 consecutive 32-bit columns, from registers.
+__device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]),
+      "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+template <int TYPE, bool E4M3, int DH>
+__global__ void __launch_bounds__(E4M3 ? 448 : 320, 1)
+attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const AttnArgs a) {
+  using T = typename Elem<TYPE>::T;
+  using Smem = TcSmem<E4M3, DH>;
+  constexpr int SLOTS = Smem::SLOTS, META = Smem::META, PANELS = DH / 64, SLOT_BYTES = TC_TILE * DH * 2;
+  extern __shared__ uint8_t raw_smem[];
+  Smem& s = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~uintptr_t(1023));
+  const lbi_paged_batch& p = a.b;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (a.zero_tail && !a.part_o)
+    for (int64_t row = (int64_t)last_row(p) + blockIdx.x; row < p.rows; row += gridDim.x)
+      for (int i = threadIdx.x; i < a.heads * DH; i += blockDim.x) ((T*)a.out)[row * a.heads * DH + i] = from_f<T>(0.f);
+
+  // ------------------------------------------------------------------ the block's rows and keys
+  const int64_t unit_block = (int64_t)gridDim.x - 1 - blockIdx.x;   // late tokens walk more keys: first
+  const int split = (int)(unit_block % a.splits);
+  const int64_t unit = unit_block / a.splits;
+  const int kh = (int)(unit % p.kv_heads);
+  const int64_t tile = unit / p.kv_heads;
+  const int b = seq_of_tile(p, tile, a.group, 2 * TC_TILE);
+  const int2 r = seq_rows(p, b);
+  const int64_t local64 = (tile - first_tile(p, b, a.group, 2 * TC_TILE)) * (2 * TC_TILE);
+  const int64_t rows_b = (int64_t)(r.y - r.x) * a.group;
+  if (local64 < 0 || local64 >= rows_b) return;
+  const int local = (int)local64, n_rows = (int)min((int64_t)2 * TC_TILE, rows_b - local64);
+  const int first_pos = __ldg(p.context + b) - (r.y - r.x);
+  const int64_t capacity = (int64_t)p.table_width << a.page_shift;
+  const int k0 = split * a.split_keys;
+  int n_kv[2], k_end = 0;   // key tiles of each row tile; one behind the last key any row sees
+#pragma unroll
+  for (int g = 0; g < 2; ++g) {
+    const int last = min(n_rows, (g + 1) * TC_TILE) - 1;   // the tile's last row
+    const int keys = last < g * TC_TILE ? 0 : (int)min((int64_t)first_pos + (local + last) / a.group + 1, capacity);
+    const int k1 = split == a.splits - 1 ? keys : min(keys, k0 + a.split_keys);
+    n_kv[g] = k1 > k0 ? (k1 - k0 + TC_TILE - 1) / TC_TILE : 0;
+    k_end = max(k_end, k1);
+  }
+  const int n_j = max(n_kv[0], n_kv[1]);
+
+  if (threadIdx.x == 0) {
+    s.abort_flag = 0;
+    mbar_init(&s.bar_q, 8);
+    for (int i = 0; i < SLOTS; ++i) {
+      mbar_init(&s.bar_full[i], E4M3 ? 4 : 1);
+      mbar_init(&s.bar_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s.bar_s[i], 1);
+      mbar_init(&s.bar_p[i], 4);
+      mbar_init(&s.bar_o[i], 1);
+    }
+    fence_barrier_init();
+    if (!E4M3) {
+      prefetch_tmap(&map_k);
+      prefetch_tmap(&map_v);
+    }
+  }
+  if (warp == 8) tmem_alloc(&s.tmem_base, 512);
+  fence_before_sync();
+  __syncthreads();
+  fence_after_sync();
+  const uint32_t tmem = s.tmem_base;
+  volatile int* abortp = &s.abort_flag;
+
+  if (warp == 8) {
+    // ======================================================================== MMA issuer (all lanes wait, lane 0 issues)
+    constexpr uint32_t F16_BITS = (1u << 7) | (1u << 10);
+    const uint32_t idesc_s = make_idesc_bf16(128, 128, 0, 0) & (TYPE == LBI_F16 ? ~F16_BITS : ~0u);
+    const uint32_t idesc_o = make_idesc_bf16(128, DH, 0, 1) & (TYPE == LBI_F16 ? ~F16_BITS : ~0u);
+    const uint64_t kmajor0 = make_smem_desc(0, 16, 1024), mnmajor0 = make_smem_desc(0, TC_PANEL, 1024);
+    const uint32_t q16 = smem_u32(s.q[0]) >> 4, kv16 = smem_u32(s.kv[0]) >> 4;
+    constexpr uint32_t SLOT16 = SLOT_BYTES >> 4, PANEL16 = TC_PANEL >> 4;
+    auto issue_s = [&](int g, int n) {   // n: index of K_j in the slot sequence
+      if (lane == 0) {
+        const uint64_t da = kmajor0 + q16 + g * SLOT16, db = kmajor0 + kv16 + (n % SLOTS) * SLOT16;
+#pragma unroll
+        for (int kk = 0; kk < DH / 16; ++kk) {
+          const uint32_t step = (kk >> 2) * PANEL16 + (kk & 3) * 2;
+          mma_bf16(tmem + g * 128, da + step, db + step, idesc_s, kk);
+        }
+        mma_commit(&s.bar_s[g]);
+      }
+    };
+    auto wait_full = [&](int n) { return mbar_wait(&s.bar_full[n % SLOTS], (n / SLOTS) & 1, abortp, p.status, 41); };
+    bool ok = n_j == 0 || (mbar_wait(&s.bar_q, 0, abortp, p.status, 42) && wait_full(0));
+    if (ok && n_j > 0) {
+      fence_after_sync();
+      for (int g = 0; g < 2; ++g)
+        if (n_kv[g] > 0) issue_s(g, 0);
+      if (lane == 0) mma_commit(&s.bar_empty[0]);
+    }
+    for (int j = 0; j < n_j && ok; ++j) {
+      const int nv = 2 * j + 1, nk = 2 * j + 2;
+      ok = wait_full(nv);
+      if (!ok) break;
+      if (!E4M3) {   // rows of V that belong to no key
+        const uint32_t* there = s.meta[j % META].there;
+        if ((there[0] & there[1] & there[2] & there[3]) != 0xffffffffu) {
+          for (int row = lane; row < TC_TILE; row += 32)
+            if (!(there[row >> 5] >> (row & 31) & 1u)) {
+              const uint32_t at = smem_u32(s.kv[nv % SLOTS]) + row * 128;
+#pragma unroll
+              for (int c = 0; c < PANELS * 8; ++c)
+                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at + (c >> 3) * TC_PANEL + (c & 7) * 16), "r"(0) : "memory");
+            }
+          fence_proxy_async();
+          __syncwarp();
+        }
+      }
+      bool next_k = j + 1 < n_j;
+      if (next_k) ok = wait_full(nk);
+      for (int g = 0; g < 2 && ok; ++g) {
+        if (j >= n_kv[g]) continue;
+        ok = mbar_wait(&s.bar_p[g], j & 1, abortp, p.status, 43);
+        if (!ok) break;
+        fence_after_sync();
+        if (lane == 0) {
+          const uint64_t db = mnmajor0 + kv16 + (nv % SLOTS) * SLOT16;
+#pragma unroll
+          for (int kk = 0; kk < 8; ++kk) mma_ts(tmem + 256 + g * DH, tmem + g * 128 + kk * 8, db + 128 * kk, idesc_o, (j > 0 || kk > 0) ? 1u : 0u);
+          if (j + 1 == n_kv[g]) mma_commit(&s.bar_o[g]);
+        }
+        if (j + 1 < n_kv[g]) issue_s(g, nk);
+      }
+      if (ok && lane == 0) {
+        mma_commit(&s.bar_empty[nv % SLOTS]);
+        if (next_k) mma_commit(&s.bar_empty[nk % SLOTS]);
+      }
+    }
+  } else if (warp == 9 && !E4M3) {
+    // ======================================================================== TMA producer: one lane per page
+    const int per = TC_TILE >> a.page_shift;   // pages of a tile, 1 .. 16
+    const int* table = p.table + (int64_t)b * p.table_stride;
+    auto load_page = [&](int j) {
+      const int pos = k0 + j * TC_TILE + (lane << a.page_shift);
+      return j < n_j && lane < per && pos < k_end ? __ldg(table + (pos >> a.page_shift)) : -1;
+    };
+    int page = load_page(0);
+    bool ok = true;
+    for (int j = 0; j < n_j && ok; ++j) {
+      const int next = load_page(j + 1);
+      const int base = k0 + j * TC_TILE;
+      const bool wanted = lane < per && base + (lane << a.page_shift) < k_end;
+      const bool good = wanted && page >= 0 && page < p.num_pages;
+      if (wanted && !good && p.status) atomicCAS(p.status, 0, 84);
+      const uint32_t pages = __ballot_sync(0xffffffffu, good);
+      const uint32_t bytes = __popc(pages) * (uint32_t)p.page_size * DH * 2;
+      const int row = (max(page, 0) * p.kv_heads + kh) * p.page_size;
+#pragma unroll
+      for (int v = 0; v < 2 && ok; ++v) {
+        const int n = 2 * j + v, st = n % SLOTS;
+        if (n >= SLOTS) ok = mbar_wait(&s.bar_empty[st], ((n / SLOTS) - 1) & 1, abortp, p.status, 44);
+        if (!ok) break;
+        if (v == 0 && lane < 4) {
+          uint32_t there = 0;
+          for (int i = 0; i < 32; ++i) {
+            const int key = lane * 32 + i;
+            if ((pages >> (key >> a.page_shift) & 1u) && base + key < k_end) there |= 1u << i;
+          }
+          s.meta[j % META].there[lane] = there;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive_expect_tx(&s.bar_full[st], bytes);
+        __syncwarp();
+        if (good) {
+#pragma unroll
+          for (int c = 0; c < PANELS; ++c)
+            tma_load_2d(s.kv[st] + c * TC_PANEL + (lane << a.page_shift) * 128, v ? &map_v : &map_k, &s.bar_full[st], c * 64, row);
+        }
+        __syncwarp();
+      }
+      page = next;
+    }
+  } else if (warp < 8) {
+    // ======================================================================== softmax warpgroups
+    const int g = warp >> 2, quarter = warp & 3;
+    const int row = quarter * 32 + lane;             // of the tile
+    // queries: 16-byte chunks of the warp's 32 rows, neighbouring lanes on neighbouring chunks, into the swizzled tile
+    for (int i = lane; i < 32 * (DH / 8); i += 32) {
+      const int rr = quarter * 32 + i / (DH / 8), c = i % (DH / 8);
+      const int at = g * TC_TILE + rr;
+      uint4 x = make_uint4(0, 0, 0, 0);
+      if (at < n_rows) {
+        const int tok = (local + at) / a.group, head = kh * a.group + (local + at) % a.group;
+        x = __ldg(reinterpret_cast<const uint4*>((const T*)a.q + (int64_t)(r.x + tok) * a.q_stride + head * DH) + c);
+      }
+      *reinterpret_cast<uint4*>(s.q[g] + (c >> 3) * TC_PANEL + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = x;
+    }
+    fence_proxy_async();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&s.bar_q);
+
+    const int mine = g == 0 ? n_kv[0] : n_kv[1];
+    const bool live = g * TC_TILE + row < n_rows;
+    const int limit = live ? first_pos + (local + g * TC_TILE + row) / a.group : -1;
+    const uint32_t t_s = tmem + ((uint32_t)(quarter * 32) << 16) + g * 128;
+    const uint32_t t_o = tmem + ((uint32_t)(quarter * 32) << 16) + 256 + g * DH;
+    float m = -INFINITY, l = 0.f;
+    bool ok = true;
+    for (int j = 0; j < mine; ++j) {
+      ok = mbar_wait(&s.bar_s[g], j & 1, abortp, p.status, 45);
+      if (!ok) break;
+      fence_after_sync();
+      const KeyMeta& meta = s.meta[j % META];
+      const int rel = limit - (k0 + j * TC_TILE);    // the row's last key, counted from the tile's first
+      uint32_t seen[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int e = rel - 32 * c;
+        seen[c] = meta.there[c] & (e >= 31 ? 0xffffffffu : e < 0 ? 0u : (2u << e) - 1u);
+      }
+      const bool masked = __any_sync(0xffffffffu, (seen[0] & seen[1] & seen[2] & seen[3]) != 0xffffffffu);
+      float top = -INFINITY;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t x[32];
+        tmem_ld_32x32(t_s + c * 32, x);
+        tmem_ld_wait();
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          float u = __uint_as_float(x[e]);
+          if (E4M3) u = fmaf(u, meta.ks[c * 32 + e], meta.lv[c * 32 + e]);
+          if (masked && !(seen[c] >> e & 1u)) u = -INFINITY;
+          top = fmaxf(top, u);
+        }
+      }
+      if (!E4M3) top *= a.scale_log2;   // scale > 0: see the entry point
+      // the reference point follows only a growth by more than 2^8
+      const bool grow = top > m + 8.f;
+      if (__any_sync(0xffffffffu, grow)) {
+        const float m_new = grow ? top : m;
+        const float keep = m == m_new ? 1.f : ex2(m - m_new);
+        m = m_new;
+        l *= keep;
+        if (j > 0) {
+#pragma unroll
+          for (int c = 0; c < DH / 16; ++c) {
+            uint32_t x[16];
+            tmem_ld_32x16(t_o + c * 16, x);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * keep);
+            tmem_st_32x16(t_o + c * 16, x);
+          }
+        }
+      }
+      const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t x[32], w[16];
+        tmem_ld_32x32(t_s + c * 32, x);
+        tmem_ld_wait();
+        float sum0 = 0.f, sum1 = 0.f;
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) {
+          float u[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            u[i] = __uint_as_float(x[e + i]);
+            if (E4M3) u[i] = ex2(fmaf(u[i], meta.ks[c * 32 + e + i], meta.lv[c * 32 + e + i]) - ref);
+            else u[i] = ex2(fmaf(u[i], a.scale_log2, -ref));
+            if (masked && !(seen[c] >> (e + i) & 1u)) u[i] = 0.f;
+          }
+          if (E4M3) {
+            sum0 = fmaf(u[0], meta.iv[c * 32 + e], sum0);
+            sum1 = fmaf(u[1], meta.iv[c * 32 + e + 1], sum1);
+          } else {
+            sum0 += u[0];
+            sum1 += u[1];
+          }
+          w[e >> 1] = pack16<TYPE>(u[0], u[1]);
+        }
+        l += sum0 + sum1;
+        tmem_st_32x16(t_s + c * 16, w);   // over columns that have been read
+      }
+      tmem_st_wait();
+      fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s.bar_p[g]);
+    }
+    if (ok && mine > 0) ok = mbar_wait(&s.bar_o[g], 0, abortp, p.status, 46);
+    if (ok) {
+      fence_after_sync();
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const int at = local + g * TC_TILE + row;
+      const int64_t o_row = (int64_t)(r.x + at / a.group) * a.heads + kh * a.group + at % a.group;
+#pragma unroll
+      for (int c = 0; c < DH / 32; ++c) {
+        uint32_t x[32];
+        if (mine > 0) {
+          tmem_ld_32x32(t_o + c * 32, x);
+          tmem_ld_wait();
+        }
+        float f[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) f[e] = mine > 0 ? __uint_as_float(x[e]) * inv : 0.f;
+        if (live) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 8) {
+            if (a.part_o) store_f<float, 8>(a.part_o + (o_row * a.splits + split) * DH + c * 32 + e, f + e);
+            else store_f<T, 8>((T*)a.out + o_row * DH + c * 32 + e, f + e);
+          }
+        }
+      }
+      if (live && a.part_o) a.part_lse[o_row * a.splits + split] = l == 0.f ? -INFINITY : m + log2f(l);
+    }
+  } else if (E4M3 && warp >= 10) {
+    // ======================================================================== converting warpgroup (warps 10 .. 13)
+    const int tid = threadIdx.x - 320;               // 0 .. 127: also the key whose slot and scales this thread looks up
+    const int* table = p.table + (int64_t)b * p.table_stride;
+    constexpr int CH = DH / 16;                      // 16-byte chunks of a row of codes
+    auto load_page = [&](int j) {
+      const int pos = k0 + j * TC_TILE + tid;
+      return j < n_j && pos < k_end ? __ldg(table + (pos >> a.page_shift)) : -1;
+    };
+    int page = load_page(0);
+    bool ok = true;
+    for (int j = 0; j < n_j; ++j) {   // after a failed wait too: all four warps meet at the barrier below
+      const int next = load_page(j + 1);
+      const int pos = k0 + j * TC_TILE + tid;
+      int slot = -1;
+      if (pos < k_end) {
+        if (page >= 0 && page < p.num_pages) slot = (page * p.kv_heads + kh) * p.page_size + (pos & (p.page_size - 1));
+        else if (p.status) atomicCAS(p.status, 0, 84);
+      }
+      page = next;
+      const float k_scale = slot >= 0 ? __ldg(p.k_scale + slot) : 0.f, v_scale = slot >= 0 ? __ldg(p.v_scale + slot) : 0.f;
+      s.slot_of[j & 1][tid] = slot;
+      const uint32_t there = __ballot_sync(0xffffffffu, slot >= 0);
+      named_barrier_sync(1, 128);
+      uint4 raw[2][CH];
+#pragma unroll
+      for (int v = 0; v < 2; ++v)
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+          const int id = i * 128 + tid;
+          const int sl = s.slot_of[j & 1][id / CH];
+          raw[v][i] = sl >= 0 ? __ldg(reinterpret_cast<const uint4*>((const uint8_t*)(v ? p.v : p.k) + (int64_t)sl * DH) + id % CH) : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+      for (int v = 0; v < 2 && ok; ++v) {
+        const int n = 2 * j + v, st = n % SLOTS;
+        if (n >= SLOTS) ok = mbar_wait(&s.bar_empty[st], ((n / SLOTS) - 1) & 1, abortp, p.status, 47);
+        if (!ok) break;
+        if (v == 0) {   // behind the wait, see META
+          KeyMeta& meta = s.meta[j % META];
+          const float vs = positive_scale(v_scale);
+          meta.ks[tid] = k_scale * a.scale_log2;
+          meta.lv[tid] = lg2(vs);
+          meta.iv[tid] = __frcp_rn(vs);
+          if (lane == 0) meta.there[warp - 10] = there;
+        }
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+          const int id = i * 128 + tid, row = id / CH, c = id % CH;
+          const uint32_t* w = reinterpret_cast<const uint32_t*>(&raw[v][i]);
+          uint32_t x[8];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) codes_to_16<TYPE>(w[e], x[2 * e], x[2 * e + 1]);
+          uint8_t* dst = s.kv[st] + (c >> 2) * TC_PANEL + row * 128;
+          *reinterpret_cast<uint4*>(dst + (((2 * (c & 3)) ^ (row & 7)) << 4)) = make_uint4(x[0], x[1], x[2], x[3]);
+          *reinterpret_cast<uint4*>(dst + (((2 * (c & 3) + 1) ^ (row & 7)) << 4)) = make_uint4(x[4], x[5], x[6], x[7]);
+        }
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s.bar_full[st]);
+      }
+    }
+  }
+
+  // ---------------------------------------------------------------------- teardown
+  __syncwarp();
+  if (s.abort_flag) {
+    const unsigned long long t0 = global_ns();
+    while (global_ns() - t0 < 2000000ull) __nanosleep(1000);  // let copies in flight land before smem is released
+  }
+  fence_before_sync();
+  __syncthreads();
+  if (warp == 8) {
+    fence_after_sync();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ host side
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
+                                  CUtensorMapFloatOOBfill);
+
+static EncodeTiledFn encode_fn() {
+  static EncodeTiledFn fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult res;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &res) == cudaSuccess && res == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeTiledFn>(ptr);
+  });
+  return fn;
+}
+
+template <int TYPE, bool E4M3, int DH>
+static int launch_tiles(const AttnArgs& a, cudaStream_t st) {
+  CUtensorMap map[2] = {};
+  if (!E4M3) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return 801;
+    const cuuint64_t dims[2] = {DH, (cuuint64_t)a.b.num_pages * a.b.kv_heads * a.b.page_size};
+    const cuuint64_t strides[1] = {DH * 2};
+    const cuuint32_t box[2] = {64, (cuuint32_t)a.b.page_size}, estr[2] = {1, 1};
+    for (int v = 0; v < 2; ++v) {
+      const CUresult rc = fn(&map[v], TYPE == LBI_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, v ? a.b.v : a.b.k, dims,
+                             strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+      if (rc != CUDA_SUCCESS) return 1000 + (int)rc;
+    }
+  }
+  auto kernel = attn_tiles_kernel<TYPE, E4M3, DH>;
+  const int smem = (int)sizeof(TcSmem<E4M3, DH>) + 1024;
+  static lbi::PerDeviceOnce once;
+  cudaError_t e = once.max_dynamic_smem(kernel, smem);
+  if (e != cudaSuccess) return (int)e;
+  const int64_t blocks = tile_bound(a.b, a.group, 2 * TC_TILE) * a.b.kv_heads * a.splits;
+  if (blocks >= (1ll << 31)) return (int)cudaErrorInvalidValue;
+  kernel<<<(unsigned)blocks, E4M3 ? 448 : 320, smem, st>>>(map[0], map[1], a);
+  return (int)cudaGetLastError();
+}
+
+int launch_attn_tiles(const AttnArgs& a, int type, cudaStream_t st) {
+  const bool e4m3 = a.b.cache_type == LBI_E4M3, wide = a.b.head_dim == 128;
+  if (type == LBI_BF16)
+    return e4m3 ? (wide ? launch_tiles<LBI_BF16, true, 128>(a, st) : launch_tiles<LBI_BF16, true, 64>(a, st))
+                : (wide ? launch_tiles<LBI_BF16, false, 128>(a, st) : launch_tiles<LBI_BF16, false, 64>(a, st));
+  return e4m3 ? (wide ? launch_tiles<LBI_F16, true, 128>(a, st) : launch_tiles<LBI_F16, true, 64>(a, st))
+              : (wide ? launch_tiles<LBI_F16, false, 128>(a, st) : launch_tiles<LBI_F16, false, 64>(a, st));
+}
+
+}  // namespace paged
+}  // namespace lbi

@@ -82,7 +82,7 @@ def attention_oracle(batch, q, scale):
                     prod = kk * qd[at + i, h]
                     p = torch.softmax(prod.sum(-1) * scale, dim=0)
                     o, size = p @ vv, p @ vv.abs()
-                    score_off = (batch.dim + 8) * F32 * float(prod.abs().sum(-1).max()) * scale
+                    score_off = (batch.dim + 8) * F32 * float(prod.abs().sum(-1).max()) * abs(scale)
                     rounded_p = eps if batch.dtype != torch.float32 else 0.0
                     out[at + i, h] = o
                     tol[at + i, h] = 1.01 * (eps * o.abs() + size * (rounded_p + 2 * score_off + (n + 16) * F32))

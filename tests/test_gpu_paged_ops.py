@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from lbi_b200 import ops
-from paged_oracle import Batch, check_append, check_attention, check_gather, check_logits
+from paged_oracle import Batch, attention_oracle, check_append, check_attention, check_gather, check_logits
 from test_paged_ops import SEQS, refusals
 
 pytestmark = pytest.mark.gpu
@@ -125,6 +125,27 @@ def test_missing_pages_are_skipped_and_recorded():
         assert ops.ext().kernel_status(like) == 84 and not bool(k[0, 0, 8:].any())
         ops.kv_append(qkv, pages, table, ctx, 1, rope=(torch.zeros(4, 32, device=DEV), torch.zeros(4, 32, device=DEV), False))
         assert ops.ext().kernel_status(like) in (83, 84)
+
+
+@pytest.mark.parametrize("dim,group,cache", [(64, 1, "same"), (128, 3, "same"), (64, 4, "e4m3"), (128, 1, "e4m3")])
+def test_chunks_skip_missing_pages_and_cut_long_contexts(dim, group, cache):
+    batch = Batch([(150, 1700)], group, 1, dim, 16, BF16, cache, DEV)     # few rows, many keys: cut into parts
+    q = batch.queries()
+    whole = ops.paged_attention(q, batch.pages, batch.table, batch.context, 0.1)
+    batch.table[0, 5] = 10 ** 6
+    got = ops.paged_attention(q, batch.pages, batch.table, batch.context, 0.1)
+    assert ops.ext().kernel_status(q) == 84
+    kept = torch.cat([torch.arange(80), torch.arange(96, 1700)])
+    shorter = Batch([(150, 1684)], group, 1, dim, 16, BF16, cache, DEV)
+    shorter.k, shorter.v = [batch.k[0][:, kept]], [batch.v[0][:, kept]]
+    want, tol = attention_oracle(shorter, q, 0.1)
+    assert bool(((got.double().cpu() - want).abs() <= tol).all()) and not torch.equal(got, whole)
+
+
+@pytest.mark.parametrize("scale", [-0.1, 0.0])
+def test_any_scale(scale):
+    check_attention(Batch([(1, 90), (70, 200)], 2, 2, 64, 16, BF16, "same", DEV), scale=scale)
+    check_attention(Batch([(70, 200)], 2, 2, 64, 16, BF16, "e4m3", DEV), scale=scale)
 
 
 def test_non_finite_rows_of_an_8_bit_cache():
