@@ -12,7 +12,11 @@ import torch
 import torch.nn.functional as F
 from torch import nn
 
-from .rope import apply_rope
+from .rope import apply_rope, rope_tables
+
+
+KV_CACHES = ("paged", "e4m3")
+KV_PAGE_SIZE = 16
 
 
 class CausalSelfAttention(nn.Module):
@@ -101,10 +105,26 @@ class CausalSelfAttention(nn.Module):
         return self.out_proj(out)
 
     # ------------------------------------------------------------------ token-by-token decoding
-    def allocate_decode_state(self, batch_size: int, max_len: int, device=None, dtype=None) -> dict:
-        """Key / value cache for ``max_len`` positions, the last ``d_conv - 1`` pre-convolution qkv rows, the position counter."""
+    def allocate_decode_state(self, batch_size: int, max_len: int, device=None, dtype=None, kv_cache: str | None = None) -> dict:
+        """Key / value cache for ``max_len`` positions, the last ``d_conv - 1`` pre-convolution qkv rows, the position counter.
+
+        ``kv_cache``: None keeps one contiguous tensor per sequence; ``"paged"`` keeps pages in ``dtype`` and ``"e4m3"`` pages in
+        8 bits with a scale per token and head, both read by the paged attention kernels (``ops.paged_attention``)."""
         device = self.in_proj.weight.device if device is None else device
         dtype = self.in_proj.weight.dtype if dtype is None else dtype
+        if kv_cache is not None:
+            if kv_cache not in KV_CACHES:
+                raise ValueError(f"kv_cache must be None or one of {KV_CACHES}, got {kv_cache!r}")
+            from lbi_b200 import ops
+
+            width = -(-max(int(max_len), 1) // KV_PAGE_SIZE)
+            state = {"pages": ops.kv_pages(max(1, batch_size * width), KV_PAGE_SIZE, self.n_kv_heads, self.head_dim,
+                                           torch.float8_e4m3fn if kv_cache == "e4m3" else dtype, device),
+                     "table": torch.arange(batch_size * width, dtype=torch.int32, device=device).view(batch_size, width),
+                     "context": torch.zeros(batch_size, dtype=torch.int32, device=device), "dtype": dtype, "max_len": int(max_len), "pos": 0}
+            if self.d_conv > 0:
+                state["conv"] = torch.zeros(batch_size, self.qkv_dim, self.d_conv - 1, device=device, dtype=dtype)
+            return state
         state = {"k": torch.zeros(batch_size, self.n_kv_heads, max_len, self.head_dim, device=device, dtype=dtype),
                  "v": torch.zeros(batch_size, self.n_kv_heads, max_len, self.head_dim, device=device, dtype=dtype), "pos": 0}
         if self.d_conv > 0:
@@ -114,6 +134,8 @@ class CausalSelfAttention(nn.Module):
     @torch.no_grad()
     def step(self, x: torch.Tensor, state: dict) -> torch.Tensor:
         """One token x [B, D] at position ``state['pos']`` -> [B, D]; equals row ``pos`` of ``forward`` on the whole sequence."""
+        if "pages" in state:
+            return self.extend(x.unsqueeze(1), state)[:, 0]
         bsz, pos = x.shape[0], int(state["pos"])
         if pos >= state["k"].shape[2]:
             raise ValueError("the key / value cache is full")
@@ -133,3 +155,28 @@ class CausalSelfAttention(nn.Module):
         keys, values = self.expand_kv(state["k"][:, :, : pos + 1]), self.expand_kv(state["v"][:, :, : pos + 1])
         out = F.scaled_dot_product_attention(q, keys.to(q.dtype), values.to(q.dtype), dropout_p=0.0, is_causal=False, scale=self.scale)
         return self.out_proj(out.transpose(1, 2).reshape(bsz, self.out_dim))
+
+    @torch.no_grad()
+    def extend(self, x: torch.Tensor, state: dict) -> torch.Tensor:
+        """The next n tokens x [B, n, D] over a paged state -> [B, n, D]; equals rows ``pos .. pos + n - 1`` of ``forward``."""
+        from lbi_b200 import ops
+
+        if "pages" not in state:
+            raise ValueError("extend needs a paged decode state (allocate_decode_state(..., kv_cache=...))")
+        bsz, n, _ = x.shape
+        end = int(state["pos"]) + n
+        if end > state["max_len"]:
+            raise ValueError("the key / value cache is full")
+        qkv = self.in_proj(x)
+        if self.d_conv > 0:
+            window = torch.cat([state["conv"], qkv.transpose(1, 2).to(state["conv"].dtype)], dim=-1)  # [B, C, d_conv - 1 + n]
+            state["conv"].copy_(window[..., n:])
+            qkv = F.conv1d(window, self.conv1d.weight.to(window.dtype), None if self.conv1d.bias is None else self.conv1d.bias.to(window.dtype),
+                           groups=self.qkv_dim).transpose(1, 2)
+        cos, sin = rope_tables(state["max_len"], self.head_dim, self.rope_base, x.device)
+        state["context"].fill_(end)
+        state["pos"] = end
+        rows = qkv.reshape(bsz * n, self.qkv_dim).to(state["dtype"])
+        q = ops.kv_append(rows, state["pages"], state["table"], state["context"], self.n_heads, rope=(cos, sin, self.rope_interleaved))
+        out = ops.paged_attention(q, state["pages"], state["table"], state["context"], self.scale, max_context=end)
+        return self.out_proj(out.view(bsz, n, self.out_dim).to(x.dtype))

@@ -1,7 +1,8 @@
 """Minimal HTTP front end for ``inference.generate``:  python -m lbi_b200.serve RUN_DIR [--host 127.0.0.1] [--port 8000]
 
 ``POST /generate`` with ``{"prompt": "text"}`` or ``{"prompt_ids": [1, 2, 3]}`` and optional ``max_new_tokens``, ``temperature``,
-``top_k``, ``seed``, ``total_len`` returns ``{"prompt_ids", "new_ids", "text"}``; ``GET /health`` reports the model.  Requests are
+``top_k``, ``seed``, ``total_len``, ``repetition_penalty``, ``presence_penalty``, ``frequency_penalty``, ``logit_bias`` ({id: value})
+and ``allowed_ids`` ([id, ...]) returns ``{"prompt_ids", "new_ids", "text"}``; ``GET /health`` reports the model.  Requests are
 served one at a time (one model, one device); the request logic is ``GenerationService.handle`` and works without the web stack.
 """
 from __future__ import annotations
@@ -11,15 +12,17 @@ from typing import Any
 
 import torch
 
-from .inference import generate, load_run, load_run_tokenizer
+from .inference import LogitRules, generate, load_run, load_run_tokenizer
 
 
 class GenerationService:
     """One loaded run (model, config, tokenizer) behind a lock; ``handle(request)`` validates, generates and decodes."""
 
-    def __init__(self, model: Any, cfg: Any, tokenizer: Any = None, *, max_new_tokens_limit: int = 1024) -> None:
+    def __init__(self, model: Any, cfg: Any, tokenizer: Any = None, *, max_new_tokens_limit: int = 1024,
+                 kv_cache: str | None = None) -> None:
         self.model, self.cfg, self.tokenizer = model, cfg, tokenizer
         self.limit = int(max_new_tokens_limit)
+        self.kv_cache = kv_cache
         self._lock = threading.Lock()
 
     @classmethod
@@ -54,6 +57,16 @@ class GenerationService:
             return bytes(i % 256 for i in ids).decode("utf-8", errors="replace")
         return None
 
+    @staticmethod
+    def _rules(request: dict) -> LogitRules:
+        try:
+            bias = {int(k): float(v) for k, v in dict(request.get("logit_bias") or {}).items()} or None
+            allowed = [int(i) for i in request.get("allowed_ids") or []] or None
+            return LogitRules(float(request.get("repetition_penalty", 1.0)), float(request.get("presence_penalty", 0.0)),
+                              float(request.get("frequency_penalty", 0.0)), bias, allowed)
+        except TypeError as exc:
+            raise ValueError(f"malformed sampling rules: {exc}") from exc
+
     def handle(self, request: dict) -> dict:
         """One generation request -> response dict; raises ValueError for a malformed request."""
         ids = self._encode(request)
@@ -62,12 +75,14 @@ class GenerationService:
             raise ValueError(f"max_new_tokens must be in 1..{self.limit}")
         temperature = float(request.get("temperature", 0.0))
         top_k = int(request.get("top_k", 0)) or None
+        rules = self._rules(request)
         device = next(self.model.parameters()).device
         prompt = torch.tensor([ids], dtype=torch.long, device=device)
         total = int(request.get("total_len", 0)) or max(int(self.cfg.seq_len), prompt.shape[1] + new)
         gen = torch.Generator(device=device).manual_seed(int(request.get("seed", 0))) if temperature > 0 else None
         with self._lock:
-            out = generate(self.model, prompt, new, total_len=total, temperature=temperature, top_k=top_k, generator=gen)
+            out = generate(self.model, prompt, new, total_len=total, temperature=temperature, top_k=top_k, generator=gen,
+                           kv_cache=self.kv_cache, rules=rules)
         new_ids = out[0, prompt.shape[1]:].tolist()
         return {"prompt_ids": ids, "new_ids": new_ids, "text": self._decode(new_ids)}
 
@@ -101,12 +116,14 @@ def main(argv: list[str] | None = None) -> None:
     p.add_argument("--port", type=int, default=8000)
     p.add_argument("--checkpoint", choices=("best", "latest"), default="latest")
     p.add_argument("--device", choices=("auto", "cpu", "cuda"), default="auto")
+    p.add_argument("--kv-cache", choices=("contiguous", "paged", "e4m3"), default="contiguous", help="layout of the key / value cache")
     p.add_argument("--max-new-tokens-limit", type=int, default=1024)
     ns = p.parse_args(argv)
     import uvicorn
 
     service = GenerationService.from_run(ns.run_dir, checkpoint=ns.checkpoint, device=ns.device,
-                                         max_new_tokens_limit=ns.max_new_tokens_limit)
+                                         max_new_tokens_limit=ns.max_new_tokens_limit,
+                                         kv_cache=None if ns.kv_cache == "contiguous" else ns.kv_cache)
     uvicorn.run(build_app(service), host=ns.host, port=ns.port)
 
 
