@@ -150,19 +150,38 @@ __device__ __forceinline__ uint32_t pack16(float a, float b) {
   return d;
 }
 
-// Four e4m3 codes -> two words of a 16-bit type, exactly.  fp16 has the conversion; for bf16 sign, exponent and mantissa are moved to
-// their places (which divides the value by 2^120, codes below the normal range included) and multiplied by 2^120.  A NaN code comes
-// out as 480 there: rows with a NaN are written with a NaN scale.
+// Four e4m3 codes -> two words of a 16-bit type, exactly: sign, exponent and mantissa are moved to their places, which divides the value
+// by 2^120 (bf16) or 2^8 (fp16), codes below the normal range included, and the quotient is multiplied back.  (fp16 has a conversion
+// instruction, but it runs on the unit of the exponentials.)  A NaN code comes out as 480: rows with a NaN carry a NaN scale.
 template <int TYPE>
 __device__ __forceinline__ void codes_to_16(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  const uint32_t a = __byte_perm(w, 0, 0x1404), b = __byte_perm(w, 0, 0x3424);
   if (TYPE == LBI_F16) {
-    asm("{\n.reg .b16 a, b;\nmov.b32 {a, b}, %2;\ncvt.rn.f16x2.e4m3x2 %0, a;\ncvt.rn.f16x2.e4m3x2 %1, b;\n}" : "=r"(lo), "=r"(hi) : "r"(w));
+    const uint32_t x = ((a >> 1) & 0x3f803f80u) | (a & 0x80008000u), y = ((b >> 1) & 0x3f803f80u) | (b & 0x80008000u);
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(lo) : "r"(x), "r"(0x5c005c00u));
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(hi) : "r"(y), "r"(0x5c005c00u));
   } else {
-    const uint32_t a = __byte_perm(w, 0, 0x1404), b = __byte_perm(w, 0, 0x3424);
     const uint32_t x = ((a >> 4) & 0x07f007f0u) | (a & 0x80008000u), y = ((b >> 4) & 0x07f007f0u) | (b & 0x80008000u);
     asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(lo) : "r"(x), "r"(0x7b807b80u));
     asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(hi) : "r"(y), "r"(0x7b807b80u));
   }
+}
+
+// Two fp32 operations per instruction (packed pairs, sm_100).
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<unsigned long long&>(d))
+      : "l"(reinterpret_cast<const unsigned long long&>(a)), "l"(reinterpret_cast<const unsigned long long&>(b)),
+        "l"(reinterpret_cast<const unsigned long long&>(c)));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<unsigned long long&>(d))
+      : "l"(reinterpret_cast<const unsigned long long&>(a)), "l"(reinterpret_cast<const unsigned long long&>(b)));
+  return d;
 }
 
 // Scale of a value row: a row of zeros has scale 0, which has no logarithm and no reciprocal; its codes are 0, so any positive

@@ -35,7 +35,8 @@ constexpr int TC_PANEL = TC_TILE * 128;    // 128 rows x 64 16-bit columns
 
 struct alignas(16) KeyMeta {
   uint32_t there[4];                       // which of the tile's 128 keys exist
-  float ks[TC_TILE], lv[TC_TILE], iv[TC_TILE];   // e4m3: scale * log2(e) * k_scale, log2 v_scale, 1 / v_scale
+  // e4m3, for two neighbouring keys: scale * log2(e) * k_scale of both, log2 v_scale of both; 1 / v_scale
+  float ks_lv[TC_TILE / 2][4], iv[TC_TILE];
 };
 
 template <bool E4M3, int DH>
@@ -78,8 +79,16 @@ __device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t* r)
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// Registers of a warpgroup: claimed ones come from those that the block was launched with and others have released.  16-bit pages
+// (384 threads, 168 each at launch): 2 x 128 x 224 + 128 x 56 = 64512; e4m3 (512 threads, 128 each): 2 x 128 x 176 + 128 x 56 +
+// 128 x 104 = 65536.
+template <int N>
+__device__ __forceinline__ void claim_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void release_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
 template <int TYPE, bool E4M3, int DH>
-__global__ void __launch_bounds__(E4M3 ? 448 : 320, 1)
+__global__ void __launch_bounds__(E4M3 ? 512 : 384, 1)
 attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const AttnArgs a) {
   using T = typename Elem<TYPE>::T;
   using Smem = TcSmem<E4M3, DH>;
@@ -144,117 +153,125 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   const uint32_t tmem = s.tmem_base;
   volatile int* abortp = &s.abort_flag;
 
-  if (warp == 8) {
-    // ======================================================================== MMA issuer (all lanes wait, lane 0 issues)
-    constexpr uint32_t F16_BITS = (1u << 7) | (1u << 10);
-    const uint32_t idesc_s = make_idesc_bf16(128, 128, 0, 0) & (TYPE == LBI_F16 ? ~F16_BITS : ~0u);
-    const uint32_t idesc_o = make_idesc_bf16(128, DH, 0, 1) & (TYPE == LBI_F16 ? ~F16_BITS : ~0u);
-    const uint64_t kmajor0 = make_smem_desc(0, 16, 1024), mnmajor0 = make_smem_desc(0, TC_PANEL, 1024);
-    const uint32_t q16 = smem_u32(s.q[0]) >> 4, kv16 = smem_u32(s.kv[0]) >> 4;
-    constexpr uint32_t SLOT16 = SLOT_BYTES >> 4, PANEL16 = TC_PANEL >> 4;
-    auto issue_s = [&](int g, int n) {   // n: index of K_j in the slot sequence
-      if (lane == 0) {
-        const uint64_t da = kmajor0 + q16 + g * SLOT16, db = kmajor0 + kv16 + (n % SLOTS) * SLOT16;
+  if (warp >= 8 && warp < 12) {
+    release_registers<56>();
+    if (warp == 8) {
+      // ====================================================================== MMA issuer (all lanes wait, lane 0 issues)
+      constexpr uint32_t F16_BITS = (1u << 7) | (1u << 10);
+      const uint32_t idesc_s = make_idesc_bf16(128, 128, 0, 0) & (TYPE == LBI_F16 ? ~F16_BITS : ~0u);
+      const uint32_t idesc_o = make_idesc_bf16(128, DH, 0, 1) & (TYPE == LBI_F16 ? ~F16_BITS : ~0u);
+      const uint64_t kmajor0 = make_smem_desc(0, 16, 1024), mnmajor0 = make_smem_desc(0, TC_PANEL, 1024);
+      const uint32_t q16 = smem_u32(s.q[0]) >> 4, kv16 = smem_u32(s.kv[0]) >> 4;
+      constexpr uint32_t SLOT16 = SLOT_BYTES >> 4, PANEL16 = TC_PANEL >> 4;
+      auto issue_s = [&](int g, int n) {   // n: index of K_j in the slot sequence
+        if (lane == 0) {
+          const uint64_t da = kmajor0 + q16 + g * SLOT16, db = kmajor0 + kv16 + (n % SLOTS) * SLOT16;
 #pragma unroll
-        for (int kk = 0; kk < DH / 16; ++kk) {
-          const uint32_t step = (kk >> 2) * PANEL16 + (kk & 3) * 2;
-          mma_bf16(tmem + g * 128, da + step, db + step, idesc_s, kk);
+          for (int kk = 0; kk < DH / 16; ++kk) {
+            const uint32_t step = (kk >> 2) * PANEL16 + (kk & 3) * 2;
+            mma_bf16(tmem + g * 128, da + step, db + step, idesc_s, kk);
+          }
+          mma_commit(&s.bar_s[g]);
         }
-        mma_commit(&s.bar_s[g]);
+      };
+      auto wait_full = [&](int n) { return mbar_wait(&s.bar_full[n % SLOTS], (n / SLOTS) & 1, abortp, p.status, 41); };
+      bool ok = n_j == 0 || (mbar_wait(&s.bar_q, 0, abortp, p.status, 42) && wait_full(0));
+      if (ok && n_j > 0) {
+        fence_after_sync();
+        for (int g = 0; g < 2; ++g)
+          if (n_kv[g] > 0) issue_s(g, 0);
+        if (lane == 0) mma_commit(&s.bar_empty[0]);
       }
-    };
-    auto wait_full = [&](int n) { return mbar_wait(&s.bar_full[n % SLOTS], (n / SLOTS) & 1, abortp, p.status, 41); };
-    bool ok = n_j == 0 || (mbar_wait(&s.bar_q, 0, abortp, p.status, 42) && wait_full(0));
-    if (ok && n_j > 0) {
-      fence_after_sync();
-      for (int g = 0; g < 2; ++g)
-        if (n_kv[g] > 0) issue_s(g, 0);
-      if (lane == 0) mma_commit(&s.bar_empty[0]);
-    }
-    for (int j = 0; j < n_j && ok; ++j) {
-      const int nv = 2 * j + 1, nk = 2 * j + 2;
-      ok = wait_full(nv);
-      if (!ok) break;
-      if (!E4M3) {   // rows of V that belong to no key
-        const uint32_t* there = s.meta[j % META].there;
-        if ((there[0] & there[1] & there[2] & there[3]) != 0xffffffffu) {
-          for (int row = lane; row < TC_TILE; row += 32)
-            if (!(there[row >> 5] >> (row & 31) & 1u)) {
-              const uint32_t at = smem_u32(s.kv[nv % SLOTS]) + row * 128;
+      for (int j = 0; j < n_j && ok; ++j) {
+        const int nv = 2 * j + 1, nk = 2 * j + 2;
+        ok = wait_full(nv);
+        if (!ok) break;
+        if (!E4M3) {   // rows of V that belong to no key (codes become finite values whatever they are)
+          const uint32_t* there = s.meta[j % META].there;
+          if ((there[0] & there[1] & there[2] & there[3]) != 0xffffffffu) {
+            for (int row = lane; row < TC_TILE; row += 32)
+              if (!(there[row >> 5] >> (row & 31) & 1u)) {
+                const uint32_t at = smem_u32(s.kv[nv % SLOTS]) + row * 128;
 #pragma unroll
-              for (int c = 0; c < PANELS * 8; ++c)
-                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at + (c >> 3) * TC_PANEL + (c & 7) * 16), "r"(0) : "memory");
+                for (int c = 0; c < PANELS * 8; ++c)
+                  asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at + (c >> 3) * TC_PANEL + (c & 7) * 16), "r"(0) : "memory");
+              }
+            fence_proxy_async();
+            __syncwarp();
+          }
+        }
+        const bool next_k = j + 1 < n_j;
+        if (next_k) ok = wait_full(nk);
+        for (int g = 0; g < 2 && ok; ++g) {
+          if (j >= n_kv[g]) continue;
+          ok = mbar_wait(&s.bar_p[g], j & 1, abortp, p.status, 43);
+          if (!ok) break;
+          fence_after_sync();
+          if (lane == 0) {
+            const uint64_t db = mnmajor0 + kv16 + (nv % SLOTS) * SLOT16;
+#pragma unroll
+            for (int kk = 0; kk < 8; ++kk) mma_ts(tmem + 256 + g * DH, tmem + g * 128 + kk * 8, db + 128 * kk, idesc_o, (j > 0 || kk > 0) ? 1u : 0u);
+            if (j + 1 == n_kv[g]) mma_commit(&s.bar_o[g]);
+          }
+          if (j + 1 < n_kv[g]) issue_s(g, nk);
+        }
+        if (ok && lane == 0) {
+          mma_commit(&s.bar_empty[nv % SLOTS]);
+          if (next_k) mma_commit(&s.bar_empty[nk % SLOTS]);
+        }
+      }
+    } else if (warp == 9 && !E4M3) {
+      // ====================================================================== TMA producer: one lane per page
+      const int per = TC_TILE >> a.page_shift;   // pages of a tile, 1 .. 16
+      const int* table = p.table + (int64_t)b * p.table_stride;
+      auto load_page = [&](int j) {
+        const int pos = k0 + j * TC_TILE + (lane << a.page_shift);
+        return j < n_j && lane < per && pos < k_end ? __ldg(table + (pos >> a.page_shift)) : -1;
+      };
+      int page = load_page(0);
+      bool ok = true;
+      for (int j = 0; j < n_j && ok; ++j) {
+        const int next = load_page(j + 1);
+        const int base = k0 + j * TC_TILE;
+        const bool wanted = lane < per && base + (lane << a.page_shift) < k_end;
+        const bool good = wanted && page >= 0 && page < p.num_pages;
+        if (wanted && !good && p.status) atomicCAS(p.status, 0, 84);
+        const uint32_t pages = __ballot_sync(0xffffffffu, good);
+        const uint32_t bytes = __popc(pages) * (uint32_t)p.page_size * DH * 2;
+        const int row = (max(page, 0) * p.kv_heads + kh) * p.page_size;
+#pragma unroll
+        for (int v = 0; v < 2 && ok; ++v) {
+          const int n = 2 * j + v, st = n % SLOTS;
+          if (n >= SLOTS) ok = mbar_wait(&s.bar_empty[st], ((n / SLOTS) - 1) & 1, abortp, p.status, 44);
+          if (!ok) break;
+          if (v == 0 && lane < 4) {
+            uint32_t there = 0;
+            if (pages == (per == 32 ? ~0u : (1u << per) - 1u) && base + TC_TILE <= k_end) {
+              there = 0xffffffffu;
+            } else {
+              for (int i = 0; i < 32; ++i) {
+                const int key = lane * 32 + i;
+                if ((pages >> (key >> a.page_shift) & 1u) && base + key < k_end) there |= 1u << i;
+              }
             }
-          fence_proxy_async();
+            s.meta[j % META].there[lane] = there;
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive_expect_tx(&s.bar_full[st], bytes);
+          __syncwarp();
+          if (good) {
+#pragma unroll
+            for (int c = 0; c < PANELS; ++c)
+              tma_load_2d(s.kv[st] + c * TC_PANEL + (lane << a.page_shift) * 128, v ? &map_v : &map_k, &s.bar_full[st], c * 64, row);
+          }
           __syncwarp();
         }
+        page = next;
       }
-      bool next_k = j + 1 < n_j;
-      if (next_k) ok = wait_full(nk);
-      for (int g = 0; g < 2 && ok; ++g) {
-        if (j >= n_kv[g]) continue;
-        ok = mbar_wait(&s.bar_p[g], j & 1, abortp, p.status, 43);
-        if (!ok) break;
-        fence_after_sync();
-        if (lane == 0) {
-          const uint64_t db = mnmajor0 + kv16 + (nv % SLOTS) * SLOT16;
-#pragma unroll
-          for (int kk = 0; kk < 8; ++kk) mma_ts(tmem + 256 + g * DH, tmem + g * 128 + kk * 8, db + 128 * kk, idesc_o, (j > 0 || kk > 0) ? 1u : 0u);
-          if (j + 1 == n_kv[g]) mma_commit(&s.bar_o[g]);
-        }
-        if (j + 1 < n_kv[g]) issue_s(g, nk);
-      }
-      if (ok && lane == 0) {
-        mma_commit(&s.bar_empty[nv % SLOTS]);
-        if (next_k) mma_commit(&s.bar_empty[nk % SLOTS]);
-      }
-    }
-  } else if (warp == 9 && !E4M3) {
-    // ======================================================================== TMA producer: one lane per page
-    const int per = TC_TILE >> a.page_shift;   // pages of a tile, 1 .. 16
-    const int* table = p.table + (int64_t)b * p.table_stride;
-    auto load_page = [&](int j) {
-      const int pos = k0 + j * TC_TILE + (lane << a.page_shift);
-      return j < n_j && lane < per && pos < k_end ? __ldg(table + (pos >> a.page_shift)) : -1;
-    };
-    int page = load_page(0);
-    bool ok = true;
-    for (int j = 0; j < n_j && ok; ++j) {
-      const int next = load_page(j + 1);
-      const int base = k0 + j * TC_TILE;
-      const bool wanted = lane < per && base + (lane << a.page_shift) < k_end;
-      const bool good = wanted && page >= 0 && page < p.num_pages;
-      if (wanted && !good && p.status) atomicCAS(p.status, 0, 84);
-      const uint32_t pages = __ballot_sync(0xffffffffu, good);
-      const uint32_t bytes = __popc(pages) * (uint32_t)p.page_size * DH * 2;
-      const int row = (max(page, 0) * p.kv_heads + kh) * p.page_size;
-#pragma unroll
-      for (int v = 0; v < 2 && ok; ++v) {
-        const int n = 2 * j + v, st = n % SLOTS;
-        if (n >= SLOTS) ok = mbar_wait(&s.bar_empty[st], ((n / SLOTS) - 1) & 1, abortp, p.status, 44);
-        if (!ok) break;
-        if (v == 0 && lane < 4) {
-          uint32_t there = 0;
-          for (int i = 0; i < 32; ++i) {
-            const int key = lane * 32 + i;
-            if ((pages >> (key >> a.page_shift) & 1u) && base + key < k_end) there |= 1u << i;
-          }
-          s.meta[j % META].there[lane] = there;
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive_expect_tx(&s.bar_full[st], bytes);
-        __syncwarp();
-        if (good) {
-#pragma unroll
-          for (int c = 0; c < PANELS; ++c)
-            tma_load_2d(s.kv[st] + c * TC_PANEL + (lane << a.page_shift) * 128, v ? &map_v : &map_k, &s.bar_full[st], c * 64, row);
-        }
-        __syncwarp();
-      }
-      page = next;
     }
   } else if (warp < 8) {
     // ======================================================================== softmax warpgroups
+    claim_registers<E4M3 ? 176 : 224>();
     const int g = warp >> 2, quarter = warp & 3;
     const int row = quarter * 32 + lane;             // of the tile
     // queries: 16-byte chunks of the warp's 32 rows, neighbouring lanes on neighbouring chunks, into the swizzled tile
@@ -277,84 +294,91 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     const int limit = live ? first_pos + (local + g * TC_TILE + row) / a.group : -1;
     const uint32_t t_s = tmem + ((uint32_t)(quarter * 32) << 16) + g * 128;
     const uint32_t t_o = tmem + ((uint32_t)(quarter * 32) << 16) + 256 + g * DH;
-    float m = -INFINITY, l = 0.f;
+    float m = -INFINITY;
+    float2 l2 = make_float2(0.f, 0.f);
     bool ok = true;
     for (int j = 0; j < mine; ++j) {
       ok = mbar_wait(&s.bar_s[g], j & 1, abortp, p.status, 45);
       if (!ok) break;
       fence_after_sync();
       const KeyMeta& meta = s.meta[j % META];
-      const int rel = limit - (k0 + j * TC_TILE);    // the row's last key, counted from the tile's first
-      uint32_t seen[4];
+      union {   // the row of S
+        uint32_t w[TC_TILE];
+        float f[TC_TILE];
+        float2 f2[TC_TILE / 2];
+      } x;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const int e = rel - 32 * c;
-        seen[c] = meta.there[c] & (e >= 31 ? 0xffffffffu : e < 0 ? 0u : (2u << e) - 1u);
-      }
-      const bool masked = __any_sync(0xffffffffu, (seen[0] & seen[1] & seen[2] & seen[3]) != 0xffffffffu);
-      float top = -INFINITY;
+      for (int c = 0; c < 4; ++c) tmem_ld_32x32(t_s + c * 32, x.w + c * 32);
+      tmem_ld_wait();
+      if (E4M3) {
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t x[32];
-        tmem_ld_32x32(t_s + c * 32, x);
-        tmem_ld_wait();
-#pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          float u = __uint_as_float(x[e]);
-          if (E4M3) u = fmaf(u, meta.ks[c * 32 + e], meta.lv[c * 32 + e]);
-          if (masked && !(seen[c] >> e & 1u)) u = -INFINITY;
-          top = fmaxf(top, u);
+        for (int e = 0; e < TC_TILE / 2; ++e) {
+          const float4 f = *reinterpret_cast<const float4*>(meta.ks_lv[e]);
+          x.f2[e] = fma2(x.f2[e], make_float2(f.x, f.y), make_float2(f.z, f.w));
         }
       }
-      if (!E4M3) top *= a.scale_log2;   // scale > 0: see the entry point
+      const int rel = limit - (k0 + j * TC_TILE);    // the row's last key, counted from the tile's first
+      uint32_t hidden = 0;
+      {
+        const uint4 there = *reinterpret_cast<const uint4*>(meta.there);
+        hidden = (there.x & there.y & there.z & there.w) != 0xffffffffu || rel < TC_TILE - 1;
+      }
+      if (__any_sync(0xffffffffu, hidden)) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const int e0 = rel - 32 * c;
+          const uint32_t seen = meta.there[c] & (e0 >= 31 ? 0xffffffffu : e0 < 0 ? 0u : (2u << e0) - 1u);
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (!(seen >> e & 1u)) x.f[c * 32 + e] = -INFINITY;
+        }
+      }
+      float t4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int e = 0; e < TC_TILE; e += 8)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) t4[i] = fmaxf(t4[i], fmaxf(x.f[e + i], x.f[e + 4 + i]));
+      float top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
+      if (!E4M3) top *= a.scale_log2;   // the scale is positive here, see the choice of the kernel
       // the reference point follows only a growth by more than 2^8
       const bool grow = top > m + 8.f;
       if (__any_sync(0xffffffffu, grow)) {
         const float m_new = grow ? top : m;
         const float keep = m == m_new ? 1.f : ex2(m - m_new);
         m = m_new;
-        l *= keep;
+        l2.x *= keep;
+        l2.y *= keep;
         if (j > 0) {
 #pragma unroll
           for (int c = 0; c < DH / 16; ++c) {
-            uint32_t x[16];
-            tmem_ld_32x16(t_o + c * 16, x);
+            uint32_t o[16];
+            tmem_ld_32x16(t_o + c * 16, o);
             tmem_ld_wait();
 #pragma unroll
-            for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * keep);
-            tmem_st_32x16(t_o + c * 16, x);
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+            tmem_st_32x16(t_o + c * 16, o);
           }
         }
       }
       const float ref = m == -INFINITY ? 0.f : m;
+      const float2 neg = make_float2(-ref, -ref), sc = make_float2(a.scale_log2, a.scale_log2);
+      float2 sum[2] = {l2, make_float2(0.f, 0.f)};
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        uint32_t x[32], w[16];
-        tmem_ld_32x32(t_s + c * 32, x);
-        tmem_ld_wait();
-        float sum0 = 0.f, sum1 = 0.f;
+        uint32_t w[16];
 #pragma unroll
-        for (int e = 0; e < 32; e += 2) {
-          float u[2];
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            u[i] = __uint_as_float(x[e + i]);
-            if (E4M3) u[i] = ex2(fmaf(u[i], meta.ks[c * 32 + e + i], meta.lv[c * 32 + e + i]) - ref);
-            else u[i] = ex2(fmaf(u[i], a.scale_log2, -ref));
-            if (masked && !(seen[c] >> (e + i) & 1u)) u[i] = 0.f;
-          }
-          if (E4M3) {
-            sum0 = fmaf(u[0], meta.iv[c * 32 + e], sum0);
-            sum1 = fmaf(u[1], meta.iv[c * 32 + e + 1], sum1);
-          } else {
-            sum0 += u[0];
-            sum1 += u[1];
-          }
-          w[e >> 1] = pack16<TYPE>(u[0], u[1]);
+        for (int e = 0; e < 16; ++e) {
+          float2 u = x.f2[c * 16 + e];
+          u = E4M3 ? add2(u, neg) : fma2(u, sc, neg);
+          u.x = ex2(u.x);
+          u.y = ex2(u.y);
+          w[e] = pack16<TYPE>(u.x, u.y);
+          if (E4M3) sum[e & 1] = fma2(u, *reinterpret_cast<const float2*>(meta.iv + c * 32 + 2 * e), sum[e & 1]);
+          else sum[e & 1] = add2(sum[e & 1], u);
         }
-        l += sum0 + sum1;
         tmem_st_32x16(t_s + c * 16, w);   // over columns that have been read
       }
+      l2 = add2(sum[0], sum[1]);
       tmem_st_wait();
       fence_before_sync();
       __syncwarp();
@@ -363,6 +387,7 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     if (ok && mine > 0) ok = mbar_wait(&s.bar_o[g], 0, abortp, p.status, 46);
     if (ok) {
       fence_after_sync();
+      const float l = l2.x + l2.y;
       const float inv = l == 0.f ? 0.f : 1.f / l;
       const int at = local + g * TC_TILE + row;
       const int64_t o_row = (int64_t)(r.x + at / a.group) * a.heads + kh * a.group + at % a.group;
@@ -386,67 +411,79 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
       }
       if (live && a.part_o) a.part_lse[o_row * a.splits + split] = l == 0.f ? -INFINITY : m + log2f(l);
     }
-  } else if (E4M3 && warp >= 10) {
-    // ======================================================================== converting warpgroup (warps 10 .. 13)
-    const int tid = threadIdx.x - 320;               // 0 .. 127: also the key whose slot and scales this thread looks up
+  } else if (E4M3) {
+    // ======================================================================== converting warpgroup (warps 12 .. 15)
+    // A thread holds 16-byte chunks of codes of one tile (K_j or V_j); as it converts them it loads the chunks of the next one in
+    // their place, so that the loads have the conversion and the wait for the next slot to arrive.
+    release_registers<104>();
+    const int tid = threadIdx.x - 384;               // 0 .. 127: also the key whose slot and scales this thread looks up
     const int* table = p.table + (int64_t)b * p.table_stride;
     constexpr int CH = DH / 16;                      // 16-byte chunks of a row of codes
     auto load_page = [&](int j) {
       const int pos = k0 + j * TC_TILE + tid;
       return j < n_j && pos < k_end ? __ldg(table + (pos >> a.page_shift)) : -1;
     };
-    int page = load_page(0);
-    bool ok = true;
-    for (int j = 0; j < n_j; ++j) {   // after a failed wait too: all four warps meet at the barrier below
-      const int next = load_page(j + 1);
+    int slot = -1;
+    float k_scale = 0.f, v_scale = 0.f;
+    auto look_up = [&](int j, int page) {            // slot and scales of key tid of tile j
       const int pos = k0 + j * TC_TILE + tid;
-      int slot = -1;
-      if (pos < k_end) {
+      slot = -1;
+      if (j < n_j && pos < k_end) {
         if (page >= 0 && page < p.num_pages) slot = (page * p.kv_heads + kh) * p.page_size + (pos & (p.page_size - 1));
         else if (p.status) atomicCAS(p.status, 0, 84);
       }
-      page = next;
-      const float k_scale = slot >= 0 ? __ldg(p.k_scale + slot) : 0.f, v_scale = slot >= 0 ? __ldg(p.v_scale + slot) : 0.f;
+      k_scale = slot >= 0 ? __ldg(p.k_scale + slot) : 0.f;
+      v_scale = slot >= 0 ? __ldg(p.v_scale + slot) : 0.f;
       s.slot_of[j & 1][tid] = slot;
-      const uint32_t there = __ballot_sync(0xffffffffu, slot >= 0);
-      named_barrier_sync(1, 128);
-      uint4 raw[2][CH];
+    };
+    uint4 raw[CH];
+    auto load_chunk = [&](int i, const void* codes, int j) {
+      const int sl = s.slot_of[j & 1][(i * 128 + tid) / CH];
+      raw[i] = sl >= 0 ? __ldg(reinterpret_cast<const uint4*>((const uint8_t*)codes + (int64_t)sl * DH) + tid % CH) : make_uint4(0, 0, 0, 0);
+    };
+    bool ok = true;
+    auto convert_tile = [&](int n, const void* next_codes, int next_j) {
+      const int st = n % SLOTS;
 #pragma unroll
-      for (int v = 0; v < 2; ++v)
-#pragma unroll
-        for (int i = 0; i < CH; ++i) {
-          const int id = i * 128 + tid;
-          const int sl = s.slot_of[j & 1][id / CH];
-          raw[v][i] = sl >= 0 ? __ldg(reinterpret_cast<const uint4*>((const uint8_t*)(v ? p.v : p.k) + (int64_t)sl * DH) + id % CH) : make_uint4(0, 0, 0, 0);
-        }
-#pragma unroll
-      for (int v = 0; v < 2 && ok; ++v) {
-        const int n = 2 * j + v, st = n % SLOTS;
-        if (n >= SLOTS) ok = mbar_wait(&s.bar_empty[st], ((n / SLOTS) - 1) & 1, abortp, p.status, 47);
-        if (!ok) break;
-        if (v == 0) {   // behind the wait, see META
-          KeyMeta& meta = s.meta[j % META];
-          const float vs = positive_scale(v_scale);
-          meta.ks[tid] = k_scale * a.scale_log2;
-          meta.lv[tid] = lg2(vs);
-          meta.iv[tid] = __frcp_rn(vs);
-          if (lane == 0) meta.there[warp - 10] = there;
-        }
-#pragma unroll
-        for (int i = 0; i < CH; ++i) {
-          const int id = i * 128 + tid, row = id / CH, c = id % CH;
-          const uint32_t* w = reinterpret_cast<const uint32_t*>(&raw[v][i]);
-          uint32_t x[8];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) codes_to_16<TYPE>(w[e], x[2 * e], x[2 * e + 1]);
-          uint8_t* dst = s.kv[st] + (c >> 2) * TC_PANEL + row * 128;
-          *reinterpret_cast<uint4*>(dst + (((2 * (c & 3)) ^ (row & 7)) << 4)) = make_uint4(x[0], x[1], x[2], x[3]);
-          *reinterpret_cast<uint4*>(dst + (((2 * (c & 3) + 1) ^ (row & 7)) << 4)) = make_uint4(x[4], x[5], x[6], x[7]);
-        }
-        fence_proxy_async();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&s.bar_full[st]);
+      for (int i = 0; i < CH; ++i) {
+        const int row = (i * 128 + tid) / CH, c = tid % CH;
+        uint32_t x[8];
+        codes_to_16<TYPE>(raw[i].x, x[0], x[1]);
+        codes_to_16<TYPE>(raw[i].y, x[2], x[3]);
+        codes_to_16<TYPE>(raw[i].z, x[4], x[5]);
+        codes_to_16<TYPE>(raw[i].w, x[6], x[7]);
+        load_chunk(i, next_codes, next_j);
+        uint8_t* dst = s.kv[st] + (c >> 2) * TC_PANEL + row * 128;
+        *reinterpret_cast<uint4*>(dst + (((2 * (c & 3)) ^ (row & 7)) << 4)) = make_uint4(x[0], x[1], x[2], x[3]);
+        *reinterpret_cast<uint4*>(dst + (((2 * (c & 3) + 1) ^ (row & 7)) << 4)) = make_uint4(x[4], x[5], x[6], x[7]);
       }
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s.bar_full[st]);
+    };
+    look_up(0, load_page(0));
+    int page = load_page(1);
+    named_barrier_sync(1, 128);
+#pragma unroll
+    for (int i = 0; i < CH; ++i) load_chunk(i, p.k, 0);
+    for (int j = 0; j < n_j; ++j) {   // after a failed wait too: all four warps meet at the barrier below
+      const int nk = 2 * j, nv = 2 * j + 1;
+      if (ok && nk >= SLOTS) ok = mbar_wait(&s.bar_empty[nk % SLOTS], ((nk / SLOTS) - 1) & 1, abortp, p.status, 47);
+      const uint32_t there = __ballot_sync(0xffffffffu, slot >= 0);
+      if (ok) {
+        KeyMeta& meta = s.meta[j % META];   // behind the wait, see META
+        const float vs = positive_scale(v_scale);
+        meta.ks_lv[tid >> 1][tid & 1] = k_scale * a.scale_log2;
+        meta.ks_lv[tid >> 1][2 + (tid & 1)] = lg2(vs);
+        meta.iv[tid] = __frcp_rn(vs);
+        if (lane == 0) meta.there[warp - 12] = there;
+        convert_tile(nk, p.v, j);
+      }
+      look_up(j + 1, page);
+      page = load_page(j + 2);
+      named_barrier_sync(1, 128);       // the slots of tile j + 1 are known, and nobody needs those of tile j any more
+      if (ok && nv >= SLOTS) ok = mbar_wait(&s.bar_empty[nv % SLOTS], ((nv / SLOTS) - 1) & 1, abortp, p.status, 47);
+      if (ok) convert_tile(nv, p.k, j + 1);
     }
   }
 
@@ -502,9 +539,15 @@ static int launch_tiles(const AttnArgs& a, cudaStream_t st) {
   static lbi::PerDeviceOnce once;
   cudaError_t e = once.max_dynamic_smem(kernel, smem);
   if (e != cudaSuccess) return (int)e;
+  // the claims of the warpgroups add up to what a block gets at launch only if the kernel was compiled to this many registers
+  static const bool registers_add_up = [&] {
+    cudaFuncAttributes attr;
+    return cudaFuncGetAttributes(&attr, kernel) == cudaSuccess && attr.numRegs == (E4M3 ? 128 : 168);
+  }();
+  if (!registers_add_up) return (int)cudaErrorInvalidConfiguration;
   const int64_t blocks = tile_bound(a.b, a.group, 2 * TC_TILE) * a.b.kv_heads * a.splits;
   if (blocks >= (1ll << 31)) return (int)cudaErrorInvalidValue;
-  kernel<<<(unsigned)blocks, E4M3 ? 448 : 320, smem, st>>>(map[0], map[1], a);
+  kernel<<<(unsigned)blocks, E4M3 ? 512 : 384, smem, st>>>(map[0], map[1], a);
   return (int)cudaGetLastError();
 }
 
