@@ -15,8 +15,8 @@
 //
 // Keys and values: 16-bit pages come by TMA, one box of page_size rows per page and 64 columns (128-byte swizzle), the ids of a
 // tile's pages read one tile ahead, a lane per page.  Slots behind the context and pages that do not exist are masked out of S, and
-// their rows of V are cleared before the product (0 * NaN would reach every row).  e4m3 pages are read by a converting warpgroup, which
-// stores the codes as 16-bit values (exact) and prepares the scales: with u_j = scale s_j k_scale_j + log2 v_scale_j the weights
+// their rows of V are cleared before the product (0 * NaN would reach every row).  Codes of e4m3 pages come 64 keys at a time; a converting
+// warpgroup stores them as 16-bit values (exact) and prepares the scales: with u_j = scale s_j k_scale_j + log2 v_scale_j the weights
 // 2^(u_j - m) carry the value's scale, and the sum of exponentials takes 2^(u_j - m) / v_scale_j.
 // Every wait is bounded (tcgen05.cuh).
 #include <algorithm>
@@ -31,6 +31,7 @@ namespace paged {
 using namespace tc;
 
 constexpr int TC_TILE = 128;
+constexpr int TC_HALF = 64;                // keys of one copy of codes
 constexpr int TC_PANEL = TC_TILE * 128;    // 128 rows x 64 16-bit columns
 
 struct alignas(16) KeyMeta {
@@ -48,7 +49,10 @@ struct TcSmem {
   alignas(1024) uint8_t q[2][TC_TILE * DH * 2];
   alignas(1024) uint8_t kv[SLOTS][TC_TILE * DH * 2];
   KeyMeta meta[META];
-  int slot_of[2][TC_TILE];                 // e4m3: where the keys of a tile are
+  static constexpr int RAW = E4M3 ? (DH == 128 ? 3 : 6) : 1;   // codes of 64 keys each, on their way to the converting warps
+  alignas(128) uint8_t raw[RAW][E4M3 ? TC_HALF * DH : 16];
+  uint64_t bar_raw_full[RAW];
+  uint64_t bar_raw_empty[RAW];
   uint64_t bar_q;
   uint64_t bar_full[SLOTS];
   uint64_t bar_empty[SLOTS];
@@ -80,8 +84,8 @@ __device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t* r)
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // Registers of a warpgroup: claimed ones come from those that the block was launched with and others have released.  16-bit pages
-// (384 threads, 168 each at launch): 2 x 128 x 224 + 128 x 56 = 64512; e4m3 (512 threads, 128 each): 2 x 128 x 176 + 128 x 56 +
-// 128 x 104 = 65536.
+// (384 threads, 168 each at launch): 2 x 128 x 224 + 128 x 56 = 64512; e4m3 (512 threads, 128 each): 2 x 128 x 200 + 128 x 48 +
+// 128 x 64 = 65536.
 template <int N>
 __device__ __forceinline__ void claim_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N>
@@ -92,7 +96,7 @@ __global__ void __launch_bounds__(E4M3 ? 512 : 384, 1)
 attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const AttnArgs a) {
   using T = typename Elem<TYPE>::T;
   using Smem = TcSmem<E4M3, DH>;
-  constexpr int SLOTS = Smem::SLOTS, META = Smem::META, PANELS = DH / 64, SLOT_BYTES = TC_TILE * DH * 2;
+  constexpr int SLOTS = Smem::SLOTS, META = Smem::META, RAW = Smem::RAW, PANELS = DH / 64, SLOT_BYTES = TC_TILE * DH * 2;
   extern __shared__ uint8_t raw_smem[];
   Smem& s = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~uintptr_t(1023));
   const lbi_paged_batch& p = a.b;
@@ -135,16 +139,18 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
       mbar_init(&s.bar_full[i], E4M3 ? 4 : 1);
       mbar_init(&s.bar_empty[i], 1);
     }
+    for (int i = 0; i < RAW; ++i) {
+      mbar_init(&s.bar_raw_full[i], 1);
+      mbar_init(&s.bar_raw_empty[i], 4);
+    }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s.bar_s[i], 1);
       mbar_init(&s.bar_p[i], 4);
       mbar_init(&s.bar_o[i], 1);
     }
     fence_barrier_init();
-    if (!E4M3) {
-      prefetch_tmap(&map_k);
-      prefetch_tmap(&map_v);
-    }
+    prefetch_tmap(&map_k);
+    prefetch_tmap(&map_v);
   }
   if (warp == 8) tmem_alloc(&s.tmem_base, 512);
   fence_before_sync();
@@ -154,7 +160,7 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   volatile int* abortp = &s.abort_flag;
 
   if (warp >= 8 && warp < 12) {
-    release_registers<56>();
+    release_registers<E4M3 ? 48 : 56>();
     if (warp == 8) {
       // ====================================================================== MMA issuer (all lanes wait, lane 0 issues)
       constexpr uint32_t F16_BITS = (1u << 7) | (1u << 10);
@@ -220,7 +226,7 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
           if (next_k) mma_commit(&s.bar_empty[nk % SLOTS]);
         }
       }
-    } else if (warp == 9 && !E4M3) {
+    } else if (warp == 9) {
       // ====================================================================== TMA producer: one lane per page
       const int per = TC_TILE >> a.page_shift;   // pages of a tile, 1 .. 16
       const int* table = p.table + (int64_t)b * p.table_stride;
@@ -237,8 +243,27 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
         const bool good = wanted && page >= 0 && page < p.num_pages;
         if (wanted && !good && p.status) atomicCAS(p.status, 0, 84);
         const uint32_t pages = __ballot_sync(0xffffffffu, good);
-        const uint32_t bytes = __popc(pages) * (uint32_t)p.page_size * DH * 2;
         const int row = (max(page, 0) * p.kv_heads + kh) * p.page_size;
+        if (E4M3) {   // codes of 64 keys at a time, for the converting warps
+          const int rows = min(p.page_size, TC_HALF);
+          for (int h = 0; h < 4 && ok; ++h) {   // K_j, then V_j
+            const int n = 4 * j + h, st = n % RAW, half = h & 1;
+            if (n >= RAW) ok = mbar_wait(&s.bar_raw_empty[st], ((n / RAW) - 1) & 1, abortp, p.status, 44);
+            if (!ok) break;
+            const bool here = good && (p.page_size > TC_HALF || (lane << a.page_shift) / TC_HALF == half);
+            const uint32_t copies = __popc(__ballot_sync(0xffffffffu, here));
+            if (lane == 0) mbar_arrive_expect_tx(&s.bar_raw_full[st], copies * (uint32_t)rows * DH);
+            __syncwarp();
+            if (here) {
+              const int at = p.page_size > TC_HALF ? 0 : (lane << a.page_shift) % TC_HALF;
+              tma_load_2d(s.raw[st] + at * DH, h < 2 ? &map_k : &map_v, &s.bar_raw_full[st], 0, row + (p.page_size > TC_HALF ? half * TC_HALF : 0));
+            }
+            __syncwarp();
+          }
+          page = next;
+          continue;
+        }
+        const uint32_t bytes = __popc(pages) * (uint32_t)p.page_size * DH * 2;
 #pragma unroll
         for (int v = 0; v < 2 && ok; ++v) {
           const int n = 2 * j + v, st = n % SLOTS;
@@ -246,7 +271,7 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
           if (!ok) break;
           if (v == 0 && lane < 4) {
             uint32_t there = 0;
-            if (pages == (per == 32 ? ~0u : (1u << per) - 1u) && base + TC_TILE <= k_end) {
+            if (pages == (1u << per) - 1u && base + TC_TILE <= k_end) {
               there = 0xffffffffu;
             } else {
               for (int i = 0; i < 32; ++i) {
@@ -271,7 +296,7 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     }
   } else if (warp < 8) {
     // ======================================================================== softmax warpgroups
-    claim_registers<E4M3 ? 176 : 224>();
+    claim_registers<E4M3 ? 200 : 224>();
     const int g = warp >> 2, quarter = warp & 3;
     const int row = quarter * 32 + lane;             // of the tile
     // queries: 16-byte chunks of the warp's 32 rows, neighbouring lanes on neighbouring chunks, into the swizzled tile
@@ -362,27 +387,37 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
       }
       const float ref = m == -INFINITY ? 0.f : m;
       const float2 neg = make_float2(-ref, -ref), sc = make_float2(a.scale_log2, a.scale_log2);
-      float2 sum[2] = {l2, make_float2(0.f, 0.f)};
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         uint32_t w[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          float2 u = x.f2[c * 16 + e];
+          float2& u = x.f2[c * 16 + e];
           u = E4M3 ? add2(u, neg) : fma2(u, sc, neg);
           u.x = ex2(u.x);
           u.y = ex2(u.y);
           w[e] = pack16<TYPE>(u.x, u.y);
-          if (E4M3) sum[e & 1] = fma2(u, *reinterpret_cast<const float2*>(meta.iv + c * 32 + 2 * e), sum[e & 1]);
-          else sum[e & 1] = add2(sum[e & 1], u);
         }
         tmem_st_32x16(t_s + c * 16, w);   // over columns that have been read
       }
-      l2 = add2(sum[0], sum[1]);
       tmem_st_wait();
       fence_before_sync();
       __syncwarp();
       if (lane == 0) mbar_arrive(&s.bar_p[g]);
+      // the sum is needed by nobody yet: behind the arrival
+      float2 sum[4] = {l2, make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+      for (int e = 0; e < TC_TILE / 2; e += 2) {
+        if (E4M3) {
+          const float4 iv = *reinterpret_cast<const float4*>(meta.iv + 2 * e);
+          sum[e & 3] = fma2(x.f2[e], make_float2(iv.x, iv.y), sum[e & 3]);
+          sum[(e & 3) + 1] = fma2(x.f2[e + 1], make_float2(iv.z, iv.w), sum[(e & 3) + 1]);
+        } else {
+          sum[e & 3] = add2(sum[e & 3], x.f2[e]);
+          sum[(e & 3) + 1] = add2(sum[(e & 3) + 1], x.f2[e + 1]);
+        }
+      }
+      l2 = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
     }
     if (ok && mine > 0) ok = mbar_wait(&s.bar_o[g], 0, abortp, p.status, 46);
     if (ok) {
@@ -413,12 +448,10 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     }
   } else if (E4M3) {
     // ======================================================================== converting warpgroup (warps 12 .. 15)
-    // A thread holds 16-byte chunks of codes of one tile (K_j or V_j); as it converts them it loads the chunks of the next one in
-    // their place, so that the loads have the conversion and the wait for the next slot to arrive.
-    release_registers<104>();
-    const int tid = threadIdx.x - 384;               // 0 .. 127: also the key whose slot and scales this thread looks up
+    release_registers<64>();
+    const int tid = threadIdx.x - 384;               // 0 .. 127: also the key whose scales this thread looks up
     const int* table = p.table + (int64_t)b * p.table_stride;
-    constexpr int CH = DH / 16;                      // 16-byte chunks of a row of codes
+    constexpr int CHUNKS = TC_HALF * DH / 16 / 128;  // 16-byte chunks of codes per thread and copy
     auto load_page = [&](int j) {
       const int pos = k0 + j * TC_TILE + tid;
       return j < n_j && pos < k_end ? __ldg(table + (pos >> a.page_shift)) : -1;
@@ -428,62 +461,55 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     auto look_up = [&](int j, int page) {            // slot and scales of key tid of tile j
       const int pos = k0 + j * TC_TILE + tid;
       slot = -1;
-      if (j < n_j && pos < k_end) {
-        if (page >= 0 && page < p.num_pages) slot = (page * p.kv_heads + kh) * p.page_size + (pos & (p.page_size - 1));
-        else if (p.status) atomicCAS(p.status, 0, 84);
-      }
+      if (j < n_j && pos < k_end && page >= 0 && page < p.num_pages) slot = (page * p.kv_heads + kh) * p.page_size + (pos & (p.page_size - 1));
       k_scale = slot >= 0 ? __ldg(p.k_scale + slot) : 0.f;
       v_scale = slot >= 0 ? __ldg(p.v_scale + slot) : 0.f;
-      s.slot_of[j & 1][tid] = slot;
-    };
-    uint4 raw[CH];
-    auto load_chunk = [&](int i, const void* codes, int j) {
-      const int sl = s.slot_of[j & 1][(i * 128 + tid) / CH];
-      raw[i] = sl >= 0 ? __ldg(reinterpret_cast<const uint4*>((const uint8_t*)codes + (int64_t)sl * DH) + tid % CH) : make_uint4(0, 0, 0, 0);
-    };
-    bool ok = true;
-    auto convert_tile = [&](int n, const void* next_codes, int next_j) {
-      const int st = n % SLOTS;
-#pragma unroll
-      for (int i = 0; i < CH; ++i) {
-        const int row = (i * 128 + tid) / CH, c = tid % CH;
-        uint32_t x[8];
-        codes_to_16<TYPE>(raw[i].x, x[0], x[1]);
-        codes_to_16<TYPE>(raw[i].y, x[2], x[3]);
-        codes_to_16<TYPE>(raw[i].z, x[4], x[5]);
-        codes_to_16<TYPE>(raw[i].w, x[6], x[7]);
-        load_chunk(i, next_codes, next_j);
-        uint8_t* dst = s.kv[st] + (c >> 2) * TC_PANEL + row * 128;
-        *reinterpret_cast<uint4*>(dst + (((2 * (c & 3)) ^ (row & 7)) << 4)) = make_uint4(x[0], x[1], x[2], x[3]);
-        *reinterpret_cast<uint4*>(dst + (((2 * (c & 3) + 1) ^ (row & 7)) << 4)) = make_uint4(x[4], x[5], x[6], x[7]);
-      }
-      fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&s.bar_full[st]);
     };
     look_up(0, load_page(0));
     int page = load_page(1);
-    named_barrier_sync(1, 128);
-#pragma unroll
-    for (int i = 0; i < CH; ++i) load_chunk(i, p.k, 0);
-    for (int j = 0; j < n_j; ++j) {   // after a failed wait too: all four warps meet at the barrier below
-      const int nk = 2 * j, nv = 2 * j + 1;
-      if (ok && nk >= SLOTS) ok = mbar_wait(&s.bar_empty[nk % SLOTS], ((nk / SLOTS) - 1) & 1, abortp, p.status, 47);
-      const uint32_t there = __ballot_sync(0xffffffffu, slot >= 0);
-      if (ok) {
-        KeyMeta& meta = s.meta[j % META];   // behind the wait, see META
+    bool ok = true;
+    for (int n = 0; n < 2 * n_j && ok; ++n) {        // K_0, V_0, K_1, ...
+      const int st = n % SLOTS, j = n >> 1;
+      if (n >= SLOTS) ok = mbar_wait(&s.bar_empty[st], ((n / SLOTS) - 1) & 1, abortp, p.status, 47);
+      if (!ok) break;
+      if ((n & 1) == 0) {
+        KeyMeta& meta = s.meta[j % META];            // behind the wait, see META
         const float vs = positive_scale(v_scale);
+        const uint32_t there = __ballot_sync(0xffffffffu, slot >= 0);
         meta.ks_lv[tid >> 1][tid & 1] = k_scale * a.scale_log2;
         meta.ks_lv[tid >> 1][2 + (tid & 1)] = lg2(vs);
         meta.iv[tid] = __frcp_rn(vs);
         if (lane == 0) meta.there[warp - 12] = there;
-        convert_tile(nk, p.v, j);
+        look_up(j + 1, page);
+        page = load_page(j + 2);
       }
-      look_up(j + 1, page);
-      page = load_page(j + 2);
-      named_barrier_sync(1, 128);       // the slots of tile j + 1 are known, and nobody needs those of tile j any more
-      if (ok && nv >= SLOTS) ok = mbar_wait(&s.bar_empty[nv % SLOTS], ((nv / SLOTS) - 1) & 1, abortp, p.status, 47);
-      if (ok) convert_tile(nv, p.k, j + 1);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int nr = 2 * n + half, sr = nr % RAW;
+        ok = mbar_wait(&s.bar_raw_full[sr], (nr / RAW) & 1, abortp, p.status, 48);
+        if (!ok) break;
+        uint4 raw[CHUNKS];
+#pragma unroll
+        for (int i = 0; i < CHUNKS; ++i) raw[i] = *reinterpret_cast<const uint4*>(s.raw[sr] + (i * 128 + tid) * 16);
+#pragma unroll
+        for (int i = 0; i < CHUNKS; ++i) {
+          const int id = i * 128 + tid, row = half * TC_HALF + id / (DH / 16), c = id % (DH / 16);
+          uint32_t x[8];
+          codes_to_16<TYPE>(raw[i].x, x[0], x[1]);
+          codes_to_16<TYPE>(raw[i].y, x[2], x[3]);
+          codes_to_16<TYPE>(raw[i].z, x[4], x[5]);
+          codes_to_16<TYPE>(raw[i].w, x[6], x[7]);
+          uint8_t* dst = s.kv[st] + (c >> 2) * TC_PANEL + row * 128;
+          *reinterpret_cast<uint4*>(dst + (((2 * (c & 3)) ^ (row & 7)) << 4)) = make_uint4(x[0], x[1], x[2], x[3]);
+          *reinterpret_cast<uint4*>(dst + (((2 * (c & 3) + 1) ^ (row & 7)) << 4)) = make_uint4(x[4], x[5], x[6], x[7]);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s.bar_raw_empty[sr]);
+      }
+      if (!ok) break;
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s.bar_full[st]);
     }
   }
 
@@ -520,19 +546,18 @@ static EncodeTiledFn encode_fn() {
 
 template <int TYPE, bool E4M3, int DH>
 static int launch_tiles(const AttnArgs& a, cudaStream_t st) {
-  CUtensorMap map[2] = {};
-  if (!E4M3) {
-    EncodeTiledFn fn = encode_fn();
-    if (!fn) return 801;
-    const cuuint64_t dims[2] = {DH, (cuuint64_t)a.b.num_pages * a.b.kv_heads * a.b.page_size};
-    const cuuint64_t strides[1] = {DH * 2};
-    const cuuint32_t box[2] = {64, (cuuint32_t)a.b.page_size}, estr[2] = {1, 1};
-    for (int v = 0; v < 2; ++v) {
-      const CUresult rc = fn(&map[v], TYPE == LBI_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, v ? a.b.v : a.b.k, dims,
-                             strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-      if (rc != CUDA_SUCCESS) return 1000 + (int)rc;
-    }
+  CUtensorMap map[2];
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return 801;
+  const cuuint64_t dims[2] = {DH, (cuuint64_t)a.b.num_pages * a.b.kv_heads * a.b.page_size};
+  const cuuint64_t strides[1] = {E4M3 ? DH : DH * 2};
+  const cuuint32_t box[2] = {E4M3 ? DH : 64, (cuuint32_t)(E4M3 ? std::min(a.b.page_size, TC_HALF) : a.b.page_size)}, estr[2] = {1, 1};
+  for (int v = 0; v < 2; ++v) {
+    const CUresult rc = fn(&map[v], E4M3 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : TYPE == LBI_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
+                           v ? a.b.v : a.b.k, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           E4M3 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (rc != CUDA_SUCCESS) return 1000 + (int)rc;
   }
   auto kernel = attn_tiles_kernel<TYPE, E4M3, DH>;
   const int smem = (int)sizeof(TcSmem<E4M3, DH>) + 1024;
