@@ -82,6 +82,40 @@ __device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t* r)
       : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// 16 lanes x 128 columns: thread t gets, for every 8 columns, columns 2 (t % 4) and + 1 of rows t / 4 and t / 4 + 8.
+__device__ __forceinline__ void tmem_ld_16x128(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x16.b32 {"
+      "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, "
+      "%22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33, %34, %35, %36, %37, %38, %39, %40, %41, "
+      "%42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, "
+      "%62, %63"
+      "}, [%64];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
+        "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]),
+        "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]),
+        "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]),
+        "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]), "=r"(r[41]), "=r"(r[42]),
+        "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]), "=r"(r[49]),
+        "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]), "=r"(r[56]),
+        "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+      : "r"(taddr)
+      : "memory");
+}
+// 16 lanes x 64 columns in the same spread: column t % 4 of every 4, rows t / 4 and t / 4 + 8.
+__device__ __forceinline__ void tmem_st_16x64(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.16x128b.x16.b32 [%32], {"
+      "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, "
+      "%22, %23, %24, %25, %26, %27, %28, %29, %30, %31"
+      "};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]),
+      "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
+      "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]),
+      "r"(taddr)
+      : "memory");
+}
 
 // Registers of a warpgroup: claimed ones come from those that the block was launched with and others have released.  16-bit pages
 // (384 threads, 168 each at launch): 2 x 128 x 224 + 128 x 56 = 64512; e4m3 (512 threads, 128 each): 2 x 128 x 200 + 128 x 48 +
@@ -319,10 +353,140 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     const int limit = live ? first_pos + (local + g * TC_TILE + row) / a.group : -1;
     const uint32_t t_s = tmem + ((uint32_t)(quarter * 32) << 16) + g * 128;
     const uint32_t t_o = tmem + ((uint32_t)(quarter * 32) << 16) + 256 + g * DH;
-    float m = -INFINITY;
-    float2 l2 = make_float2(0.f, 0.f);
+    float m = -INFINITY, l = 0.f;                    // of the thread's row, in base-2 logarithms and relative to m
     bool ok = true;
-    for (int j = 0; j < mine; ++j) {
+    if (E4M3) {
+      // Every column has its own scales.  A thread per row would read all 3 x 128 of them from shared memory, 393 KB per pair of
+      // tiles, which takes longer than the exponentials; in the spread of the 16-lane loads a thread has a quarter of the columns
+      // for four rows (t / 4 + 8 k of the warp's 32) and reads a quarter of that.  A row is shared by the four threads of a quad.
+      const int t = lane & 3;
+      int lim[4];
+      float mr[4], lr[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int rr = g * TC_TILE + quarter * 32 + (lane >> 2) + 8 * k;
+        lim[k] = rr < n_rows ? first_pos + (local + rr) / a.group : -1;
+        mr[k] = -INFINITY;
+        lr[k] = 0.f;
+      }
+      for (int j = 0; j < mine; ++j) {
+        ok = mbar_wait(&s.bar_s[g], j & 1, abortp, p.status, 45);
+        if (!ok) break;
+        fence_after_sync();
+        const KeyMeta& meta = s.meta[j % META];
+        union {   // [16 rows][8 columns][row + 8][column]
+          uint32_t w[2][16 * 4];
+          float2 f2[2][16][2];
+        } x;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) tmem_ld_16x128(t_s + ((uint32_t)(16 * h) << 16), x.w[h]);
+        tmem_ld_wait();
+#pragma unroll
+        for (int n = 0; n < 16; ++n) {
+          const float4 f = *reinterpret_cast<const float4*>(meta.ks_lv[4 * n + t]);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) x.f2[k >> 1][n][k & 1] = fma2(x.f2[k >> 1][n][k & 1], make_float2(f.x, f.y), make_float2(f.z, f.w));
+        }
+        const int base = k0 + j * TC_TILE;
+        const uint4 there = *reinterpret_cast<const uint4*>(meta.there);
+        if (__any_sync(0xffffffffu, (there.x & there.y & there.z & there.w) != 0xffffffffu || min(min(lim[0], lim[1]), min(lim[2], lim[3])) - base < TC_TILE - 1)) {
+#pragma unroll
+          for (int n = 0; n < 16; ++n) {
+            const uint32_t bits = meta.there[n >> 2] >> ((n & 3) * 8 + 2 * t);
+            const int key = base + 8 * n + 2 * t;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              float2& u = x.f2[k >> 1][n][k & 1];
+              if (!(bits & 1u) || key > lim[k]) u.x = -INFINITY;
+              if (!(bits & 2u) || key + 1 > lim[k]) u.y = -INFINITY;
+            }
+          }
+        }
+        float top[4];
+        bool grow = false;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          float t0 = -INFINITY, t1 = -INFINITY;
+#pragma unroll
+          for (int n = 0; n < 16; n += 2) {
+            const float2 u = x.f2[k >> 1][n][k & 1], w = x.f2[k >> 1][n + 1][k & 1];
+            t0 = fmaxf(t0, fmaxf(u.x, u.y));
+            t1 = fmaxf(t1, fmaxf(w.x, w.y));
+          }
+          top[k] = fmaxf(t0, t1);
+          top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], 1));
+          top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], 2));
+          grow = grow || top[k] > mr[k] + 8.f;
+        }
+        if (__any_sync(0xffffffffu, grow)) {
+          float row_keep = 1.f;   // of row `lane`, for O
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float m_new = top[k] > mr[k] + 8.f ? top[k] : mr[k];
+            const float keep = mr[k] == m_new ? 1.f : ex2(mr[k] - m_new);
+            mr[k] = m_new;
+            lr[k] *= keep;
+            const float k_row = __shfl_sync(0xffffffffu, keep, (lane & 7) * 4);
+            if (lane >> 3 == k) row_keep = k_row;
+          }
+          if (j > 0) {
+#pragma unroll
+            for (int c = 0; c < DH / 16; ++c) {
+              uint32_t o[16];
+              tmem_ld_32x16(t_o + c * 16, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * row_keep);
+              tmem_st_32x16(t_o + c * 16, o);
+            }
+          }
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t w[32];
+#pragma unroll
+          for (int n = 0; n < 16; ++n)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const float ref = mr[2 * h + k] == -INFINITY ? 0.f : mr[2 * h + k];
+              float2& u = x.f2[h][n][k];
+              u = add2(u, make_float2(-ref, -ref));
+              u.x = ex2(u.x);
+              u.y = ex2(u.y);
+              w[2 * n + k] = pack16<TYPE>(u.x, u.y);
+            }
+          tmem_st_16x64(t_s + ((uint32_t)(16 * h) << 16), w);
+        }
+        tmem_st_wait();
+        fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s.bar_p[g]);
+        // the sums are needed by nobody yet: behind the arrival
+        float2 sum[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sum[k] = make_float2(lr[k], 0.f);
+#pragma unroll
+        for (int n = 0; n < 16; ++n) {
+          const float2 iv = *reinterpret_cast<const float2*>(meta.iv + 8 * n + 2 * t);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) sum[k] = fma2(x.f2[k >> 1][n][k & 1], iv, sum[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) lr[k] = sum[k].x + sum[k].y;
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {   // to the thread of the row
+        lr[k] += __shfl_xor_sync(0xffffffffu, lr[k], 1);
+        lr[k] += __shfl_xor_sync(0xffffffffu, lr[k], 2);
+        const float l_row = __shfl_sync(0xffffffffu, lr[k], (lane & 7) * 4), m_row = __shfl_sync(0xffffffffu, mr[k], (lane & 7) * 4);
+        if (lane >> 3 == k) {
+          l = l_row;
+          m = m_row;
+        }
+      }
+    }
+    float2 l2 = make_float2(0.f, 0.f);
+    for (int j = 0; !E4M3 && j < mine; ++j) {
       ok = mbar_wait(&s.bar_s[g], j & 1, abortp, p.status, 45);
       if (!ok) break;
       fence_after_sync();
@@ -335,13 +499,6 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
 #pragma unroll
       for (int c = 0; c < 4; ++c) tmem_ld_32x32(t_s + c * 32, x.w + c * 32);
       tmem_ld_wait();
-      if (E4M3) {
-#pragma unroll
-        for (int e = 0; e < TC_TILE / 2; ++e) {
-          const float4 f = *reinterpret_cast<const float4*>(meta.ks_lv[e]);
-          x.f2[e] = fma2(x.f2[e], make_float2(f.x, f.y), make_float2(f.z, f.w));
-        }
-      }
       const int rel = limit - (k0 + j * TC_TILE);    // the row's last key, counted from the tile's first
       uint32_t hidden = 0;
       {
@@ -364,7 +521,7 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
 #pragma unroll
         for (int i = 0; i < 4; ++i) t4[i] = fmaxf(t4[i], fmaxf(x.f[e + i], x.f[e + 4 + i]));
       float top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
-      if (!E4M3) top *= a.scale_log2;   // the scale is positive here, see the choice of the kernel
+      top *= a.scale_log2;   // the scale is positive here, see the choice of the kernel
       // the reference point follows only a growth by more than 2^8
       const bool grow = top > m + 8.f;
       if (__any_sync(0xffffffffu, grow)) {
@@ -393,7 +550,7 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           float2& u = x.f2[c * 16 + e];
-          u = E4M3 ? add2(u, neg) : fma2(u, sc, neg);
+          u = fma2(u, sc, neg);
           u.x = ex2(u.x);
           u.y = ex2(u.y);
           w[e] = pack16<TYPE>(u.x, u.y);
@@ -408,21 +565,15 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
       float2 sum[4] = {l2, make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
       for (int e = 0; e < TC_TILE / 2; e += 2) {
-        if (E4M3) {
-          const float4 iv = *reinterpret_cast<const float4*>(meta.iv + 2 * e);
-          sum[e & 3] = fma2(x.f2[e], make_float2(iv.x, iv.y), sum[e & 3]);
-          sum[(e & 3) + 1] = fma2(x.f2[e + 1], make_float2(iv.z, iv.w), sum[(e & 3) + 1]);
-        } else {
-          sum[e & 3] = add2(sum[e & 3], x.f2[e]);
-          sum[(e & 3) + 1] = add2(sum[(e & 3) + 1], x.f2[e + 1]);
-        }
+        sum[e & 3] = add2(sum[e & 3], x.f2[e]);
+        sum[(e & 3) + 1] = add2(sum[(e & 3) + 1], x.f2[e + 1]);
       }
       l2 = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
     }
+    if (!E4M3) l = l2.x + l2.y;
     if (ok && mine > 0) ok = mbar_wait(&s.bar_o[g], 0, abortp, p.status, 46);
     if (ok) {
       fence_after_sync();
-      const float l = l2.x + l2.y;
       const float inv = l == 0.f ? 0.f : 1.f / l;
       const int at = local + g * TC_TILE + row;
       const int64_t o_row = (int64_t)(r.x + at / a.group) * a.heads + kh * a.group + at % a.group;
