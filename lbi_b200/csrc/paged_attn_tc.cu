@@ -1,26 +1,30 @@
 // Causal attention of a chunk of new tokens over a paged cache, on tcgen05 / TMEM / TMA: 16-bit queries, head_dim 64 or 128.
 //
 // A block owns 256 rows (token x head of a group, heads fastest, so that a key is loaded once for all heads of its group): two tiles
-// of 128 rows, each with a softmax warpgroup of its own (one thread per row), and walks the keys 128 at a time:
-//     S_g = Q_g K_j^T        M 128 x N 128, TMEM columns [128 g, 128 g + 128)
-//     P_g = 2^(S_g - m)      rounded to the queries' type and stored over S_g in TMEM (columns [128 g, 128 g + 64)): the second
-//                            product takes its left operand from there, so P never passes through shared memory
-//     O_g += P_g V_j         M 128 x N head_dim, accumulated in TMEM columns [256 + head_dim g, ..)
+// of 128 rows, each with a softmax warpgroup of its own, and walks the keys KEYS (64 or 128) at a time:
+//     S_g = Q_g K_j^T        M 128 x N KEYS, TMEM columns [KEYS g, ..)
+//     P_g = 2^(S_g - m)      rounded to the queries' type and stored over S_g in TMEM: the second product takes its left operand
+//                            from there, so P never passes through shared memory
+//     O_g += P_g V_j         M 128 x N head_dim, accumulated in TMEM columns [2 KEYS + head_dim g, ..)
 // Products of a thread run in the order in which they are issued, so S_g of the next tile may be issued right behind the product that
 // still reads P_g, and the barrier that announces S_g(j + 1) also says that O_g holds tile j.  The running maximum follows the row only
 // when it has grown by more than 2^8: P stays in (0, 2^8], and O is rescaled (a read and a write of TMEM) in the first tiles only.
 // While one warpgroup computes exponentials the tensor core works for the other.
 //
-// Bound by the exponentials (16 per clock and SM: 1024 cycles per 128 x 128 tile) and, at head_dim 128, equally by the products.
+// What bounds it: the chain S -> maximum -> exponentials -> P -> products of a row tile, of which two (head_dim 128) or four
+// (head_dim 64: two blocks per SM, 256 columns of TMEM each) run at a time.  The special-function unit would be the next bound (16
+// exponentials per clock and SM: 1024 cycles per 128 x 128 tile, as long as the products take at head_dim 128), so a part of the
+// exponentials is computed by a polynomial on the FMA units.
 //
-// Keys and values: 16-bit pages come by TMA, one box of page_size rows per page and 64 columns (128-byte swizzle), the ids of a
-// tile's pages read one tile ahead, a lane per page.  Slots behind the context and pages that do not exist are masked out of S, and
-// their rows of V are cleared before the product (0 * NaN would reach every row).  Codes of e4m3 pages come 64 keys at a time; a converting
-// warpgroup stores them as 16-bit values (exact) and prepares the scales: with u_j = scale s_j k_scale_j + log2 v_scale_j the weights
-// 2^(u_j - m) carry the value's scale, and the sum of exponentials takes 2^(u_j - m) / v_scale_j.
+// Keys and values: 16-bit pages come by TMA, one box per page and 64 columns (128-byte swizzle), the ids of a tile's pages read one
+// tile ahead, a lane per page.  Slots behind the context and pages that do not exist are masked out of S, and their rows of V are
+// cleared before the product (0 * NaN would reach every row).  Codes of e4m3 pages come 64 keys at a time; converting warps store
+// them as 16-bit values (exact) and prepare the scales: with u_j = scale s_j k_scale_j + log2 v_scale_j the weights 2^(u_j - m) carry
+// the value's scale, and the sum of exponentials takes 2^(u_j - m) / v_scale_j.
 // Every wait is bounded (tcgen05.cuh).
 #include <algorithm>
 #include <mutex>
+#include <type_traits>
 
 #include "paged.cuh"
 #include "tcgen05.cuh"
@@ -30,35 +34,57 @@ namespace paged {
 
 using namespace tc;
 
-constexpr int TC_TILE = 128;
-constexpr int TC_HALF = 64;                // keys of one copy of codes
-constexpr int TC_PANEL = TC_TILE * 128;    // 128 rows x 64 16-bit columns
+#ifndef POLY_PAIRS
+#define POLY_PAIRS 3
+#define POLY_PAIRS_E4M3 0
+#endif
+constexpr int ROWS = 128;                  // rows of a tile
+constexpr int COPY_KEYS = 64;              // keys of one copy of codes
 
+template <bool E4M3, int DH>
+struct TcConfig {
+  static constexpr int BLOCKS = DH == 64 ? 2 : 1;                 // per SM
+  static constexpr int KEYS = DH == 64 || E4M3 ? 64 : 128;        // of a tile
+  static constexpr int SLOTS = DH == 64 ? 6 : E4M3 ? 8 : 4;       // K_0, V_0, K_1, V_1, ...
+  // Masks and scales of a key tile: K_j is stored when S_(j - SLOTS / 2) is complete, which follows the softmax of the tile before
+  // that one, so SLOTS / 2 + 2 entries never meet one that is still read.
+  static constexpr int META = SLOTS / 2 + 2;
+  static constexpr int RAW = E4M3 ? (DH == 64 ? 4 : 3) : 1;       // copies of codes on their way to the converting warps
+  // warps 0-3, 4-7 softmax; 8 products; 9 copies; 16-bit pages: 10 clears V; e4m3: converting warps
+  static constexpr int CONVERT = E4M3 ? (DH == 64 ? 2 : 4) : 0, FIRST_CONVERT = DH == 64 ? 10 : 12;
+  static constexpr int THREADS = E4M3 && DH == 128 ? 512 : 384;
+  // Registers at launch and of the warpgroups afterwards (softmax, warps 8-11, warps 12-15): claimed ones come from those that the
+  // block was launched with and others have released, so the shares add up to at most threads x LAUNCH.
+  static constexpr int LAUNCH = DH == 64 ? 80 : E4M3 ? 128 : 168;
+  static constexpr int SOFTMAX = DH == 64 ? 96 : E4M3 ? 200 : 224, ISSUE = DH == 64 ? 48 : E4M3 ? 48 : 56, WIDE = 64;
+  static_assert(256 * SOFTMAX + 128 * ISSUE + (THREADS == 512 ? 128 * WIDE : 0) <= THREADS * LAUNCH, "register shares");
+  static constexpr int TMEM = DH == 64 ? 256 : 512;
+  static_assert(2 * KEYS + 2 * DH <= TMEM, "columns");
+};
+
+template <int KEYS>
 struct alignas(16) KeyMeta {
-  uint32_t there[4];                       // which of the tile's 128 keys exist
+  uint32_t there[4];                       // which of the tile's keys exist
   // e4m3, for two neighbouring keys: scale * log2(e) * k_scale of both, log2 v_scale of both; 1 / v_scale
-  float ks_lv[TC_TILE / 2][4], iv[TC_TILE];
+  float ks_lv[KEYS / 2][4], iv[KEYS];
 };
 
 template <bool E4M3, int DH>
 struct TcSmem {
-  static constexpr int SLOTS = DH == 128 ? 4 : 8;   // K_0, V_0, K_1, V_1, ...
-  // Masks and scales of a key tile: K_j is stored when S_(j - SLOTS / 2) is complete, which follows the softmax of the tile before
-  // that one, so SLOTS / 2 + 2 entries never meet one that is still read.
-  static constexpr int META = SLOTS / 2 + 2;
-  alignas(1024) uint8_t q[2][TC_TILE * DH * 2];
-  alignas(1024) uint8_t kv[SLOTS][TC_TILE * DH * 2];
-  KeyMeta meta[META];
-  static constexpr int RAW = E4M3 ? (DH == 128 ? 3 : 6) : 1;   // codes of 64 keys each, on their way to the converting warps
-  alignas(128) uint8_t raw[RAW][E4M3 ? TC_HALF * DH : 16];
-  uint64_t bar_raw_full[RAW];
-  uint64_t bar_raw_empty[RAW];
+  using C = TcConfig<E4M3, DH>;
+  alignas(1024) uint8_t q[2][ROWS * DH * 2];
+  alignas(1024) uint8_t kv[C::SLOTS][C::KEYS * DH * 2];
+  alignas(128) uint8_t raw[C::RAW][E4M3 ? COPY_KEYS * DH : 16];
+  KeyMeta<E4M3 ? C::KEYS : 4> meta[C::META];
+  uint64_t bar_raw_full[C::RAW];
+  uint64_t bar_raw_empty[C::RAW];
   uint64_t bar_q;
-  uint64_t bar_full[SLOTS];
-  uint64_t bar_empty[SLOTS];
-  uint64_t bar_s[2];
-  uint64_t bar_p[2];
-  uint64_t bar_o[2];
+  uint64_t bar_full[C::SLOTS];
+  uint64_t bar_empty[C::SLOTS];
+  uint64_t bar_clean[C::SLOTS];            // 16-bit pages: V without the rows that belong to no key
+  uint64_t bar_s[2];                       // S_g(j) is there (and O_g holds tile j - 1)
+  uint64_t bar_p[2];                       // P_g(j) is there, O_g is scaled for it
+  uint64_t bar_o[2];                       // O_g is complete
   uint32_t tmem_base;
   volatile int abort_flag;
 };
@@ -76,61 +102,72 @@ __device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_
 // 32 lanes x 16 consecutive 32-bit columns, from registers.
 __device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t* r) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]),
-      "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {"
+      "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15 "
+      "};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
       : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-// 16 lanes x 128 columns: thread t gets, for every 8 columns, columns 2 (t % 4) and + 1 of rows t / 4 and t / 4 + 8.
-__device__ __forceinline__ void tmem_ld_16x128(uint32_t taddr, uint32_t* r) {
+// 16 lanes x 64 columns: thread t gets, for every 8 columns, columns 2 (t % 4) and + 1 of rows t / 4 and t / 4 + 8.
+__device__ __forceinline__ void tmem_ld_16x64(uint32_t taddr, uint32_t* r) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.16x256b.x16.b32 {"
-      "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, "
-      "%22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33, %34, %35, %36, %37, %38, %39, %40, %41, "
-      "%42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, "
-      "%62, %63"
-      "}, [%64];"
+      "tcgen05.ld.sync.aligned.16x256b.x8.b32 {"
+      "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31 "
+      "}, [%32];"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
-        "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]),
-        "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]),
-        "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]),
-        "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]), "=r"(r[41]), "=r"(r[42]),
-        "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]), "=r"(r[49]),
-        "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]), "=r"(r[56]),
-        "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(taddr)
       : "memory");
 }
-// 16 lanes x 64 columns in the same spread: column t % 4 of every 4, rows t / 4 and t / 4 + 8.
-__device__ __forceinline__ void tmem_st_16x64(uint32_t taddr, const uint32_t* r) {
+// 16 lanes x 32 columns in the same spread: column t % 4 of every 4, rows t / 4 and t / 4 + 8.
+__device__ __forceinline__ void tmem_st_16x32(uint32_t taddr, const uint32_t* r) {
   asm volatile(
-      "tcgen05.st.sync.aligned.16x128b.x16.b32 [%32], {"
-      "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, "
-      "%22, %23, %24, %25, %26, %27, %28, %29, %30, %31"
-      "};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
-      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]),
-      "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
-      "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]),
-      "r"(taddr)
+      "tcgen05.st.sync.aligned.16x128b.x8.b32 [%16], {"
+      "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15 "
+      "};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
       : "memory");
 }
-
-// Registers of a warpgroup: claimed ones come from those that the block was launched with and others have released.  16-bit pages
-// (384 threads, 168 each at launch): 2 x 128 x 224 + 128 x 56 = 64512; e4m3 (512 threads, 128 each): 2 x 128 x 200 + 128 x 48 +
-// 128 x 64 = 65536.
 template <int N>
 __device__ __forceinline__ void claim_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N>
 __device__ __forceinline__ void release_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
+// 2^x for x in [-126, 128) on the FMA units, for the share of the exponentials that the special-function unit has no time for:
+// x = n + f with n the nearest whole number, 2^f by the minimax polynomial of degree 3 (bf16; relative error 7.5e-5, a fiftieth of the
+// half step to which P is rounded) or 4 (fp16; 2.6e-6) on [-1/2, 1/2], n added to the exponent.
+template <int TYPE>
+__device__ __forceinline__ float2 exp2_by_polynomial(float2 x) {
+  x = make_float2(fmaxf(x.x, -126.f), fmaxf(x.y, -126.f));
+  const float2 t = add2(x, make_float2(12582912.f, 12582912.f));   // 1.5 * 2^23: n in the low bits
+  const float2 n = add2(t, make_float2(-12582912.f, -12582912.f));
+  const float2 f = fma2(n, make_float2(-1.f, -1.f), x);
+  float2 r;
+  if (TYPE == LBI_F16) {
+    r = fma2(make_float2(0.009570102207362652f, 0.009570102207362652f), f, make_float2(0.05591785907745361f, 0.05591785907745361f));
+    r = fma2(r, f, make_float2(0.240247443318367f, 0.240247443318367f));
+    r = fma2(r, f, make_float2(0.6931217908859253f, 0.6931217908859253f));
+    r = fma2(r, f, make_float2(0.9999992847442627f, 0.9999992847442627f));
+  } else {
+    r = fma2(make_float2(0.0551716685295105f, 0.0551716685295105f), f, make_float2(0.2426111251115799f, 0.2426111251115799f));
+    r = fma2(r, f, make_float2(0.6932609677314758f, 0.6932609677314758f));
+    r = fma2(r, f, make_float2(0.9999280571937561f, 0.9999280571937561f));
+  }
+  return make_float2(__int_as_float(__float_as_int(r.x) + (__float_as_int(t.x) << 23)), __int_as_float(__float_as_int(r.y) + (__float_as_int(t.y) << 23)));
+}
+
 template <int TYPE, bool E4M3, int DH>
-__global__ void __launch_bounds__(E4M3 ? 512 : 384, 1)
+__global__ void __launch_bounds__(TcConfig<E4M3, DH>::THREADS, TcConfig<E4M3, DH>::BLOCKS)
 attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const AttnArgs a) {
   using T = typename Elem<TYPE>::T;
+  using C = TcConfig<E4M3, DH>;
   using Smem = TcSmem<E4M3, DH>;
-  constexpr int SLOTS = Smem::SLOTS, META = Smem::META, RAW = Smem::RAW, PANELS = DH / 64, SLOT_BYTES = TC_TILE * DH * 2;
+  constexpr int KEYS = C::KEYS, SLOTS = C::SLOTS, META = C::META, RAW = C::RAW, PANELS = DH / 64;
+  constexpr int Q_BYTES = ROWS * DH * 2, Q_PANEL = ROWS * 128, KV_BYTES = KEYS * DH * 2, KV_PANEL = KEYS * 128;   // panels of 64 columns
   extern __shared__ uint8_t raw_smem[];
   Smem& s = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~uintptr_t(1023));
   const lbi_paged_batch& p = a.b;
@@ -146,22 +183,22 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   const int64_t unit = unit_block / a.splits;
   const int kh = (int)(unit % p.kv_heads);
   const int64_t tile = unit / p.kv_heads;
-  const int b = seq_of_tile(p, tile, a.group, 2 * TC_TILE);
+  const int b = seq_of_tile(p, tile, a.group, 2 * ROWS);
   const int2 r = seq_rows(p, b);
-  const int64_t local64 = (tile - first_tile(p, b, a.group, 2 * TC_TILE)) * (2 * TC_TILE);
+  const int64_t local64 = (tile - first_tile(p, b, a.group, 2 * ROWS)) * (2 * ROWS);
   const int64_t rows_b = (int64_t)(r.y - r.x) * a.group;
   if (local64 < 0 || local64 >= rows_b) return;
-  const int local = (int)local64, n_rows = (int)min((int64_t)2 * TC_TILE, rows_b - local64);
+  const int local = (int)local64, n_rows = (int)min((int64_t)2 * ROWS, rows_b - local64);
   const int first_pos = __ldg(p.context + b) - (r.y - r.x);
   const int64_t capacity = (int64_t)p.table_width << a.page_shift;
   const int k0 = split * a.split_keys;
   int n_kv[2], k_end = 0;   // key tiles of each row tile; one behind the last key any row sees
 #pragma unroll
   for (int g = 0; g < 2; ++g) {
-    const int last = min(n_rows, (g + 1) * TC_TILE) - 1;   // the tile's last row
-    const int keys = last < g * TC_TILE ? 0 : (int)min((int64_t)first_pos + (local + last) / a.group + 1, capacity);
+    const int last = min(n_rows, (g + 1) * ROWS) - 1;   // the tile's last row
+    const int keys = last < g * ROWS ? 0 : (int)min((int64_t)first_pos + (local + last) / a.group + 1, capacity);
     const int k1 = split == a.splits - 1 ? keys : min(keys, k0 + a.split_keys);
-    n_kv[g] = k1 > k0 ? (k1 - k0 + TC_TILE - 1) / TC_TILE : 0;
+    n_kv[g] = k1 > k0 ? (k1 - k0 + KEYS - 1) / KEYS : 0;
     k_end = max(k_end, k1);
   }
   const int n_j = max(n_kv[0], n_kv[1]);
@@ -170,12 +207,13 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     s.abort_flag = 0;
     mbar_init(&s.bar_q, 8);
     for (int i = 0; i < SLOTS; ++i) {
-      mbar_init(&s.bar_full[i], E4M3 ? 4 : 1);
+      mbar_init(&s.bar_full[i], E4M3 ? C::CONVERT : 1);
       mbar_init(&s.bar_empty[i], 1);
+      mbar_init(&s.bar_clean[i], 1);
     }
     for (int i = 0; i < RAW; ++i) {
       mbar_init(&s.bar_raw_full[i], 1);
-      mbar_init(&s.bar_raw_empty[i], 4);
+      mbar_init(&s.bar_raw_empty[i], E4M3 ? C::CONVERT : 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s.bar_s[i], 1);
@@ -186,212 +224,310 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     prefetch_tmap(&map_k);
     prefetch_tmap(&map_v);
   }
-  if (warp == 8) tmem_alloc(&s.tmem_base, 512);
+  if (warp == 8) tmem_alloc(&s.tmem_base, C::TMEM);
   fence_before_sync();
   __syncthreads();
   fence_after_sync();
   const uint32_t tmem = s.tmem_base;
   volatile int* abortp = &s.abort_flag;
 
-  if (warp >= 8 && warp < 12) {
-    release_registers<E4M3 ? 48 : 56>();
-    if (warp == 8) {
-      // ====================================================================== MMA issuer (all lanes wait, lane 0 issues)
-      constexpr uint32_t F16_BITS = (1u << 7) | (1u << 10);
-      const uint32_t idesc_s = make_idesc_bf16(128, 128, 0, 0) & (TYPE == LBI_F16 ? ~F16_BITS : ~0u);
-      const uint32_t idesc_o = make_idesc_bf16(128, DH, 0, 1) & (TYPE == LBI_F16 ? ~F16_BITS : ~0u);
-      const uint64_t kmajor0 = make_smem_desc(0, 16, 1024), mnmajor0 = make_smem_desc(0, TC_PANEL, 1024);
-      const uint32_t q16 = smem_u32(s.q[0]) >> 4, kv16 = smem_u32(s.kv[0]) >> 4;
-      constexpr uint32_t SLOT16 = SLOT_BYTES >> 4, PANEL16 = TC_PANEL >> 4;
-      auto issue_s = [&](int g, int n) {   // n: index of K_j in the slot sequence
-        if (lane == 0) {
-          const uint64_t da = kmajor0 + q16 + g * SLOT16, db = kmajor0 + kv16 + (n % SLOTS) * SLOT16;
+  // ---------------------------------------------------------------------- converting warps (called by theirs)
+  auto convert = [&] {
+    if constexpr (E4M3) {
+      constexpr int THREADS = C::CONVERT * 32, EACH = KEYS / THREADS > 1 ? KEYS / THREADS : 1;
+      const int tid = threadIdx.x - C::FIRST_CONVERT * 32;   // the keys tid, tid + THREADS, .. whose scales this thread looks up
+      const int* table = p.table + (int64_t)b * p.table_stride;
+      constexpr int CHUNKS = COPY_KEYS * DH / 16 / THREADS;    // 16-byte chunks of codes per thread and copy
+      static_assert(KEYS == COPY_KEYS && CHUNKS % 2 == 0, "one copy per tile");
+      float k_scale[EACH], v_scale[EACH];
+      uint32_t there[EACH];
+      int page[EACH];
+      auto load_pages = [&](int j) {
 #pragma unroll
-          for (int kk = 0; kk < DH / 16; ++kk) {
-            const uint32_t step = (kk >> 2) * PANEL16 + (kk & 3) * 2;
-            mma_bf16(tmem + g * 128, da + step, db + step, idesc_s, kk);
-          }
-          mma_commit(&s.bar_s[g]);
+        for (int i = 0; i < EACH; ++i) {
+          const int key = tid + i * THREADS, pos = k0 + j * KEYS + key;
+          page[i] = j < n_j && key < KEYS && pos < k_end ? __ldg(table + (pos >> a.page_shift)) : -1;
         }
       };
-      auto wait_full = [&](int n) { return mbar_wait(&s.bar_full[n % SLOTS], (n / SLOTS) & 1, abortp, p.status, 41); };
-      bool ok = n_j == 0 || (mbar_wait(&s.bar_q, 0, abortp, p.status, 42) && wait_full(0));
-      if (ok && n_j > 0) {
-        fence_after_sync();
-        for (int g = 0; g < 2; ++g)
-          if (n_kv[g] > 0) issue_s(g, 0);
-        if (lane == 0) mma_commit(&s.bar_empty[0]);
-      }
-      for (int j = 0; j < n_j && ok; ++j) {
-        const int nv = 2 * j + 1, nk = 2 * j + 2;
-        ok = wait_full(nv);
+      auto look_up = [&](int j) {
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+          const int pos = k0 + j * KEYS + tid + i * THREADS;
+          const bool good = page[i] >= 0 && page[i] < p.num_pages;
+          const int slot = good ? (page[i] * p.kv_heads + kh) * p.page_size + (pos & (p.page_size - 1)) : 0;
+          k_scale[i] = good ? __ldg(p.k_scale + slot) : 0.f;
+          v_scale[i] = good ? __ldg(p.v_scale + slot) : 0.f;
+          there[i] = __ballot_sync(0xffffffffu, good);
+        }
+      };
+      load_pages(0);
+      look_up(0);
+      load_pages(1);
+      bool ok = true;
+      for (int n = 0; n < 2 * n_j && ok; ++n) {        // K_0, V_0, K_1, ...
+        const int st = n % SLOTS, sr = n % RAW, j = n >> 1;
+        if (n >= SLOTS) ok = mbar_wait(&s.bar_empty[st], ((n / SLOTS) - 1) & 1, abortp, p.status, 47);
         if (!ok) break;
-        if (!E4M3) {   // rows of V that belong to no key (codes become finite values whatever they are)
-          const uint32_t* there = s.meta[j % META].there;
-          if ((there[0] & there[1] & there[2] & there[3]) != 0xffffffffu) {
-            for (int row = lane; row < TC_TILE; row += 32)
-              if (!(there[row >> 5] >> (row & 31) & 1u)) {
-                const uint32_t at = smem_u32(s.kv[nv % SLOTS]) + row * 128;
+        if ((n & 1) == 0) {
+          auto& meta = s.meta[j % META];               // behind the wait, see META
 #pragma unroll
-                for (int c = 0; c < PANELS * 8; ++c)
-                  asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at + (c >> 3) * TC_PANEL + (c & 7) * 16), "r"(0) : "memory");
-              }
-            fence_proxy_async();
-            __syncwarp();
+          for (int i = 0; i < EACH; ++i) {
+            const int key = tid + i * THREADS;
+            if (key < KEYS) {
+              const float vs = positive_scale(v_scale[i]);
+              meta.ks_lv[key >> 1][key & 1] = k_scale[i] * a.scale_log2;
+              meta.ks_lv[key >> 1][2 + (key & 1)] = lg2(vs);
+              meta.iv[key] = __frcp_rn(vs);
+              if (lane == 0) meta.there[key >> 5] = there[i];
+            }
+          }
+          look_up(j + 1);
+          load_pages(j + 2);
+        }
+        ok = mbar_wait(&s.bar_raw_full[sr], (n / RAW) & 1, abortp, p.status, 48);
+        if (!ok) break;
+#pragma unroll
+        for (int i0 = 0; i0 < CHUNKS; i0 += 2) {
+          uint4 raw[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) raw[i] = *reinterpret_cast<const uint4*>(s.raw[sr] + ((i0 + i) * THREADS + tid) * 16);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int id = (i0 + i) * THREADS + tid, row = id / (DH / 16), c = id % (DH / 16);
+            uint32_t x[8];
+            codes_to_16<TYPE>(raw[i].x, x[0], x[1]);
+            codes_to_16<TYPE>(raw[i].y, x[2], x[3]);
+            codes_to_16<TYPE>(raw[i].z, x[4], x[5]);
+            codes_to_16<TYPE>(raw[i].w, x[6], x[7]);
+            uint8_t* dst = s.kv[st] + (c >> 2) * KV_PANEL + row * 128;
+            *reinterpret_cast<uint4*>(dst + (((2 * (c & 3)) ^ (row & 7)) << 4)) = make_uint4(x[0], x[1], x[2], x[3]);
+            *reinterpret_cast<uint4*>(dst + (((2 * (c & 3) + 1) ^ (row & 7)) << 4)) = make_uint4(x[4], x[5], x[6], x[7]);
           }
         }
-        const bool next_k = j + 1 < n_j;
-        if (next_k) ok = wait_full(nk);
-        for (int g = 0; g < 2 && ok; ++g) {
-          if (j >= n_kv[g]) continue;
-          ok = mbar_wait(&s.bar_p[g], j & 1, abortp, p.status, 43);
-          if (!ok) break;
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&s.bar_raw_empty[sr]);
+          mbar_arrive(&s.bar_full[st]);
+        }
+      }
+    }
+  };
+
+  if (warp >= 12) {
+    release_registers<C::WIDE>();
+    convert();
+  } else if (warp >= 8) {
+    release_registers<C::ISSUE>();
+    if (warp == 8) {
+      // ====================================================================== MMA issuer (one thread)
+      // The loop over g stays a loop, so that not all descriptors are kept in registers.
+      if (elect_one()) {
+        constexpr uint32_t F16_BITS = (1u << 7) | (1u << 10);
+        constexpr uint32_t idesc_s = make_idesc_bf16(ROWS, KEYS, 0, 0) & (TYPE == LBI_F16 ? ~F16_BITS : ~0u);
+        constexpr uint32_t idesc_o = make_idesc_bf16(ROWS, DH, 0, 1) & (TYPE == LBI_F16 ? ~F16_BITS : ~0u);
+        const uint64_t kmajor = make_smem_desc(0, 16, 1024), mnmajor = make_smem_desc(0, KV_PANEL, 1024);
+        const uint32_t q16 = smem_u32(s.q[0]) >> 4, kv16 = smem_u32(s.kv[0]) >> 4;
+        auto issue_s = [&](int g, int n) {   // n: index of K_j in the slot sequence
+          const uint64_t da = kmajor + (q16 + g * (Q_BYTES >> 4)), db = kmajor + (kv16 + (n % SLOTS) * (KV_BYTES >> 4));
+#pragma unroll
+          for (int kk = 0; kk < DH / 16; ++kk)
+            mma_bf16(tmem + g * KEYS, da + ((kk >> 2) * (Q_PANEL >> 4) + (kk & 3) * 2), db + ((kk >> 2) * (KV_PANEL >> 4) + (kk & 3) * 2), idesc_s, kk);
+          mma_commit(&s.bar_s[g]);
+        };
+        auto wait_full = [&](int n) { return mbar_wait(&s.bar_full[n % SLOTS], (n / SLOTS) & 1, abortp, p.status, 41); };
+        bool ok = n_j == 0 || (mbar_wait(&s.bar_q, 0, abortp, p.status, 42) && wait_full(0));
+        if (ok && n_j > 0) {
           fence_after_sync();
-          if (lane == 0) {
-            const uint64_t db = mnmajor0 + kv16 + (nv % SLOTS) * SLOT16;
-#pragma unroll
-            for (int kk = 0; kk < 8; ++kk) mma_ts(tmem + 256 + g * DH, tmem + g * 128 + kk * 8, db + 128 * kk, idesc_o, (j > 0 || kk > 0) ? 1u : 0u);
-            if (j + 1 == n_kv[g]) mma_commit(&s.bar_o[g]);
-          }
-          if (j + 1 < n_kv[g]) issue_s(g, nk);
+#pragma unroll 1
+          for (int g = 0; g < 2; ++g)
+            if (n_kv[g] > 0) issue_s(g, 0);
+          mma_commit(&s.bar_empty[0]);
         }
-        if (ok && lane == 0) {
-          mma_commit(&s.bar_empty[nv % SLOTS]);
-          if (next_k) mma_commit(&s.bar_empty[nk % SLOTS]);
+        for (int j = 0; j < n_j && ok; ++j) {
+          const int nv = 2 * j + 1, nk = 2 * j + 2;
+          const bool next_k = j + 1 < n_j;
+          ok = wait_full(nv) && (E4M3 || mbar_wait(&s.bar_clean[nv % SLOTS], (nv / SLOTS) & 1, abortp, p.status, 51)) && (!next_k || wait_full(nk));
+#pragma unroll 1
+          for (int g = 0; g < 2 && ok; ++g) {
+            if (j >= n_kv[g]) continue;
+            ok = mbar_wait(&s.bar_p[g], j & 1, abortp, p.status, 43);
+            if (!ok) break;
+            fence_after_sync();
+            const uint64_t db = mnmajor + (kv16 + (nv % SLOTS) * (KV_BYTES >> 4));
+#pragma unroll
+            for (int kk = 0; kk < KEYS / 16; ++kk)
+              mma_ts(tmem + 2 * KEYS + g * DH, tmem + g * KEYS + kk * 8, db + 128 * kk, idesc_o, (j > 0 || kk > 0) ? 1u : 0u);
+            if (j + 1 == n_kv[g]) mma_commit(&s.bar_o[g]);
+            else issue_s(g, nk);
+          }
+          if (ok) {
+            mma_commit(&s.bar_empty[nv % SLOTS]);
+            if (next_k) mma_commit(&s.bar_empty[nk % SLOTS]);
+          }
         }
       }
     } else if (warp == 9) {
       // ====================================================================== TMA producer: one lane per page
-      const int per = TC_TILE >> a.page_shift;   // pages of a tile, 1 .. 16
+      const int box = min(p.page_size, KEYS);    // rows of a copy: a page, or a tile's part of it
+      const int per = KEYS / box;                // copies of a tile, 1 .. 16
       const int* table = p.table + (int64_t)b * p.table_stride;
       auto load_page = [&](int j) {
-        const int pos = k0 + j * TC_TILE + (lane << a.page_shift);
+        const int pos = k0 + j * KEYS + lane * box;
         return j < n_j && lane < per && pos < k_end ? __ldg(table + (pos >> a.page_shift)) : -1;
       };
       int page = load_page(0);
       bool ok = true;
       for (int j = 0; j < n_j && ok; ++j) {
         const int next = load_page(j + 1);
-        const int base = k0 + j * TC_TILE;
-        const bool wanted = lane < per && base + (lane << a.page_shift) < k_end;
+        const int base = k0 + j * KEYS, pos = base + lane * box;
+        const bool wanted = lane < per && pos < k_end;
         const bool good = wanted && page >= 0 && page < p.num_pages;
         if (wanted && !good && p.status) atomicCAS(p.status, 0, 84);
         const uint32_t pages = __ballot_sync(0xffffffffu, good);
-        const int row = (max(page, 0) * p.kv_heads + kh) * p.page_size;
-        if (E4M3) {   // codes of 64 keys at a time, for the converting warps
-          const int rows = min(p.page_size, TC_HALF);
-          for (int h = 0; h < 4 && ok; ++h) {   // K_j, then V_j
-            const int n = 4 * j + h, st = n % RAW, half = h & 1;
-            if (n >= RAW) ok = mbar_wait(&s.bar_raw_empty[st], ((n / RAW) - 1) & 1, abortp, p.status, 44);
-            if (!ok) break;
-            const bool here = good && (p.page_size > TC_HALF || (lane << a.page_shift) / TC_HALF == half);
-            const uint32_t copies = __popc(__ballot_sync(0xffffffffu, here));
-            if (lane == 0) mbar_arrive_expect_tx(&s.bar_raw_full[st], copies * (uint32_t)rows * DH);
-            __syncwarp();
-            if (here) {
-              const int at = p.page_size > TC_HALF ? 0 : (lane << a.page_shift) % TC_HALF;
-              tma_load_2d(s.raw[st] + at * DH, h < 2 ? &map_k : &map_v, &s.bar_raw_full[st], 0, row + (p.page_size > TC_HALF ? half * TC_HALF : 0));
-            }
-            __syncwarp();
-          }
-          page = next;
-          continue;
-        }
-        const uint32_t bytes = __popc(pages) * (uint32_t)p.page_size * DH * 2;
+        const int row = (max(page, 0) * p.kv_heads + kh) * p.page_size + (pos & (p.page_size - 1));
+        const uint32_t bytes = __popc(pages) * (uint32_t)box * DH * (E4M3 ? 1 : 2);
 #pragma unroll
         for (int v = 0; v < 2 && ok; ++v) {
-          const int n = 2 * j + v, st = n % SLOTS;
-          if (n >= SLOTS) ok = mbar_wait(&s.bar_empty[st], ((n / SLOTS) - 1) & 1, abortp, p.status, 44);
+          const int n = 2 * j + v, ring = E4M3 ? RAW : SLOTS, st = n % ring;
+          uint64_t* full = E4M3 ? &s.bar_raw_full[st] : &s.bar_full[st];
+          if (n >= ring) ok = mbar_wait(E4M3 ? &s.bar_raw_empty[st] : &s.bar_empty[st], ((n / ring) - 1) & 1, abortp, p.status, 44);
           if (!ok) break;
-          if (v == 0 && lane < 4) {
+          if (!E4M3 && v == 0 && lane < 4) {
             uint32_t there = 0;
-            if (pages == (1u << per) - 1u && base + TC_TILE <= k_end) {
+            if (lane >= KEYS / 32 || (pages == (1u << per) - 1u && base + KEYS <= k_end)) {
               there = 0xffffffffu;
             } else {
               for (int i = 0; i < 32; ++i) {
                 const int key = lane * 32 + i;
-                if ((pages >> (key >> a.page_shift) & 1u) && base + key < k_end) there |= 1u << i;
+                if ((pages >> (key / box) & 1u) && base + key < k_end) there |= 1u << i;
               }
             }
             s.meta[j % META].there[lane] = there;
           }
           __syncwarp();
-          if (lane == 0) mbar_arrive_expect_tx(&s.bar_full[st], bytes);
+          if (lane == 0) mbar_arrive_expect_tx(full, bytes);
           __syncwarp();
           if (good) {
+            if (E4M3) {
+              tma_load_2d(s.raw[st] + lane * box * DH, v ? &map_v : &map_k, full, 0, row);
+            } else {
 #pragma unroll
-            for (int c = 0; c < PANELS; ++c)
-              tma_load_2d(s.kv[st] + c * TC_PANEL + (lane << a.page_shift) * 128, v ? &map_v : &map_k, &s.bar_full[st], c * 64, row);
+              for (int c = 0; c < PANELS; ++c) tma_load_2d(s.kv[st] + c * KV_PANEL + lane * box * 128, v ? &map_v : &map_k, full, c * 64, row);
+            }
           }
           __syncwarp();
         }
         page = next;
       }
+    } else if (E4M3) {
+      if (warp >= C::FIRST_CONVERT) convert();
+    } else if (warp == 10) {
+      // ====================================================================== rows of V that belong to no key: 0 * NaN is NaN
+      // (codes become finite values whatever they are)
+      bool ok = true;
+      for (int j = 0; j < n_j && ok; ++j) {
+        const int nv = 2 * j + 1, st = nv % SLOTS;
+        ok = mbar_wait(&s.bar_full[st], (nv / SLOTS) & 1, abortp, p.status, 52);
+        if (!ok) break;
+        const uint32_t* there = s.meta[j % META].there;
+        if ((there[0] & there[1] & there[2] & there[3]) != 0xffffffffu) {
+          for (int row = lane; row < KEYS; row += 32)
+            if (!(there[row >> 5] >> (row & 31) & 1u)) {
+              const uint32_t at = smem_u32(s.kv[st]) + row * 128;
+#pragma unroll
+              for (int c = 0; c < PANELS * 8; ++c)
+                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at + (c >> 3) * KV_PANEL + (c & 7) * 16), "r"(0) : "memory");
+            }
+          fence_proxy_async();
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s.bar_clean[st]);
+      }
     }
-  } else if (warp < 8) {
+  } else {
     // ======================================================================== softmax warpgroups
-    claim_registers<E4M3 ? 200 : 224>();
+    claim_registers<C::SOFTMAX>();
     const int g = warp >> 2, quarter = warp & 3;
     const int row = quarter * 32 + lane;             // of the tile
     // queries: 16-byte chunks of the warp's 32 rows, neighbouring lanes on neighbouring chunks, into the swizzled tile
     for (int i = lane; i < 32 * (DH / 8); i += 32) {
       const int rr = quarter * 32 + i / (DH / 8), c = i % (DH / 8);
-      const int at = g * TC_TILE + rr;
+      const int at = g * ROWS + rr;
       uint4 x = make_uint4(0, 0, 0, 0);
       if (at < n_rows) {
         const int tok = (local + at) / a.group, head = kh * a.group + (local + at) % a.group;
         x = __ldg(reinterpret_cast<const uint4*>((const T*)a.q + (int64_t)(r.x + tok) * a.q_stride + head * DH) + c);
       }
-      *reinterpret_cast<uint4*>(s.q[g] + (c >> 3) * TC_PANEL + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = x;
+      *reinterpret_cast<uint4*>(s.q[g] + (c >> 3) * Q_PANEL + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = x;
     }
     fence_proxy_async();
     __syncwarp();
     if (lane == 0) mbar_arrive(&s.bar_q);
 
     const int mine = g == 0 ? n_kv[0] : n_kv[1];
-    const bool live = g * TC_TILE + row < n_rows;
-    const int limit = live ? first_pos + (local + g * TC_TILE + row) / a.group : -1;
-    const uint32_t t_s = tmem + ((uint32_t)(quarter * 32) << 16) + g * 128;
-    const uint32_t t_o = tmem + ((uint32_t)(quarter * 32) << 16) + 256 + g * DH;
+    const bool live = g * ROWS + row < n_rows;
+    const uint32_t t_s = tmem + ((uint32_t)(quarter * 32) << 16) + g * KEYS;   // P too
+    const uint32_t t_o = tmem + ((uint32_t)(quarter * 32) << 16) + 2 * KEYS + g * DH;
+    auto rescale = [&](float keep) {
+#pragma unroll
+      for (int c = 0; c < DH / 16; ++c) {
+        uint32_t o[16];
+        tmem_ld_32x16(t_o + c * 16, o);
+        tmem_ld_wait();
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+        tmem_st_32x16(t_o + c * 16, o);
+      }
+    };
+    auto hand_over = [&] {
+      tmem_st_wait();
+      fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s.bar_p[g]);
+    };
     float m = -INFINITY, l = 0.f;                    // of the thread's row, in base-2 logarithms and relative to m
     bool ok = true;
-    if (E4M3) {
-      // Every column has its own scales.  A thread per row would read all 3 x 128 of them from shared memory, 393 KB per pair of
-      // tiles, which takes longer than the exponentials; in the spread of the 16-lane loads a thread has a quarter of the columns
-      // for four rows (t / 4 + 8 k of the warp's 32) and reads a quarter of that.  A row is shared by the four threads of a quad.
+    if constexpr (E4M3) {
+      // Every column has its own scales.  A thread per row would read all of them from shared memory, 393 KB per 128 keys, which
+      // takes longer than the exponentials; in the spread of the 16-lane loads a thread has a quarter of the columns for four rows
+      // (t / 4 + 8 k of the warp's 32) and reads a quarter of that.  A row is shared by the four threads of a quad.
       const int t = lane & 3;
       int lim[4];
       float mr[4], lr[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const int rr = g * TC_TILE + quarter * 32 + (lane >> 2) + 8 * k;
+        const int rr = g * ROWS + quarter * 32 + (lane >> 2) + 8 * k;
         lim[k] = rr < n_rows ? first_pos + (local + rr) / a.group : -1;
         mr[k] = -INFINITY;
         lr[k] = 0.f;
       }
+      constexpr int N = KEYS / 8;
+      static_assert(N == 8, "one load per 16 lanes");
       for (int j = 0; j < mine; ++j) {
         ok = mbar_wait(&s.bar_s[g], j & 1, abortp, p.status, 45);
         if (!ok) break;
         fence_after_sync();
-        const KeyMeta& meta = s.meta[j % META];
+        const auto& meta = s.meta[j % META];
         union {   // [16 rows][8 columns][row + 8][column]
-          uint32_t w[2][16 * 4];
-          float2 f2[2][16][2];
+          uint32_t w[2][N * 4];
+          float2 f2[2][N][2];
         } x;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) tmem_ld_16x128(t_s + ((uint32_t)(16 * h) << 16), x.w[h]);
+        for (int h = 0; h < 2; ++h) tmem_ld_16x64(t_s + ((uint32_t)(16 * h) << 16), x.w[h]);
         tmem_ld_wait();
 #pragma unroll
-        for (int n = 0; n < 16; ++n) {
+        for (int n = 0; n < N; ++n) {
           const float4 f = *reinterpret_cast<const float4*>(meta.ks_lv[4 * n + t]);
 #pragma unroll
           for (int k = 0; k < 4; ++k) x.f2[k >> 1][n][k & 1] = fma2(x.f2[k >> 1][n][k & 1], make_float2(f.x, f.y), make_float2(f.z, f.w));
         }
-        const int base = k0 + j * TC_TILE;
-        const uint4 there = *reinterpret_cast<const uint4*>(meta.there);
-        if (__any_sync(0xffffffffu, (there.x & there.y & there.z & there.w) != 0xffffffffu || min(min(lim[0], lim[1]), min(lim[2], lim[3])) - base < TC_TILE - 1)) {
+        const int base = k0 + j * KEYS;
+        const bool masked = __any_sync(0xffffffffu, (meta.there[0] & meta.there[1]) != 0xffffffffu ||
+                                                        min(min(lim[0], lim[1]), min(lim[2], lim[3])) - base < KEYS - 1);
+        if (masked) {
 #pragma unroll
-          for (int n = 0; n < 16; ++n) {
+          for (int n = 0; n < N; ++n) {
             const uint32_t bits = meta.there[n >> 2] >> ((n & 3) * 8 + 2 * t);
             const int key = base + 8 * n + 2 * t;
 #pragma unroll
@@ -408,7 +544,7 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
         for (int k = 0; k < 4; ++k) {
           float t0 = -INFINITY, t1 = -INFINITY;
 #pragma unroll
-          for (int n = 0; n < 16; n += 2) {
+          for (int n = 0; n < N; n += 2) {
             const float2 u = x.f2[k >> 1][n][k & 1], w = x.f2[k >> 1][n + 1][k & 1];
             t0 = fmaxf(t0, fmaxf(u.x, u.y));
             t1 = fmaxf(t1, fmaxf(w.x, w.y));
@@ -429,44 +565,35 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
             const float k_row = __shfl_sync(0xffffffffu, keep, (lane & 7) * 4);
             if (lane >> 3 == k) row_keep = k_row;
           }
-          if (j > 0) {
+          if (j > 0) rescale(row_keep);
+        }
+        auto exponentials = [&](auto by_polynomial) {
 #pragma unroll
-            for (int c = 0; c < DH / 16; ++c) {
-              uint32_t o[16];
-              tmem_ld_32x16(t_o + c * 16, o);
-              tmem_ld_wait();
+          for (int h = 0; h < 2; ++h) {
+            uint32_t w[16];
 #pragma unroll
-              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * row_keep);
-              tmem_st_32x16(t_o + c * 16, o);
-            }
+            for (int n = 0; n < N; ++n)
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                const float ref = mr[2 * h + k] == -INFINITY ? 0.f : mr[2 * h + k];
+                float2& u = x.f2[h][n][k];
+                u = add2(u, make_float2(-ref, -ref));
+                if (decltype(by_polynomial)::value && (2 * n + k) % 8 < POLY_PAIRS_E4M3) u = exp2_by_polynomial<TYPE>(u);
+                else u = make_float2(ex2(u.x), ex2(u.y));
+                w[2 * n + k] = pack16<TYPE>(u.x, u.y);
+              }
+            tmem_st_16x32(t_s + ((uint32_t)(16 * h) << 16), w);
           }
-        }
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t w[32];
-#pragma unroll
-          for (int n = 0; n < 16; ++n)
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              const float ref = mr[2 * h + k] == -INFINITY ? 0.f : mr[2 * h + k];
-              float2& u = x.f2[h][n][k];
-              u = add2(u, make_float2(-ref, -ref));
-              u.x = ex2(u.x);
-              u.y = ex2(u.y);
-              w[2 * n + k] = pack16<TYPE>(u.x, u.y);
-            }
-          tmem_st_16x64(t_s + ((uint32_t)(16 * h) << 16), w);
-        }
-        tmem_st_wait();
-        fence_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&s.bar_p[g]);
+        };
+        if (masked || POLY_PAIRS_E4M3 == 0) exponentials(std::false_type{});   // 2^-inf is 0 there, the polynomial's smallest value is 2^-126
+        else exponentials(std::true_type{});
+        hand_over();
         // the sums are needed by nobody yet: behind the arrival
         float2 sum[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) sum[k] = make_float2(lr[k], 0.f);
 #pragma unroll
-        for (int n = 0; n < 16; ++n) {
+        for (int n = 0; n < N; ++n) {
           const float2 iv = *reinterpret_cast<const float2*>(meta.iv + 8 * n + 2 * t);
 #pragma unroll
           for (int k = 0; k < 4; ++k) sum[k] = fma2(x.f2[k >> 1][n][k & 1], iv, sum[k]);
@@ -484,98 +611,84 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
           m = m_row;
         }
       }
-    }
-    float2 l2 = make_float2(0.f, 0.f);
-    for (int j = 0; !E4M3 && j < mine; ++j) {
-      ok = mbar_wait(&s.bar_s[g], j & 1, abortp, p.status, 45);
-      if (!ok) break;
-      fence_after_sync();
-      const KeyMeta& meta = s.meta[j % META];
-      union {   // the row of S
-        uint32_t w[TC_TILE];
-        float f[TC_TILE];
-        float2 f2[TC_TILE / 2];
-      } x;
+    } else {
+      const int limit = live ? first_pos + (local + g * ROWS + row) / a.group : -1;
+      float2 l2 = make_float2(0.f, 0.f);
+      for (int j = 0; j < mine; ++j) {
+        ok = mbar_wait(&s.bar_s[g], j & 1, abortp, p.status, 45);
+        if (!ok) break;
+        fence_after_sync();
+        const auto& meta = s.meta[j % META];
+        union {   // the row of S
+          uint32_t w[KEYS];
+          float f[KEYS];
+          float2 f2[KEYS / 2];
+        } x;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld_32x32(t_s + c * 32, x.w + c * 32);
-      tmem_ld_wait();
-      const int rel = limit - (k0 + j * TC_TILE);    // the row's last key, counted from the tile's first
-      uint32_t hidden = 0;
-      {
+        for (int c = 0; c < KEYS / 32; ++c) tmem_ld_32x32(t_s + c * 32, x.w + c * 32);
+        tmem_ld_wait();
+        const int rel = limit - (k0 + j * KEYS);     // the row's last key, counted from the tile's first
         const uint4 there = *reinterpret_cast<const uint4*>(meta.there);
-        hidden = (there.x & there.y & there.z & there.w) != 0xffffffffu || rel < TC_TILE - 1;
-      }
-      if (__any_sync(0xffffffffu, hidden)) {
+        const bool masked = __any_sync(0xffffffffu, (there.x & there.y & there.z & there.w) != 0xffffffffu || rel < KEYS - 1);
+        if (masked) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const int e0 = rel - 32 * c;
-          const uint32_t seen = meta.there[c] & (e0 >= 31 ? 0xffffffffu : e0 < 0 ? 0u : (2u << e0) - 1u);
+          for (int c = 0; c < KEYS / 32; ++c) {
+            const int e0 = rel - 32 * c;
+            const uint32_t seen = meta.there[c] & (e0 >= 31 ? 0xffffffffu : e0 < 0 ? 0u : (2u << e0) - 1u);
 #pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (!(seen >> e & 1u)) x.f[c * 32 + e] = -INFINITY;
-        }
-      }
-      float t4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-      for (int e = 0; e < TC_TILE; e += 8)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) t4[i] = fmaxf(t4[i], fmaxf(x.f[e + i], x.f[e + 4 + i]));
-      float top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
-      top *= a.scale_log2;   // the scale is positive here, see the choice of the kernel
-      // the reference point follows only a growth by more than 2^8
-      const bool grow = top > m + 8.f;
-      if (__any_sync(0xffffffffu, grow)) {
-        const float m_new = grow ? top : m;
-        const float keep = m == m_new ? 1.f : ex2(m - m_new);
-        m = m_new;
-        l2.x *= keep;
-        l2.y *= keep;
-        if (j > 0) {
-#pragma unroll
-          for (int c = 0; c < DH / 16; ++c) {
-            uint32_t o[16];
-            tmem_ld_32x16(t_o + c * 16, o);
-            tmem_ld_wait();
-#pragma unroll
-            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
-            tmem_st_32x16(t_o + c * 16, o);
+            for (int e = 0; e < 32; ++e)
+              if (!(seen >> e & 1u)) x.f[c * 32 + e] = -INFINITY;
           }
         }
-      }
-      const float ref = m == -INFINITY ? 0.f : m;
-      const float2 neg = make_float2(-ref, -ref), sc = make_float2(a.scale_log2, a.scale_log2);
+        float t4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t w[16];
+        for (int e = 0; e < KEYS; e += 8)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          float2& u = x.f2[c * 16 + e];
-          u = fma2(u, sc, neg);
-          u.x = ex2(u.x);
-          u.y = ex2(u.y);
-          w[e] = pack16<TYPE>(u.x, u.y);
+          for (int i = 0; i < 4; ++i) t4[i] = fmaxf(t4[i], fmaxf(x.f[e + i], x.f[e + 4 + i]));
+        const float top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])) * a.scale_log2;   // positive, see the choice of the kernel
+        // the reference point follows only a growth by more than 2^8
+        const bool grow = top > m + 8.f;
+        if (__any_sync(0xffffffffu, grow)) {
+          const float m_new = grow ? top : m;
+          const float keep = m == m_new ? 1.f : ex2(m - m_new);
+          m = m_new;
+          l2.x *= keep;
+          l2.y *= keep;
+          if (j > 0) rescale(keep);
         }
-        tmem_st_32x16(t_s + c * 16, w);   // over columns that have been read
-      }
-      tmem_st_wait();
-      fence_before_sync();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&s.bar_p[g]);
-      // the sum is needed by nobody yet: behind the arrival
-      float2 sum[4] = {l2, make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        const float ref = m == -INFINITY ? 0.f : m;
+        const float2 neg = make_float2(-ref, -ref), sc = make_float2(a.scale_log2, a.scale_log2);
+        auto exponentials = [&](auto by_polynomial) {
 #pragma unroll
-      for (int e = 0; e < TC_TILE / 2; e += 2) {
-        sum[e & 3] = add2(sum[e & 3], x.f2[e]);
-        sum[(e & 3) + 1] = add2(sum[(e & 3) + 1], x.f2[e + 1]);
+          for (int c = 0; c < KEYS / 32; ++c) {
+            uint32_t w[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              float2& u = x.f2[c * 16 + e];
+              u = fma2(u, sc, neg);
+              if (decltype(by_polynomial)::value && e % 8 < POLY_PAIRS) u = exp2_by_polynomial<TYPE>(u);
+              else u = make_float2(ex2(u.x), ex2(u.y));
+              w[e] = pack16<TYPE>(u.x, u.y);
+            }
+            tmem_st_32x16(t_s + c * 16, w);
+          }
+        };
+        if (masked) exponentials(std::false_type{});   // 2^-inf is 0 there, the polynomial's smallest value is 2^-126
+        else exponentials(std::true_type{});
+        hand_over();
+        // the sum is needed by nobody yet: behind the arrival
+        float2 sum[4] = {l2, make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+        for (int e = 0; e < KEYS / 2; ++e) sum[e & 3] = add2(sum[e & 3], x.f2[e]);
+        l2 = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
       }
-      l2 = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
+      l = l2.x + l2.y;
     }
-    if (!E4M3) l = l2.x + l2.y;
     if (ok && mine > 0) ok = mbar_wait(&s.bar_o[g], 0, abortp, p.status, 46);
     if (ok) {
       fence_after_sync();
       const float inv = l == 0.f ? 0.f : 1.f / l;
-      const int at = local + g * TC_TILE + row;
+      const int at = local + g * ROWS + row;
       const int64_t o_row = (int64_t)(r.x + at / a.group) * a.heads + kh * a.group + at % a.group;
 #pragma unroll
       for (int c = 0; c < DH / 32; ++c) {
@@ -584,83 +697,18 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
           tmem_ld_32x32(t_o + c * 32, x);
           tmem_ld_wait();
         }
-        float f[32];
-#pragma unroll
-        for (int e = 0; e < 32; ++e) f[e] = mine > 0 ? __uint_as_float(x[e]) * inv : 0.f;
         if (live) {
 #pragma unroll
           for (int e = 0; e < 32; e += 8) {
-            if (a.part_o) store_f<float, 8>(a.part_o + (o_row * a.splits + split) * DH + c * 32 + e, f + e);
-            else store_f<T, 8>((T*)a.out + o_row * DH + c * 32 + e, f + e);
+            float f[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = mine > 0 ? __uint_as_float(x[e + i]) * inv : 0.f;
+            if (a.part_o) store_f<float, 8>(a.part_o + (o_row * a.splits + split) * DH + c * 32 + e, f);
+            else store_f<T, 8>((T*)a.out + o_row * DH + c * 32 + e, f);
           }
         }
       }
       if (live && a.part_o) a.part_lse[o_row * a.splits + split] = l == 0.f ? -INFINITY : m + log2f(l);
-    }
-  } else if (E4M3) {
-    // ======================================================================== converting warpgroup (warps 12 .. 15)
-    release_registers<64>();
-    const int tid = threadIdx.x - 384;               // 0 .. 127: also the key whose scales this thread looks up
-    const int* table = p.table + (int64_t)b * p.table_stride;
-    constexpr int CHUNKS = TC_HALF * DH / 16 / 128;  // 16-byte chunks of codes per thread and copy
-    auto load_page = [&](int j) {
-      const int pos = k0 + j * TC_TILE + tid;
-      return j < n_j && pos < k_end ? __ldg(table + (pos >> a.page_shift)) : -1;
-    };
-    int slot = -1;
-    float k_scale = 0.f, v_scale = 0.f;
-    auto look_up = [&](int j, int page) {            // slot and scales of key tid of tile j
-      const int pos = k0 + j * TC_TILE + tid;
-      slot = -1;
-      if (j < n_j && pos < k_end && page >= 0 && page < p.num_pages) slot = (page * p.kv_heads + kh) * p.page_size + (pos & (p.page_size - 1));
-      k_scale = slot >= 0 ? __ldg(p.k_scale + slot) : 0.f;
-      v_scale = slot >= 0 ? __ldg(p.v_scale + slot) : 0.f;
-    };
-    look_up(0, load_page(0));
-    int page = load_page(1);
-    bool ok = true;
-    for (int n = 0; n < 2 * n_j && ok; ++n) {        // K_0, V_0, K_1, ...
-      const int st = n % SLOTS, j = n >> 1;
-      if (n >= SLOTS) ok = mbar_wait(&s.bar_empty[st], ((n / SLOTS) - 1) & 1, abortp, p.status, 47);
-      if (!ok) break;
-      if ((n & 1) == 0) {
-        KeyMeta& meta = s.meta[j % META];            // behind the wait, see META
-        const float vs = positive_scale(v_scale);
-        const uint32_t there = __ballot_sync(0xffffffffu, slot >= 0);
-        meta.ks_lv[tid >> 1][tid & 1] = k_scale * a.scale_log2;
-        meta.ks_lv[tid >> 1][2 + (tid & 1)] = lg2(vs);
-        meta.iv[tid] = __frcp_rn(vs);
-        if (lane == 0) meta.there[warp - 12] = there;
-        look_up(j + 1, page);
-        page = load_page(j + 2);
-      }
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int nr = 2 * n + half, sr = nr % RAW;
-        ok = mbar_wait(&s.bar_raw_full[sr], (nr / RAW) & 1, abortp, p.status, 48);
-        if (!ok) break;
-        uint4 raw[CHUNKS];
-#pragma unroll
-        for (int i = 0; i < CHUNKS; ++i) raw[i] = *reinterpret_cast<const uint4*>(s.raw[sr] + (i * 128 + tid) * 16);
-#pragma unroll
-        for (int i = 0; i < CHUNKS; ++i) {
-          const int id = i * 128 + tid, row = half * TC_HALF + id / (DH / 16), c = id % (DH / 16);
-          uint32_t x[8];
-          codes_to_16<TYPE>(raw[i].x, x[0], x[1]);
-          codes_to_16<TYPE>(raw[i].y, x[2], x[3]);
-          codes_to_16<TYPE>(raw[i].z, x[4], x[5]);
-          codes_to_16<TYPE>(raw[i].w, x[6], x[7]);
-          uint8_t* dst = s.kv[st] + (c >> 2) * TC_PANEL + row * 128;
-          *reinterpret_cast<uint4*>(dst + (((2 * (c & 3)) ^ (row & 7)) << 4)) = make_uint4(x[0], x[1], x[2], x[3]);
-          *reinterpret_cast<uint4*>(dst + (((2 * (c & 3) + 1) ^ (row & 7)) << 4)) = make_uint4(x[4], x[5], x[6], x[7]);
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&s.bar_raw_empty[sr]);
-      }
-      if (!ok) break;
-      fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&s.bar_full[st]);
     }
   }
 
@@ -674,7 +722,7 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   __syncthreads();
   if (warp == 8) {
     fence_after_sync();
-    tmem_dealloc(tmem, 512);
+    tmem_dealloc(tmem, C::TMEM);
   }
 }
 
@@ -702,7 +750,7 @@ static int launch_tiles(const AttnArgs& a, cudaStream_t st) {
   if (!fn) return 801;
   const cuuint64_t dims[2] = {DH, (cuuint64_t)a.b.num_pages * a.b.kv_heads * a.b.page_size};
   const cuuint64_t strides[1] = {E4M3 ? DH : DH * 2};
-  const cuuint32_t box[2] = {E4M3 ? DH : 64, (cuuint32_t)(E4M3 ? std::min(a.b.page_size, TC_HALF) : a.b.page_size)}, estr[2] = {1, 1};
+  const cuuint32_t box[2] = {E4M3 ? DH : 64, (cuuint32_t)std::min(a.b.page_size, TcConfig<E4M3, DH>::KEYS)}, estr[2] = {1, 1};
   for (int v = 0; v < 2; ++v) {
     const CUresult rc = fn(&map[v], E4M3 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : TYPE == LBI_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
                            v ? a.b.v : a.b.k, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
@@ -718,12 +766,12 @@ static int launch_tiles(const AttnArgs& a, cudaStream_t st) {
   // the claims of the warpgroups add up to what a block gets at launch only if the kernel was compiled to this many registers
   static const bool registers_add_up = [&] {
     cudaFuncAttributes attr;
-    return cudaFuncGetAttributes(&attr, kernel) == cudaSuccess && attr.numRegs == (E4M3 ? 128 : 168);
+    return cudaFuncGetAttributes(&attr, kernel) == cudaSuccess && attr.numRegs == TcConfig<E4M3, DH>::LAUNCH;
   }();
   if (!registers_add_up) return (int)cudaErrorInvalidConfiguration;
-  const int64_t blocks = tile_bound(a.b, a.group, 2 * TC_TILE) * a.b.kv_heads * a.splits;
+  const int64_t blocks = tile_bound(a.b, a.group, 2 * ROWS) * a.b.kv_heads * a.splits;
   if (blocks >= (1ll << 31)) return (int)cudaErrorInvalidValue;
-  kernel<<<(unsigned)blocks, E4M3 ? 512 : 384, smem, st>>>(map[0], map[1], a);
+  kernel<<<(unsigned)blocks, TcConfig<E4M3, DH>::THREADS, smem, st>>>(map[0], map[1], a);
   return (int)cudaGetLastError();
 }
 
