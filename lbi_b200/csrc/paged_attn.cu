@@ -490,11 +490,11 @@ extern "C" lbi_attention_plan lbi_paged_attention_plan(const lbi_paged_batch* p,
   // the tcgen05 kernel takes its row maximum before the scale, so it needs a positive one
   plan.kernel = p->head_dim >= 64 && (int64_t)p->rows * group >= 64ll * p->batch && scale > 0.f ? 2 : 1;
   if (plan.kernel == 2) {
-    // One block per SM (head_dim 128) or two.  Parts of a context pay where whole units leave the last round of blocks half empty: the
+    // One block per SM, or two (head_dim 64, 16-bit pages).  Parts of a context pay where whole units leave the last round of blocks half empty: the
     // number of parts (of 512 keys at least) with the fewest key tiles per SM, 4 % added per part for the partial results and the
     // block's own start.
     const int64_t units = tile_bound(*p, group, 256) * p->kv_heads;
-    sm_count *= p->head_dim == 64 ? 2 : 1;
+    sm_count *= p->head_dim == 64 && p->cache_type != LBI_E4M3 ? 2 : 1;
     double best = 0;
     for (int splits = 1; splits <= 16 && (splits == 1 || longest / splits >= 512); ++splits) {
       const double cost = (double)((units * splits + sm_count - 1) / sm_count) / splits * (1 + 0.04 * (splits - 1));

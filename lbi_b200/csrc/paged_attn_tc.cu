@@ -43,23 +43,26 @@ constexpr int COPY_KEYS = 64;              // keys of one copy of codes
 
 template <bool E4M3, int DH>
 struct TcConfig {
-  static constexpr int BLOCKS = DH == 64 ? 2 : 1;                 // per SM
+  static constexpr int BLOCKS = DH == 64 && !E4M3 ? 2 : 1;        // per SM
   static constexpr int KEYS = DH == 64 || E4M3 ? 64 : 128;        // of a tile
-  static constexpr int SLOTS = DH == 64 ? 6 : E4M3 ? 8 : 4;       // K_0, V_0, K_1, V_1, ...
+  static constexpr int SLOTS = E4M3 ? 10 : DH == 64 ? 6 : 4;       // K_0, V_0, K_1, V_1, ...
   // Masks and scales of a key tile: K_j is stored when S_(j - SLOTS / 2) is complete, which follows the softmax of the tile before
   // that one, so SLOTS / 2 + 2 entries never meet one that is still read.
   static constexpr int META = SLOTS / 2 + 2;
-  static constexpr int RAW = E4M3 ? (DH == 64 ? 4 : 3) : 1;       // copies of codes on their way to the converting warps
-  // warps 0-3, 4-7 softmax; 8 products; 9 copies; 16-bit pages: 10 clears V; e4m3: converting warps
-  static constexpr int CONVERT = E4M3 ? (DH == 64 ? 2 : 4) : 0, FIRST_CONVERT = DH == 64 ? 10 : 12;
-  static constexpr int THREADS = E4M3 && DH == 128 ? 512 : 384;
-  // Registers at launch and of the warpgroups afterwards (softmax, warps 8-11, warps 12-15): claimed ones come from those that the
+  static constexpr int RAW = E4M3 ? 6 : 1;                         // copies of codes on their way to the converting warps
+  // warps 0-3, 4-7 softmax; 8 products; 9 copies; 16-bit pages: 10 clears V; e4m3: 10 and 11 scales, 12-19 conversion
+  static constexpr int CONVERT = E4M3 ? 8 : 0, FIRST_CONVERT = 12;
+  static constexpr int THREADS = 384 + CONVERT * 32;
+  // Registers at launch and of the warpgroups afterwards (softmax, warps 8-11, conversion): claimed ones come from those that the
   // block was launched with and others have released, so the shares add up to at most threads x LAUNCH.
-  static constexpr int LAUNCH = DH == 64 ? 80 : E4M3 ? 128 : 168;
-  static constexpr int SOFTMAX = DH == 64 ? 96 : E4M3 ? 200 : 224, ISSUE = DH == 64 ? 48 : E4M3 ? 48 : 56, WIDE = 64;
-  static_assert(256 * SOFTMAX + 128 * ISSUE + (THREADS == 512 ? 128 * WIDE : 0) <= THREADS * LAUNCH, "register shares");
-  static constexpr int TMEM = DH == 64 ? 256 : 512;
-  static_assert(2 * KEYS + 2 * DH <= TMEM, "columns");
+  static constexpr int LAUNCH = E4M3 ? 96 : DH == 64 ? 80 : 168;
+  static constexpr int SOFTMAX = E4M3 ? 160 : DH == 64 ? 96 : 224, ISSUE = E4M3 || DH == 64 ? 48 : 56, WIDE = 56;
+  static_assert(256 * SOFTMAX + 128 * ISSUE + CONVERT * 32 * WIDE <= THREADS * LAUNCH, "register shares");
+  static constexpr int TMEM = DH == 64 && !E4M3 ? 256 : 512;
+  // e4m3: Q is read from TMEM, too.  Shared memory is what runs short there (the conversion writes 2 bytes per code, the softmax reads
+  // scales), and Q is the larger operand of S.
+  static constexpr bool Q_IN_TMEM = E4M3;
+  static_assert(2 * KEYS + 2 * DH + (Q_IN_TMEM ? DH : 0) <= TMEM, "columns");
 };
 
 template <int KEYS>
@@ -72,9 +75,9 @@ struct alignas(16) KeyMeta {
 template <bool E4M3, int DH>
 struct TcSmem {
   using C = TcConfig<E4M3, DH>;
-  alignas(1024) uint8_t q[2][ROWS * DH * 2];
+  alignas(1024) uint8_t q[C::Q_IN_TMEM ? 1 : 2][C::Q_IN_TMEM ? 16 : ROWS * DH * 2];
   alignas(1024) uint8_t kv[C::SLOTS][C::KEYS * DH * 2];
-  alignas(128) uint8_t raw[C::RAW][E4M3 ? COPY_KEYS * DH : 16];
+  alignas(1024) uint8_t raw[C::RAW][E4M3 ? COPY_KEYS * DH : 16];
   KeyMeta<E4M3 ? C::KEYS : 4> meta[C::META];
   uint64_t bar_raw_full[C::RAW];
   uint64_t bar_raw_empty[C::RAW];
@@ -192,22 +195,23 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   const int first_pos = __ldg(p.context + b) - (r.y - r.x);
   const int64_t capacity = (int64_t)p.table_width << a.page_shift;
   const int k0 = split * a.split_keys;
-  int n_kv[2], k_end = 0;   // key tiles of each row tile; one behind the last key any row sees
-#pragma unroll
-  for (int g = 0; g < 2; ++g) {
+  int k_end = 0;            // one behind the last key that any row sees
+  auto key_tiles = [&](int g) {   // of row tile g
+
     const int last = min(n_rows, (g + 1) * ROWS) - 1;   // the tile's last row
     const int keys = last < g * ROWS ? 0 : (int)min((int64_t)first_pos + (local + last) / a.group + 1, capacity);
     const int k1 = split == a.splits - 1 ? keys : min(keys, k0 + a.split_keys);
-    n_kv[g] = k1 > k0 ? (k1 - k0 + KEYS - 1) / KEYS : 0;
     k_end = max(k_end, k1);
-  }
-  const int n_j = max(n_kv[0], n_kv[1]);
+    return k1 > k0 ? (k1 - k0 + KEYS - 1) / KEYS : 0;
+  };
+  // two variables, not an array, which an index known at run time only would put into local memory
+  const int n_kv0 = key_tiles(0), n_kv1 = key_tiles(1), n_j = max(n_kv0, n_kv1);
 
   if (threadIdx.x == 0) {
     s.abort_flag = 0;
     mbar_init(&s.bar_q, 8);
     for (int i = 0; i < SLOTS; ++i) {
-      mbar_init(&s.bar_full[i], E4M3 ? C::CONVERT : 1);
+      mbar_init(&s.bar_full[i], E4M3 ? C::CONVERT + (i % 2 == 0 ? 2 : 0) : 1);   // K comes with its scales
       mbar_init(&s.bar_empty[i], 1);
       mbar_init(&s.bar_clean[i], 1);
     }
@@ -231,78 +235,42 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   const uint32_t tmem = s.tmem_base;
   volatile int* abortp = &s.abort_flag;
 
-  // ---------------------------------------------------------------------- converting warps (called by theirs)
-  auto convert = [&] {
+  if (warp >= 12) {
+    // ======================================================================== converting warps: codes -> 16-bit values
+    release_registers<C::WIDE>();
     if constexpr (E4M3) {
-      constexpr int THREADS = C::CONVERT * 32, EACH = KEYS / THREADS > 1 ? KEYS / THREADS : 1;
-      const int tid = threadIdx.x - C::FIRST_CONVERT * 32;   // the keys tid, tid + THREADS, .. whose scales this thread looks up
-      const int* table = p.table + (int64_t)b * p.table_stride;
-      constexpr int CHUNKS = COPY_KEYS * DH / 16 / THREADS;    // 16-byte chunks of codes per thread and copy
-      static_assert(KEYS == COPY_KEYS && CHUNKS % 2 == 0, "one copy per tile");
-      float k_scale[EACH], v_scale[EACH];
-      uint32_t there[EACH];
-      int page[EACH];
-      auto load_pages = [&](int j) {
-#pragma unroll
-        for (int i = 0; i < EACH; ++i) {
-          const int key = tid + i * THREADS, pos = k0 + j * KEYS + key;
-          page[i] = j < n_j && key < KEYS && pos < k_end ? __ldg(table + (pos >> a.page_shift)) : -1;
-        }
-      };
-      auto look_up = [&](int j) {
-#pragma unroll
-        for (int i = 0; i < EACH; ++i) {
-          const int pos = k0 + j * KEYS + tid + i * THREADS;
-          const bool good = page[i] >= 0 && page[i] < p.num_pages;
-          const int slot = good ? (page[i] * p.kv_heads + kh) * p.page_size + (pos & (p.page_size - 1)) : 0;
-          k_scale[i] = good ? __ldg(p.k_scale + slot) : 0.f;
-          v_scale[i] = good ? __ldg(p.v_scale + slot) : 0.f;
-          there[i] = __ballot_sync(0xffffffffu, good);
-        }
-      };
-      load_pages(0);
-      look_up(0);
-      load_pages(1);
+      constexpr int THREADS = C::CONVERT * 32, CHUNKS = COPY_KEYS * DH / 16 / THREADS;    // 16-byte chunks of codes per thread and copy
+      static_assert(KEYS == COPY_KEYS, "one copy per tile");
+      const int tid = threadIdx.x - C::FIRST_CONVERT * 32;
+      // Which row and 16-byte chunk of codes a thread takes: eight neighbouring threads read and write without bank conflicts.
+      // head_dim 64: two rows of four chunks.  head_dim 128: four chunks of the rows r and r ^ 5, which differ in the bit that decides
+      // between the halves of the swizzled row of codes and in the lowest, which decides between the even and the odd chunks of the
+      // converted row.
+      const int row0 = DH == 128 ? (tid >> 6) * 8 + (tid & 4 ? (tid >> 3 & 3) ^ 5 : tid >> 3 & 3) : tid >> 2;
+      const int chunk = DH == 128 ? (tid >> 5 & 1) * 4 + (tid & 3) : tid & 3;
+      const int from = row0 * DH + ((DH == 128 ? chunk ^ (row0 & 7) : chunk) << 4);
+      const int to0 = (chunk >> 2) * KV_PANEL + row0 * 128 + (((2 * (chunk & 3)) ^ (row0 & 7)) << 4), to1 = to0 ^ 16;
+      constexpr int STEP = THREADS * 16 / DH;          // rows between a thread's chunks: a multiple of 8
+      static_assert(STEP % 8 == 0, "the swizzle repeats");
       bool ok = true;
       for (int n = 0; n < 2 * n_j && ok; ++n) {        // K_0, V_0, K_1, ...
-        const int st = n % SLOTS, sr = n % RAW, j = n >> 1;
-        if (n >= SLOTS) ok = mbar_wait(&s.bar_empty[st], ((n / SLOTS) - 1) & 1, abortp, p.status, 47);
-        if (!ok) break;
-        if ((n & 1) == 0) {
-          auto& meta = s.meta[j % META];               // behind the wait, see META
-#pragma unroll
-          for (int i = 0; i < EACH; ++i) {
-            const int key = tid + i * THREADS;
-            if (key < KEYS) {
-              const float vs = positive_scale(v_scale[i]);
-              meta.ks_lv[key >> 1][key & 1] = k_scale[i] * a.scale_log2;
-              meta.ks_lv[key >> 1][2 + (key & 1)] = lg2(vs);
-              meta.iv[key] = __frcp_rn(vs);
-              if (lane == 0) meta.there[key >> 5] = there[i];
-            }
-          }
-          look_up(j + 1);
-          load_pages(j + 2);
-        }
+        const int st = n % SLOTS, sr = n % RAW;
         ok = mbar_wait(&s.bar_raw_full[sr], (n / RAW) & 1, abortp, p.status, 48);
         if (!ok) break;
+        uint4 raw[CHUNKS];
 #pragma unroll
-        for (int i0 = 0; i0 < CHUNKS; i0 += 2) {
-          uint4 raw[2];
+        for (int i = 0; i < CHUNKS; ++i) raw[i] = *reinterpret_cast<const uint4*>(s.raw[sr] + from + i * STEP * DH);
+        if (n >= SLOTS) ok = mbar_wait(&s.bar_empty[st], ((n / SLOTS) - 1) & 1, abortp, p.status, 47);
+        if (!ok) break;
 #pragma unroll
-          for (int i = 0; i < 2; ++i) raw[i] = *reinterpret_cast<const uint4*>(s.raw[sr] + ((i0 + i) * THREADS + tid) * 16);
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int id = (i0 + i) * THREADS + tid, row = id / (DH / 16), c = id % (DH / 16);
-            uint32_t x[8];
-            codes_to_16<TYPE>(raw[i].x, x[0], x[1]);
-            codes_to_16<TYPE>(raw[i].y, x[2], x[3]);
-            codes_to_16<TYPE>(raw[i].z, x[4], x[5]);
-            codes_to_16<TYPE>(raw[i].w, x[6], x[7]);
-            uint8_t* dst = s.kv[st] + (c >> 2) * KV_PANEL + row * 128;
-            *reinterpret_cast<uint4*>(dst + (((2 * (c & 3)) ^ (row & 7)) << 4)) = make_uint4(x[0], x[1], x[2], x[3]);
-            *reinterpret_cast<uint4*>(dst + (((2 * (c & 3) + 1) ^ (row & 7)) << 4)) = make_uint4(x[4], x[5], x[6], x[7]);
-          }
+        for (int i = 0; i < CHUNKS; ++i) {
+          uint32_t x[8];
+          codes_to_16<TYPE>(raw[i].x, x[0], x[1]);
+          codes_to_16<TYPE>(raw[i].y, x[2], x[3]);
+          codes_to_16<TYPE>(raw[i].z, x[4], x[5]);
+          codes_to_16<TYPE>(raw[i].w, x[6], x[7]);
+          *reinterpret_cast<uint4*>(s.kv[st] + to0 + i * STEP * 128) = make_uint4(x[0], x[1], x[2], x[3]);
+          *reinterpret_cast<uint4*>(s.kv[st] + to1 + i * STEP * 128) = make_uint4(x[4], x[5], x[6], x[7]);
         }
         fence_proxy_async();
         __syncwarp();
@@ -312,11 +280,6 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
         }
       }
     }
-  };
-
-  if (warp >= 12) {
-    release_registers<C::WIDE>();
-    convert();
   } else if (warp >= 8) {
     release_registers<C::ISSUE>();
     if (warp == 8) {
@@ -331,8 +294,10 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
         auto issue_s = [&](int g, int n) {   // n: index of K_j in the slot sequence
           const uint64_t da = kmajor + (q16 + g * (Q_BYTES >> 4)), db = kmajor + (kv16 + (n % SLOTS) * (KV_BYTES >> 4));
 #pragma unroll
-          for (int kk = 0; kk < DH / 16; ++kk)
-            mma_bf16(tmem + g * KEYS, da + ((kk >> 2) * (Q_PANEL >> 4) + (kk & 3) * 2), db + ((kk >> 2) * (KV_PANEL >> 4) + (kk & 3) * 2), idesc_s, kk);
+          for (int kk = 0; kk < DH / 16; ++kk) {
+            if (C::Q_IN_TMEM) mma_ts(tmem + g * KEYS, tmem + 2 * KEYS + 2 * DH + g * (DH / 2) + kk * 8, db + ((kk >> 2) * (KV_PANEL >> 4) + (kk & 3) * 2), idesc_s, kk);
+            else mma_bf16(tmem + g * KEYS, da + ((kk >> 2) * (Q_PANEL >> 4) + (kk & 3) * 2), db + ((kk >> 2) * (KV_PANEL >> 4) + (kk & 3) * 2), idesc_s, kk);
+          }
           mma_commit(&s.bar_s[g]);
         };
         auto wait_full = [&](int n) { return mbar_wait(&s.bar_full[n % SLOTS], (n / SLOTS) & 1, abortp, p.status, 41); };
@@ -341,7 +306,7 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
           fence_after_sync();
 #pragma unroll 1
           for (int g = 0; g < 2; ++g)
-            if (n_kv[g] > 0) issue_s(g, 0);
+            if ((g == 0 ? n_kv0 : n_kv1) > 0) issue_s(g, 0);
           mma_commit(&s.bar_empty[0]);
         }
         for (int j = 0; j < n_j && ok; ++j) {
@@ -350,7 +315,8 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
           ok = wait_full(nv) && (E4M3 || mbar_wait(&s.bar_clean[nv % SLOTS], (nv / SLOTS) & 1, abortp, p.status, 51)) && (!next_k || wait_full(nk));
 #pragma unroll 1
           for (int g = 0; g < 2 && ok; ++g) {
-            if (j >= n_kv[g]) continue;
+            const int n_g = g == 0 ? n_kv0 : n_kv1;
+            if (j >= n_g) continue;
             ok = mbar_wait(&s.bar_p[g], j & 1, abortp, p.status, 43);
             if (!ok) break;
             fence_after_sync();
@@ -358,7 +324,7 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
 #pragma unroll
             for (int kk = 0; kk < KEYS / 16; ++kk)
               mma_ts(tmem + 2 * KEYS + g * DH, tmem + g * KEYS + kk * 8, db + 128 * kk, idesc_o, (j > 0 || kk > 0) ? 1u : 0u);
-            if (j + 1 == n_kv[g]) mma_commit(&s.bar_o[g]);
+            if (j + 1 == n_g) mma_commit(&s.bar_o[g]);
             else issue_s(g, nk);
           }
           if (ok) {
@@ -421,7 +387,40 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
         page = next;
       }
     } else if (E4M3) {
-      if (warp >= C::FIRST_CONVERT) convert();
+      // ====================================================================== scales and presence of the keys, one thread per key
+      const int key = threadIdx.x - 320;               // 0 .. 63
+      const int* table = p.table + (int64_t)b * p.table_stride;
+      auto load_page = [&](int j) {
+        const int pos = k0 + j * KEYS + key;
+        return j < n_j && pos < k_end ? __ldg(table + (pos >> a.page_shift)) : -1;
+      };
+      float k_scale, v_scale;
+      bool good;
+      auto look_up = [&](int j, int page) {
+        good = page >= 0 && page < p.num_pages;
+        const int slot = good ? (page * p.kv_heads + kh) * p.page_size + ((k0 + j * KEYS + key) & (p.page_size - 1)) : 0;
+        k_scale = good ? __ldg(p.k_scale + slot) : 0.f;
+        v_scale = good ? __ldg(p.v_scale + slot) : 0.f;
+      };
+      look_up(0, load_page(0));
+      int page = load_page(1);
+      bool ok = true;
+      for (int j = 0; j < n_j && ok; ++j) {
+        const int n = 2 * j, st = n % SLOTS;
+        if (n >= SLOTS) ok = mbar_wait(&s.bar_empty[st], ((n / SLOTS) - 1) & 1, abortp, p.status, 49);   // see META
+        if (!ok) break;
+        auto& meta = s.meta[j % META];
+        const float vs = positive_scale(v_scale);
+        const uint32_t there = __ballot_sync(0xffffffffu, good);
+        meta.ks_lv[key >> 1][key & 1] = k_scale * a.scale_log2;
+        meta.ks_lv[key >> 1][2 + (key & 1)] = lg2(vs);
+        meta.iv[key] = __frcp_rn(vs);
+        if (lane == 0) meta.there[key >> 5] = there;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s.bar_full[st]);
+        look_up(j + 1, page);
+        page = load_page(j + 2);
+      }
     } else if (warp == 10) {
       // ====================================================================== rows of V that belong to no key: 0 * NaN is NaN
       // (codes become finite values whatever they are)
@@ -450,23 +449,36 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     claim_registers<C::SOFTMAX>();
     const int g = warp >> 2, quarter = warp & 3;
     const int row = quarter * 32 + lane;             // of the tile
-    // queries: 16-byte chunks of the warp's 32 rows, neighbouring lanes on neighbouring chunks, into the swizzled tile
-    for (int i = lane; i < 32 * (DH / 8); i += 32) {
-      const int rr = quarter * 32 + i / (DH / 8), c = i % (DH / 8);
-      const int at = g * ROWS + rr;
-      uint4 x = make_uint4(0, 0, 0, 0);
-      if (at < n_rows) {
-        const int tok = (local + at) / a.group, head = kh * a.group + (local + at) % a.group;
-        x = __ldg(reinterpret_cast<const uint4*>((const T*)a.q + (int64_t)(r.x + tok) * a.q_stride + head * DH) + c);
+    const bool live = g * ROWS + row < n_rows;
+    if constexpr (C::Q_IN_TMEM) {   // a thread's row into its lane, two elements per column
+      const int at = local + g * ROWS + row;
+      const T* src = (const T*)a.q + (int64_t)(r.x + (live ? at / a.group : 0)) * a.q_stride + (kh * a.group + (live ? at % a.group : 0)) * DH;
+#pragma unroll
+      for (int c = 0; c < DH / 32; ++c) {
+        uint4 x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = live ? __ldg(reinterpret_cast<const uint4*>(src) + c * 4 + e) : make_uint4(0, 0, 0, 0);
+        tmem_st_32x16(tmem + ((uint32_t)(quarter * 32) << 16) + 2 * KEYS + 2 * DH + g * (DH / 2) + c * 16, reinterpret_cast<const uint32_t*>(x));
       }
-      *reinterpret_cast<uint4*>(s.q[g] + (c >> 3) * Q_PANEL + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = x;
+      tmem_st_wait();
+      fence_before_sync();
+    } else {   // 16-byte chunks of the warp's 32 rows, neighbouring lanes on neighbouring chunks, into the swizzled tile
+      for (int i = lane; i < 32 * (DH / 8); i += 32) {
+        const int rr = quarter * 32 + i / (DH / 8), c = i % (DH / 8);
+        const int at = g * ROWS + rr;
+        uint4 x = make_uint4(0, 0, 0, 0);
+        if (at < n_rows) {
+          const int tok = (local + at) / a.group, head = kh * a.group + (local + at) % a.group;
+          x = __ldg(reinterpret_cast<const uint4*>((const T*)a.q + (int64_t)(r.x + tok) * a.q_stride + head * DH) + c);
+        }
+        *reinterpret_cast<uint4*>(s.q[g] + (c >> 3) * Q_PANEL + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = x;
+      }
+      fence_proxy_async();
     }
-    fence_proxy_async();
     __syncwarp();
     if (lane == 0) mbar_arrive(&s.bar_q);
 
-    const int mine = g == 0 ? n_kv[0] : n_kv[1];
-    const bool live = g * ROWS + row < n_rows;
+    const int mine = g == 0 ? n_kv0 : n_kv1;
     const uint32_t t_s = tmem + ((uint32_t)(quarter * 32) << 16) + g * KEYS;   // P too
     const uint32_t t_o = tmem + ((uint32_t)(quarter * 32) << 16) + 2 * KEYS + g * DH;
     auto rescale = [&](float keep) {
@@ -754,7 +766,7 @@ static int launch_tiles(const AttnArgs& a, cudaStream_t st) {
   for (int v = 0; v < 2; ++v) {
     const CUresult rc = fn(&map[v], E4M3 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : TYPE == LBI_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
                            v ? a.b.v : a.b.k, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                           E4M3 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                           E4M3 && DH == 64 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (rc != CUDA_SUCCESS) return 1000 + (int)rc;
   }
