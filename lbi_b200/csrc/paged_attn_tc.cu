@@ -11,10 +11,13 @@
 // when it has grown by more than 2^8: P stays in (0, 2^8], and O is rescaled (a read and a write of TMEM) in the first tiles only.
 // While one warpgroup computes exponentials the tensor core works for the other.
 //
-// What bounds it: the chain S -> maximum -> exponentials -> P -> products of a row tile, of which two (head_dim 128) or four
-// (head_dim 64: two blocks per SM, 256 columns of TMEM each) run at a time.  The special-function unit would be the next bound (16
+// What bounds it: the chain S -> maximum -> exponentials -> P -> products of a row tile, of which two (or, with 16-bit pages at head_dim
+// 64, four: two blocks per SM, 256 columns of TMEM each) run at a time.  The special-function unit would be the next bound (16
 // exponentials per clock and SM: 1024 cycles per 128 x 128 tile, as long as the products take at head_dim 128), so a part of the
-// exponentials is computed by a polynomial on the FMA units.
+// exponentials is computed by a polynomial on the FMA units.  Measured on a B200 with 2368 new tokens over 8192 keys, 32 heads on 8:
+// head_dim 128 fp16 pages 231 us, 1170 TFLOP/s (0.71 of the measured bf16 product rate), e4m3 314 us, 866 TFLOP/s; head_dim 64 200 us,
+// 680 TFLOP/s, and 283 us.  Two warpgroups per row tile, each with half of the columns, were slower (261 us at head_dim 128): the
+// exchange of the maxima costs more than the shorter chain gives.
 //
 // Keys and values: 16-bit pages come by TMA, one box per page and 64 columns (128-byte swizzle), the ids of a tile's pages read one
 // tile ahead, a lane per page.  Slots behind the context and pages that do not exist are masked out of S, and their rows of V are
@@ -34,34 +37,34 @@ namespace paged {
 
 using namespace tc;
 
-#ifndef POLY_PAIRS
-#define POLY_PAIRS 3
-#define POLY_PAIRS_E4M3 0
-#endif
 constexpr int ROWS = 128;                  // rows of a tile
 constexpr int COPY_KEYS = 64;              // keys of one copy of codes
 
 template <bool E4M3, int DH>
 struct TcConfig {
   static constexpr int BLOCKS = DH == 64 && !E4M3 ? 2 : 1;        // per SM
-  static constexpr int KEYS = DH == 64 || E4M3 ? 64 : 128;        // of a tile
-  static constexpr int SLOTS = E4M3 ? 10 : DH == 64 ? 6 : 4;       // K_0, V_0, K_1, V_1, ...
+  static constexpr int KEYS = DH == 64 && !E4M3 ? 64 : 128;       // of a tile
+  static constexpr int SLOTS = DH == 128 ? 4 : E4M3 ? 8 : 6;      // K_0, V_0, K_1, V_1, ...
   // Masks and scales of a key tile: K_j is stored when S_(j - SLOTS / 2) is complete, which follows the softmax of the tile before
   // that one, so SLOTS / 2 + 2 entries never meet one that is still read.
   static constexpr int META = SLOTS / 2 + 2;
-  static constexpr int RAW = E4M3 ? 6 : 1;                         // copies of codes on their way to the converting warps
-  // warps 0-3, 4-7 softmax; 8 products; 9 copies; 16-bit pages: 10 clears V; e4m3: 10 and 11 scales, 12-19 conversion
-  static constexpr int CONVERT = E4M3 ? 8 : 0, FIRST_CONVERT = 12;
+  static constexpr int RAW = E4M3 ? (DH == 128 ? 3 : 6) : 1;        // copies of codes on their way to the converting warps
+  // warps 0-3, 4-7 softmax; 8 products; 9 copies; 16-bit pages: 10 clears V; e4m3: 10 and 11 scales, 12-15 conversion
+  static constexpr int CONVERT = E4M3 ? 4 : 0, FIRST_CONVERT = 12;
   static constexpr int THREADS = 384 + CONVERT * 32;
   // Registers at launch and of the warpgroups afterwards (softmax, warps 8-11, conversion): claimed ones come from those that the
   // block was launched with and others have released, so the shares add up to at most threads x LAUNCH.
-  static constexpr int LAUNCH = E4M3 ? 96 : DH == 64 ? 80 : 168;
-  static constexpr int SOFTMAX = E4M3 ? 160 : DH == 64 ? 96 : 224, ISSUE = E4M3 || DH == 64 ? 48 : 56, WIDE = 56;
+  static constexpr int LAUNCH = E4M3 ? 128 : DH == 64 ? 80 : 168;
+  static constexpr int SOFTMAX = E4M3 ? 200 : DH == 64 ? 96 : 224, ISSUE = E4M3 || DH == 64 ? 48 : 56, WIDE = 64;
   static_assert(256 * SOFTMAX + 128 * ISSUE + CONVERT * 32 * WIDE <= THREADS * LAUNCH, "register shares");
   static constexpr int TMEM = DH == 64 && !E4M3 ? 256 : 512;
-  // e4m3: Q is read from TMEM, too.  Shared memory is what runs short there (the conversion writes 2 bytes per code, the softmax reads
-  // scales), and Q is the larger operand of S.
-  static constexpr bool Q_IN_TMEM = E4M3;
+  // Of every 8 pairs of exponentials so many by the polynomial.  Measured at 0 / 2 / 3 / 4, 2368 tokens over 8192 keys, 32 heads:
+  // head_dim 128 261 / 232 / 229 / 235 us, head_dim 64 206 / 201 / 217 / 224 us.  e4m3: none; the conversion takes the issue slots (2:
+  // 464 against 314 us).
+  static constexpr int POLY = E4M3 ? 0 : DH == 64 ? 2 : 3;
+  // e4m3, where the columns suffice: Q is read from TMEM, too.  Shared memory is what runs short there (the conversion writes 2 bytes
+  // per code, the softmax reads scales).
+  static constexpr bool Q_IN_TMEM = E4M3 && DH == 64;
   static_assert(2 * KEYS + 2 * DH + (Q_IN_TMEM ? DH : 0) <= TMEM, "columns");
 };
 
@@ -75,7 +78,7 @@ struct alignas(16) KeyMeta {
 template <bool E4M3, int DH>
 struct TcSmem {
   using C = TcConfig<E4M3, DH>;
-  alignas(1024) uint8_t q[C::Q_IN_TMEM ? 1 : 2][C::Q_IN_TMEM ? 16 : ROWS * DH * 2];
+  alignas(1024) uint8_t q[2][C::Q_IN_TMEM ? 512 : ROWS * DH * 2];
   alignas(1024) uint8_t kv[C::SLOTS][C::KEYS * DH * 2];
   alignas(1024) uint8_t raw[C::RAW][E4M3 ? COPY_KEYS * DH : 16];
   KeyMeta<E4M3 ? C::KEYS : 4> meta[C::META];
@@ -112,17 +115,23 @@ __device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t* r)
       : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-// 16 lanes x 64 columns: thread t gets, for every 8 columns, columns 2 (t % 4) and + 1 of rows t / 4 and t / 4 + 8.
-__device__ __forceinline__ void tmem_ld_16x64(uint32_t taddr, uint32_t* r) {
+// 16 lanes x 128 columns: thread t gets, for every 8 columns, columns 2 (t % 4) and + 1 of rows t / 4 and t / 4 + 8.
+__device__ __forceinline__ void tmem_ld_16x128(uint32_t taddr, uint32_t* r) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.16x256b.x8.b32 {"
+      "tcgen05.ld.sync.aligned.16x256b.x16.b32 {"
       "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31 "
-      "}, [%32];"
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, "
+      "%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, "
+      "%48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63 "
+      "}, [%64];"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
         "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
         "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
+        "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
+        "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
+        "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
+        "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
       : "r"(taddr)
       : "memory");
 }
@@ -240,7 +249,6 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     release_registers<C::WIDE>();
     if constexpr (E4M3) {
       constexpr int THREADS = C::CONVERT * 32, CHUNKS = COPY_KEYS * DH / 16 / THREADS;    // 16-byte chunks of codes per thread and copy
-      static_assert(KEYS == COPY_KEYS, "one copy per tile");
       const int tid = threadIdx.x - C::FIRST_CONVERT * 32;
       // Which row and 16-byte chunk of codes a thread takes: eight neighbouring threads read and write without bank conflicts.
       // head_dim 64: two rows of four chunks.  head_dim 128: four chunks of the rows r and r ^ 5, which differ in the bit that decides
@@ -254,30 +262,34 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
       static_assert(STEP % 8 == 0, "the swizzle repeats");
       bool ok = true;
       for (int n = 0; n < 2 * n_j && ok; ++n) {        // K_0, V_0, K_1, ...
-        const int st = n % SLOTS, sr = n % RAW;
-        ok = mbar_wait(&s.bar_raw_full[sr], (n / RAW) & 1, abortp, p.status, 48);
-        if (!ok) break;
-        uint4 raw[CHUNKS];
+        const int st = n % SLOTS;
+        for (int half = 0; half < KEYS / COPY_KEYS && ok; ++half) {
+          const int nr = n * (KEYS / COPY_KEYS) + half, sr = nr % RAW;
+          ok = mbar_wait(&s.bar_raw_full[sr], (nr / RAW) & 1, abortp, p.status, 48);
+          if (!ok) break;
+          uint4 raw[CHUNKS];
 #pragma unroll
-        for (int i = 0; i < CHUNKS; ++i) raw[i] = *reinterpret_cast<const uint4*>(s.raw[sr] + from + i * STEP * DH);
-        if (n >= SLOTS) ok = mbar_wait(&s.bar_empty[st], ((n / SLOTS) - 1) & 1, abortp, p.status, 47);
-        if (!ok) break;
+          for (int i = 0; i < CHUNKS; ++i) raw[i] = *reinterpret_cast<const uint4*>(s.raw[sr] + from + i * STEP * DH);
+          if (half == 0 && n >= SLOTS) ok = mbar_wait(&s.bar_empty[st], ((n / SLOTS) - 1) & 1, abortp, p.status, 47);
+          if (!ok) break;
+          uint8_t* to = s.kv[st] + half * COPY_KEYS * 128;
 #pragma unroll
-        for (int i = 0; i < CHUNKS; ++i) {
-          uint32_t x[8];
-          codes_to_16<TYPE>(raw[i].x, x[0], x[1]);
-          codes_to_16<TYPE>(raw[i].y, x[2], x[3]);
-          codes_to_16<TYPE>(raw[i].z, x[4], x[5]);
-          codes_to_16<TYPE>(raw[i].w, x[6], x[7]);
-          *reinterpret_cast<uint4*>(s.kv[st] + to0 + i * STEP * 128) = make_uint4(x[0], x[1], x[2], x[3]);
-          *reinterpret_cast<uint4*>(s.kv[st] + to1 + i * STEP * 128) = make_uint4(x[4], x[5], x[6], x[7]);
+          for (int i = 0; i < CHUNKS; ++i) {
+            uint32_t x[8];
+            codes_to_16<TYPE>(raw[i].x, x[0], x[1]);
+            codes_to_16<TYPE>(raw[i].y, x[2], x[3]);
+            codes_to_16<TYPE>(raw[i].z, x[4], x[5]);
+            codes_to_16<TYPE>(raw[i].w, x[6], x[7]);
+            *reinterpret_cast<uint4*>(to + to0 + i * STEP * 128) = make_uint4(x[0], x[1], x[2], x[3]);
+            *reinterpret_cast<uint4*>(to + to1 + i * STEP * 128) = make_uint4(x[4], x[5], x[6], x[7]);
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&s.bar_raw_empty[sr]);
         }
+        if (!ok) break;
         fence_proxy_async();
         __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&s.bar_raw_empty[sr]);
-          mbar_arrive(&s.bar_full[st]);
-        }
+        if (lane == 0) mbar_arrive(&s.bar_full[st]);
       }
     }
   } else if (warp >= 8) {
@@ -335,8 +347,9 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
       }
     } else if (warp == 9) {
       // ====================================================================== TMA producer: one lane per page
-      const int box = min(p.page_size, KEYS);    // rows of a copy: a page, or a tile's part of it
-      const int per = KEYS / box;                // copies of a tile, 1 .. 16
+      constexpr int COPY = E4M3 ? COPY_KEYS : KEYS, COPIES = KEYS / COPY, RING = E4M3 ? RAW : SLOTS;   // keys of a ring entry
+      const int box = min(p.page_size, COPY);    // rows of a box: a page, or an entry's part of it
+      const int per = KEYS / box;                // boxes of a tile, 1 .. 16
       const int* table = p.table + (int64_t)b * p.table_stride;
       auto load_page = [&](int j) {
         const int pos = k0 + j * KEYS + lane * box;
@@ -350,36 +363,36 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
         const bool wanted = lane < per && pos < k_end;
         const bool good = wanted && page >= 0 && page < p.num_pages;
         if (wanted && !good && p.status) atomicCAS(p.status, 0, 84);
-        const uint32_t pages = __ballot_sync(0xffffffffu, good);
+        const uint32_t boxes = __ballot_sync(0xffffffffu, good);
         const int row = (max(page, 0) * p.kv_heads + kh) * p.page_size + (pos & (p.page_size - 1));
-        const uint32_t bytes = __popc(pages) * (uint32_t)box * DH * (E4M3 ? 1 : 2);
-#pragma unroll
-        for (int v = 0; v < 2 && ok; ++v) {
-          const int n = 2 * j + v, ring = E4M3 ? RAW : SLOTS, st = n % ring;
+        for (int i = 0; i < 2 * COPIES && ok; ++i) {
+          const int v = i / COPIES, n = 2 * COPIES * j + i, st = n % RING;
           uint64_t* full = E4M3 ? &s.bar_raw_full[st] : &s.bar_full[st];
-          if (n >= ring) ok = mbar_wait(E4M3 ? &s.bar_raw_empty[st] : &s.bar_empty[st], ((n / ring) - 1) & 1, abortp, p.status, 44);
+          if (n >= RING) ok = mbar_wait(E4M3 ? &s.bar_raw_empty[st] : &s.bar_empty[st], ((n / RING) - 1) & 1, abortp, p.status, 44);
           if (!ok) break;
           if (!E4M3 && v == 0 && lane < 4) {
             uint32_t there = 0;
-            if (lane >= KEYS / 32 || (pages == (1u << per) - 1u && base + KEYS <= k_end)) {
+            if (lane >= KEYS / 32 || (boxes == (1u << per) - 1u && base + KEYS <= k_end)) {
               there = 0xffffffffu;
             } else {
-              for (int i = 0; i < 32; ++i) {
-                const int key = lane * 32 + i;
-                if ((pages >> (key / box) & 1u) && base + key < k_end) there |= 1u << i;
+              for (int e = 0; e < 32; ++e) {
+                const int key = lane * 32 + e;
+                if ((boxes >> (key / box) & 1u) && base + key < k_end) there |= 1u << e;
               }
             }
             s.meta[j % META].there[lane] = there;
           }
-          __syncwarp();
+          const int at = lane * box - (i % COPIES) * COPY;   // row in the entry
+          const bool here = good && at >= 0 && at < COPY;
+          const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, here)) * (uint32_t)box * DH * (E4M3 ? 1 : 2);
           if (lane == 0) mbar_arrive_expect_tx(full, bytes);
           __syncwarp();
-          if (good) {
+          if (here) {
             if (E4M3) {
-              tma_load_2d(s.raw[st] + lane * box * DH, v ? &map_v : &map_k, full, 0, row);
+              tma_load_2d(s.raw[st] + at * DH, v ? &map_v : &map_k, full, 0, row);
             } else {
 #pragma unroll
-              for (int c = 0; c < PANELS; ++c) tma_load_2d(s.kv[st] + c * KV_PANEL + lane * box * 128, v ? &map_v : &map_k, full, c * 64, row);
+              for (int c = 0; c < PANELS; ++c) tma_load_2d(s.kv[st] + c * KV_PANEL + at * 128, v ? &map_v : &map_k, full, c * 64, row);
             }
           }
           __syncwarp();
@@ -387,39 +400,52 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
         page = next;
       }
     } else if (E4M3) {
-      // ====================================================================== scales and presence of the keys, one thread per key
-      const int key = threadIdx.x - 320;               // 0 .. 63
+      // ====================================================================== scales and presence of the keys, two per thread
+      constexpr int EACH = KEYS / 64;
+      const int key0 = threadIdx.x - 320;              // 0 .. 63
       const int* table = p.table + (int64_t)b * p.table_stride;
-      auto load_page = [&](int j) {
-        const int pos = k0 + j * KEYS + key;
-        return j < n_j && pos < k_end ? __ldg(table + (pos >> a.page_shift)) : -1;
+      int page[EACH];
+      float k_scale[EACH], v_scale[EACH];
+      bool good[EACH];
+      auto load_pages = [&](int j) {
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+          const int pos = k0 + j * KEYS + key0 + i * 64;
+          page[i] = j < n_j && pos < k_end ? __ldg(table + (pos >> a.page_shift)) : -1;
+        }
       };
-      float k_scale, v_scale;
-      bool good;
-      auto look_up = [&](int j, int page) {
-        good = page >= 0 && page < p.num_pages;
-        const int slot = good ? (page * p.kv_heads + kh) * p.page_size + ((k0 + j * KEYS + key) & (p.page_size - 1)) : 0;
-        k_scale = good ? __ldg(p.k_scale + slot) : 0.f;
-        v_scale = good ? __ldg(p.v_scale + slot) : 0.f;
+      auto look_up = [&](int j) {
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+          good[i] = page[i] >= 0 && page[i] < p.num_pages;
+          const int slot = good[i] ? (page[i] * p.kv_heads + kh) * p.page_size + ((k0 + j * KEYS + key0 + i * 64) & (p.page_size - 1)) : 0;
+          k_scale[i] = good[i] ? __ldg(p.k_scale + slot) : 0.f;
+          v_scale[i] = good[i] ? __ldg(p.v_scale + slot) : 0.f;
+        }
       };
-      look_up(0, load_page(0));
-      int page = load_page(1);
+      load_pages(0);
+      look_up(0);
+      load_pages(1);
       bool ok = true;
       for (int j = 0; j < n_j && ok; ++j) {
         const int n = 2 * j, st = n % SLOTS;
         if (n >= SLOTS) ok = mbar_wait(&s.bar_empty[st], ((n / SLOTS) - 1) & 1, abortp, p.status, 49);   // see META
         if (!ok) break;
         auto& meta = s.meta[j % META];
-        const float vs = positive_scale(v_scale);
-        const uint32_t there = __ballot_sync(0xffffffffu, good);
-        meta.ks_lv[key >> 1][key & 1] = k_scale * a.scale_log2;
-        meta.ks_lv[key >> 1][2 + (key & 1)] = lg2(vs);
-        meta.iv[key] = __frcp_rn(vs);
-        if (lane == 0) meta.there[key >> 5] = there;
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+          const int key = key0 + i * 64;
+          const float vs = positive_scale(v_scale[i]);
+          const uint32_t there = __ballot_sync(0xffffffffu, good[i]);
+          meta.ks_lv[key >> 1][key & 1] = k_scale[i] * a.scale_log2;
+          meta.ks_lv[key >> 1][2 + (key & 1)] = lg2(vs);
+          meta.iv[key] = __frcp_rn(vs);
+          if (lane == 0) meta.there[key >> 5] = there;
+        }
         __syncwarp();
         if (lane == 0) mbar_arrive(&s.bar_full[st]);
-        look_up(j + 1, page);
-        page = load_page(j + 2);
+        look_up(j + 1);
+        load_pages(j + 2);
       }
     } else if (warp == 10) {
       // ====================================================================== rows of V that belong to no key: 0 * NaN is NaN
@@ -515,7 +541,7 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
         lr[k] = 0.f;
       }
       constexpr int N = KEYS / 8;
-      static_assert(N == 8, "one load per 16 lanes");
+      static_assert(N == 16, "one load per 16 lanes");
       for (int j = 0; j < mine; ++j) {
         ok = mbar_wait(&s.bar_s[g], j & 1, abortp, p.status, 45);
         if (!ok) break;
@@ -526,7 +552,7 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
           float2 f2[2][N][2];
         } x;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) tmem_ld_16x64(t_s + ((uint32_t)(16 * h) << 16), x.w[h]);
+        for (int h = 0; h < 2; ++h) tmem_ld_16x128(t_s + ((uint32_t)(16 * h) << 16), x.w[h]);
         tmem_ld_wait();
 #pragma unroll
         for (int n = 0; n < N; ++n) {
@@ -535,7 +561,7 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
           for (int k = 0; k < 4; ++k) x.f2[k >> 1][n][k & 1] = fma2(x.f2[k >> 1][n][k & 1], make_float2(f.x, f.y), make_float2(f.z, f.w));
         }
         const int base = k0 + j * KEYS;
-        const bool masked = __any_sync(0xffffffffu, (meta.there[0] & meta.there[1]) != 0xffffffffu ||
+        const bool masked = __any_sync(0xffffffffu, (meta.there[0] & meta.there[1] & meta.there[2] & meta.there[3]) != 0xffffffffu ||
                                                         min(min(lim[0], lim[1]), min(lim[2], lim[3])) - base < KEYS - 1);
         if (masked) {
 #pragma unroll
@@ -579,26 +605,28 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
           }
           if (j > 0) rescale(row_keep);
         }
-        auto exponentials = [&](auto by_polynomial) {
+        float2 neg[4];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
+        for (int k = 0; k < 4; ++k) {
+          const float ref = mr[k] == -INFINITY ? 0.f : mr[k];
+          neg[k] = make_float2(-ref, -ref);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int n0 = 0; n0 < N; n0 += 8) {
             uint32_t w[16];
 #pragma unroll
-            for (int n = 0; n < N; ++n)
+            for (int n = 0; n < 8; ++n)
 #pragma unroll
               for (int k = 0; k < 2; ++k) {
-                const float ref = mr[2 * h + k] == -INFINITY ? 0.f : mr[2 * h + k];
-                float2& u = x.f2[h][n][k];
-                u = add2(u, make_float2(-ref, -ref));
-                if (decltype(by_polynomial)::value && (2 * n + k) % 8 < POLY_PAIRS_E4M3) u = exp2_by_polynomial<TYPE>(u);
-                else u = make_float2(ex2(u.x), ex2(u.y));
+                float2& u = x.f2[h][n0 + n][k];
+                u = add2(u, neg[2 * h + k]);
+                u = make_float2(ex2(u.x), ex2(u.y));
                 w[2 * n + k] = pack16<TYPE>(u.x, u.y);
               }
-            tmem_st_16x32(t_s + ((uint32_t)(16 * h) << 16), w);
+            tmem_st_16x32(t_s + ((uint32_t)(16 * h) << 16) + n0 * 4, w);
           }
-        };
-        if (masked || POLY_PAIRS_E4M3 == 0) exponentials(std::false_type{});   // 2^-inf is 0 there, the polynomial's smallest value is 2^-126
-        else exponentials(std::true_type{});
         hand_over();
         // the sums are needed by nobody yet: behind the arrival
         float2 sum[4];
@@ -678,7 +706,7 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
             for (int e = 0; e < 16; ++e) {
               float2& u = x.f2[c * 16 + e];
               u = fma2(u, sc, neg);
-              if (decltype(by_polynomial)::value && e % 8 < POLY_PAIRS) u = exp2_by_polynomial<TYPE>(u);
+              if (decltype(by_polynomial)::value && e % 8 < C::POLY) u = exp2_by_polynomial<TYPE>(u);
               else u = make_float2(ex2(u.x), ex2(u.y));
               w[e] = pack16<TYPE>(u.x, u.y);
             }
@@ -762,7 +790,7 @@ static int launch_tiles(const AttnArgs& a, cudaStream_t st) {
   if (!fn) return 801;
   const cuuint64_t dims[2] = {DH, (cuuint64_t)a.b.num_pages * a.b.kv_heads * a.b.page_size};
   const cuuint64_t strides[1] = {E4M3 ? DH : DH * 2};
-  const cuuint32_t box[2] = {E4M3 ? DH : 64, (cuuint32_t)std::min(a.b.page_size, TcConfig<E4M3, DH>::KEYS)}, estr[2] = {1, 1};
+  const cuuint32_t box[2] = {E4M3 ? DH : 64, (cuuint32_t)std::min(a.b.page_size, E4M3 ? COPY_KEYS : TcConfig<E4M3, DH>::KEYS)}, estr[2] = {1, 1};
   for (int v = 0; v < 2; ++v) {
     const CUresult rc = fn(&map[v], E4M3 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : TYPE == LBI_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
                            v ? a.b.v : a.b.k, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
