@@ -49,7 +49,7 @@ lbi_attention_plan lbi_paged_attention_plan(const lbi_paged_batch* p, int type, 
 
 // out [rows, heads * head_dim] = causal attention of the new tokens q (row stride q_stride elements) over the sequences' pages.
 int lbi_paged_attention(const lbi_paged_batch* p, const void* q, int64_t q_stride, void* out, float* part_o, float* part_lse,
-                        lbi_attention_plan plan, int type, int heads, float scale, int zero_tail, cudaStream_t stream);
+                        lbi_attention_plan plan, int type, int heads, float scale, int zero_tail, int sm_count, cudaStream_t stream);
 
 // out fp32 [batch, vocab] from logits [batch, vocab] (row stride, type), the rules of logits.cu.  Null pointers: the scalar is used.
 typedef struct {
@@ -71,7 +71,7 @@ typedef struct {
   float repetition, presence, frequency;
   int type, batch, vocab, history;
 } lbi_logit_rules;
-int lbi_adjust_logits(const lbi_logit_rules* p, cudaStream_t stream);
+int lbi_adjust_logits(const lbi_logit_rules* p, int sm_count, cudaStream_t stream);
 
 #ifdef __cplusplus
 }

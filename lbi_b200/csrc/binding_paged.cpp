@@ -163,13 +163,14 @@ Tensor paged_attention(const Tensor& q_in, const Tensor& k, const Tensor& v, con
   const Tensor q = aligned_rows(packed ? q_in : q_in.contiguous());
   Tensor o = output(out, q.sizes(), q, q.scalar_type(), p.batch == 0);
   const int type = type_of(q, "q");
-  const lbi_attention_plan plan = lbi_paged_attention_plan(&p, type, (int)heads, (float)scale, max_context, at::cuda::getCurrentDeviceProperties()->multiProcessorCount);
+  const int sm_count = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
+  const lbi_attention_plan plan = lbi_paged_attention_plan(&p, type, (int)heads, (float)scale, max_context, sm_count);
   Tensor parts;   // results of the parts of a long context, then the logarithms of their sums
   const int64_t part_rows = q.size(0) * heads * plan.splits;
   if (plan.splits > 1) parts = torch::empty({part_rows * (p.head_dim + 1)}, q.options().dtype(at::kFloat));
   float* part_o = plan.splits > 1 ? parts.data_ptr<float>() : nullptr;
   check(lbi_paged_attention(&p, q.data_ptr(), q.size(0) > 1 ? q.stride(0) : heads * p.head_dim, o.data_ptr(), part_o,
-                            part_o ? part_o + part_rows * p.head_dim : nullptr, plan, type, (int)heads, (float)scale, given(out) ? 0 : 1, cur_stream()),
+                            part_o ? part_o + part_rows * p.head_dim : nullptr, plan, type, (int)heads, (float)scale, given(out) ? 0 : 1, sm_count, cur_stream()),
         "paged_attention");
   return o;
 }
@@ -232,7 +233,7 @@ Tensor adjust_logits(const Tensor& logits, const Tensor& tokens, const OptTensor
   Tensor o = output(out, logits.sizes(), logits, at::kFloat);
   p.out = o.data_ptr<float>();
   p.out_stride = vocab;
-  check(lbi_adjust_logits(&p, cur_stream()), "adjust_logits");
+  check(lbi_adjust_logits(&p, at::cuda::getCurrentDeviceProperties()->multiProcessorCount, cur_stream()), "adjust_logits");
   return o;
 }
 

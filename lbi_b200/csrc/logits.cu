@@ -5,65 +5,106 @@
 //   x = x - presence * [made > 0] - frequency * made + bias;   not allowed -> -inf (whatever the logit was, NaN included)
 //
 // Bound by memory (logits in, fp32 out).  A block owns a tile of the vocabulary of one row: it counts the history's tokens that
-// fall into the tile in shared memory (whole numbers: the order of the atomics does not matter), bit 31 marks a token that occurs
-// in the prompt only.  Every block of a row reads the row's history again, which stays in L2.
+// fall into the tile in shared memory (whole numbers: the order of the atomics does not matter); the count's highest bit marks a token
+// that occurs in the prompt.  Every block of a row reads the row's history again, which stays in L2, so tiles are large: 16-bit counts,
+// two to a word, while the history is shorter than 2^15, else 32-bit counts of half as many tokens.
+#include <algorithm>
+
 #include "paged.cuh"
 
 namespace lbi {
 namespace paged {
 
-constexpr int TILE_V = 4096;
-constexpr int LOGIT_THREADS = 256;
+constexpr int COUNT_BYTES = 32768;
+constexpr int LOGIT_THREADS = 512;
 
-template <int TYPE>
-__global__ void __launch_bounds__(LOGIT_THREADS) logits_kernel(const lbi_logit_rules p) {
+template <int TYPE, typename COUNT>
+__global__ void __launch_bounds__(LOGIT_THREADS) logits_kernel(const lbi_logit_rules p, int tile) {
   using T = typename Elem<TYPE>::T;
-  __shared__ uint32_t count[TILE_V];
-  const int b = blockIdx.y, v0 = blockIdx.x * TILE_V, n = min(TILE_V, p.vocab - v0);
-  for (int i = threadIdx.x; i < TILE_V; i += LOGIT_THREADS) count[i] = 0;
-  __syncthreads();
+  constexpr bool WIDE = sizeof(COUNT) == 4;
+  constexpr uint32_t PROMPT = WIDE ? 0x80000000u : 0x8000u;
+  __shared__ alignas(16) COUNT count[COUNT_BYTES / sizeof(COUNT)];
+  const int b = blockIdx.y, v0 = blockIdx.x * tile, n = min(tile, p.vocab - v0);
+  for (int i = threadIdx.x; i < tile * (int)sizeof(COUNT) / 16; i += LOGIT_THREADS) reinterpret_cast<uint4*>(count)[i] = make_uint4(0, 0, 0, 0);
   const int len = p.lengths ? min(max(p.lengths[b], 0), p.history) : p.history;
   const int prompt = p.prompt_lengths ? p.prompt_lengths[b] : 0;
-  const int64_t* hist = p.tokens + (int64_t)b * p.tokens_stride;
-  for (int i = threadIdx.x; i < len; i += LOGIT_THREADS) {
-    const int64_t t = hist[i] - v0;
-    if (t >= 0 && t < n) {
-      if (i < prompt) atomicOr(&count[t], 0x80000000u);
-      else atomicAdd(&count[t], 1u);
-    }
-  }
-  __syncthreads();
   const float rep = p.repetition_row ? p.repetition_row[b] : p.repetition;
   const float pres = p.presence_row ? p.presence_row[b] : p.presence;
   const float freq = p.frequency_row ? p.frequency_row[b] : p.frequency;
+  const int64_t* hist = p.tokens + (int64_t)b * p.tokens_stride;
+  __syncthreads();
+  for (int i0 = threadIdx.x; i0 < len; i0 += 4 * LOGIT_THREADS) {
+    int64_t t[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) t[e] = i0 + e * LOGIT_THREADS < len ? __ldg(hist + i0 + e * LOGIT_THREADS) - v0 : -1;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (t[e] >= 0 && t[e] < n) {
+        const bool first = i0 + e * LOGIT_THREADS < prompt;
+        uint32_t* word = reinterpret_cast<uint32_t*>(count) + (WIDE ? t[e] : t[e] >> 1);
+        const int shift = WIDE ? 0 : (int)(t[e] & 1) * 16;
+        if (first) atomicOr(word, PROMPT << shift);
+        else atomicAdd(word, 1u << shift);
+      }
+  }
+  __syncthreads();
   const T* x = (const T*)p.logits + (int64_t)b * p.logits_stride + v0;
   float* out = p.out + (int64_t)b * p.out_stride + v0;
   const float* bias = p.bias ? p.bias + (int64_t)b * p.bias_stride + v0 : nullptr;
   const int* allowed = p.allowed ? p.allowed + (int64_t)b * p.allowed_stride + (v0 >> 5) : nullptr;
-  for (int i = threadIdx.x; i < n; i += LOGIT_THREADS) {
-    float f = to_f<T>(x[i]);
-    const uint32_t c = count[i];
-    if (c) {
-      f = f > 0.f ? __fdiv_rn(f, rep) : f * rep;
-      const uint32_t made = c & 0x7fffffffu;
-      if (made) f = __fsub_rn(__fsub_rn(f, pres), __fmul_rn(freq, (float)made));
+  constexpr int EACH = 8;   // rows of odd vocabularies start anywhere, so an element per thread and access, several in flight
+  for (int i0 = threadIdx.x; i0 < n; i0 += EACH * LOGIT_THREADS) {
+    float f[EACH], add[EACH];
+    uint32_t bits[EACH];
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+      const int i = i0 + e * LOGIT_THREADS;
+      f[e] = add[e] = 0.f;
+      bits[e] = 0xffffffffu;
+      if (i < n) {
+        f[e] = to_f<T>(x[i]);
+        if (bias) add[e] = __ldg(bias + i);
+        if (allowed) bits[e] = (uint32_t)__ldg(allowed + (i >> 5));
+      }
     }
-    if (bias) f += bias[i];
-    if (allowed && !((uint32_t)allowed[i >> 5] >> (i & 31) & 1u)) f = -INFINITY;
-    out[i] = f;
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+      const int i = i0 + e * LOGIT_THREADS;
+      if (i >= n) break;
+      const uint32_t c = count[i];
+      if (c) {
+        f[e] = f[e] > 0.f ? __fdiv_rn(f[e], rep) : f[e] * rep;
+        const uint32_t made = c & (PROMPT - 1);
+        if (made) f[e] = __fsub_rn(__fsub_rn(f[e], pres), __fmul_rn(freq, (float)made));
+      }
+      if (bias) f[e] += add[e];
+      if (!(bits[e] >> (i & 31) & 1u)) f[e] = -INFINITY;
+      out[i] = f[e];
+    }
   }
+}
+
+template <int TYPE>
+static void launch_logits(const lbi_logit_rules& p, int sm_count, cudaStream_t st) {
+  // Full tiles, unless they leave SMs without a block: then as many as there are SMs, of 1024 tokens at least.
+  const bool wide = p.history >= 32768;
+  const int most = COUNT_BYTES / (wide ? 4 : 2);
+  const int64_t per_row = std::max<int64_t>(1, sm_count / p.batch);
+  const int tile = (int)std::min<int64_t>(most, std::max<int64_t>(1024, ((p.vocab + per_row - 1) / per_row + 1023) / 1024 * 1024));
+  const dim3 grid((p.vocab + tile - 1) / tile, p.batch);
+  if (wide) logits_kernel<TYPE, uint32_t><<<grid, LOGIT_THREADS, 0, st>>>(p, tile);
+  else logits_kernel<TYPE, uint16_t><<<grid, LOGIT_THREADS, 0, st>>>(p, tile);
 }
 
 }  // namespace paged
 }  // namespace lbi
 
-extern "C" int lbi_adjust_logits(const lbi_logit_rules* p, cudaStream_t st) {
+extern "C" int lbi_adjust_logits(const lbi_logit_rules* p, int sm_count, cudaStream_t st) {
   using namespace lbi::paged;
   if (p->batch == 0 || p->vocab == 0) return 0;
   if (p->batch > 65535 || p->type < 0 || p->type > LBI_F16) return (int)cudaErrorInvalidValue;
-  dim3 grid((p->vocab + TILE_V - 1) / TILE_V, p->batch);
-  if (p->type == LBI_F32) logits_kernel<LBI_F32><<<grid, LOGIT_THREADS, 0, st>>>(*p);
-  else if (p->type == LBI_BF16) logits_kernel<LBI_BF16><<<grid, LOGIT_THREADS, 0, st>>>(*p);
-  else logits_kernel<LBI_F16><<<grid, LOGIT_THREADS, 0, st>>>(*p);
+  if (p->type == LBI_F32) launch_logits<LBI_F32>(*p, sm_count, st);
+  else if (p->type == LBI_BF16) launch_logits<LBI_BF16>(*p, sm_count, st);
+  else launch_logits<LBI_F16>(*p, sm_count, st);
   return (int)cudaGetLastError();
 }

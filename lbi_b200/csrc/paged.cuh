@@ -78,16 +78,26 @@ __device__ __forceinline__ int2 seq_rows(const lbi_paged_batch& p, int b) {
   return make_int2(lo, min(max(__ldg(p.cu + b + 1), lo), p.rows));
 }
 
-// Sequence that row `row` belongs to (the last b with cu[b] <= row), or batch when the row lies behind the last sequence.
-__device__ __forceinline__ int seq_of_row(const lbi_paged_batch& p, int row) {
-  if (!p.cu) return row / (p.rows / p.batch);
-  int lo = 0, hi = p.batch;   // cu[lo] <= row < cu[hi + 1]
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (__ldg(p.cu + mid) <= row) lo = mid;
-    else hi = mid - 1;
+// The last b of [0, n) with below(b), which holds for a first part of them (0 if for none); a full warp calls, 32 candidates are tried
+// at a time.
+template <typename F>
+__device__ __forceinline__ int last_below(int n, F below) {
+  int lo = 0;
+  const int lane = threadIdx.x & 31;
+  while (n > 1) {
+    const int step = (n + 31) >> 5;
+    const bool yes = lane * step < n && below(lo + lane * step);
+    const int hit = max(__popc(__ballot_sync(0xffffffffu, yes)) - 1, 0);
+    n = min(step, n - hit * step);
+    lo += hit * step;
   }
   return lo;
+}
+
+// Sequence that row `row` belongs to; a full warp calls.
+__device__ __forceinline__ int seq_of_row(const lbi_paged_batch& p, int row) {
+  if (!p.cu) return row / (p.rows / p.batch);
+  return last_below(p.batch, [&](int b) { return __ldg(p.cu + b) <= row; });
 }
 
 __device__ __forceinline__ int last_row(const lbi_paged_batch& p) {
@@ -115,19 +125,9 @@ __device__ __forceinline__ int64_t first_tile(const lbi_paged_batch& p, int b, i
 }
 inline int64_t tile_bound(const lbi_paged_batch& p, int group, int per_tile) { return (int64_t)p.rows * group / per_tile + p.batch; }
 
-// Sequence of tile `tile` (the last b with first_tile(b) <= tile); a full warp calls, 32 candidates are read at a time.
+// Sequence of tile `tile`; a full warp calls.
 __device__ __forceinline__ int seq_of_tile(const lbi_paged_batch& p, int64_t tile, int group, int per_tile) {
-  int lo = 0, n = p.batch;
-  const int lane = threadIdx.x & 31;
-  while (n > 1) {
-    const int step = (n + 31) >> 5;
-    const int b = lo + lane * step;
-    const bool below = lane * step < n && first_tile(p, b, group, per_tile) <= tile;
-    const int hit = max(__popc(__ballot_sync(0xffffffffu, below)) - 1, 0);
-    n = min(step, n - hit * step);
-    lo += hit * step;
-  }
-  return lo;
+  return last_below(p.batch, [&](int b) { return first_tile(p, b, group, per_tile) <= tile; });
 }
 
 __device__ __forceinline__ float ex2(float x) {

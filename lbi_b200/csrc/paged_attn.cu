@@ -351,38 +351,75 @@ __global__ void __launch_bounds__(WARPS * 32, 2) attn_rows_kernel(const AttnArgs
   }
 }
 
-// Joins the parts of a context: o = sum_s 2^(lse_s - max) o_s / sum_s 2^(lse_s - max); one warp per (token, head), the parts in
-// their order.
-template <int TYPE>
-__global__ void __launch_bounds__(128) combine_kernel(const AttnArgs a) {
+// Joins the parts of a context: o = sum_s 2^(lse_s - max) o_s / sum_s 2^(lse_s - max).  A group of LANES threads owns a (token, head),
+// four elements each; with SHARE > 1 so many groups share its parts (few rows, many parts), which are then added in their order.
+constexpr int COMBINE_THREADS = 128;
+
+template <int TYPE, int LANES, int SHARE>
+__global__ void __launch_bounds__(COMBINE_THREADS) combine_kernel(const AttnArgs a) {
   using T = typename Elem<TYPE>::T;
+  constexpr int GROUPS = COMBINE_THREADS / LANES, ROWS = GROUPS / SHARE;
+  __shared__ float part[SHARE > 1 ? GROUPS : 1][LANES * 4 + 1];
   const lbi_paged_batch& p = a.b;
-  const int lane = threadIdx.x & 31, dim = p.head_dim;
-  const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (at >= (int64_t)p.rows * a.heads) return;
-  const bool owned = at / a.heads < last_row(p);
-  if (!owned && !a.zero_tail) return;
+  const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES, share = group % SHARE, dim = p.head_dim, d = lane * 4;
+  const int64_t at = (int64_t)blockIdx.x * ROWS + group / SHARE;
+  const bool exists = at < (int64_t)p.rows * a.heads;
+  const bool owned = exists && at / a.heads < last_row(p);
   const float* lse = a.part_lse + at * a.splits;
   float top = -INFINITY;
   if (owned)
-    for (int s = lane; s < a.splits; s += 32) top = fmaxf(top, lse[s]);
-  top = warp_max(top);
+    for (int s = lane; s < a.splits; s += LANES) top = fmaxf(top, lse[s]);
+#pragma unroll
+  for (int o = 1; o < LANES; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   const float ref = top == -INFINITY ? 0.f : top;
-  for (int d = lane * 4; d < dim; d += 128) {
-    float acc[4] = {0.f, 0.f, 0.f, 0.f}, sum = 0.f;
-    for (int s = 0; owned && s < a.splits; ++s) {
-      const float w = ex2(lse[s] - ref);
-      float x[4];
-      load_f<float, 4>(a.part_o + (at * a.splits + s) * dim + d, x);
+  float acc[4] = {0.f, 0.f, 0.f, 0.f}, sum = 0.f;
+  if (owned) {
+#pragma unroll 4
+    for (int s = share; s < a.splits; s += SHARE) {
+      const float w = ex2(__ldg(lse + s) - ref);
+      const float4 x = d < dim ? __ldg(reinterpret_cast<const float4*>(a.part_o + (at * a.splits + s) * dim + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
       sum += w;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[e] += w * x[e];
+      acc[0] += w * x.x;
+      acc[1] += w * x.y;
+      acc[2] += w * x.z;
+      acc[3] += w * x.w;
     }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) acc[e] *= inv;
-    store_f<T, 4>((T*)a.out + at * dim + d, acc);
   }
+  if (SHARE > 1) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) part[group][d + e] = acc[e];
+    if (lane == 0) part[group][LANES * 4] = sum;
+    __syncthreads();
+    if (share == 0) {
+#pragma unroll
+      for (int g = 1; g < SHARE; ++g) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] += part[group + g][d + e];
+        sum += part[group + g][LANES * 4];
+      }
+    }
+  }
+  if (share != 0 || !exists || d >= dim || (!owned && !a.zero_tail)) return;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) acc[e] *= inv;
+  store_f<T, 4>((T*)a.out + at * dim + d, acc);
+}
+
+template <int TYPE>
+int launch_combine(const AttnArgs& a, int sm_count, cudaStream_t st) {
+  // several groups per row where the rows alone give less than two blocks per SM
+  const int64_t rows = (int64_t)a.b.rows * a.heads;
+  const bool few = rows < 2ll * sm_count * 4 && a.splits >= 8;
+  const int lanes = a.b.head_dim <= 32 ? 8 : a.b.head_dim <= 64 ? 16 : a.b.head_dim <= 128 ? 32 : 64;
+  const int64_t per_block = COMBINE_THREADS / lanes / (few ? (lanes == 64 ? 2 : 4) : 1), blocks = (rows + per_block - 1) / per_block;
+  if (blocks >= (1ll << 31)) return (int)cudaErrorInvalidValue;
+#define LBI_COMBINE(L, S) combine_kernel<TYPE, L, S><<<(unsigned)blocks, COMBINE_THREADS, 0, st>>>(a)
+  if (lanes == 8) { if (few) LBI_COMBINE(8, 4); else LBI_COMBINE(8, 1); }
+  else if (lanes == 16) { if (few) LBI_COMBINE(16, 4); else LBI_COMBINE(16, 1); }
+  else { if (few) LBI_COMBINE(32, 4); else LBI_COMBINE(32, 1); }
+#undef LBI_COMBINE
+  return (int)cudaGetLastError();
 }
 
 // ------------------------------------------------------------------------------------------------ one warp per row
@@ -505,12 +542,13 @@ extern "C" lbi_attention_plan lbi_paged_attention_plan(const lbi_paged_batch* p,
     }
     plan.split_keys = (int)std::max<int64_t>(128, ((longest + plan.splits - 1) / plan.splits + 127) / 128 * 128);
   } else {
-    // Parts of equal length, so that a batch of uneven contexts is balanced by the order in which blocks finish: as long as two
-    // blocks per SM are there, at most 2048 keys (the partial results are under 2 % of the bytes read), and not below 256.
-    const int64_t units = tile_bound(*p, group, ROW_TILE) * p->kv_heads;
-    const int64_t wanted = std::max<int64_t>(1, 2 * sm_count / units);
-    int64_t keys = (longest + wanted - 1) / wanted;
-    keys = std::min<int64_t>(2048, std::max<int64_t>(256, (keys + 63) / 64 * 64));
+    // Parts of equal length, so that a batch of uneven contexts is balanced by the order in which blocks finish: of about 2048 keys
+    // (the partial results are under 2 % of the bytes read), so many that the blocks fill whole rounds of two per SM, and not below
+    // 256 keys.
+    const int64_t units = tile_bound(*p, group, ROW_TILE) * p->kv_heads, slots = 2 * sm_count;
+    const int64_t rounds = std::max<int64_t>(1, (longest * units + slots * 2048 - 1) / (slots * 2048));
+    const int64_t parts = std::max<int64_t>(1, rounds * slots / units);
+    const int64_t keys = std::max<int64_t>(256, ((longest + parts - 1) / parts + 63) / 64 * 64);
     plan.splits = (int)std::max<int64_t>(1, (longest + keys - 1) / keys);
     plan.split_keys = (int)keys;
   }
@@ -518,7 +556,7 @@ extern "C" lbi_attention_plan lbi_paged_attention_plan(const lbi_paged_batch* p,
 }
 
 extern "C" int lbi_paged_attention(const lbi_paged_batch* p, const void* q, int64_t q_stride, void* out, float* part_o, float* part_lse,
-                                   lbi_attention_plan plan, int type, int heads, float scale, int zero_tail, cudaStream_t st) {
+                                   lbi_attention_plan plan, int type, int heads, float scale, int zero_tail, int sm_count, cudaStream_t st) {
   using namespace lbi::paged;
   if (p->head_dim % 16 != 0 || p->head_dim > 256 || type < 0 || type > LBI_F16 || heads % p->kv_heads != 0) return (int)cudaErrorInvalidValue;
   if (p->rows == 0 || p->batch == 0) return 0;
@@ -529,9 +567,5 @@ extern "C" int lbi_paged_attention(const lbi_paged_batch* p, const void* q, int6
     return type == LBI_F32 ? launch_row<LBI_F32>(a, st) : type == LBI_BF16 ? launch_row<LBI_BF16>(a, st) : launch_row<LBI_F16>(a, st);
   const int rc = plan.kernel == 2 ? launch_attn_tiles(a, type, st) : type == LBI_BF16 ? launch_rows<LBI_BF16>(a, st) : launch_rows<LBI_F16>(a, st);
   if (rc != 0 || plan.splits == 1) return rc;
-  const int64_t blocks = ((int64_t)p->rows * heads + 3) / 4;
-  if (blocks >= (1ll << 31)) return (int)cudaErrorInvalidValue;
-  if (type == LBI_BF16) combine_kernel<LBI_BF16><<<(unsigned)blocks, 128, 0, st>>>(a);
-  else combine_kernel<LBI_F16><<<(unsigned)blocks, 128, 0, st>>>(a);
-  return (int)cudaGetLastError();
+  return type == LBI_BF16 ? launch_combine<LBI_BF16>(a, sm_count, st) : launch_combine<LBI_F16>(a, sm_count, st);
 }

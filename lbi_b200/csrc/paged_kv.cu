@@ -15,6 +15,7 @@ namespace lbi {
 namespace paged {
 
 constexpr int APPEND_THREADS = 128;
+constexpr int BATCH = 4;   // head rows of a thread whose loads are in flight together
 
 struct AppendArgs {
   lbi_paged_batch b;
@@ -36,10 +37,25 @@ __global__ void __launch_bounds__(APPEND_THREADS) append_kernel(const AppendArgs
   const int group = 1 << a.group_shift, lane = threadIdx.x & (group - 1);
   const int d0 = a.interleaved ? lane * 16 : lane * 8, d1 = a.interleaved ? d0 + 8 : d0 + half;   // two runs of 8 elements
   const bool active = lane * 16 < dim;
-  const int total = a.heads + 2 * p.kv_heads;
+  const int total = a.heads + 2 * p.kv_heads, per_pass = APPEND_THREADS >> a.group_shift, first = threadIdx.x >> a.group_shift;
+  const T* src = (const T*)a.qkv + (int64_t)row * a.qkv_stride;
   T* q_out = (T*)a.q_out + (int64_t)row * a.heads * dim;
 
+  Vec<T, 8> raw[BATCH][2];
+  auto load = [&](int h0) {
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
+      const int h = h0 + i * per_pass + first;
+      if (h < total && active) {
+        raw[i][0] = *reinterpret_cast<const Vec<T, 8>*>(src + (int64_t)h * dim + d0);
+        raw[i][1] = *reinterpret_cast<const Vec<T, 8>*>(src + (int64_t)h * dim + d1);
+      }
+    }
+  };
+  load(0);   // before anything is known about the token
+
   const bool owned = row < last_row(p);
+  if (!owned && !a.zero_tail) return;
   int pos = -1, page = -1;
   bool turn_ok = true;
   if (owned) {
@@ -52,7 +68,6 @@ __global__ void __launch_bounds__(APPEND_THREADS) append_kernel(const AppendArgs
       if (threadIdx.x == 0 && p.status) atomicCAS(p.status, 0, 83);
     }
   }
-  if (!owned && !a.zero_tail) return;
   const bool dead = pos < 0 || !turn_ok;   // no position: q is zero, nothing is written
   float cs[8], sn[8];
 #pragma unroll
@@ -61,61 +76,77 @@ __global__ void __launch_bounds__(APPEND_THREADS) append_kernel(const AppendArgs
     load_f<float, 8>(a.cos_tab + (int64_t)pos * half + lane * 8, cs);
     load_f<float, 8>(a.sin_tab + (int64_t)pos * half + lane * 8, sn);
   }
-  const T* src = (const T*)a.qkv + (int64_t)row * a.qkv_stride;
-  for (int h0 = 0; h0 < total; h0 += APPEND_THREADS >> a.group_shift) {
-    const int h = h0 + (threadIdx.x >> a.group_shift);
-    float x[16];
+  for (int h0 = 0; h0 < total; h0 += BATCH * per_pass) {
+    if (h0 > 0) load(h0);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) x[i] = 0.f;
-    if (h < total && active && !dead) {
-      load_f<T, 8>(src + (int64_t)h * dim + d0, x);
-      load_f<T, 8>(src + (int64_t)h * dim + d1, x + 8);
+    for (int i = 0; i < BATCH; ++i) {
+      const int h = h0 + i * per_pass + first;
+      if (h0 + i * per_pass >= total) break;   // the same for the whole block
+      const bool here = h < total && active;
+      float x[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) x[e] = here && !dead ? to_f<T>(raw[i][e >> 3].v[e & 7]) : 0.f;
       if (a.cos_tab && h < a.heads + p.kv_heads) {
         // separate roundings (no fused multiply-add), so that the values that get quantised do not depend on contraction
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int ia = a.interleaved ? 2 * i : i, ib = a.interleaved ? 2 * i + 1 : 8 + i;
-          const float u = x[ia], w = x[ib];
-          x[ia] = __fsub_rn(__fmul_rn(u, cs[i]), __fmul_rn(w, sn[i]));
-          x[ib] = __fadd_rn(__fmul_rn(u, sn[i]), __fmul_rn(w, cs[i]));
+        for (int e = 0; e < 8; ++e) {
+          if (a.interleaved) {
+            const float u = x[2 * e], w = x[2 * e + 1];
+            x[2 * e] = __fsub_rn(__fmul_rn(u, cs[e]), __fmul_rn(w, sn[e]));
+            x[2 * e + 1] = __fadd_rn(__fmul_rn(u, sn[e]), __fmul_rn(w, cs[e]));
+          } else {
+            const float u = x[e], w = x[8 + e];
+            x[e] = __fsub_rn(__fmul_rn(u, cs[e]), __fmul_rn(w, sn[e]));
+            x[8 + e] = __fadd_rn(__fmul_rn(u, sn[e]), __fmul_rn(w, cs[e]));
+          }
         }
       }
-    }
-    float top = 0.f;
-    if (E4M3) {   // every thread of the warp takes part in the exchange
+      float top = 0.f;
+      if (E4M3) {   // every thread of the warp takes part in the exchange
 #pragma unroll
-      for (int i = 0; i < 16; ++i) top = max_nan(top, fabsf(x[i]));
-      for (int o = 1; o < group; o <<= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
-    }
-    if (h >= total || !active) continue;
-    if (h < a.heads) {
-      store_f<T, 8>(q_out + (int64_t)h * dim + d0, x);
-      store_f<T, 8>(q_out + (int64_t)h * dim + d1, x + 8);
-      continue;
-    }
-    if (dead || page < 0) continue;
-    const int kh = h - a.heads < p.kv_heads ? h - a.heads : h - a.heads - p.kv_heads;
-    const bool is_k = h - a.heads < p.kv_heads;
-    const int64_t slot = ((int64_t)page * p.kv_heads + kh) * p.page_size + (pos & (p.page_size - 1));
-    C* dst = (C*)(is_k ? p.k : p.v) + slot * dim;
-    if (E4M3) {
-      const float scale = __fdiv_rn(top, 448.f);
-      uint32_t w[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint32_t lo = 0, hi = 0;
-        if (top != 0.f) {
-          lo = __nv_cvt_float2_to_fp8x2(make_float2(__fdiv_rn(x[4 * i], scale), __fdiv_rn(x[4 * i + 1], scale)), __NV_SATFINITE, __NV_E4M3);
-          hi = __nv_cvt_float2_to_fp8x2(make_float2(__fdiv_rn(x[4 * i + 2], scale), __fdiv_rn(x[4 * i + 3], scale)), __NV_SATFINITE, __NV_E4M3);
-        }
-        w[i] = lo | hi << 16;
+        for (int e = 0; e < 16; ++e) top = max_nan(top, fabsf(x[e]));
+        for (int o = 1; o < group; o <<= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
       }
-      *reinterpret_cast<uint2*>(dst + d0) = make_uint2(w[0], w[1]);
-      *reinterpret_cast<uint2*>(dst + d1) = make_uint2(w[2], w[3]);
-      if (lane == 0) (is_k ? p.k_scale : p.v_scale)[slot] = scale;
-    } else {
-      store_f<T, 8>((T*)dst + d0, x);
-      store_f<T, 8>((T*)dst + d1, x + 8);
+      if (!here) continue;
+      if (h < a.heads) {
+        store_f<T, 8>(q_out + (int64_t)h * dim + d0, x);
+        store_f<T, 8>(q_out + (int64_t)h * dim + d1, x + 8);
+        continue;
+      }
+      if (dead || page < 0) continue;
+      const bool is_k = h - a.heads < p.kv_heads;
+      const int kh = is_k ? h - a.heads : h - a.heads - p.kv_heads;
+      const int64_t slot = ((int64_t)page * p.kv_heads + kh) * p.page_size + (pos & (p.page_size - 1));
+      C* dst = (C*)(is_k ? p.k : p.v) + slot * dim;
+      if (E4M3) {
+        const float scale = __fdiv_rn(top, 448.f);
+        // One division per head row: x * (1 / scale) is within 2^-23 of x / scale, a millionth of the code's half step.  A scale below
+        // the normal range has no reciprocal: those rows divide.
+        const float inv = __fdiv_rn(1.f, scale);
+        if (top == 0.f) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) x[e] = 0.f;
+        } else if (scale >= 1.17549435e-38f || scale != scale) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) x[e] = __fmul_rn(x[e], inv);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) x[e] = __fdiv_rn(x[e], scale);
+        }
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(x[4 * e], x[4 * e + 1]), __NV_SATFINITE, __NV_E4M3);
+          const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(x[4 * e + 2], x[4 * e + 3]), __NV_SATFINITE, __NV_E4M3);
+          w[e] = lo | hi << 16;
+        }
+        *reinterpret_cast<uint2*>(dst + d0) = make_uint2(w[0], w[1]);
+        *reinterpret_cast<uint2*>(dst + d1) = make_uint2(w[2], w[3]);
+        if (lane == 0) (is_k ? p.k_scale : p.v_scale)[slot] = scale;
+      } else {
+        store_f<T, 8>((T*)dst + d0, x);
+        store_f<T, 8>((T*)dst + d1, x + 8);
+      }
     }
   }
 }
