@@ -24,6 +24,18 @@ struct PerDeviceOnce {
     if (e == cudaSuccess && tracked) done[dev >> 6].fetch_or(bit, std::memory_order_release);
     return e;
   }
+  // Asks for the largest shared-memory share of the L1 (a hint: static shared memory alone does not move it, and blocks per SM follow
+  // from it).
+  template <typename Kernel>
+  void all_shared(Kernel kernel) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return;
+    const bool tracked = dev >= 0 && dev < 256;
+    const unsigned long long bit = 1ull << (dev & 63);
+    if (tracked && (done[dev >> 6].load(std::memory_order_acquire) & bit)) return;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared) == cudaSuccess && tracked)
+      done[dev >> 6].fetch_or(bit, std::memory_order_release);
+  }
 };
 
 // Debug build (python -m lbi_b200.build --bounds-check, extension lbi_b200._Cdbg): index checks that record the first violation

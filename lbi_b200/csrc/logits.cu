@@ -16,10 +16,10 @@ namespace lbi {
 namespace paged {
 
 constexpr int COUNT_BYTES = 32768;
-constexpr int LOGIT_THREADS = 512;
+constexpr int LOGIT_THREADS = 512;   // four blocks per SM: 2048 threads, 128 KB of counts
 
 template <int TYPE, typename COUNT>
-__global__ void __launch_bounds__(LOGIT_THREADS) logits_kernel(const lbi_logit_rules p, int tile) {
+__global__ void __launch_bounds__(LOGIT_THREADS, 4) logits_kernel(const lbi_logit_rules p, int tile) {
   using T = typename Elem<TYPE>::T;
   constexpr bool WIDE = sizeof(COUNT) == 4;
   constexpr uint32_t PROMPT = WIDE ? 0x80000000u : 0x8000u;
@@ -52,36 +52,35 @@ __global__ void __launch_bounds__(LOGIT_THREADS) logits_kernel(const lbi_logit_r
   float* out = p.out + (int64_t)b * p.out_stride + v0;
   const float* bias = p.bias ? p.bias + (int64_t)b * p.bias_stride + v0 : nullptr;
   const int* allowed = p.allowed ? p.allowed + (int64_t)b * p.allowed_stride + (v0 >> 5) : nullptr;
-  constexpr int EACH = 8;   // rows of odd vocabularies start anywhere, so an element per thread and access, several in flight
-  for (int i0 = threadIdx.x; i0 < n; i0 += EACH * LOGIT_THREADS) {
+  // Rows of odd vocabularies start anywhere, so an element per thread and access, several in flight; the tile's end is a case of its
+  // own.  A tile starts at a multiple of 32, so a warp's 32 elements share a word of the mask.
+  constexpr int EACH = 8;
+  auto rules = [&](int i, float f, float add, uint32_t bits) {
+    const uint32_t c = count[i];
+    if (c) {
+      f = f > 0.f ? __fdiv_rn(f, rep) : f * rep;
+      const uint32_t made = c & (PROMPT - 1);
+      if (made) f = __fsub_rn(__fsub_rn(f, pres), __fmul_rn(freq, (float)made));
+    }
+    if (bias) f += add;
+    out[i] = bits >> (threadIdx.x & 31) & 1u ? f : -INFINITY;
+  };
+  int i = threadIdx.x;
+  for (; i + (EACH - 1) * LOGIT_THREADS < n; i += EACH * LOGIT_THREADS) {
     float f[EACH], add[EACH];
     uint32_t bits[EACH];
 #pragma unroll
-    for (int e = 0; e < EACH; ++e) {
-      const int i = i0 + e * LOGIT_THREADS;
-      f[e] = add[e] = 0.f;
-      bits[e] = 0xffffffffu;
-      if (i < n) {
-        f[e] = to_f<T>(x[i]);
-        if (bias) add[e] = __ldg(bias + i);
-        if (allowed) bits[e] = (uint32_t)__ldg(allowed + (i >> 5));
-      }
-    }
+    for (int e = 0; e < EACH; ++e) f[e] = to_f<T>(x[i + e * LOGIT_THREADS]);
 #pragma unroll
     for (int e = 0; e < EACH; ++e) {
-      const int i = i0 + e * LOGIT_THREADS;
-      if (i >= n) break;
-      const uint32_t c = count[i];
-      if (c) {
-        f[e] = f[e] > 0.f ? __fdiv_rn(f[e], rep) : f[e] * rep;
-        const uint32_t made = c & (PROMPT - 1);
-        if (made) f[e] = __fsub_rn(__fsub_rn(f[e], pres), __fmul_rn(freq, (float)made));
-      }
-      if (bias) f[e] += add[e];
-      if (!(bits[e] >> (i & 31) & 1u)) f[e] = -INFINITY;
-      out[i] = f[e];
+      add[e] = bias ? __ldg(bias + i + e * LOGIT_THREADS) : 0.f;
+      bits[e] = allowed ? (uint32_t)__ldg(allowed + ((i + e * LOGIT_THREADS) >> 5)) : 0xffffffffu;
     }
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) rules(i + e * LOGIT_THREADS, f[e], add[e], bits[e]);
   }
+  for (; i < n; i += LOGIT_THREADS)
+    rules(i, to_f<T>(x[i]), bias ? __ldg(bias + i) : 0.f, allowed ? (uint32_t)__ldg(allowed + (i >> 5)) : 0xffffffffu);
 }
 
 template <int TYPE>
@@ -92,6 +91,9 @@ static void launch_logits(const lbi_logit_rules& p, int sm_count, cudaStream_t s
   const int64_t per_row = std::max<int64_t>(1, sm_count / p.batch);
   const int tile = (int)std::min<int64_t>(most, std::max<int64_t>(1024, ((p.vocab + per_row - 1) / per_row + 1023) / 1024 * 1024));
   const dim3 grid((p.vocab + tile - 1) / tile, p.batch);
+  static lbi::PerDeviceOnce narrow_once, wide_once;
+  narrow_once.all_shared(logits_kernel<TYPE, uint16_t>);
+  wide_once.all_shared(logits_kernel<TYPE, uint32_t>);
   if (wide) logits_kernel<TYPE, uint32_t><<<grid, LOGIT_THREADS, 0, st>>>(p, tile);
   else logits_kernel<TYPE, uint16_t><<<grid, LOGIT_THREADS, 0, st>>>(p, tile);
 }

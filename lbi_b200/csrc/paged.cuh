@@ -60,13 +60,6 @@ __device__ __forceinline__ void store_f(T* p, const float* f) {
   *reinterpret_cast<Vec<T, N>*>(p) = x;
 }
 
-// max that keeps a NaN (fmaxf drops it): a row with a NaN gets a NaN scale, as the plain form's amax gives
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-
 // [first, last) rows of the new tokens of sequence b.  Offsets are clamped to the rows that exist: a wrong one can leave tokens
 // out but never reach outside q.
 __device__ __forceinline__ int2 seq_rows(const lbi_paged_batch& p, int b) {
@@ -174,6 +167,13 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
       : "=l"(reinterpret_cast<unsigned long long&>(d))
       : "l"(reinterpret_cast<const unsigned long long&>(a)), "l"(reinterpret_cast<const unsigned long long&>(b)),
         "l"(reinterpret_cast<const unsigned long long&>(c)));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<unsigned long long&>(d))
+      : "l"(reinterpret_cast<const unsigned long long&>(a)), "l"(reinterpret_cast<const unsigned long long&>(b)));
   return d;
 }
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {

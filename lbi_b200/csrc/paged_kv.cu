@@ -15,44 +15,41 @@ namespace lbi {
 namespace paged {
 
 constexpr int APPEND_THREADS = 128;
-constexpr int BATCH = 4;   // head rows of a thread whose loads are in flight together
 
 struct AppendArgs {
   lbi_paged_batch b;
   const void* qkv;
   int64_t qkv_stride;
   void* q_out;
-  int heads, interleaved, zero_tail, page_shift, group_shift;   // 1 << group_shift threads serve one head row
+  int heads, zero_tail, page_shift, group_shift;   // 1 << group_shift threads serve one head row
   const float* cos_tab;
   const float* sin_tab;
   int64_t rope_rows;
 };
 
-template <int TYPE, bool E4M3>
-__global__ void __launch_bounds__(APPEND_THREADS) append_kernel(const AppendArgs a) {
+// PAIRED: the turn's partners are neighbours (2 i, 2 i + 1), else i and i + head_dim / 2.
+template <int TYPE, bool E4M3, bool PAIRED>
+__global__ void __launch_bounds__(APPEND_THREADS, 8) append_kernel(const AppendArgs a) {
   using T = typename Elem<TYPE>::T;
   using C = typename Elem<E4M3 ? LBI_E4M3 : TYPE>::T;
   const lbi_paged_batch& p = a.b;
   const int row = blockIdx.x, dim = p.head_dim, half = dim >> 1;
   const int group = 1 << a.group_shift, lane = threadIdx.x & (group - 1);
-  const int d0 = a.interleaved ? lane * 16 : lane * 8, d1 = a.interleaved ? d0 + 8 : d0 + half;   // two runs of 8 elements
+  const int d0 = PAIRED ? lane * 16 : lane * 8, d1 = PAIRED ? d0 + 8 : d0 + half;   // two runs of 8 elements
   const bool active = lane * 16 < dim;
   const int total = a.heads + 2 * p.kv_heads, per_pass = APPEND_THREADS >> a.group_shift, first = threadIdx.x >> a.group_shift;
   const T* src = (const T*)a.qkv + (int64_t)row * a.qkv_stride;
   T* q_out = (T*)a.q_out + (int64_t)row * a.heads * dim;
 
-  Vec<T, 8> raw[BATCH][2];
-  auto load = [&](int h0) {
-#pragma unroll
-    for (int i = 0; i < BATCH; ++i) {
-      const int h = h0 + i * per_pass + first;
-      if (h < total && active) {
-        raw[i][0] = *reinterpret_cast<const Vec<T, 8>*>(src + (int64_t)h * dim + d0);
-        raw[i][1] = *reinterpret_cast<const Vec<T, 8>*>(src + (int64_t)h * dim + d1);
-      }
+  Vec<T, 8> next[2] = {};
+  bool dead = false;   // no position: q is zero, nothing is written
+  auto load = [&](int h) {
+    if (h < total && active && !dead) {
+      next[0] = *reinterpret_cast<const Vec<T, 8>*>(src + h * dim + d0);
+      next[1] = *reinterpret_cast<const Vec<T, 8>*>(src + h * dim + d1);
     }
   };
-  load(0);   // before anything is known about the token
+  load(first);   // before anything is known about the token, and then one head row ahead
 
   const bool owned = row < last_row(p);
   if (!owned && !a.zero_tail) return;
@@ -68,85 +65,100 @@ __global__ void __launch_bounds__(APPEND_THREADS) append_kernel(const AppendArgs
       if (threadIdx.x == 0 && p.status) atomicCAS(p.status, 0, 83);
     }
   }
-  const bool dead = pos < 0 || !turn_ok;   // no position: q is zero, nothing is written
-  float cs[8], sn[8];
+  dead = pos < 0 || !turn_ok;
+  if (dead) next[0] = next[1] = Vec<T, 8>{};
+  union Eight {
+    float f[8];
+    float2 f2[4];
+  } cs, sn;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) cs[i] = 1.f, sn[i] = 0.f;
+  for (int i = 0; i < 8; ++i) cs.f[i] = 1.f, sn.f[i] = 0.f;
   if (a.cos_tab && !dead && active) {
-    load_f<float, 8>(a.cos_tab + (int64_t)pos * half + lane * 8, cs);
-    load_f<float, 8>(a.sin_tab + (int64_t)pos * half + lane * 8, sn);
+    load_f<float, 8>(a.cos_tab + (int64_t)pos * half + lane * 8, cs.f);
+    load_f<float, 8>(a.sin_tab + (int64_t)pos * half + lane * 8, sn.f);
   }
-  for (int h0 = 0; h0 < total; h0 += BATCH * per_pass) {
-    if (h0 > 0) load(h0);
+#pragma unroll 1
+  for (int h0 = 0; h0 < total; h0 += per_pass) {
+    const int h = h0 + first;
+    const bool here = h < total && active;
+    Eight u, w;   // the partners of eight turns (or 16 elements of a value row)
 #pragma unroll
-    for (int i = 0; i < BATCH; ++i) {
-      const int h = h0 + i * per_pass + first;
-      if (h0 + i * per_pass >= total) break;   // the same for the whole block
-      const bool here = h < total && active;
-      float x[16];
+    for (int e = 0; e < 8; ++e) {
+      u.f[e] = PAIRED ? to_f<T>(next[e >> 2].v[2 * (e & 3)]) : to_f<T>(next[0].v[e]);
+      w.f[e] = PAIRED ? to_f<T>(next[e >> 2].v[2 * (e & 3) + 1]) : to_f<T>(next[1].v[e]);
+    }
+    load(h + per_pass);
+    if (a.cos_tab && h < a.heads + p.kv_heads) {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) x[e] = here && !dead ? to_f<T>(raw[i][e >> 3].v[e & 7]) : 0.f;
-      if (a.cos_tab && h < a.heads + p.kv_heads) {
-        // separate roundings (no fused multiply-add), so that the values that get quantised do not depend on contraction
+      for (int e = 0; e < 4; ++e) {
+        const float2 un = u.f2[e], wn = w.f2[e], minus = make_float2(-sn.f2[e].x, -sn.f2[e].y);
+        u.f2[e] = fma2(wn, minus, mul2(un, cs.f2[e]));
+        w.f2[e] = fma2(un, sn.f2[e], mul2(wn, cs.f2[e]));
+      }
+    }
+    float top = 0.f;
+    if (E4M3) {   // every thread of the warp takes part in the exchange
+      // as whole numbers, magnitudes are in order, with a NaN (which has to reach the scale) above all
+      int most = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) most = max(most, max(__float_as_int(u.f[e]) & 0x7fffffff, __float_as_int(w.f[e]) & 0x7fffffff));
+      for (int o = 1; o < group; o <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+      top = __int_as_float(most);
+    }
+    if (!here) continue;
+    float x[16];   // in the order of memory: run d0, run d1
+    auto in_order = [&] {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        x[PAIRED ? 2 * e : e] = u.f[e];
+        x[PAIRED ? 2 * e + 1 : 8 + e] = w.f[e];
+      }
+    };
+    if (h < a.heads) {
+      in_order();
+      store_f<T, 8>(q_out + h * dim + d0, x);
+      store_f<T, 8>(q_out + h * dim + d1, x + 8);
+      continue;
+    }
+    if (dead || page < 0) continue;
+    const bool is_k = h - a.heads < p.kv_heads;
+    const int kh = is_k ? h - a.heads : h - a.heads - p.kv_heads;
+    const int slot = (page * p.kv_heads + kh) * p.page_size + (pos & (p.page_size - 1));
+    C* dst = (C*)(is_k ? p.k : p.v) + (int64_t)slot * dim;
+    if (E4M3) {
+      const float scale = __fmul_rn(top, 1.f / 448.f);
+      // One reciprocal per head row: x * (1 / scale) is within 2^-22 of x / scale, some millionths of the code's half step.  A scale
+      // below the normal range has no reciprocal: those rows divide.
+      if (scale < 1.17549435e-38f) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          if (a.interleaved) {
-            const float u = x[2 * e], w = x[2 * e + 1];
-            x[2 * e] = __fsub_rn(__fmul_rn(u, cs[e]), __fmul_rn(w, sn[e]));
-            x[2 * e + 1] = __fadd_rn(__fmul_rn(u, sn[e]), __fmul_rn(w, cs[e]));
-          } else {
-            const float u = x[e], w = x[8 + e];
-            x[e] = __fsub_rn(__fmul_rn(u, cs[e]), __fmul_rn(w, sn[e]));
-            x[8 + e] = __fadd_rn(__fmul_rn(u, sn[e]), __fmul_rn(w, cs[e]));
-          }
+          u.f[e] = scale == 0.f ? 0.f : __fdiv_rn(u.f[e], scale);
+          w.f[e] = scale == 0.f ? 0.f : __fdiv_rn(w.f[e], scale);
         }
-      }
-      float top = 0.f;
-      if (E4M3) {   // every thread of the warp takes part in the exchange
-#pragma unroll
-        for (int e = 0; e < 16; ++e) top = max_nan(top, fabsf(x[e]));
-        for (int o = 1; o < group; o <<= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
-      }
-      if (!here) continue;
-      if (h < a.heads) {
-        store_f<T, 8>(q_out + (int64_t)h * dim + d0, x);
-        store_f<T, 8>(q_out + (int64_t)h * dim + d1, x + 8);
-        continue;
-      }
-      if (dead || page < 0) continue;
-      const bool is_k = h - a.heads < p.kv_heads;
-      const int kh = is_k ? h - a.heads : h - a.heads - p.kv_heads;
-      const int64_t slot = ((int64_t)page * p.kv_heads + kh) * p.page_size + (pos & (p.page_size - 1));
-      C* dst = (C*)(is_k ? p.k : p.v) + slot * dim;
-      if (E4M3) {
-        const float scale = __fdiv_rn(top, 448.f);
-        // One division per head row: x * (1 / scale) is within 2^-23 of x / scale, a millionth of the code's half step.  A scale below
-        // the normal range has no reciprocal: those rows divide.
-        const float inv = __fdiv_rn(1.f, scale);
-        if (top == 0.f) {
-#pragma unroll
-          for (int e = 0; e < 16; ++e) x[e] = 0.f;
-        } else if (scale >= 1.17549435e-38f || scale != scale) {
-#pragma unroll
-          for (int e = 0; e < 16; ++e) x[e] = __fmul_rn(x[e], inv);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 16; ++e) x[e] = __fdiv_rn(x[e], scale);
-        }
-        uint32_t w[4];
+      } else {
+        float inv;
+        asm("rcp.approx.f32 %0, %1;" : "=f"(inv) : "f"(scale));
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(x[4 * e], x[4 * e + 1]), __NV_SATFINITE, __NV_E4M3);
-          const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(x[4 * e + 2], x[4 * e + 3]), __NV_SATFINITE, __NV_E4M3);
-          w[e] = lo | hi << 16;
+          u.f2[e] = mul2(u.f2[e], make_float2(inv, inv));
+          w.f2[e] = mul2(w.f2[e], make_float2(inv, inv));
         }
-        *reinterpret_cast<uint2*>(dst + d0) = make_uint2(w[0], w[1]);
-        *reinterpret_cast<uint2*>(dst + d1) = make_uint2(w[2], w[3]);
-        if (lane == 0) (is_k ? p.k_scale : p.v_scale)[slot] = scale;
-      } else {
-        store_f<T, 8>((T*)dst + d0, x);
-        store_f<T, 8>((T*)dst + d1, x + 8);
       }
+      in_order();
+      uint32_t code[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(x[4 * e], x[4 * e + 1]), __NV_SATFINITE, __NV_E4M3);
+        const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(x[4 * e + 2], x[4 * e + 3]), __NV_SATFINITE, __NV_E4M3);
+        code[e] = __byte_perm(lo, hi, 0x5410);
+      }
+      *reinterpret_cast<uint2*>(dst + d0) = make_uint2(code[0], code[1]);
+      *reinterpret_cast<uint2*>(dst + d1) = make_uint2(code[2], code[3]);
+      if (lane == 0) (is_k ? p.k_scale : p.v_scale)[slot] = scale;
+    } else {
+      in_order();
+      store_f<T, 8>((T*)dst + d0, x);
+      store_f<T, 8>((T*)dst + d1, x + 8);
     }
   }
 }
@@ -186,9 +198,9 @@ __global__ void __launch_bounds__(256) gather_kernel(const lbi_paged_batch p, vo
 
 #define LBI_BY_TYPE(type, e4m3, CALL)                                              \
   do {                                                                             \
-    if ((type) == LBI_F32) { if (e4m3) CALL(LBI_F32, true); else CALL(LBI_F32, false); }      \
-    else if ((type) == LBI_BF16) { if (e4m3) CALL(LBI_BF16, true); else CALL(LBI_BF16, false); } \
-    else { if (e4m3) CALL(LBI_F16, true); else CALL(LBI_F16, false); }             \
+    if ((type) == LBI_F32) { if (e4m3) { CALL(LBI_F32, true); } else { CALL(LBI_F32, false); } }      \
+    else if ((type) == LBI_BF16) { if (e4m3) { CALL(LBI_BF16, true); } else { CALL(LBI_BF16, false); } } \
+    else { if (e4m3) { CALL(LBI_F16, true); } else { CALL(LBI_F16, false); } }     \
   } while (0)
 
 extern "C" int lbi_kv_append(const lbi_paged_batch* p, const void* qkv, int64_t qkv_stride, void* q_out, int type, int heads,
@@ -196,8 +208,12 @@ extern "C" int lbi_kv_append(const lbi_paged_batch* p, const void* qkv, int64_t 
   using namespace lbi::paged;
   if (p->head_dim % 16 != 0 || p->head_dim > 256 || p->rows < 0 || type < 0 || type > LBI_F16) return (int)cudaErrorInvalidValue;
   if (p->rows == 0) return 0;
-  AppendArgs a{*p, qkv, qkv_stride, q_out, heads, interleaved, zero_tail, shift_of(p->page_size), shift_of(p->head_dim / 16), cos_tab, sin_tab, rope_rows};
-#define LBI_APPEND(T, E) append_kernel<T, E><<<p->rows, APPEND_THREADS, 0, st>>>(a)
+  AppendArgs a{*p, qkv, qkv_stride, q_out, heads, zero_tail, shift_of(p->page_size), shift_of(p->head_dim / 16), cos_tab, sin_tab, rope_rows};
+#define LBI_APPEND(T, E)                                                             \
+  do {                                                                                \
+    if (interleaved) append_kernel<T, E, true><<<p->rows, APPEND_THREADS, 0, st>>>(a); \
+    else append_kernel<T, E, false><<<p->rows, APPEND_THREADS, 0, st>>>(a);            \
+  } while (0)
   LBI_BY_TYPE(type, p->cache_type == LBI_E4M3, LBI_APPEND);
 #undef LBI_APPEND
   return (int)cudaGetLastError();
