@@ -87,10 +87,27 @@ __device__ __forceinline__ int last_below(int n, F below) {
   return lo;
 }
 
-// Sequence that row `row` belongs to; a full warp calls.
-__device__ __forceinline__ int seq_of_row(const lbi_paged_batch& p, int row) {
-  if (!p.cu) return row / (p.rows / p.batch);
-  return last_below(p.batch, [&](int b) { return __ldg(p.cu + b) <= row; });
+// Sequence of row `row`, its rows [first, last), and whether the row belongs to any; a full warp calls.  Batches of up to 31 sequences
+// read all offsets at once.
+struct Place {
+  int b, first, last;
+  bool owned;
+};
+__device__ __forceinline__ Place place_of_row(const lbi_paged_batch& p, int row) {
+  if (!p.cu) {
+    const int each = p.rows / p.batch, b = row / each;
+    return {b, b * each, (b + 1) * each, true};
+  }
+  if (p.batch < 32) {
+    const int lane = threadIdx.x & 31;
+    const int v = min(max(__ldg(p.cu + min(lane, p.batch)), 0), p.rows);
+    const int b = min(max(__popc(__ballot_sync(0xffffffffu, lane < p.batch && v <= row)) - 1, 0), p.batch - 1);
+    const int lo = __shfl_sync(0xffffffffu, v, b), hi = max(__shfl_sync(0xffffffffu, v, b + 1), lo);
+    return {b, lo, hi, row >= lo && row < hi};
+  }
+  const int b = last_below(p.batch, [&](int i) { return __ldg(p.cu + i) <= row; });
+  const int2 r = seq_rows(p, b);
+  return {b, r.x, r.y, row >= r.x && row < r.y};
 }
 
 __device__ __forceinline__ int last_row(const lbi_paged_batch& p) {
@@ -158,6 +175,16 @@ __device__ __forceinline__ void codes_to_16(uint32_t w, uint32_t& lo, uint32_t& 
     asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(lo) : "r"(x), "r"(0x7b807b80u));
     asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(hi) : "r"(y), "r"(0x7b807b80u));
   }
+}
+
+// The same by the conversion instruction, for kernels that have time on its unit.
+__device__ __forceinline__ void codes_to_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  asm("{\n.reg .b16 a, b;\nmov.b32 {a, b}, %2;\ncvt.rn.f16x2.e4m3x2 %0, a;\ncvt.rn.f16x2.e4m3x2 %1, b;\n}" : "=r"(lo), "=r"(hi) : "r"(w));
+}
+__device__ __forceinline__ float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
 // Two fp32 operations per instruction (packed pairs, sm_100).

@@ -2,10 +2,10 @@
 //
 //   o_i = sum_j softmax_j(scale q_i . k_j) v_j   over the positions j <= context - new + i of the sequence; no position: o_i = 0.
 //
-// Three kernels:
+// Kernels:
 //   attn_rows_kernel   16 query rows at a time (tokens x heads of a group) for 16-bit queries: decoding, a few new tokens.
 //   attn_tiles_kernel  256 rows at a time on tcgen05 (paged_attn_tc.cu): chunks of a prompt.
-//   attn_row_kernel    one warp per (token, head): fp32 queries and head sizes that the tiles do not cover.
+//   attn_any_kernel    16 rows at a time in (almost) full precision: fp32 queries, and head sizes that the other tiles do not cover.
 //   combine_kernel     joins the parts of a long context.
 #include <algorithm>
 
@@ -71,6 +71,80 @@ __device__ __forceinline__ uint32_t swz(int r, int c) {
   return (uint32_t)(r * RB + ((c ^ ((r / ROWS) & (IN_LINE - 1))) << 4));
 }
 
+// What a block of 16 rows works on.
+struct RowsUnit {
+  int split, kh, b, first_row, local, n_rows, first_pos, k0, k1;   // local: first row of the tile in the sequence's tile space
+  bool any;
+};
+__device__ __forceinline__ RowsUnit rows_unit(const AttnArgs& a) {
+  const lbi_paged_batch& p = a.b;
+  RowsUnit u;
+  u.split = blockIdx.x % a.splits;
+  const int64_t unit = blockIdx.x / a.splits;
+  u.kh = (int)(unit % p.kv_heads);
+  const int64_t tile = unit / p.kv_heads;
+  u.b = seq_of_tile(p, tile, a.group, ROW_TILE);
+  const int2 r = seq_rows(p, u.b);
+  u.first_row = r.x;
+  u.local = (int)(tile - first_tile(p, u.b, a.group, ROW_TILE)) * ROW_TILE;
+  const int rows_b = (r.y - r.x) * a.group;
+  u.any = u.local >= 0 && u.local < rows_b;
+  u.n_rows = min(ROW_TILE, rows_b - u.local);
+  u.first_pos = __ldg(p.context + u.b) - (r.y - r.x);              // position of the sequence's first new token
+  const int64_t capacity = (int64_t)p.table_width << a.page_shift;
+  const int keys = (int)min((int64_t)u.first_pos + (u.local + u.n_rows - 1) / a.group + 1, capacity);
+  u.k0 = u.split * a.split_keys;
+  u.k1 = u.split == a.splits - 1 ? keys : min(keys, u.k0 + a.split_keys);
+  return u;
+}
+template <typename T>
+__device__ __forceinline__ void zero_rows_of_nobody(const AttnArgs& a) {
+  if (a.zero_tail && !a.part_o)
+    for (int64_t row = (int64_t)last_row(a.b) + blockIdx.x; row < a.b.rows; row += gridDim.x)
+      for (int i = threadIdx.x; i < a.heads * a.b.head_dim; i += blockDim.x) ((T*)a.out)[row * a.heads * a.b.head_dim + i] = from_f<T>(0.f);
+}
+// Slot of key `lane` of a tile that starts at `base`, or -1 where there is no such key or page.
+__device__ __forceinline__ int key_slot(const AttnArgs& a, const RowsUnit& u, int pos, bool wanted, int page) {
+  const lbi_paged_batch& p = a.b;
+  if (!wanted) return -1;
+  if (page >= 0 && page < p.num_pages) return (page * p.kv_heads + u.kh) * p.page_size + (pos & (p.page_size - 1));
+  if (p.status) atomicCAS(p.status, 0, 84);
+  return -1;
+}
+// Joins the warps of a block and stores the result (or the part): `m`, `l` of rows g and g + 8 in every thread, the output row parts
+// behind ml in shared memory as [warp][row][dim + 4].
+template <typename T>
+__device__ __forceinline__ void join_and_store(const AttnArgs& a, const RowsUnit& u, const float* ml, int dim) {
+  const float* os = ml + 2 * WARPS * ROW_TILE;
+  for (int i = threadIdx.x; i < u.n_rows * (dim / 8); i += WARPS * 32) {
+    const int rr = i / (dim / 8), d = i % (dim / 8) * 8;
+    float top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) top = fmaxf(top, ml[w * ROW_TILE + rr]);
+    const float ref = top == -INFINITY ? 0.f : top;
+    float sum = 0.f, acc[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[e] = 0.f;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      const float f = ex2(ml[w * ROW_TILE + rr] - ref);
+      sum += f * ml[(WARPS + w) * ROW_TILE + rr];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[e] += f * os[(w * ROW_TILE + rr) * (dim + 4) + d + e];
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[e] *= inv;
+    const int64_t at = (int64_t)(u.first_row + (u.local + rr) / a.group) * a.heads + u.kh * a.group + (u.local + rr) % a.group;
+    if (a.part_o) {
+      store_f<float, 8>(a.part_o + (at * a.splits + u.split) * dim + d, acc);
+      if (d == 0) a.part_lse[at * a.splits + u.split] = sum == 0.f ? -INFINITY : top + log2f(sum);
+    } else {
+      store_f<T, 8>((T*)a.out + at * dim + d, acc);
+    }
+  }
+}
+
 template <int TYPE, bool E4M3, int DH, int KEYS, int STAGES>
 struct RowsTile {
   static constexpr int RB = DH * (E4M3 ? 1 : 2);
@@ -88,43 +162,50 @@ __global__ void __launch_bounds__(WARPS * 32, 2) attn_rows_kernel(const AttnArgs
   extern __shared__ __align__(128) uint8_t smem[];
   const lbi_paged_batch& p = a.b;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int split = blockIdx.x % a.splits;
-  const int64_t unit = blockIdx.x / a.splits;
-  const int kh = (int)(unit % p.kv_heads);
-  const int64_t tile = unit / p.kv_heads;
-
-  if (a.zero_tail && !a.part_o)
-    for (int64_t row = (int64_t)last_row(p) + blockIdx.x; row < p.rows; row += gridDim.x)
-      for (int i = threadIdx.x; i < a.heads * DH; i += WARPS * 32) ((T*)a.out)[row * a.heads * DH + i] = from_f<T>(0.f);
-
-  const int b = seq_of_tile(p, tile, a.group, ROW_TILE);
-  const int2 r = seq_rows(p, b);
-  const int local = (int)(tile - first_tile(p, b, a.group, ROW_TILE)) * ROW_TILE;   // first row of the tile in the sequence's tile space
-  const int rows_b = (r.y - r.x) * a.group;
-  if (local < 0 || local >= rows_b) return;
-  const int n_rows = min(ROW_TILE, rows_b - local);
-  const int ctx = __ldg(p.context + b);
-  const int first_pos = ctx - (r.y - r.x);                                          // position of the sequence's first new token
-  const int64_t capacity = (int64_t)p.table_width << a.page_shift;
-  const int keys = (int)min((int64_t)first_pos + (local + n_rows - 1) / a.group + 1, capacity);
-  const int k0 = split * a.split_keys;
-  const int k1 = split == a.splits - 1 ? keys : min(keys, k0 + a.split_keys);
+  zero_rows_of_nobody<T>(a);
+  const RowsUnit u = rows_unit(a);
+  if (!u.any) return;
+  const int kh = u.kh, local = u.local, n_rows = u.n_rows, k0 = u.k0, k1 = u.k1;
 
   // query fragments: row g (and g + 8) of the tile; the order of the head's elements within a product of 16 is free as long as Q and
   // K agree: natural for 16-bit pages (ldmatrix), 4 neighbours per thread for codes (one 32-bit load)
+  // e4m3: the products run in fp16, which holds the codes and, behind a power of two per row that brings its largest element to
+  // [2^14, 2^15), a bf16 query as well (29 binades below the largest to the normal range's end: nothing that an fp32 sum would notice)
+  constexpr int MATH = E4M3 ? LBI_F16 : TYPE;
   uint32_t qf[DH / 16][4];
   int limit[2];
+  float row_scale[2];
 #pragma unroll
   for (int hh = 0; hh < 2; ++hh) {
     const int rr = local + g + 8 * hh;
     const bool live = g + 8 * hh < n_rows;
     const int token = live ? rr / a.group : 0, head = kh * a.group + (live ? rr % a.group : 0);
-    limit[hh] = live ? first_pos + token : -1;
-    const uint32_t* src = reinterpret_cast<const uint32_t*>((const T*)a.q + (int64_t)(r.x + token) * a.q_stride + head * DH);
+    limit[hh] = live ? u.first_pos + token : -1;
+    row_scale[hh] = a.scale_log2;
+    const uint32_t* src = reinterpret_cast<const uint32_t*>((const T*)a.q + (int64_t)(u.first_row + token) * a.q_stride + head * DH);
 #pragma unroll
     for (int ks = 0; ks < DH / 16; ++ks) {
       qf[ks][hh] = live ? src[ks * 8 + (E4M3 ? 2 * t : t)] : 0u;
       qf[ks][2 + hh] = live ? src[ks * 8 + (E4M3 ? 2 * t + 1 : t + 4)] : 0u;
+    }
+    if (E4M3 && TYPE == LBI_BF16) {
+      int most = 0;   // as whole numbers, magnitudes are in order
+#pragma unroll
+      for (int ks = 0; ks < DH / 16; ++ks)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) most = max(most, max(qf[ks][2 * i + hh] << 16 & 0x7fff0000, qf[ks][2 * i + hh] & 0x7fff0000));
+      most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+      most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+      const int e = min(max(14 + 127 - (most >> 23), -100), 120);
+      const float up = __int_as_float((e + 127) << 23);
+      row_scale[hh] *= __int_as_float((127 - e) << 23);
+#pragma unroll
+      for (int ks = 0; ks < DH / 16; ++ks)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          uint32_t& w = qf[ks][2 * i + hh];
+          w = pack16<LBI_F16>(__uint_as_float(w << 16) * up, __uint_as_float(w & 0xffff0000u) * up);
+        }
     }
   }
   float o[DH / 8][4];
@@ -137,7 +218,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2) attn_rows_kernel(const AttnArgs
   const uint32_t ring = smem_addr(smem) + warp * L::RING;
   const int n_tiles = k1 > k0 ? (k1 - k0 + KEYS - 1) / KEYS : 0;
   const int mine = n_tiles > warp ? (n_tiles - warp + WARPS - 1) / WARPS : 0;      // tiles warp, warp + 4, ...
-  const int* table = p.table + (int64_t)b * p.table_stride;
+  const int* table = p.table + (int64_t)u.b * p.table_stride;
   auto load_page = [&](int i) {   // page id of key `lane` of this warp's i-th tile; -1: not there
     const int pos = k0 + (warp + i * WARPS) * KEYS + lane;
     return i < mine && lane < KEYS && pos < k1 ? __ldg(table + (pos >> a.page_shift)) : -1;
@@ -145,12 +226,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2) attn_rows_kernel(const AttnArgs
   auto copy_tile = [&](int i, int page) {
     const int st = i % STAGES;
     const int pos = k0 + (warp + i * WARPS) * KEYS + lane;
-    const bool wanted = lane < KEYS && pos < k1;
-    int slot = -1;
-    if (wanted) {
-      if (page >= 0 && page < p.num_pages) slot = (page * p.kv_heads + kh) * p.page_size + (pos & (p.page_size - 1));
-      else if (p.status) atomicCAS(p.status, 0, 84);
-    }
+    const int slot = key_slot(a, u, pos, lane < KEYS && pos < k1, page);
     const uint32_t kd = ring + st * L::STAGE, vd = kd + L::TILE;
     constexpr int CH = L::RB / 16;
 #pragma unroll
@@ -210,8 +286,8 @@ __global__ void __launch_bounds__(WARPS * 32, 2) attn_rows_kernel(const AttnArgs
         for (int n = 0; n < KEYS / 8; ++n) {
           const uint32_t w = lds32(kd + swz<L::RB>(n * 8 + g, ks) + 4 * t);
           uint32_t f0, f1;
-          codes_to_16<TYPE>(w, f0, f1);
-          mma16816<TYPE>(s[n], qf[ks], f0, f1);
+          codes_to_f16(w, f0, f1);
+          mma16816<MATH>(s[n], qf[ks], f0, f1);
         }
     }
 
@@ -220,21 +296,21 @@ __global__ void __launch_bounds__(WARPS * 32, 2) attn_rows_kernel(const AttnArgs
     float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
     for (int n = 0; n < KEYS / 8; ++n) {
-      float ks[2] = {a.scale_log2, a.scale_log2}, lv[2] = {0.f, 0.f};
+      float ks[2] = {1.f, 1.f}, lv[2] = {0.f, 0.f};
       if (E4M3) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          ks[e] *= __uint_as_float(lds32(vd + L::TILE + (n * 8 + 2 * t + e) * 4));
+          ks[e] = __uint_as_float(lds32(vd + L::TILE + (n * 8 + 2 * t + e) * 4));
           const float vs = positive_scale(__uint_as_float(lds32(vd + L::TILE + (KEYS + n * 8 + 2 * t + e) * 4)));
           lv[e] = lg2(vs);
-          inv_vs[n][e] = __frcp_rn(vs);
+          inv_vs[n][e] = rcp(vs);
         }
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int key = n * 8 + 2 * t + (e & 1);
         const bool seen = base + key <= limit[e >> 1] && (there >> key & 1u);
-        s[n][e] = seen ? fmaf(s[n][e], ks[e & 1], lv[e & 1]) : -INFINITY;
+        s[n][e] = seen ? fmaf(s[n][e] * row_scale[e >> 1], ks[e & 1], lv[e & 1]) : -INFINITY;
         top[e >> 1] = fmaxf(top[e >> 1], s[n][e]);
       }
     }
@@ -257,8 +333,8 @@ __global__ void __launch_bounds__(WARPS * 32, 2) attn_rows_kernel(const AttnArgs
         s[n][e] = ex2(s[n][e] - ref[e >> 1]);
         l[e >> 1] += E4M3 ? s[n][e] * inv_vs[n][e & 1] : s[n][e];
       }
-      pf[n >> 1][(n & 1) * 2] = pack16<TYPE>(s[n][0], s[n][1]);
-      pf[n >> 1][(n & 1) * 2 + 1] = pack16<TYPE>(s[n][2], s[n][3]);
+      pf[n >> 1][(n & 1) * 2] = pack16<MATH>(s[n][0], s[n][1]);
+      pf[n >> 1][(n & 1) * 2 + 1] = pack16<MATH>(s[n][2], s[n][3]);
     }
 #pragma unroll
     for (int n = 0; n < DH / 8; ++n)
@@ -285,12 +361,12 @@ __global__ void __launch_bounds__(WARPS * 32, 2) attn_rows_kernel(const AttnArgs
           for (int q4 = 0; q4 < 4; ++q4)
             w[q4] = lds32(vd + swz<L::RB>(kk * 16 + 2 * t + (q4 & 1) + (q4 >> 1) * 8, 2 * c + (g >> 2)) + 4 * (g & 3));
           uint32_t lo[4], hi[4];
-          codes_to_16<TYPE>(__byte_perm(w[0], w[1], 0x5140), lo[0], lo[1]);
-          codes_to_16<TYPE>(__byte_perm(w[0], w[1], 0x7362), lo[2], lo[3]);
-          codes_to_16<TYPE>(__byte_perm(w[2], w[3], 0x5140), hi[0], hi[1]);
-          codes_to_16<TYPE>(__byte_perm(w[2], w[3], 0x7362), hi[2], hi[3]);
+          codes_to_f16(__byte_perm(w[0], w[1], 0x5140), lo[0], lo[1]);
+          codes_to_f16(__byte_perm(w[0], w[1], 0x7362), lo[2], lo[3]);
+          codes_to_f16(__byte_perm(w[2], w[3], 0x5140), hi[0], hi[1]);
+          codes_to_f16(__byte_perm(w[2], w[3], 0x7362), hi[2], hi[3]);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) mma16816<TYPE>(o[4 * c + e], pf[kk], lo[e], hi[e]);
+          for (int e = 0; e < 4; ++e) mma16816<MATH>(o[4 * c + e], pf[kk], lo[e], hi[e]);
         }
     }
     __syncwarp();   // the stage may be overwritten
@@ -322,46 +398,20 @@ __global__ void __launch_bounds__(WARPS * 32, 2) attn_rows_kernel(const AttnArgs
       os[(warp * ROW_TILE + g + 8 * (e >> 1)) * (DH + 4) + d] = o[n][e];
     }
   __syncthreads();
-  for (int i = threadIdx.x; i < n_rows * (DH / 8); i += WARPS * 32) {
-    const int rr = i / (DH / 8), d = i % (DH / 8) * 8;
-    float top = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) top = fmaxf(top, ml[w * ROW_TILE + rr]);
-    const float ref = top == -INFINITY ? 0.f : top;
-    float sum = 0.f, acc[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) acc[e] = 0.f;
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) {
-      const float f = ex2(ml[w * ROW_TILE + rr] - ref);
-      sum += f * ml[(WARPS + w) * ROW_TILE + rr];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) acc[e] += f * os[(w * ROW_TILE + rr) * (DH + 4) + d + e];
-    }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) acc[e] *= inv;
-    const int64_t at = (int64_t)(r.x + (local + rr) / a.group) * a.heads + kh * a.group + (local + rr) % a.group;
-    if (a.part_o) {
-      store_f<float, 8>(a.part_o + (at * a.splits + split) * DH + d, acc);
-      if (d == 0) a.part_lse[at * a.splits + split] = sum == 0.f ? -INFINITY : top + log2f(sum);
-    } else {
-      store_f<T, 8>((T*)a.out + at * DH + d, acc);
-    }
-  }
+  join_and_store<T>(a, u, ml, DH);
 }
 
 // Joins the parts of a context: o = sum_s 2^(lse_s - max) o_s / sum_s 2^(lse_s - max).  A group of LANES threads owns a (token, head),
 // four elements each; with SHARE > 1 so many groups share its parts (few rows, many parts), which are then added in their order.
 constexpr int COMBINE_THREADS = 128;
 
-template <int TYPE, int LANES, int SHARE>
+template <int TYPE, int LANES, int RUNS, int SHARE>
 __global__ void __launch_bounds__(COMBINE_THREADS) combine_kernel(const AttnArgs a) {
   using T = typename Elem<TYPE>::T;
-  constexpr int GROUPS = COMBINE_THREADS / LANES, ROWS = GROUPS / SHARE;
-  __shared__ float part[SHARE > 1 ? GROUPS : 1][LANES * 4 + 1];
+  constexpr int GROUPS = COMBINE_THREADS / LANES, ROWS = GROUPS / SHARE, WIDTH = LANES * 4 * RUNS;
+  __shared__ float part[SHARE > 1 ? GROUPS : 1][SHARE > 1 ? WIDTH + 1 : 1];
   const lbi_paged_batch& p = a.b;
-  const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES, share = group % SHARE, dim = p.head_dim, d = lane * 4;
+  const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES, share = group % SHARE, dim = p.head_dim;
   const int64_t at = (int64_t)blockIdx.x * ROWS + group / SHARE;
   const bool exists = at < (int64_t)p.rows * a.heads;
   const bool owned = exists && at / a.heads < last_row(p);
@@ -372,38 +422,55 @@ __global__ void __launch_bounds__(COMBINE_THREADS) combine_kernel(const AttnArgs
 #pragma unroll
   for (int o = 1; o < LANES; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   const float ref = top == -INFINITY ? 0.f : top;
-  float acc[4] = {0.f, 0.f, 0.f, 0.f}, sum = 0.f;
+  float acc[RUNS][4], sum = 0.f;
+#pragma unroll
+  for (int r = 0; r < RUNS; ++r)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[r][e] = 0.f;
   if (owned) {
 #pragma unroll 4
     for (int s = share; s < a.splits; s += SHARE) {
       const float w = ex2(__ldg(lse + s) - ref);
-      const float4 x = d < dim ? __ldg(reinterpret_cast<const float4*>(a.part_o + (at * a.splits + s) * dim + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
       sum += w;
-      acc[0] += w * x.x;
-      acc[1] += w * x.y;
-      acc[2] += w * x.z;
-      acc[3] += w * x.w;
+#pragma unroll
+      for (int r = 0; r < RUNS; ++r) {
+        const int d = (r * LANES + lane) * 4;
+        const float4 x = d < dim ? __ldg(reinterpret_cast<const float4*>(a.part_o + (at * a.splits + s) * dim + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        acc[r][0] += w * x.x;
+        acc[r][1] += w * x.y;
+        acc[r][2] += w * x.z;
+        acc[r][3] += w * x.w;
+      }
     }
   }
   if (SHARE > 1) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) part[group][d + e] = acc[e];
-    if (lane == 0) part[group][LANES * 4] = sum;
+    for (int r = 0; r < RUNS; ++r)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) part[group][(r * LANES + lane) * 4 + e] = acc[r][e];
+    if (lane == 0) part[group][WIDTH] = sum;
     __syncthreads();
     if (share == 0) {
 #pragma unroll
       for (int g = 1; g < SHARE; ++g) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[e] += part[group + g][d + e];
-        sum += part[group + g][LANES * 4];
+        for (int r = 0; r < RUNS; ++r)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[r][e] += part[group + g][(r * LANES + lane) * 4 + e];
+        sum += part[group + g][WIDTH];
       }
     }
   }
-  if (share != 0 || !exists || d >= dim || (!owned && !a.zero_tail)) return;
+  if (share != 0 || !exists || (!owned && !a.zero_tail)) return;
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) acc[e] *= inv;
-  store_f<T, 4>((T*)a.out + at * dim + d, acc);
+  for (int r = 0; r < RUNS; ++r) {
+    const int d = (r * LANES + lane) * 4;
+    if (d >= dim) break;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[r][e] *= inv;
+    store_f<T, 4>((T*)a.out + at * dim + d, acc[r]);
+  }
 }
 
 template <int TYPE>
@@ -411,75 +478,254 @@ int launch_combine(const AttnArgs& a, int sm_count, cudaStream_t st) {
   // several groups per row where the rows alone give less than two blocks per SM
   const int64_t rows = (int64_t)a.b.rows * a.heads;
   const bool few = rows < 2ll * sm_count * 4 && a.splits >= 8;
-  const int lanes = a.b.head_dim <= 32 ? 8 : a.b.head_dim <= 64 ? 16 : a.b.head_dim <= 128 ? 32 : 64;
-  const int64_t per_block = COMBINE_THREADS / lanes / (few ? (lanes == 64 ? 2 : 4) : 1), blocks = (rows + per_block - 1) / per_block;
+  const int dim = a.b.head_dim, lanes = dim <= 32 ? 8 : dim <= 64 ? 16 : 32;
+  const int64_t per_block = COMBINE_THREADS / lanes / (few ? 4 : 1), blocks = (rows + per_block - 1) / per_block;
   if (blocks >= (1ll << 31)) return (int)cudaErrorInvalidValue;
-#define LBI_COMBINE(L, S) combine_kernel<TYPE, L, S><<<(unsigned)blocks, COMBINE_THREADS, 0, st>>>(a)
-  if (lanes == 8) { if (few) LBI_COMBINE(8, 4); else LBI_COMBINE(8, 1); }
-  else if (lanes == 16) { if (few) LBI_COMBINE(16, 4); else LBI_COMBINE(16, 1); }
-  else { if (few) LBI_COMBINE(32, 4); else LBI_COMBINE(32, 1); }
+#define LBI_COMBINE(L, R)                                                                          \
+  do {                                                                                             \
+    if (few) combine_kernel<TYPE, L, R, 4><<<(unsigned)blocks, COMBINE_THREADS, 0, st>>>(a);        \
+    else combine_kernel<TYPE, L, R, 1><<<(unsigned)blocks, COMBINE_THREADS, 0, st>>>(a);            \
+  } while (0)
+  if (lanes == 8) LBI_COMBINE(8, 1);
+  else if (lanes == 16) LBI_COMBINE(16, 1);
+  else if (dim <= 128) LBI_COMBINE(32, 1);
+  else LBI_COMBINE(32, 2);
 #undef LBI_COMBINE
   return (int)cudaGetLastError();
 }
 
-// ------------------------------------------------------------------------------------------------ one warp per row
-// fp32 queries and head sizes without a tile: the lanes share the head's elements, the running maximum, sum and output stay in
-// registers in fp32 and every key is read once.  e4m3 pages: the key's scale multiplies its score, the value's its probability.
-
-template <int TYPE, bool E4M3>
-__global__ void __launch_bounds__(128) attn_row_kernel(const AttnArgs a) {
-  using T = typename Elem<TYPE>::T;
+// ------------------------------------------------------------------------------------------------ 16-row tiles, any type and size
+// The same division of work with mma.sync m16n8k8 on tf32 operands: an fp32 value is the sum of two tf32 values up to 2^-22 of it, and
+// hi hi + hi lo + lo hi of two such sums lacks only lo lo.  16-bit values and codes are tf32 values as they stand, and need one product
+// less.  P is split like an fp32 operand for fp32 queries, and rounded to tf32 for 16-bit ones (as fine as fp16, finer than bf16).
+// Queries lie in shared memory in the order of the fragments; keys and values as they come, a row padded by 16 bytes, so that the eight
+// keys (or four pairs of them) of a fragment lie in different banks.
+template <int TYPE, bool E4M3, int DHP>
+struct AnyTile {   // DHP: head_dim rounded up to 64, 128 or 256
+  using Q = typename Elem<TYPE>::T;
   using C = typename Elem<E4M3 ? LBI_E4M3 : TYPE>::T;
-  const lbi_paged_batch& p = a.b;
-  const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31, dim = p.head_dim;
-  const int row = (int)(unit / a.heads), head = (int)(unit % a.heads);
-  if (row >= p.rows) return;
-  T* out = (T*)a.out + ((int64_t)row * a.heads + head) * dim;
-  float q[8], o[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) q[e] = o[e] = 0.f;
-  float l = 0.f;
-  if (row < last_row(p)) {
-    const int b = seq_of_row(p, row);
-    const int2 r = seq_rows(p, b);
-    const int ctx = __ldg(p.context + b);
-    const int keys = min(ctx - (r.y - row) + 1, p.table_width << a.page_shift);
-    const int kh = head / (a.heads / p.kv_heads);
-    const T* src = (const T*)a.q + (int64_t)row * a.q_stride + head * dim;
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (lane + 32 * e < dim) q[e] = to_f<T>(src[lane + 32 * e]) * a.scale_log2;
-    float m = -INFINITY;
-    for (int j = 0; j < keys; ++j) {
-      const int page = page_of(p, b, j, a.page_shift);
-      if (page < 0) continue;
-      const int64_t slot = ((int64_t)page * p.kv_heads + kh) * p.page_size + (j & (p.page_size - 1));
-      const C* kp = (const C*)p.k + slot * dim;
-      const C* vp = (const C*)p.v + slot * dim;
-      float s = 0.f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (lane + 32 * e < dim) s += q[e] * to_f<C>(kp[lane + 32 * e]);
-      s = warp_sum(s);
-      if (E4M3) s *= __ldg(p.k_scale + slot);
-      const float mn = fmaxf(m, s);
-      const float keep = exp2f(m - mn);
-      float w = exp2f(s - mn);
-      l = l * keep + w;
-      m = mn;
-      if (E4M3) w *= __ldg(p.v_scale + slot);
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (lane + 32 * e < dim) o[e] = o[e] * keep + w * to_f<C>(vp[lane + 32 * e]);
-    }
-  } else if (!a.zero_tail) {
-    return;
+  static constexpr int KEYS = DHP == 256 ? 8 : 16, STAGES = 2;
+  static constexpr bool Q_LO = TYPE == LBI_F32, C_LO = TYPE == LBI_F32 && !E4M3, P_LO = TYPE == LBI_F32;
+  static constexpr int Q_BYTES = DHP / 8 * 32 * 16 * (Q_LO ? 2 : 1);
+  __host__ __device__ static int pitch(int dim) { return dim * (int)sizeof(C) + 16; }
+  __host__ __device__ static int stage(int dim) { return 2 * KEYS * pitch(dim) + 8 * KEYS + 16; }   // K, V, scales, which keys exist
+  __host__ __device__ static int smem(int dim) {
+    const int join = WARPS * ROW_TILE * (dim + 4) * 4 + WARPS * ROW_TILE * 8, ring = WARPS * STAGES * stage(dim);
+    return Q_BYTES + (join > ring ? join : ring);
   }
-  const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
+};
+
+__device__ __forceinline__ uint32_t tf32(float x) {
+  uint32_t r;
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ void mma1688(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+template <int TYPE, bool E4M3, int DHP>
+__global__ void __launch_bounds__(WARPS * 32) attn_any_kernel(const AttnArgs a) {
+  using L = AnyTile<TYPE, E4M3, DHP>;
+  using T = typename L::Q;
+  using C = typename L::C;
+  constexpr int KEYS = L::KEYS, STAGES = L::STAGES;
+  extern __shared__ __align__(128) uint8_t smem[];
+  const lbi_paged_batch& p = a.b;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, dim = p.head_dim;
+  zero_rows_of_nobody<T>(a);
+  const RowsUnit u = rows_unit(a);
+  if (!u.any) return;
+
+  uint4* qs = reinterpret_cast<uint4*>(smem);   // [8 elements][lane]: hi, then (fp32) lo
+  int limit[2];
+  for (int ks = warp; ks < dim / 8; ks += WARPS) {
+    float x[4];
 #pragma unroll
-  for (int e = 0; e < 8; ++e)
-    if (lane + 32 * e < dim) out[lane + 32 * e] = from_f<T>(o[e] * inv);
+    for (int e = 0; e < 4; ++e) {
+      const int r = g + 8 * (e & 1), rr = u.local + r;
+      x[e] = r < u.n_rows ? to_f<T>(((const T*)a.q)[(int64_t)(u.first_row + rr / a.group) * a.q_stride + (u.kh * a.group + rr % a.group) * dim + ks * 8 + t + 4 * (e >> 1)]) : 0.f;
+    }
+    uint32_t hi[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) hi[e] = tf32(x[e]);
+    qs[(ks * 32 + lane) * (L::Q_LO ? 2 : 1)] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+    if (L::Q_LO)
+      qs[(ks * 32 + lane) * 2 + 1] = make_uint4(tf32(x[0] - __uint_as_float(hi[0])), tf32(x[1] - __uint_as_float(hi[1])),
+                                                tf32(x[2] - __uint_as_float(hi[2])), tf32(x[3] - __uint_as_float(hi[3])));
+  }
+#pragma unroll
+  for (int hh = 0; hh < 2; ++hh) limit[hh] = g + 8 * hh < u.n_rows ? u.first_pos + (u.local + g + 8 * hh) / a.group : -1;
+  __syncthreads();
+
+  float o[DHP / 8][4];
+#pragma unroll
+  for (int i = 0; i < DHP / 8; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+
+  const int pitch = L::pitch(dim), stage = L::stage(dim), tile_bytes = KEYS * pitch;
+  uint8_t* ring = smem + L::Q_BYTES + warp * STAGES * stage;
+  const int n_tiles = u.k1 > u.k0 ? (u.k1 - u.k0 + KEYS - 1) / KEYS : 0;
+  const int mine = n_tiles > warp ? (n_tiles - warp + WARPS - 1) / WARPS : 0;
+  const int* table = p.table + (int64_t)u.b * p.table_stride;
+  auto load_page = [&](int i) {
+    const int pos = u.k0 + (warp + i * WARPS) * KEYS + lane;
+    return i < mine && lane < KEYS && pos < u.k1 ? __ldg(table + (pos >> a.page_shift)) : -1;
+  };
+  const int row_chunks = dim * (int)sizeof(C) / 16;
+  auto copy_tile = [&](int i, int page) {
+    const int pos = u.k0 + (warp + i * WARPS) * KEYS + lane;
+    const int slot = key_slot(a, u, pos, lane < KEYS && pos < u.k1, page);
+    uint8_t* k_dst = ring + (i % STAGES) * stage;
+    uint8_t* v_dst = k_dst + tile_bytes;
+    for (int j = 0; j < KEYS * row_chunks; j += 32) {   // KEYS * row_chunks is a multiple of 8, the last round may be partial
+      const int row = min((j + lane) / row_chunks, KEYS - 1), c = (j + lane) - row * row_chunks;
+      const int s = __shfl_sync(0xffffffffu, slot, row);
+      if (c < row_chunks) {
+        const int64_t off = (int64_t)max(s, 0) * dim * sizeof(C) + c * 16;
+        cp_async16(smem_addr(k_dst + row * pitch + c * 16), (const uint8_t*)p.k + off, s >= 0);
+        cp_async16(smem_addr(v_dst + row * pitch + c * 16), (const uint8_t*)p.v + off, s >= 0);
+      }
+    }
+    uint8_t* extra = k_dst + 2 * tile_bytes;
+    if (E4M3 && lane < KEYS) {
+      cp_async4(smem_addr(extra + lane * 4), p.k_scale + max(slot, 0), slot >= 0);
+      cp_async4(smem_addr(extra + (KEYS + lane) * 4), p.v_scale + max(slot, 0), slot >= 0);
+    }
+    const uint32_t there = __ballot_sync(0xffffffffu, slot >= 0);
+    if (lane == 0) *reinterpret_cast<volatile uint32_t*>(extra + 8 * KEYS) = there;
+  };
+
+  int page = load_page(0);
+#pragma unroll
+  for (int i = 0; i < STAGES - 1; ++i) {
+    const int next = load_page(i + 1);
+    if (i < mine) copy_tile(i, page);
+    cp_async_commit();
+    page = next;
+  }
+  for (int i = 0; i < mine; ++i) {
+    cp_async_wait<STAGES - 2>();
+    __syncwarp();
+    const int next = load_page(i + STAGES);
+    if (i + STAGES - 1 < mine) copy_tile(i + STAGES - 1, page);
+    cp_async_commit();
+    page = next;
+    const uint8_t* k_src = ring + (i % STAGES) * stage;
+    const uint8_t* v_src = k_src + tile_bytes;
+    const uint8_t* extra = v_src + tile_bytes;
+    const int base = u.k0 + (warp + i * WARPS) * KEYS;
+
+    float s[KEYS / 8][4];
+#pragma unroll
+    for (int n = 0; n < KEYS / 8; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
+#pragma unroll 4
+    for (int ks = 0; ks < dim / 8; ++ks) {
+      const uint4 qh = qs[(ks * 32 + lane) * (L::Q_LO ? 2 : 1)];
+      alignas(16) uint32_t ql[4] = {0, 0, 0, 0};
+      if (L::Q_LO) *reinterpret_cast<uint4*>(ql) = qs[(ks * 32 + lane) * 2 + 1];
+#pragma unroll
+      for (int n = 0; n < KEYS / 8; ++n) {
+        const C* row = reinterpret_cast<const C*>(k_src + (n * 8 + g) * pitch) + ks * 8 + t;
+        const float x0 = to_f<C>(row[0]), x1 = to_f<C>(row[4]);
+        const uint32_t h0 = tf32(x0), h1 = tf32(x1);
+        if (L::C_LO) mma1688(s[n], reinterpret_cast<const uint32_t*>(&qh), tf32(x0 - __uint_as_float(h0)), tf32(x1 - __uint_as_float(h1)));
+        if (L::Q_LO) mma1688(s[n], ql, h0, h1);
+        mma1688(s[n], reinterpret_cast<const uint32_t*>(&qh), h0, h1);
+      }
+    }
+
+    const uint32_t there = *reinterpret_cast<const volatile uint32_t*>(extra + 8 * KEYS);
+    float vs[KEYS / 8][2], top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int n = 0; n < KEYS / 8; ++n) {
+      float ks[2] = {a.scale_log2, a.scale_log2};
+      if (E4M3) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          ks[e] *= reinterpret_cast<const float*>(extra)[n * 8 + 2 * t + e];
+          vs[n][e] = reinterpret_cast<const float*>(extra)[KEYS + n * 8 + 2 * t + e];
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int key = n * 8 + 2 * t + (e & 1);
+        const bool seen = base + key <= limit[e >> 1] && (there >> key & 1u);
+        s[n][e] = seen ? s[n][e] * ks[e & 1] : -INFINITY;
+        top[e >> 1] = fmaxf(top[e >> 1], s[n][e]);
+      }
+    }
+    float keep[2], ref[2];
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh) {
+      top[hh] = fmaxf(top[hh], __shfl_xor_sync(0xffffffffu, top[hh], 1));
+      top[hh] = fmaxf(top[hh], __shfl_xor_sync(0xffffffffu, top[hh], 2));
+      const float mn = fmaxf(m[hh], top[hh]);
+      ref[hh] = mn == -INFINITY ? 0.f : mn;
+      keep[hh] = ex2(m[hh] - ref[hh]);
+      m[hh] = mn;
+      l[hh] *= keep[hh];
+    }
+#pragma unroll
+    for (int n = 0; n < DHP / 8; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[n][e] *= keep[e >> 1];
+#pragma unroll
+    for (int kk = 0; kk < KEYS / 8; ++kk) {
+      // keys 2 t and 2 t + 1 of the eight take the places t and t + 4 of the product's inner index, for P and V alike
+      uint32_t ph[4], pl[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float w = ex2(s[kk][e] - ref[e >> 1]);
+        l[e >> 1] += w;
+        if (E4M3) w *= vs[kk][e & 1];
+        const int at = (e >> 1) + 2 * (e & 1);
+        ph[at] = tf32(w);
+        pl[at] = tf32(w - __uint_as_float(ph[at]));
+      }
+      const C* row0 = reinterpret_cast<const C*>(v_src + (kk * 8 + 2 * t) * pitch) + g;
+      const C* row1 = reinterpret_cast<const C*>(v_src + (kk * 8 + 2 * t + 1) * pitch) + g;
+#pragma unroll
+      for (int n = 0; n < DHP / 8; ++n) {
+        if (n * 8 >= dim) break;
+        const float x0 = to_f<C>(row0[n * 8]), x1 = to_f<C>(row1[n * 8]);
+        const uint32_t h0 = tf32(x0), h1 = tf32(x1);
+        if (L::C_LO) mma1688(o[n], ph, tf32(x0 - __uint_as_float(h0)), tf32(x1 - __uint_as_float(h1)));
+        if (L::P_LO) mma1688(o[n], pl, h0, h1);
+        mma1688(o[n], ph, h0, h1);
+      }
+    }
+    __syncwarp();
+  }
+  cp_async_wait<0>();
+#pragma unroll
+  for (int hh = 0; hh < 2; ++hh) {
+    l[hh] += __shfl_xor_sync(0xffffffffu, l[hh], 1);
+    l[hh] += __shfl_xor_sync(0xffffffffu, l[hh], 2);
+  }
+  __syncthreads();
+  float* ml = reinterpret_cast<float*>(smem + L::Q_BYTES);
+  float* os = ml + 2 * WARPS * ROW_TILE;
+  if (t == 0) {
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh) {
+      ml[warp * ROW_TILE + g + 8 * hh] = m[hh];
+      ml[(WARPS + warp) * ROW_TILE + g + 8 * hh] = l[hh];
+    }
+  }
+#pragma unroll
+  for (int n = 0; n < DHP / 8; ++n) {
+    if (n * 8 >= dim) break;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) os[(warp * ROW_TILE + g + 8 * (e >> 1)) * (dim + 4) + 8 * n + 2 * t + (e & 1)] = o[n][e];
+  }
+  __syncthreads();
+  join_and_store<T>(a, u, ml, dim);
 }
 
 // ------------------------------------------------------------------------------------------------ host side
@@ -505,13 +751,24 @@ int launch_rows(const AttnArgs& a, cudaStream_t st) {   // about 8 KB of keys an
        : a.b.head_dim == 64  ? launch_rows<TYPE, false, 64, 32, 3>(a, st) : launch_rows<TYPE, false, 32, 32, 5>(a, st);
 }
 
-template <int TYPE>
-int launch_row(const AttnArgs& a, cudaStream_t st) {
-  const int64_t blocks = ((int64_t)a.b.rows * a.heads + 3) / 4;
+template <int TYPE, bool E4M3, int DHP>
+int launch_any(const AttnArgs& a, cudaStream_t st) {
+  using L = AnyTile<TYPE, E4M3, DHP>;
+  auto kernel = attn_any_kernel<TYPE, E4M3, DHP>;
+  static lbi::PerDeviceOnce once;
+  cudaError_t e = once.max_dynamic_smem(kernel, L::smem(DHP));
+  if (e != cudaSuccess) return (int)e;
+  const int64_t blocks = tile_bound(a.b, a.group, ROW_TILE) * a.b.kv_heads * a.splits;
   if (blocks >= (1ll << 31)) return (int)cudaErrorInvalidValue;
-  if (a.b.cache_type == LBI_E4M3) attn_row_kernel<TYPE, true><<<(unsigned)blocks, 128, 0, st>>>(a);
-  else attn_row_kernel<TYPE, false><<<(unsigned)blocks, 128, 0, st>>>(a);
+  kernel<<<(unsigned)blocks, WARPS * 32, L::smem(a.b.head_dim), st>>>(a);
   return (int)cudaGetLastError();
+}
+template <int TYPE>
+int launch_any(const AttnArgs& a, cudaStream_t st) {
+  const int dim = a.b.head_dim;
+  if (a.b.cache_type == LBI_E4M3)
+    return dim <= 64 ? launch_any<TYPE, true, 64>(a, st) : dim <= 128 ? launch_any<TYPE, true, 128>(a, st) : launch_any<TYPE, true, 256>(a, st);
+  return dim <= 64 ? launch_any<TYPE, false, 64>(a, st) : dim <= 128 ? launch_any<TYPE, false, 128>(a, st) : launch_any<TYPE, false, 256>(a, st);
 }
 
 }  // namespace paged
@@ -520,12 +777,13 @@ int launch_row(const AttnArgs& a, cudaStream_t st) {
 extern "C" lbi_attention_plan lbi_paged_attention_plan(const lbi_paged_batch* p, int type, int heads, float scale, int64_t max_context, int sm_count) {
   using namespace lbi::paged;
   lbi_attention_plan plan{0, 1, 1 << 30};
-  if (type == LBI_F32 || p->rows == 0 || p->batch == 0 || !(p->head_dim == 32 || p->head_dim == 64 || p->head_dim == 128)) return plan;
+  if (p->rows == 0 || p->batch == 0) return plan;
   const int group = heads / p->kv_heads;
   const int64_t capacity = (int64_t)p->table_width * p->page_size;
   const int64_t longest = max_context > 0 ? std::min(max_context, capacity) : capacity;
   // the tcgen05 kernel takes its row maximum before the scale, so it needs a positive one
-  plan.kernel = p->head_dim >= 64 && (int64_t)p->rows * group >= 64ll * p->batch && scale > 0.f ? 2 : 1;
+  const bool tiled = type != LBI_F32 && (p->head_dim == 32 || p->head_dim == 64 || p->head_dim == 128);
+  plan.kernel = !tiled ? 0 : p->head_dim >= 64 && (int64_t)p->rows * group >= 64ll * p->batch && scale > 0.f ? 2 : 1;
   if (plan.kernel == 2) {
     // One block per SM, or two (head_dim 64, 16-bit pages).  Parts of a context pay where whole units leave the last round of blocks half empty: the
     // number of parts (of 512 keys at least) with the fewest key tiles per SM, 4 % added per part for the partial results and the
@@ -563,9 +821,10 @@ extern "C" int lbi_paged_attention(const lbi_paged_batch* p, const void* q, int6
   if ((plan.splits > 1) != (part_o != nullptr)) return (int)cudaErrorInvalidValue;
   AttnArgs a{*p, q, q_stride, out, part_o, part_lse, heads, heads / p->kv_heads, zero_tail, shift_of(p->page_size), plan.splits, plan.split_keys,
              scale * 1.4426950408889634f};
-  if (plan.kernel == 0)
-    return type == LBI_F32 ? launch_row<LBI_F32>(a, st) : type == LBI_BF16 ? launch_row<LBI_BF16>(a, st) : launch_row<LBI_F16>(a, st);
-  const int rc = plan.kernel == 2 ? launch_attn_tiles(a, type, st) : type == LBI_BF16 ? launch_rows<LBI_BF16>(a, st) : launch_rows<LBI_F16>(a, st);
+  int rc;
+  if (plan.kernel == 0) rc = type == LBI_F32 ? launch_any<LBI_F32>(a, st) : type == LBI_BF16 ? launch_any<LBI_BF16>(a, st) : launch_any<LBI_F16>(a, st);
+  else if (plan.kernel == 1) rc = type == LBI_BF16 ? launch_rows<LBI_BF16>(a, st) : launch_rows<LBI_F16>(a, st);
+  else rc = launch_attn_tiles(a, type, st);
   if (rc != 0 || plan.splits == 1) return rc;
-  return type == LBI_BF16 ? launch_combine<LBI_BF16>(a, sm_count, st) : launch_combine<LBI_F16>(a, sm_count, st);
+  return type == LBI_F32 ? launch_combine<LBI_F32>(a, sm_count, st) : type == LBI_BF16 ? launch_combine<LBI_BF16>(a, sm_count, st) : launch_combine<LBI_F16>(a, sm_count, st);
 }

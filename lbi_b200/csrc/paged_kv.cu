@@ -51,15 +51,14 @@ __global__ void __launch_bounds__(APPEND_THREADS, 8) append_kernel(const AppendA
   };
   load(first);   // before anything is known about the token, and then one head row ahead
 
-  const bool owned = row < last_row(p);
-  if (!owned && !a.zero_tail) return;
   int pos = -1, page = -1;
   bool turn_ok = true;
-  if (owned) {
-    const int b = seq_of_row(p, row);
-    const int2 r = seq_rows(p, b);
-    pos = __ldg(p.context + b) - (r.y - r.x) + (row - r.x);
-    if (pos >= 0) page = page_of(p, b, pos, a.page_shift);
+  Place at = {0, 0, 0, false};
+  if (p.batch > 0) at = place_of_row(p, row);
+  if (!at.owned && !a.zero_tail) return;
+  if (at.owned) {
+    pos = __ldg(p.context + at.b) - (at.last - row);
+    if (pos >= 0) page = page_of(p, at.b, pos, a.page_shift);
     if (a.cos_tab && pos >= a.rope_rows) {
       turn_ok = false;
       if (threadIdx.x == 0 && p.status) atomicCAS(p.status, 0, 83);
