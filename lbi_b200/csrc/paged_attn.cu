@@ -496,7 +496,9 @@ int launch_combine(const AttnArgs& a, int sm_count, cudaStream_t st) {
 
 // ------------------------------------------------------------------------------------------------ 16-row tiles, any type and size
 // The same division of work with mma.sync m16n8k8 on tf32 operands: an fp32 value is the sum of two tf32 values up to 2^-22 of it, and
-// hi hi + hi lo + lo hi of two such sums lacks only lo lo.  16-bit values and codes are tf32 values as they stand, and need one product
+// hi hi + hi lo + lo hi of two such sums lacks only lo lo.  The products of one step of eight (of one key tile) start from zero and are
+// added to the running sums by the FMA units, which round to nearest: the tensor core truncates, and over thousands of keys that is a
+// drift (2 to 3 e-6 of the result, against 3.5 e-7).  16-bit values and codes are tf32 values as they stand, and need one product
 // less.  P is split like an fp32 operand for fp32 queries, and rounded to tf32 for 16-bit ones (as fine as fp16, finer than bf16).
 // Queries lie in shared memory in the order of the fragments; keys and values as they come, a row padded by 16 bytes, so that the eight
 // keys (or four pairs of them) of a fragment lie in different banks.
@@ -634,9 +636,12 @@ __global__ void __launch_bounds__(WARPS * 32) attn_any_kernel(const AttnArgs a) 
         const C* row = reinterpret_cast<const C*>(k_src + (n * 8 + g) * pitch) + ks * 8 + t;
         const float x0 = to_f<C>(row[0]), x1 = to_f<C>(row[4]);
         const uint32_t h0 = tf32(x0), h1 = tf32(x1);
-        if (L::C_LO) mma1688(s[n], reinterpret_cast<const uint32_t*>(&qh), tf32(x0 - __uint_as_float(h0)), tf32(x1 - __uint_as_float(h1)));
-        if (L::Q_LO) mma1688(s[n], ql, h0, h1);
-        mma1688(s[n], reinterpret_cast<const uint32_t*>(&qh), h0, h1);
+        float c[4] = {0.f, 0.f, 0.f, 0.f};
+        if (L::C_LO) mma1688(c, reinterpret_cast<const uint32_t*>(&qh), tf32(x0 - __uint_as_float(h0)), tf32(x1 - __uint_as_float(h1)));
+        if (L::Q_LO) mma1688(c, ql, h0, h1);
+        mma1688(c, reinterpret_cast<const uint32_t*>(&qh), h0, h1);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[n][e] += c[e];
       }
     }
 
@@ -671,34 +676,35 @@ __global__ void __launch_bounds__(WARPS * 32) attn_any_kernel(const AttnArgs a) 
       m[hh] = mn;
       l[hh] *= keep[hh];
     }
+    // keys 2 t and 2 t + 1 of eight take the places t and t + 4 of the product's inner index, for P and V alike
+    uint32_t ph[KEYS / 8][4], pl[KEYS / 8][4];
 #pragma unroll
-    for (int n = 0; n < DHP / 8; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[n][e] *= keep[e >> 1];
-#pragma unroll
-    for (int kk = 0; kk < KEYS / 8; ++kk) {
-      // keys 2 t and 2 t + 1 of the eight take the places t and t + 4 of the product's inner index, for P and V alike
-      uint32_t ph[4], pl[4];
+    for (int kk = 0; kk < KEYS / 8; ++kk)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         float w = ex2(s[kk][e] - ref[e >> 1]);
         l[e >> 1] += w;
         if (E4M3) w *= vs[kk][e & 1];
         const int at = (e >> 1) + 2 * (e & 1);
-        ph[at] = tf32(w);
-        pl[at] = tf32(w - __uint_as_float(ph[at]));
+        ph[kk][at] = tf32(w);
+        pl[kk][at] = tf32(w - __uint_as_float(ph[kk][at]));
       }
-      const C* row0 = reinterpret_cast<const C*>(v_src + (kk * 8 + 2 * t) * pitch) + g;
-      const C* row1 = reinterpret_cast<const C*>(v_src + (kk * 8 + 2 * t + 1) * pitch) + g;
 #pragma unroll
-      for (int n = 0; n < DHP / 8; ++n) {
-        if (n * 8 >= dim) break;
+    for (int n = 0; n < DHP / 8; ++n) {
+      if (n * 8 >= dim) break;
+      float c[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int kk = 0; kk < KEYS / 8; ++kk) {
+        const C* row0 = reinterpret_cast<const C*>(v_src + (kk * 8 + 2 * t) * pitch) + g;
+        const C* row1 = reinterpret_cast<const C*>(v_src + (kk * 8 + 2 * t + 1) * pitch) + g;
         const float x0 = to_f<C>(row0[n * 8]), x1 = to_f<C>(row1[n * 8]);
         const uint32_t h0 = tf32(x0), h1 = tf32(x1);
-        if (L::C_LO) mma1688(o[n], ph, tf32(x0 - __uint_as_float(h0)), tf32(x1 - __uint_as_float(h1)));
-        if (L::P_LO) mma1688(o[n], pl, h0, h1);
-        mma1688(o[n], ph, h0, h1);
+        if (L::C_LO) mma1688(c, ph[kk], tf32(x0 - __uint_as_float(h0)), tf32(x1 - __uint_as_float(h1)));
+        if (L::P_LO) mma1688(c, pl[kk], h0, h1);
+        mma1688(c, ph[kk], h0, h1);
       }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[n][e] = fmaf(o[n][e], keep[e >> 1], c[e]);
     }
     __syncwarp();
   }
