@@ -1,6 +1,7 @@
 // Python bindings of the serving operators over a paged key / value cache.  Arguments are checked here (ValueError); what only the
 // device knows (lengths, page ids) is bounds-checked by the kernels.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -95,7 +96,10 @@ Tensor aligned_rows(const Tensor& x) {
 }
 
 Tensor output(const OptTensor& out, at::IntArrayRef sizes, const Tensor& like, at::ScalarType type, bool nobody = false) {
-  if (!given(out)) return nobody ? torch::zeros(sizes, like.options().dtype(type)) : torch::empty(sizes, like.options().dtype(type));
+  if (!given(out)) {
+    Tensor made = at::detail::empty_cuda(sizes, type, like.device(), c10::nullopt);   // without the dispatcher: a decode loop waits for the host
+    return nobody ? made.zero_() : made;
+  }
   TORCH_CHECK_VALUE(out->sizes() == sizes && out->scalar_type() == type && out->device() == like.device() && out->is_contiguous() &&
                         (uintptr_t)out->data_ptr() % 16 == 0,
                     "out must be a contiguous tensor of the result's shape and type on its device");
@@ -141,8 +145,8 @@ std::tuple<Tensor, Tensor> kv_gather(const Tensor& k, const Tensor& v, const Opt
   TORCH_CHECK_VALUE(max_len >= 0, "max_len must not be negative");
   c10::cuda::CUDAGuard guard(k.device());
   const lbi_paged_batch p = paged_batch(k, v, k_scale, v_scale, table, context, c10::nullopt, 0);
-  Tensor ko = torch::empty({p.batch, p.kv_heads, max_len, p.head_dim}, k.options().dtype(dtype));
-  Tensor vo = torch::empty_like(ko);
+  Tensor ko = output(c10::nullopt, {p.batch, p.kv_heads, max_len, p.head_dim}, k, dtype);
+  Tensor vo = output(c10::nullopt, {p.batch, p.kv_heads, max_len, p.head_dim}, k, dtype);
   const int type = type_of(ko, "dtype");
   TORCH_CHECK_VALUE(p.cache_type == LBI_E4M3 || p.cache_type == type, "pages that are not e4m3 are read back in their own type");
   check(lbi_kv_gather(&p, ko.data_ptr(), vo.data_ptr(), max_len, type, cur_stream()), "kv_gather");
@@ -167,7 +171,7 @@ Tensor paged_attention(const Tensor& q_in, const Tensor& k, const Tensor& v, con
   const lbi_attention_plan plan = lbi_paged_attention_plan(&p, type, (int)heads, (float)scale, max_context, sm_count);
   Tensor parts;   // results of the parts of a long context, then the logarithms of their sums
   const int64_t part_rows = q.size(0) * heads * plan.splits;
-  if (plan.splits > 1) parts = torch::empty({part_rows * (p.head_dim + 1)}, q.options().dtype(at::kFloat));
+  if (plan.splits > 1) parts = at::detail::empty_cuda({part_rows * (p.head_dim + 1)}, at::kFloat, q.device(), c10::nullopt);
   float* part_o = plan.splits > 1 ? parts.data_ptr<float>() : nullptr;
   check(lbi_paged_attention(&p, q.data_ptr(), q.size(0) > 1 ? q.stride(0) : heads * p.head_dim, o.data_ptr(), part_o,
                             part_o ? part_o + part_rows * p.head_dim : nullptr, plan, type, (int)heads, (float)scale, given(out) ? 0 : 1, sm_count, cur_stream()),
@@ -175,16 +179,20 @@ Tensor paged_attention(const Tensor& q_in, const Tensor& k, const Tensor& v, con
   return o;
 }
 
-const float* per_row(const OptTensor& x, const Tensor& like, const char* name) {
-  if (!given(x)) return nullptr;
-  TORCH_CHECK_VALUE(x->scalar_type() == at::kFloat && x->dim() == 1 && x->size(0) == like.size(0) && x->is_contiguous() && x->device() == like.device(),
+// A penalty is a number or one fp32 entry per row: fills whichever it is.
+void penalty(const py::object& x, const Tensor& like, const char* name, const float** row, float* number) {
+  if (!THPVariable_Check(x.ptr())) {
+    *number = (float)x.cast<double>();
+    return;
+  }
+  const Tensor& t = THPVariable_Unpack(x.ptr());
+  TORCH_CHECK_VALUE(t.scalar_type() == at::kFloat && t.dim() == 1 && t.size(0) == like.size(0) && t.is_contiguous() && t.device() == like.device(),
                     name, " must be a number or a contiguous fp32 tensor with one entry per row");
-  return x->data_ptr<float>();
+  *row = t.data_ptr<float>();
 }
 
-Tensor adjust_logits(const Tensor& logits, const Tensor& tokens, const OptTensor& lengths, const OptTensor& prompt_lengths, const OptTensor& repetition_row,
-                     const OptTensor& presence_row, const OptTensor& frequency_row, double repetition, double presence, double frequency,
-                     const OptTensor& bias, const OptTensor& allowed, const OptTensor& out) {
+Tensor adjust_logits(const Tensor& logits, const Tensor& tokens, const OptTensor& lengths, const OptTensor& prompt_lengths, const py::object& repetition,
+                     const py::object& presence, const py::object& frequency, const OptTensor& bias, const OptTensor& allowed, const OptTensor& out) {
   TORCH_CHECK_VALUE(logits.is_cuda() && logits.dim() == 2 && (logits.size(1) <= 1 || logits.stride(1) == 1),
                     "logits must be a CUDA tensor [batch, vocab], contiguous along the vocabulary");
   c10::cuda::CUDAGuard guard(logits.device());
@@ -208,13 +216,10 @@ Tensor adjust_logits(const Tensor& logits, const Tensor& tokens, const OptTensor
     TORCH_CHECK_VALUE((*x.first)->size(0) == batch, "lengths must have one entry per row");
     *x.second = (*x.first)->data_ptr<int>();
   }
-  p.repetition_row = per_row(repetition_row, logits, "repetition");
-  p.presence_row = per_row(presence_row, logits, "presence");
-  p.frequency_row = per_row(frequency_row, logits, "frequency");
-  TORCH_CHECK_VALUE(p.repetition_row || repetition > 0, "repetition must be positive");
-  p.repetition = (float)repetition;
-  p.presence = (float)presence;
-  p.frequency = (float)frequency;
+  penalty(repetition, logits, "repetition", &p.repetition_row, &p.repetition);
+  penalty(presence, logits, "presence", &p.presence_row, &p.presence);
+  penalty(frequency, logits, "frequency", &p.frequency_row, &p.frequency);
+  TORCH_CHECK_VALUE(p.repetition_row || p.repetition > 0, "repetition must be positive");
   if (given(bias)) {
     TORCH_CHECK_VALUE(bias->scalar_type() == at::kFloat && bias->device() == logits.device() && bias->size(-1) == vocab &&
                           (bias->dim() == 1 || (bias->dim() == 2 && bias->size(0) == batch)) && (vocab <= 1 || bias->stride(-1) == 1),

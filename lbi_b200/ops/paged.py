@@ -23,7 +23,7 @@ from typing import NamedTuple
 import torch
 
 from . import reference as ref
-from .dispatch import _count, fell_back
+from .dispatch import KERNEL_LAUNCHES, fell_back
 from .native import ext, native_available
 
 _TYPES = (torch.float32, torch.bfloat16, torch.float16)
@@ -55,13 +55,14 @@ def kv_pages(num_pages: int, page_size: int, n_kv_heads: int, head_dim: int, dty
     return KVPages(k, v, *(torch.zeros(shape[:3], dtype=torch.float32, device=device) for _ in range(2)))
 
 
-def _no_grad(*tensors) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+def _refuse_grad() -> None:
+    if torch.is_grad_enabled():
         raise ValueError("the cache operators have no backward pass: call them under torch.no_grad()")
 
 
 def _kernel_shape(x, head_dim) -> bool:
-    return x.is_cuda and native_available() and head_dim % 16 == 0 and head_dim <= 256 and x.dtype in _TYPES
+    """Whether the kernels take rows ``x`` (checked on every call of a decode loop, the cheap conditions first)."""
+    return x.is_cuda and head_dim % 16 == 0 and head_dim <= 256 and x.dtype in _TYPES and native_available()
 
 
 def _check(pages, page_table, context_lens, cu_seqlens, rows) -> None:
@@ -104,12 +105,13 @@ def kv_append(qkv, pages, page_table, context_lens, n_heads, cu_seqlens=None, ro
     ``qkv`` [rows, (n_heads + 2 kv_heads) * head_dim] are packed projections; ``rope = (cos, sin, interleaved)`` (fp32 tables
     [positions, head_dim / 2]) turns q and k by their positions first.  Into e4m3 pages a head row goes as
     ``round(x / scale)`` with ``scale = max |x| / 448``.  Two sequences must not share a page that new tokens are written to."""
-    pages = KVPages(*pages)
-    _no_grad(qkv)
+    if qkv.requires_grad:
+        _refuse_grad()
     cos, sin, interleaved = rope if rope is not None else (None, None, False)
-    if _kernel_shape(qkv, pages.k.shape[-1]):
-        _count()
-        return ext().kv_append(qkv, *pages, page_table, context_lens, n_heads, cu_seqlens, cos, sin, bool(interleaved), out)
+    if _kernel_shape(qkv, pages[0].size(-1)):
+        KERNEL_LAUNCHES["count"] += 1
+        return ext().kv_append(qkv, *pages, page_table, context_lens, n_heads, cu_seqlens, cos, sin, interleaved, out)
+    pages = KVPages(*pages)
     fell_back("kv_append", qkv)
     _check(pages, page_table, context_lens, cu_seqlens, qkv.shape[0])
     kv_heads, head_dim = pages.k.shape[1], pages.k.shape[3]
@@ -124,11 +126,12 @@ def kv_append(qkv, pages, page_table, context_lens, n_heads, cu_seqlens=None, ro
 def kv_gather(pages, page_table, context_lens, max_len, dtype=None):
     """The cached keys and values as contiguous [B, kv_heads, max_len, head_dim] tensors, zero behind each context (the layout of
     ``CausalSelfAttention.step``).  ``dtype``: type of the result for e4m3 pages (default bf16); other pages keep theirs."""
-    pages = KVPages(*pages)
-    dtype = dtype or (torch.bfloat16 if pages.k.dtype == torch.float8_e4m3fn else pages.k.dtype)
-    if pages.k.is_cuda and native_available() and pages.k.shape[-1] % 16 == 0 and pages.k.shape[-1] <= 256:
-        _count()
+    k = pages[0]
+    dtype = dtype or (torch.bfloat16 if k.dtype == torch.float8_e4m3fn else k.dtype)
+    if k.is_cuda and k.size(-1) % 16 == 0 and k.size(-1) <= 256 and native_available():
+        KERNEL_LAUNCHES["count"] += 1
         return ext().kv_gather(*pages, page_table, context_lens, max_len, dtype)
+    pages = KVPages(*pages)
     fell_back("kv_gather", pages.k)
     _check(pages, page_table, context_lens, None, 0)
     if max_len < 0:
@@ -144,11 +147,12 @@ def paged_attention(q, pages, page_table, context_lens, scale, cu_seqlens=None, 
 
     ``max_context``: the longest context if the host knows it (a hint that sizes the launch, default: what the page table can
     hold); a longer context still gives right results.  ``out`` must not overlap ``q``."""
+    if q.requires_grad:
+        _refuse_grad()
+    if _kernel_shape(q, pages[0].size(-1)):
+        KERNEL_LAUNCHES["count"] += 1
+        return ext().paged_attention(q, *pages, page_table, context_lens, scale, cu_seqlens, max_context or 0, out)
     pages = KVPages(*pages)
-    _no_grad(q)
-    if _kernel_shape(q, pages.k.shape[-1]):
-        _count()
-        return ext().paged_attention(q, *pages, page_table, context_lens, scale, cu_seqlens, 0 if max_context is None else max_context, out)
     fell_back("paged_attention", q)
     _check(pages, page_table, context_lens, cu_seqlens, q.shape[0])
     if q.dim() != 3 or q.shape[2] != pages.k.shape[3] or q.shape[1] == 0 or q.shape[1] % pages.k.shape[1] != 0:
@@ -181,12 +185,13 @@ def adjust_logits(logits, tokens, lengths=None, prompt_lengths=None, *, repetiti
     * a token whose bit in ``allowed`` (``pack_token_mask``; [ceil(V / 32)] or one row each) is not set: -inf
 
     The three penalties are numbers or fp32 [B].  ``out`` may be ``logits`` itself when that is fp32."""
-    _no_grad(logits, bias)
+    if logits.requires_grad or (bias is not None and bias.requires_grad):
+        _refuse_grad()
+    if logits.is_cuda and logits.dtype in _TYPES and native_available():
+        KERNEL_LAUNCHES["count"] += 1
+        return ext().adjust_logits(logits, tokens, lengths, prompt_lengths, repetition, presence, frequency, bias, allowed, out)
     rows = [x if torch.is_tensor(x) else None for x in (repetition, presence, frequency)]
     numbers = [d if torch.is_tensor(x) else x for x, d in ((repetition, 1.0), (presence, 0.0), (frequency, 0.0))]
-    if logits.is_cuda and native_available() and logits.dtype in _TYPES:
-        _count()
-        return ext().adjust_logits(logits, tokens, lengths, prompt_lengths, *rows, *numbers, bias, allowed, out)
     fell_back("adjust_logits", logits)
     batch, vocab = logits.shape if logits.dim() == 2 else (-1, -1)
     if batch < 0 or logits.dtype not in _TYPES:
