@@ -40,11 +40,11 @@ __global__ void __launch_bounds__(LOGIT_THREADS, 4) logits_kernel(const lbi_logi
 #pragma unroll
     for (int e = 0; e < 4; ++e)
       if (t[e] >= 0 && t[e] < n) {
-        const bool first = i0 + e * LOGIT_THREADS < prompt;
         uint32_t* word = reinterpret_cast<uint32_t*>(count) + (WIDE ? t[e] : t[e] >> 1);
         const int shift = WIDE ? 0 : (int)(t[e] & 1) * 16;
-        if (first) atomicOr(word, PROMPT << shift);
-        else atomicAdd(word, 1u << shift);
+        // text repeats itself: what the prompt has set already is not set again
+        if (i0 + e * LOGIT_THREADS >= prompt) atomicAdd(word, 1u << shift);
+        else if (!(*reinterpret_cast<volatile uint32_t*>(word) >> shift & PROMPT)) atomicOr(word, PROMPT << shift);
       }
   }
   __syncthreads();
@@ -85,11 +85,13 @@ __global__ void __launch_bounds__(LOGIT_THREADS, 4) logits_kernel(const lbi_logi
 
 template <int TYPE>
 static void launch_logits(const lbi_logit_rules& p, int sm_count, cudaStream_t st) {
-  // Full tiles, unless they leave SMs without a block: then as many as there are SMs, of 1024 tokens at least.
+  // As few tiles as the counts allow, then so many more as fit into the same number of rounds of four blocks per SM (192 x 128001: 9
+  // instead of 8 per row), of 1024 tokens at least.
   const bool wide = p.history >= 32768;
-  const int most = COUNT_BYTES / (wide ? 4 : 2);
-  const int64_t per_row = std::max<int64_t>(1, sm_count / p.batch);
-  const int tile = (int)std::min<int64_t>(most, std::max<int64_t>(1024, ((p.vocab + per_row - 1) / per_row + 1023) / 1024 * 1024));
+  const int64_t most = COUNT_BYTES / (wide ? 4 : 2), slots = 4ll * sm_count;
+  const int64_t fewest = (p.vocab + most - 1) / most, rounds = (fewest * p.batch + slots - 1) / slots;
+  const int64_t tiles = std::max(fewest, rounds * slots / p.batch);
+  const int tile = (int)std::min<int64_t>(most, std::max<int64_t>(1024, ((p.vocab + tiles - 1) / tiles + 31) / 32 * 32));
   const dim3 grid((p.vocab + tile - 1) / tile, p.batch);
   static lbi::PerDeviceOnce narrow_once, wide_once;
   narrow_once.all_shared(logits_kernel<TYPE, uint16_t>);
