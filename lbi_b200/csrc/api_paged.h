@@ -43,6 +43,7 @@ int lbi_kv_gather(const lbi_paged_batch* p, void* k_out, void* v_out, int64_t ma
 // supplies part_o fp32 [rows * heads, splits, head_dim] and part_lse fp32 [rows * heads, splits].
 typedef struct {
   int kernel;   // 0 tiles of 16 rows for any type and head size, 1 tiles of 16 rows, 2 tiles of 256 rows
+  int rows;     // of a tile of kernels 0 and 1
   int splits, split_keys;
 } lbi_attention_plan;
 lbi_attention_plan lbi_paged_attention_plan(const lbi_paged_batch* p, int type, int heads, float scale, int64_t max_context, int sm_count);

@@ -16,18 +16,20 @@ namespace paged {
 
 // ------------------------------------------------------------------------------------------------ 16-row tiles
 // Bound by reading the cache once: 2 head_dim sizeof(code) bytes per key and kv head.  All query heads of a group (and several new
-// tokens, if there are) share a tile of 16 rows, so that one read of a key serves them all, and mma.sync m16n8k16 does the products:
-// with at most 16 rows the tensor work is a few per cent of the time, and the operands come straight from the copies below, which
-// tcgen05 (128 rows, operands through descriptors) would only add steps to.  Every warp works alone on its own keys: a ring of
-// cp.async tiles in shared memory (no block barrier in the loop), S = Q K^T, running maximum and sum, O += P V in registers; the
-// four warps of a block are joined through shared memory at the end.  The page ids of a tile are loaded one tile ahead of its copies.
+// tokens, if there are) share a tile of 8 or 16 rows, so that one read of a key serves them all, and mma.sync m16n8k16 does the
+// products with the keys (then the head's elements) as its 16 rows and the query rows as its 8 columns: S^T = K Q^T, O^T = V^T P^T.
+// With at most 16 rows the tensor work is a few per cent of the time, and the operands come straight from the copies below, which
+// tcgen05 (128 rows, operands through descriptors) would only add steps to.  P^T leaves the first product with a key's rows in one
+// thread and enters the second with a row's keys in one thread: movmatrix turns it.  Every warp works alone on its own keys: a ring of
+// cp.async tiles in shared memory (no block barrier in the loop), running maximum and sum, O^T in registers; the four warps of a block
+// are joined through shared memory at the end.  The page ids of a tile are loaded one tile ahead of its copies.
 //
-// e4m3 pages: codes become 16-bit values exactly.  With u_j = scale s_j k_scale_j + log2 v_scale_j the weights 2^(u_j - max u) carry
+// e4m3 pages: codes become fp16 values exactly.  With u_j = scale s_j k_scale_j + log2 v_scale_j the weights 2^(u_j - max u) carry
 // the value's scale and stay in (0, 1] (fp16 has no range for p * v_scale); the sum of exponentials takes 2^(u_j - max u) / v_scale_j.
-// P is rounded to the queries' 16-bit type before the second product (half a step of the result's type, as the result itself);
+// P is rounded to the 16-bit type of the products before the second one (half a step of that type, as the result itself is rounded);
 // maximum, sum and output stay in fp32.
 
-constexpr int ROW_TILE = 16;
+constexpr int ROW_TILE = 16;   // rows of attn_any_kernel; attn_rows_kernel has tiles of 8, too
 constexpr int WARPS = 4;
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -76,20 +78,20 @@ struct RowsUnit {
   int split, kh, b, first_row, local, n_rows, first_pos, k0, k1;   // local: first row of the tile in the sequence's tile space
   bool any;
 };
-__device__ __forceinline__ RowsUnit rows_unit(const AttnArgs& a) {
+__device__ __forceinline__ RowsUnit rows_unit(const AttnArgs& a, int per_tile) {
   const lbi_paged_batch& p = a.b;
   RowsUnit u;
   u.split = blockIdx.x % a.splits;
   const int64_t unit = blockIdx.x / a.splits;
   u.kh = (int)(unit % p.kv_heads);
   const int64_t tile = unit / p.kv_heads;
-  u.b = seq_of_tile(p, tile, a.group, ROW_TILE);
+  u.b = seq_of_tile(p, tile, a.group, per_tile);
   const int2 r = seq_rows(p, u.b);
   u.first_row = r.x;
-  u.local = (int)(tile - first_tile(p, u.b, a.group, ROW_TILE)) * ROW_TILE;
+  u.local = (int)(tile - first_tile(p, u.b, a.group, per_tile)) * per_tile;
   const int rows_b = (r.y - r.x) * a.group;
   u.any = u.local >= 0 && u.local < rows_b;
-  u.n_rows = min(ROW_TILE, rows_b - u.local);
+  u.n_rows = min(per_tile, rows_b - u.local);
   u.first_pos = __ldg(p.context + u.b) - (r.y - r.x);              // position of the sequence's first new token
   const int64_t capacity = (int64_t)p.table_width << a.page_shift;
   const int keys = (int)min((int64_t)u.first_pos + (u.local + u.n_rows - 1) / a.group + 1, capacity);
@@ -113,24 +115,24 @@ __device__ __forceinline__ int key_slot(const AttnArgs& a, const RowsUnit& u, in
 }
 // Joins the warps of a block and stores the result (or the part): `m`, `l` of rows g and g + 8 in every thread, the output row parts
 // behind ml in shared memory as [warp][row][dim + 4].
-template <typename T>
+template <typename T, int ROWS>
 __device__ __forceinline__ void join_and_store(const AttnArgs& a, const RowsUnit& u, const float* ml, int dim) {
-  const float* os = ml + 2 * WARPS * ROW_TILE;
+  const float* os = ml + 2 * WARPS * ROWS;
   for (int i = threadIdx.x; i < u.n_rows * (dim / 8); i += WARPS * 32) {
     const int rr = i / (dim / 8), d = i % (dim / 8) * 8;
     float top = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w) top = fmaxf(top, ml[w * ROW_TILE + rr]);
+    for (int w = 0; w < WARPS; ++w) top = fmaxf(top, ml[w * ROWS + rr]);
     const float ref = top == -INFINITY ? 0.f : top;
     float sum = 0.f, acc[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) acc[e] = 0.f;
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) {
-      const float f = ex2(ml[w * ROW_TILE + rr] - ref);
-      sum += f * ml[(WARPS + w) * ROW_TILE + rr];
+      const float f = ex2(ml[w * ROWS + rr] - ref);
+      sum += f * ml[(WARPS + w) * ROWS + rr];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) acc[e] += f * os[(w * ROW_TILE + rr) * (dim + 4) + d + e];
+      for (int e = 0; e < 8; ++e) acc[e] += f * os[(w * ROWS + rr) * (dim + 4) + d + e];
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
@@ -145,75 +147,98 @@ __device__ __forceinline__ void join_and_store(const AttnArgs& a, const RowsUnit
   }
 }
 
-template <int TYPE, bool E4M3, int DH, int KEYS, int STAGES>
+template <bool E4M3, int DH, int KEYS, int STAGES, int NT>
 struct RowsTile {
+  static constexpr int ROWS = 8 * NT;
   static constexpr int RB = DH * (E4M3 ? 1 : 2);
   static constexpr int TILE = KEYS * RB;
   static constexpr int STAGE = 2 * TILE + (E4M3 ? 8 * KEYS : 0) + 16;   // K, V, scales, which keys exist
   static constexpr int RING = STAGES * STAGE;
-  static constexpr int JOIN = WARPS * ROW_TILE * (DH + 4) * 4 + WARPS * ROW_TILE * 8;
+  static constexpr int JOIN = WARPS * ROWS * (DH + 4) * 4 + WARPS * ROWS * 8;
   static constexpr int SMEM = WARPS * RING > JOIN ? WARPS * RING : JOIN;
 };
 
-template <int TYPE, bool E4M3, int DH, int KEYS, int STAGES, int BLOCKS>
+// An 8 x 8 matrix of 16-bit values, two per thread, transposed across the warp.
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+template <int TYPE, bool E4M3, int DH, int KEYS, int STAGES, int BLOCKS, int NT>
 __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_rows_kernel(const AttnArgs a) {
   using T = typename Elem<TYPE>::T;
-  using L = RowsTile<TYPE, E4M3, DH, KEYS, STAGES>;
+  using L = RowsTile<E4M3, DH, KEYS, STAGES, NT>;
+  constexpr int ROWS = L::ROWS, KT = KEYS / 16;
   extern __shared__ __align__(128) uint8_t smem[];
   const lbi_paged_batch& p = a.b;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   zero_rows_of_nobody<T>(a);
-  const RowsUnit u = rows_unit(a);
+  const RowsUnit u = rows_unit(a, ROWS);
   if (!u.any) return;
-  const int kh = u.kh, local = u.local, n_rows = u.n_rows, k0 = u.k0, k1 = u.k1;
+  const int kh = u.kh, k0 = u.k0, k1 = u.k1;
 
-  // query fragments: row g (and g + 8) of the tile; the order of the head's elements within a product of 16 is free as long as Q and
-  // K agree: natural for 16-bit pages (ldmatrix), 4 neighbours per thread for codes (one 32-bit load)
+  // Query fragments: row 8 n + g of the tile.  The order of the head's elements within a product of 16 is free as long as Q and K
+  // agree: natural for 16-bit pages (ldmatrix), 4 neighbours per thread for codes (one 32-bit load).
   // e4m3: the products run in fp16, which holds the codes and, behind a power of two per row that brings its largest element to
-  // [2^14, 2^15), a bf16 query as well (29 binades below the largest to the normal range's end: nothing that an fp32 sum would notice)
+  // [2^14, 2^15), a bf16 query as well (29 binades below the largest to the normal range's end: nothing that an fp32 sum would notice).
   constexpr int MATH = E4M3 ? LBI_F16 : TYPE;
-  uint32_t qf[DH / 16][4];
-  int limit[2];
-  float row_scale[2];
+  uint32_t qf[NT][DH / 16][2];
+  int limit[NT][2];         // of the rows 8 n + 2 t and + 1, whose scores the thread has
+  float row_scale[NT][2];
 #pragma unroll
-  for (int hh = 0; hh < 2; ++hh) {
-    const int rr = local + g + 8 * hh;
-    const bool live = g + 8 * hh < n_rows;
+  for (int n = 0; n < NT; ++n) {
+    const int r = 8 * n + g, rr = u.local + r;
+    const bool live = r < u.n_rows;
     const int token = live ? rr / a.group : 0, head = kh * a.group + (live ? rr % a.group : 0);
-    limit[hh] = live ? u.first_pos + token : 0x7fffffff;   // rows that do not exist (queries of zero, never stored) ask for no mask
-    row_scale[hh] = a.scale_log2;
     const uint32_t* src = reinterpret_cast<const uint32_t*>((const T*)a.q + (int64_t)(u.first_row + token) * a.q_stride + head * DH);
 #pragma unroll
     for (int ks = 0; ks < DH / 16; ++ks) {
-      qf[ks][hh] = live ? src[ks * 8 + (E4M3 ? 2 * t : t)] : 0u;
-      qf[ks][2 + hh] = live ? src[ks * 8 + (E4M3 ? 2 * t + 1 : t + 4)] : 0u;
+      qf[n][ks][0] = live ? src[ks * 8 + (E4M3 ? 2 * t : t)] : 0u;
+      qf[n][ks][1] = live ? src[ks * 8 + (E4M3 ? 2 * t + 1 : t + 4)] : 0u;
     }
+    float scale = a.scale_log2;
     if (E4M3 && TYPE == LBI_BF16) {
       int most = 0;   // as whole numbers, magnitudes are in order
 #pragma unroll
       for (int ks = 0; ks < DH / 16; ++ks)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) most = max(most, max(qf[ks][2 * i + hh] << 16 & 0x7fff0000, qf[ks][2 * i + hh] & 0x7fff0000));
+        for (int i = 0; i < 2; ++i) most = max(most, max((int)(qf[n][ks][i] << 16 & 0x7fff0000u), (int)(qf[n][ks][i] & 0x7fff0000u)));
       most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
       most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
       const int e = min(max(14 + 127 - (most >> 23), -100), 120);
       const float up = __int_as_float((e + 127) << 23);
-      row_scale[hh] *= __int_as_float((127 - e) << 23);
+      scale *= __int_as_float((127 - e) << 23);
 #pragma unroll
       for (int ks = 0; ks < DH / 16; ++ks)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          uint32_t& w = qf[ks][2 * i + hh];
+          uint32_t& w = qf[n][ks][i];
           w = pack16<LBI_F16>(__uint_as_float(w << 16) * up, __uint_as_float(w & 0xffff0000u) * up);
         }
     }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int at = 8 * n + 2 * t + e;
+      row_scale[n][e] = __shfl_sync(0xffffffffu, scale, (2 * t + e) * 4);
+      // rows that do not exist (queries of zero, never stored) ask for no mask
+      limit[n][e] = at < u.n_rows ? u.first_pos + (u.local + at) / a.group : 0x7fffffff;
+    }
   }
-  float o[DH / 8][4];
+  int lowest = min(limit[0][0], limit[0][1]);
+  if (NT == 2) lowest = min(lowest, min(limit[NT - 1][0], limit[NT - 1][1]));
+  float o[DH / 16][NT][4];
 #pragma unroll
-  for (int i = 0; i < DH / 8; ++i)
+  for (int i = 0; i < DH / 16; ++i)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[i][n][e] = 0.f;
+  float m[NT][2], l[NT][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) m[n][e] = -INFINITY, l[n][e] = 0.f;
 
   const uint32_t ring = smem_addr(smem) + warp * L::RING;
   const int n_tiles = k1 > k0 ? (k1 - k0 + KEYS - 1) / KEYS : 0;
@@ -262,153 +287,166 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_rows_kernel(const Att
     page = next;
     const uint32_t kd = ring + (i % STAGES) * L::STAGE, vd = kd + L::TILE;
     const int base = k0 + (warp + i * WARPS) * KEYS;
+    const int mi = lane >> 3, row = lane & 7;   // ldmatrix: which of the four matrices, which of its rows
 
-    float s[KEYS / 8][4];
+    float s[KT][NT][4];   // keys 16 kt + g (0, 1) and + 8 (2, 3), rows 8 n + 2 t and + 1
 #pragma unroll
-    for (int n = 0; n < KEYS / 8; ++n)
+    for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
-    if (!E4M3) {
-      const int mi = lane >> 3, row = lane & 7;
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int ks = 0; ks < DH / 16; ++ks)
+        for (int e = 0; e < 4; ++e) s[kt][n][e] = 0.f;
 #pragma unroll
-        for (int np = 0; np < KEYS / 16; ++np) {
-          uint32_t f[4];
-          ldsm4(kd + swz<L::RB>(np * 16 + (mi >> 1) * 8 + row, 2 * ks + (mi & 1)), f);
-          mma16816<TYPE>(s[2 * np], qf[ks], f[0], f[1]);
-          mma16816<TYPE>(s[2 * np + 1], qf[ks], f[2], f[3]);
+    for (int ks = 0; ks < DH / 16; ++ks)
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt) {
+        uint32_t f[4];
+        if (!E4M3) {
+          ldsm4(kd + swz<L::RB>(kt * 16 + (mi & 1) * 8 + row, 2 * ks + (mi >> 1)), f);
+        } else {
+          codes_to_f16(lds32(kd + swz<L::RB>(kt * 16 + g, ks) + 4 * t), f[0], f[2]);
+          codes_to_f16(lds32(kd + swz<L::RB>(kt * 16 + 8 + g, ks) + 4 * t), f[1], f[3]);
         }
-    } else {
 #pragma unroll
-      for (int ks = 0; ks < DH / 16; ++ks)
-#pragma unroll
-        for (int n = 0; n < KEYS / 8; ++n) {
-          const uint32_t w = lds32(kd + swz<L::RB>(n * 8 + g, ks) + 4 * t);
-          uint32_t f0, f1;
-          codes_to_f16(w, f0, f1);
-          mma16816<MATH>(s[n], qf[ks], f0, f1);
-        }
-    }
+        for (int n = 0; n < NT; ++n) mma16816<MATH>(s[kt][n], f, qf[n][ks][0], qf[n][ks][1]);
+      }
 
     const uint32_t there = lds32(kd + L::STAGE - 16);
-    float inv_vs[KEYS / 8][2];
-    float top[2] = {-INFINITY, -INFINITY};
+    float inv_vs[KT][2];
 #pragma unroll
-    for (int n = 0; n < KEYS / 8; ++n) {
-      float ks[2] = {1.f, 1.f}, lv[2] = {0.f, 0.f};
-      if (E4M3) {
+    for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          ks[e] = __uint_as_float(lds32(vd + L::TILE + (n * 8 + 2 * t + e) * 4));
-          const float vs = positive_scale(__uint_as_float(lds32(vd + L::TILE + (KEYS + n * 8 + 2 * t + e) * 4)));
-          lv[e] = lg2(vs);
-          inv_vs[n][e] = rcp(vs);
+      for (int h = 0; h < 2; ++h) {
+        float ks = 1.f, lv = 0.f;
+        if (E4M3) {
+          const int key = kt * 16 + 8 * h + g;
+          ks = __uint_as_float(lds32(vd + L::TILE + key * 4));
+          const float vs = positive_scale(__uint_as_float(lds32(vd + L::TILE + (KEYS + key) * 4)));
+          lv = lg2(vs);
+          inv_vs[kt][h] = rcp(vs);
         }
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float& x = s[kt][n][2 * h + e];
+            x = E4M3 ? fmaf(x * row_scale[n][e], ks, lv) : x * row_scale[n][e];
+          }
       }
+    if (__any_sync(0xffffffffu, there != (KEYS == 32 ? 0xffffffffu : (1u << KEYS) - 1u) || base + KEYS - 1 > lowest)) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[n][e] = E4M3 ? fmaf(s[n][e] * row_scale[e >> 1], ks[e & 1], lv[e & 1]) : s[n][e] * row_scale[e >> 1];
+      for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int key = kt * 16 + 8 * (e >> 1) + g;
+            if (base + key > limit[n][e & 1] || !(there >> key & 1u)) s[kt][n][e] = -INFINITY;
+          }
     }
-    if (__any_sync(0xffffffffu, there != (KEYS == 32 ? 0xffffffffu : (1u << KEYS) - 1u) || base + KEYS - 1 > min(limit[0], limit[1]))) {
+    float keep[NT][2], ref[NT][2];
+    bool changed = false;
 #pragma unroll
-      for (int n = 0; n < KEYS / 8; ++n)
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int key = n * 8 + 2 * t + (e & 1);
-          if (base + key > limit[e >> 1] || !(there >> key & 1u)) s[n][e] = -INFINITY;
+      for (int e = 0; e < 2; ++e) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) top = fmaxf(top, fmaxf(s[kt][n][e], s[kt][n][2 + e]));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+        const float mn = fmaxf(m[n][e], top);
+        ref[n][e] = mn == -INFINITY ? 0.f : mn;      // a row that has seen no key yet
+        keep[n][e] = ex2(m[n][e] - ref[n][e]);
+        m[n][e] = mn;
+        l[n][e] *= keep[n][e];
+        changed = changed || keep[n][e] != 1.f;
+      }
+    uint32_t pf[KT][NT][2];
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float w[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            w[e] = ex2(s[kt][n][2 * h + e] - ref[n][e]);
+            l[n][e] += E4M3 ? w[e] * inv_vs[kt][h] : w[e];
+          }
+          pf[kt][n][h] = transpose8x8(pack16<MATH>(w[0], w[1]));
         }
+    if (__any_sync(0xffffffffu, changed)) {
+#pragma unroll
+      for (int d = 0; d < DH / 16; ++d)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[d][n][e] *= keep[n][e & 1];
     }
 #pragma unroll
-    for (int n = 0; n < KEYS / 8; ++n)
+    for (int kt = 0; kt < KT; ++kt) {
+      if (!E4M3) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) top[e >> 1] = fmaxf(top[e >> 1], s[n][e]);
-    float keep[2], ref[2];
-#pragma unroll
-    for (int hh = 0; hh < 2; ++hh) {
-      top[hh] = fmaxf(top[hh], __shfl_xor_sync(0xffffffffu, top[hh], 1));
-      top[hh] = fmaxf(top[hh], __shfl_xor_sync(0xffffffffu, top[hh], 2));
-      const float mn = fmaxf(m[hh], top[hh]);
-      ref[hh] = mn == -INFINITY ? 0.f : mn;      // a row that has seen no key yet
-      keep[hh] = ex2(m[hh] - ref[hh]);
-      m[hh] = mn;
-      l[hh] *= keep[hh];
-    }
-    uint32_t pf[KEYS / 16][4];
-#pragma unroll
-    for (int n = 0; n < KEYS / 8; ++n) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        s[n][e] = ex2(s[n][e] - ref[e >> 1]);
-        l[e >> 1] += E4M3 ? s[n][e] * inv_vs[n][e & 1] : s[n][e];
-      }
-      pf[n >> 1][(n & 1) * 2] = pack16<MATH>(s[n][0], s[n][1]);
-      pf[n >> 1][(n & 1) * 2 + 1] = pack16<MATH>(s[n][2], s[n][3]);
-    }
-    if (__any_sync(0xffffffffu, keep[0] != 1.f || keep[1] != 1.f)) {
-#pragma unroll
-      for (int n = 0; n < DH / 8; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[n][e] *= keep[e >> 1];
-    }
-    if (!E4M3) {
-      const int mi = lane >> 3, row = lane & 7;
-#pragma unroll
-      for (int kk = 0; kk < KEYS / 16; ++kk)
-#pragma unroll
-        for (int n = 0; n < DH / 16; ++n) {
+        for (int d = 0; d < DH / 16; ++d) {
           uint32_t f[4];
-          ldsm4_t(vd + swz<L::RB>(kk * 16 + (mi & 1) * 8 + row, 2 * n + (mi >> 1)), f);
-          mma16816<TYPE>(o[2 * n], pf[kk], f[0], f[1]);
-          mma16816<TYPE>(o[2 * n + 1], pf[kk], f[2], f[3]);
+          ldsm4_t(vd + swz<L::RB>(kt * 16 + (mi >> 1) * 8 + row, 2 * d + (mi & 1)), f);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma16816<MATH>(o[d][n], f, pf[kt][n][0], pf[kt][n][1]);
         }
-    } else {
+      } else {
 #pragma unroll
-      for (int kk = 0; kk < KEYS / 16; ++kk)
-#pragma unroll
-        for (int c = 0; c < DH / 32; ++c) {   // elements 32 c + 4 g .. + 3 of four keys: column g of four products
-          uint32_t w[4];
+        for (int c = 0; c < DH / 32; ++c) {   // elements 32 c + 4 g .. + 3 of four keys: rows g and g + 8 of two products
+          uint32_t w[4], lo[4], hi[4];
 #pragma unroll
           for (int q4 = 0; q4 < 4; ++q4)
-            w[q4] = lds32(vd + swz<L::RB>(kk * 16 + 2 * t + (q4 & 1) + (q4 >> 1) * 8, 2 * c + (g >> 2)) + 4 * (g & 3));
-          uint32_t lo[4], hi[4];
+            w[q4] = lds32(vd + swz<L::RB>(kt * 16 + 2 * t + (q4 & 1) + (q4 >> 1) * 8, 2 * c + (g >> 2)) + 4 * (g & 3));
           codes_to_f16(__byte_perm(w[0], w[1], 0x5140), lo[0], lo[1]);
           codes_to_f16(__byte_perm(w[0], w[1], 0x7362), lo[2], lo[3]);
           codes_to_f16(__byte_perm(w[2], w[3], 0x5140), hi[0], hi[1]);
           codes_to_f16(__byte_perm(w[2], w[3], 0x7362), hi[2], hi[3]);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) mma16816<MATH>(o[4 * c + e], pf[kk], lo[e], hi[e]);
+          for (int i2 = 0; i2 < 2; ++i2) {
+            const uint32_t f[4] = {lo[2 * i2], lo[2 * i2 + 1], hi[2 * i2], hi[2 * i2 + 1]};
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma16816<MATH>(o[2 * c + i2][n], f, pf[kt][n][0], pf[kt][n][1]);
+          }
         }
+      }
     }
     __syncwarp();   // the stage may be overwritten
   }
   cp_async_wait<0>();
 #pragma unroll
-  for (int hh = 0; hh < 2; ++hh) {
-    l[hh] += __shfl_xor_sync(0xffffffffu, l[hh], 1);
-    l[hh] += __shfl_xor_sync(0xffffffffu, l[hh], 2);
-  }
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+#pragma unroll
+      for (int x = 4; x < 32; x <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], x);
 
   // ------------------------------------------------------------------ join the warps
   __syncthreads();
   float* ml = reinterpret_cast<float*>(smem);                     // [warp][row] maximum, then sum
-  float* os = ml + 2 * WARPS * ROW_TILE;                          // [warp][row][DH + 4]
-  if (t == 0) {
+  float* os = ml + 2 * WARPS * ROWS;                              // [warp][row][DH + 4]
 #pragma unroll
-    for (int hh = 0; hh < 2; ++hh) {
-      ml[warp * ROW_TILE + g + 8 * hh] = m[hh];
-      ml[(WARPS + warp) * ROW_TILE + g + 8 * hh] = l[hh];
-    }
-  }
+  for (int n = 0; n < NT; ++n)
 #pragma unroll
-  for (int n = 0; n < DH / 8; ++n)
+    for (int e = 0; e < 2; ++e) {
+      if (g == 0) {
+        ml[warp * ROWS + 8 * n + 2 * t + e] = m[n][e];
+        ml[(WARPS + warp) * ROWS + 8 * n + 2 * t + e] = l[n][e];
+      }
+      float* to = os + (warp * ROWS + 8 * n + 2 * t + e) * (DH + 4);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int col = 2 * t + (e & 1);
-      const int d = E4M3 ? 32 * (n >> 2) + 4 * col + (n & 3) : 8 * n + col;
-      os[(warp * ROW_TILE + g + 8 * (e >> 1)) * (DH + 4) + d] = o[n][e];
+      for (int d = 0; d < DH / 16; ++d) {
+        to[E4M3 ? 32 * (d >> 1) + 4 * g + 2 * (d & 1) : 16 * d + g] = o[d][n][e];
+        to[E4M3 ? 32 * (d >> 1) + 4 * g + 2 * (d & 1) + 1 : 16 * d + g + 8] = o[d][n][2 + e];
+      }
     }
   __syncthreads();
-  join_and_store<T>(a, u, ml, DH);
+  join_and_store<T, ROWS>(a, u, ml, DH);
 }
 
 // Joins the parts of a context: o = sum_s 2^(lse_s - max) o_s / sum_s 2^(lse_s - max).  A group of LANES threads owns a (token, head),
@@ -547,7 +585,7 @@ __global__ void __launch_bounds__(WARPS * 32) attn_any_kernel(const AttnArgs a) 
   const lbi_paged_batch& p = a.b;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, dim = p.head_dim;
   zero_rows_of_nobody<T>(a);
-  const RowsUnit u = rows_unit(a);
+  const RowsUnit u = rows_unit(a, ROW_TILE);
   if (!u.any) return;
 
   uint4* qs = reinterpret_cast<uint4*>(smem);   // [8 elements][lane]: hi, then (fp32) lo
@@ -741,32 +779,31 @@ __global__ void __launch_bounds__(WARPS * 32) attn_any_kernel(const AttnArgs a) 
     for (int e = 0; e < 4; ++e) os[(warp * ROW_TILE + g + 8 * (e >> 1)) * (dim + 4) + 8 * n + 2 * t + (e & 1)] = o[n][e];
   }
   __syncthreads();
-  join_and_store<T>(a, u, ml, dim);
+  join_and_store<T, ROW_TILE>(a, u, ml, dim);
 }
 
 // ------------------------------------------------------------------------------------------------ host side
-template <int TYPE, bool E4M3, int DH, int KEYS, int STAGES, int BLOCKS>
+template <int TYPE, bool E4M3, int DH, int KEYS, int STAGES, int BLOCKS, int NT>
 int launch_rows(const AttnArgs& a, cudaStream_t st) {
-  using L = RowsTile<TYPE, E4M3, DH, KEYS, STAGES>;
-  auto kernel = attn_rows_kernel<TYPE, E4M3, DH, KEYS, STAGES, BLOCKS>;
+  using L = RowsTile<E4M3, DH, KEYS, STAGES, NT>;
+  auto kernel = attn_rows_kernel<TYPE, E4M3, DH, KEYS, STAGES, BLOCKS, NT>;
   static lbi::PerDeviceOnce once;
   cudaError_t e = once.max_dynamic_smem(kernel, L::SMEM);
   if (e != cudaSuccess) return (int)e;
-  const int64_t blocks = tile_bound(a.b, a.group, ROW_TILE) * a.b.kv_heads * a.splits;
+  const int64_t blocks = tile_bound(a.b, a.group, L::ROWS) * a.b.kv_heads * a.splits;
   if (blocks >= (1ll << 31)) return (int)cudaErrorInvalidValue;
   kernel<<<(unsigned)blocks, WARPS * 32, L::SMEM, st>>>(a);
   return (int)cudaGetLastError();
 }
 
-template <int TYPE>
-int launch_rows(const AttnArgs& a, cudaStream_t st) {
-  // Keys per tile, tiles in flight per warp, blocks per SM.  Measured, 64 sequences of up to 8192 tokens, bf16 queries: e4m3 head_dim 128
-  // 153 us (16, 4, 3: 163), head_dim 64 267 us (32, 5, 2: 298), head_dim 32 with 16-bit pages 66 us (32, 5, 2: 76).
+template <int TYPE, int NT>
+int launch_rows(const AttnArgs& a, cudaStream_t st) {   // keys per tile, tiles in flight per warp, blocks per SM
+  // Measured, 64 sequences of 8192 tokens: e4m3 head_dim 128 134 us (32, 3, 2: 138), head_dim 64 218 us (16, 4, 4: 256).
   if (a.b.cache_type == LBI_E4M3)
-    return a.b.head_dim == 128 ? launch_rows<TYPE, true, 128, 32, 3, 2>(a, st)
-         : a.b.head_dim == 64  ? launch_rows<TYPE, true, 64, 32, 4, 3>(a, st) : launch_rows<TYPE, true, 32, 32, 6, 3>(a, st);
-  return a.b.head_dim == 128 ? launch_rows<TYPE, false, 128, 16, 3, 2>(a, st)
-       : a.b.head_dim == 64  ? launch_rows<TYPE, false, 64, 16, 4, 3>(a, st) : launch_rows<TYPE, false, 32, 32, 4, 3>(a, st);
+    return a.b.head_dim == 128 ? launch_rows<TYPE, true, 128, 16, 3, NT == 1 ? 4 : 3, NT>(a, st)
+         : a.b.head_dim == 64  ? launch_rows<TYPE, true, 64, 32, 3, 4, NT>(a, st) : launch_rows<TYPE, true, 32, 32, 6, 3, NT>(a, st);
+  return a.b.head_dim == 128 ? launch_rows<TYPE, false, 128, 16, 3, 2, NT>(a, st)
+       : a.b.head_dim == 64  ? launch_rows<TYPE, false, 64, 16, 4, 3, NT>(a, st) : launch_rows<TYPE, false, 32, 32, 4, 3, NT>(a, st);
 }
 
 template <int TYPE, bool E4M3, int DHP>
@@ -794,14 +831,17 @@ int launch_any(const AttnArgs& a, cudaStream_t st) {
 
 extern "C" lbi_attention_plan lbi_paged_attention_plan(const lbi_paged_batch* p, int type, int heads, float scale, int64_t max_context, int sm_count) {
   using namespace lbi::paged;
-  lbi_attention_plan plan{0, 1, 1 << 30};
+  lbi_attention_plan plan{0, ROW_TILE, 1, 1 << 30};
   if (p->rows == 0 || p->batch == 0) return plan;
   const int group = heads / p->kv_heads;
   const int64_t capacity = (int64_t)p->table_width * p->page_size;
   const int64_t longest = max_context > 0 ? std::min(max_context, capacity) : capacity;
-  // the tcgen05 kernel takes its row maximum before the scale, so it needs a positive one
+  // Which tiles: by the rows (tokens x heads of a group) of an average sequence.  Measured with 32 / 8 heads of 128, 8 sequences over
+  // 4000 keys, 16-row against 256-row tiles: 16-bit pages 67 / 57 us at 32 rows, 91 / 80 us at 64, 170 / 81 us at 128; e4m3 46 / 74 us
+  // at 32, 90 / 104 us at 64, 145 / 94 us at 128.  The tcgen05 kernel takes its row maximum before the scale, so it needs a positive one.
   const bool tiled = type != LBI_F32 && (p->head_dim == 32 || p->head_dim == 64 || p->head_dim == 128);
-  plan.kernel = !tiled ? 0 : p->head_dim >= 64 && (int64_t)p->rows * group >= 64ll * p->batch && scale > 0.f ? 2 : 1;
+  const int64_t enough = p->cache_type == LBI_E4M3 ? 96 : 32;
+  plan.kernel = !tiled ? 0 : p->head_dim >= 64 && (int64_t)p->rows * group >= enough * p->batch && scale > 0.f ? 2 : 1;
   if (plan.kernel == 2) {
     // One block per SM, or two (head_dim 64, 16-bit pages).  Parts of a context pay where whole units leave the last round of blocks half empty: the
     // number of parts (of 512 keys at least) with the fewest key tiles per SM, 4 % added per part for the partial results and the
@@ -821,7 +861,8 @@ extern "C" lbi_attention_plan lbi_paged_attention_plan(const lbi_paged_batch* p,
     // Parts of equal length, so that a batch of uneven contexts is balanced by the order in which blocks finish: of about 2048 keys
     // (the partial results are under 2 % of the bytes read), so many that the blocks fill whole rounds of two per SM, and not below
     // 256 keys.
-    const int64_t units = tile_bound(*p, group, ROW_TILE) * p->kv_heads, slots = 2 * sm_count;
+    if (plan.kernel == 1 && (int64_t)p->rows * group <= 8ll * p->batch) plan.rows = 8;
+    const int64_t units = tile_bound(*p, group, plan.rows) * p->kv_heads, slots = 2 * sm_count;
     const int64_t rounds = std::max<int64_t>(1, (longest * units + slots * 2048 - 1) / (slots * 2048));
     const int64_t parts = std::max<int64_t>(1, rounds * slots / units);
     const int64_t keys = std::max<int64_t>(256, ((longest + parts - 1) / parts + 63) / 64 * 64);
@@ -841,7 +882,8 @@ extern "C" int lbi_paged_attention(const lbi_paged_batch* p, const void* q, int6
              scale * 1.4426950408889634f};
   int rc;
   if (plan.kernel == 0) rc = type == LBI_F32 ? launch_any<LBI_F32>(a, st) : type == LBI_BF16 ? launch_any<LBI_BF16>(a, st) : launch_any<LBI_F16>(a, st);
-  else if (plan.kernel == 1) rc = type == LBI_BF16 ? launch_rows<LBI_BF16>(a, st) : launch_rows<LBI_F16>(a, st);
+  else if (plan.kernel == 1 && plan.rows == 8) rc = type == LBI_BF16 ? launch_rows<LBI_BF16, 1>(a, st) : launch_rows<LBI_F16, 1>(a, st);
+  else if (plan.kernel == 1) rc = type == LBI_BF16 ? launch_rows<LBI_BF16, 2>(a, st) : launch_rows<LBI_F16, 2>(a, st);
   else rc = launch_attn_tiles(a, type, st);
   if (rc != 0 || plan.splits == 1) return rc;
   return type == LBI_F32 ? launch_combine<LBI_F32>(a, sm_count, st) : type == LBI_BF16 ? launch_combine<LBI_BF16>(a, sm_count, st) : launch_combine<LBI_F16>(a, sm_count, st);
