@@ -543,36 +543,45 @@ int launch_combine(const AttnArgs& a, int sm_count, cudaStream_t st) {
 }
 
 // ------------------------------------------------------------------------------------------------ 16-row tiles, any type and size
-// The same division of work with mma.sync m16n8k8 on tf32 operands: an fp32 value is the sum of two tf32 values up to 2^-22 of it, and
-// hi hi + hi lo + lo hi of two such sums lacks only lo lo.  The products of one step of eight (of one key tile) start from zero and are
+// The same division of work (one warp, its own keys) for fp32 queries and head sizes without tiles of their own.  An fp32 value is the
+// sum of three bf16 values (24 bits), an fp16 value of two, a bf16 value or a code is one; a product of two such sums is the products
+// of their terms down to 2^-16 of the first (six for fp32 against fp32), by mma.sync m16n8k16 with bf16 operands.  (tf32 products
+// would take two terms, but m16n8k8 occupies the tensor pipe for 32 cycles here, as long as plain FMAs would take, and m16n8k16 with
+// bf16 operands for 9.)  The products of one step of sixteen elements (of one key tile) start from zero and are
 // added to the running sums by the FMA units, which round to nearest: the tensor core truncates, and over thousands of keys that is a
-// drift (2 to 3 e-6 of the result, against 3.5 e-7).  16-bit values and codes are tf32 values as they stand, and need one product
-// less.  P is split like an fp32 operand for fp32 queries, and rounded to tf32 for 16-bit ones (as fine as fp16, finer than bf16).
-// Queries lie in shared memory in the order of the fragments; keys and values as they come, a row padded by 16 bytes, so that the eight
-// keys (or four pairs of them) of a fragment lie in different banks.
+// drift (2 to 3 e-6 of the result, against 3.5 e-7).
+// Queries lie in shared memory in the order of the fragments; keys and values as they come, their rows padded so that the accesses of a
+// fragment fall into different banks.
+template <int TYPE>
+struct Terms {
+  static constexpr int N = TYPE == LBI_F32 ? 3 : TYPE == LBI_F16 ? 2 : 1;
+};
 template <int TYPE, bool E4M3, int DHP>
 struct AnyTile {   // DHP: head_dim rounded up to 64, 128 or 256
   using Q = typename Elem<TYPE>::T;
   using C = typename Elem<E4M3 ? LBI_E4M3 : TYPE>::T;
-  static constexpr int KEYS = DHP == 256 ? 8 : 16, STAGES = 2;
-  static constexpr bool Q_LO = TYPE == LBI_F32, C_LO = TYPE == LBI_F32 && !E4M3, P_LO = TYPE == LBI_F32;
-  static constexpr int Q_BYTES = DHP / 8 * 32 * 16 * (Q_LO ? 2 : 1);
-  __host__ __device__ static int pitch(int dim) { return dim * (int)sizeof(C) + 16; }
-  __host__ __device__ static int stage(int dim) { return 2 * KEYS * pitch(dim) + 8 * KEYS + 16; }   // K, V, scales, which keys exist
+  static constexpr int KEYS = 16, STAGES = DHP == 256 && sizeof(C) == 4 ? 1 : 2;
+  static constexpr int NQ = Terms<TYPE>::N, NC = E4M3 ? 1 : Terms<TYPE>::N, NP = TYPE == LBI_F32 ? 3 : 2;
+  static constexpr int LAST = TYPE == LBI_F32 ? 2 : 1;   // terms i and j are multiplied if i + j <= LAST
+  static constexpr int Q_BYTES = DHP / 16 * 32 * 16 * NQ;
+  __host__ __device__ static int k_pitch(int dim) { return dim * (int)sizeof(C) + (sizeof(C) == 4 ? 32 : 16); }
+  __host__ __device__ static int v_pitch(int dim) { return dim * (int)sizeof(C) + 16; }
+  __host__ __device__ static int stage(int dim) { return KEYS * (k_pitch(dim) + v_pitch(dim)) + 8 * KEYS + 16; }   // K, V, scales, which keys exist
   __host__ __device__ static int smem(int dim) {
     const int join = WARPS * ROW_TILE * (dim + 4) * 4 + WARPS * ROW_TILE * 8, ring = WARPS * STAGES * stage(dim);
     return Q_BYTES + (join > ring ? join : ring);
   }
 };
 
-__device__ __forceinline__ uint32_t tf32(float x) {
-  uint32_t r;
-  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
-  return r;
-}
-__device__ __forceinline__ void mma1688(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+// The bf16 terms of two values, as words of two.
+template <int N>
+__device__ __forceinline__ void split_bf16(float x0, float x1, uint32_t* w) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    w[i] = pack16<LBI_BF16>(x0, x1);
+    x0 -= __uint_as_float(w[i] << 16);
+    x1 -= __uint_as_float(w[i] & 0xffff0000u);
+  }
 }
 
 template <int TYPE, bool E4M3, int DHP>
@@ -588,22 +597,20 @@ __global__ void __launch_bounds__(WARPS * 32) attn_any_kernel(const AttnArgs a) 
   const RowsUnit u = rows_unit(a, ROW_TILE);
   if (!u.any) return;
 
-  uint4* qs = reinterpret_cast<uint4*>(smem);   // [8 elements][lane]: hi, then (fp32) lo
+  constexpr int NQ = L::NQ, NC = L::NC, NP = L::NP, LAST = L::LAST;
+  uint4* qs = reinterpret_cast<uint4*>(smem);   // [16 elements][term][lane]
   int limit[2];
-  for (int ks = warp; ks < dim / 8; ks += WARPS) {
-    float x[4];
+  for (int ks = warp; ks < dim / 16; ks += WARPS) {
+    uint32_t w[4][NQ];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
+    for (int e = 0; e < 4; ++e) {   // rows g and g + 8, elements 2 t, + 1 and 2 t + 8, + 9
       const int r = g + 8 * (e & 1), rr = u.local + r;
-      x[e] = r < u.n_rows ? to_f<T>(((const T*)a.q)[(int64_t)(u.first_row + rr / a.group) * a.q_stride + (u.kh * a.group + rr % a.group) * dim + ks * 8 + t + 4 * (e >> 1)]) : 0.f;
+      const T* src = (const T*)a.q + (int64_t)(u.first_row + rr / a.group) * a.q_stride + (u.kh * a.group + rr % a.group) * dim + ks * 16 + 2 * t + 8 * (e >> 1);
+      const bool live = r < u.n_rows;
+      split_bf16<NQ>(live ? to_f<T>(src[0]) : 0.f, live ? to_f<T>(src[1]) : 0.f, w[e]);
     }
-    uint32_t hi[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) hi[e] = tf32(x[e]);
-    qs[(ks * 32 + lane) * (L::Q_LO ? 2 : 1)] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-    if (L::Q_LO)
-      qs[(ks * 32 + lane) * 2 + 1] = make_uint4(tf32(x[0] - __uint_as_float(hi[0])), tf32(x[1] - __uint_as_float(hi[1])),
-                                                tf32(x[2] - __uint_as_float(hi[2])), tf32(x[3] - __uint_as_float(hi[3])));
+    for (int i = 0; i < NQ; ++i) qs[(ks * NQ + i) * 32 + lane] = make_uint4(w[0][i], w[1][i], w[2][i], w[3][i]);
   }
 #pragma unroll
   for (int hh = 0; hh < 2; ++hh) limit[hh] = g + 8 * hh < u.n_rows ? u.first_pos + (u.local + g + 8 * hh) / a.group : -1;
@@ -616,7 +623,7 @@ __global__ void __launch_bounds__(WARPS * 32) attn_any_kernel(const AttnArgs a) 
     for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 
-  const int pitch = L::pitch(dim), stage = L::stage(dim), tile_bytes = KEYS * pitch;
+  const int k_pitch = L::k_pitch(dim), v_pitch = L::v_pitch(dim), stage = L::stage(dim);
   uint8_t* ring = smem + L::Q_BYTES + warp * STAGES * stage;
   const int n_tiles = u.k1 > u.k0 ? (u.k1 - u.k0 + KEYS - 1) / KEYS : 0;
   const int mine = n_tiles > warp ? (n_tiles - warp + WARPS - 1) / WARPS : 0;
@@ -630,17 +637,17 @@ __global__ void __launch_bounds__(WARPS * 32) attn_any_kernel(const AttnArgs a) 
     const int pos = u.k0 + (warp + i * WARPS) * KEYS + lane;
     const int slot = key_slot(a, u, pos, lane < KEYS && pos < u.k1, page);
     uint8_t* k_dst = ring + (i % STAGES) * stage;
-    uint8_t* v_dst = k_dst + tile_bytes;
+    uint8_t* v_dst = k_dst + KEYS * k_pitch;
     for (int j = 0; j < KEYS * row_chunks; j += 32) {   // KEYS * row_chunks is a multiple of 8, the last round may be partial
       const int row = min((j + lane) / row_chunks, KEYS - 1), c = (j + lane) - row * row_chunks;
       const int s = __shfl_sync(0xffffffffu, slot, row);
       if (c < row_chunks) {
         const int64_t off = (int64_t)max(s, 0) * dim * sizeof(C) + c * 16;
-        cp_async16(smem_addr(k_dst + row * pitch + c * 16), (const uint8_t*)p.k + off, s >= 0);
-        cp_async16(smem_addr(v_dst + row * pitch + c * 16), (const uint8_t*)p.v + off, s >= 0);
+        cp_async16(smem_addr(k_dst + row * k_pitch + c * 16), (const uint8_t*)p.k + off, s >= 0);
+        cp_async16(smem_addr(v_dst + row * v_pitch + c * 16), (const uint8_t*)p.v + off, s >= 0);
       }
     }
-    uint8_t* extra = k_dst + 2 * tile_bytes;
+    uint8_t* extra = v_dst + KEYS * v_pitch;
     if (E4M3 && lane < KEYS) {
       cp_async4(smem_addr(extra + lane * 4), p.k_scale + max(slot, 0), slot >= 0);
       cp_async4(smem_addr(extra + (KEYS + lane) * 4), p.v_scale + max(slot, 0), slot >= 0);
@@ -658,15 +665,21 @@ __global__ void __launch_bounds__(WARPS * 32) attn_any_kernel(const AttnArgs a) 
     page = next;
   }
   for (int i = 0; i < mine; ++i) {
-    cp_async_wait<STAGES - 2>();
-    __syncwarp();
+    if (STAGES > 1) {
+      cp_async_wait<STAGES - 2>();
+      __syncwarp();
+    }
     const int next = load_page(i + STAGES);
     if (i + STAGES - 1 < mine) copy_tile(i + STAGES - 1, page);
     cp_async_commit();
     page = next;
+    if (STAGES == 1) {   // no room for a tile ahead
+      cp_async_wait<0>();
+      __syncwarp();
+    }
     const uint8_t* k_src = ring + (i % STAGES) * stage;
-    const uint8_t* v_src = k_src + tile_bytes;
-    const uint8_t* extra = v_src + tile_bytes;
+    const uint8_t* v_src = k_src + KEYS * k_pitch;
+    const uint8_t* extra = v_src + KEYS * v_pitch;
     const int base = u.k0 + (warp + i * WARPS) * KEYS;
 
     float s[KEYS / 8][4];
@@ -674,23 +687,38 @@ __global__ void __launch_bounds__(WARPS * 32) attn_any_kernel(const AttnArgs a) 
     for (int n = 0; n < KEYS / 8; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
-#pragma unroll 4
-    for (int ks = 0; ks < dim / 8; ++ks) {
-      const uint4 qh = qs[(ks * 32 + lane) * (L::Q_LO ? 2 : 1)];
-      alignas(16) uint32_t ql[4] = {0, 0, 0, 0};
-      if (L::Q_LO) *reinterpret_cast<uint4*>(ql) = qs[(ks * 32 + lane) * 2 + 1];
+    // products of one sum wait for each other, and the compiler keeps them in the order in which they stand here: term by term
+    constexpr int KN = KEYS / 8;
+#pragma unroll 2
+    for (int ks = 0; ks < dim / 16; ++ks) {
+      alignas(16) uint32_t q[NQ][4];
+      uint32_t k[KN][2][NC];
+      float c[KN][2][4];   // the leading products and the others
 #pragma unroll
-      for (int n = 0; n < KEYS / 8; ++n) {
-        const C* row = reinterpret_cast<const C*>(k_src + (n * 8 + g) * pitch) + ks * 8 + t;
-        const float x0 = to_f<C>(row[0]), x1 = to_f<C>(row[4]);
-        const uint32_t h0 = tf32(x0), h1 = tf32(x1);
-        float c[4] = {0.f, 0.f, 0.f, 0.f};
-        if (L::C_LO) mma1688(c, reinterpret_cast<const uint32_t*>(&qh), tf32(x0 - __uint_as_float(h0)), tf32(x1 - __uint_as_float(h1)));
-        if (L::Q_LO) mma1688(c, ql, h0, h1);
-        mma1688(c, reinterpret_cast<const uint32_t*>(&qh), h0, h1);
+      for (int i = 0; i < NQ; ++i) *reinterpret_cast<uint4*>(q[i]) = qs[(ks * NQ + i) * 32 + lane];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[n][e] += c[e];
+      for (int n = 0; n < KN; ++n) {
+        const C* row = reinterpret_cast<const C*>(k_src + (n * 8 + g) * k_pitch) + ks * 16 + 2 * t;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float x[2];
+          load_f<C, 2>(row + 8 * h, x);
+          split_bf16<NC>(x[0], x[1], k[n][h]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) c[n][h][e] = 0.f;
+        }
       }
+#pragma unroll
+      for (int j = NC - 1; j >= 0; --j)
+#pragma unroll
+        for (int i = NQ - 1; i >= 0; --i)
+#pragma unroll
+          for (int n = 0; n < KN; ++n)
+            if (i + j <= LAST) mma16816<LBI_BF16>(c[n][i + j == 0 ? 0 : 1], q[i], k[n][0][j], k[n][1][j]);
+#pragma unroll
+      for (int n = 0; n < KN; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[n][e] += c[n][0][e] + c[n][1][e];
     }
 
     const uint32_t there = *reinterpret_cast<const volatile uint32_t*>(extra + 8 * KEYS);
@@ -724,35 +752,54 @@ __global__ void __launch_bounds__(WARPS * 32) attn_any_kernel(const AttnArgs a) 
       m[hh] = mn;
       l[hh] *= keep[hh];
     }
-    // keys 2 t and 2 t + 1 of eight take the places t and t + 4 of the product's inner index, for P and V alike
-    uint32_t ph[KEYS / 8][4], pl[KEYS / 8][4];
+    uint32_t pf[4][NP];   // rows g and g + 8, keys 2 t, + 1 and 8 + 2 t, + 1
 #pragma unroll
-    for (int kk = 0; kk < KEYS / 8; ++kk)
+    for (int n = 0; n < KN; ++n)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float w = ex2(s[kk][e] - ref[e >> 1]);
-        l[e >> 1] += w;
-        if (E4M3) w *= vs[kk][e & 1];
-        const int at = (e >> 1) + 2 * (e & 1);
-        ph[kk][at] = tf32(w);
-        pl[kk][at] = tf32(w - __uint_as_float(ph[kk][at]));
+      for (int hh = 0; hh < 2; ++hh) {
+        float w[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          w[e] = ex2(s[n][2 * hh + e] - ref[hh]);
+          l[hh] += w[e];
+          if (E4M3) w[e] *= vs[n][e];
+        }
+        split_bf16<NP>(w[0], w[1], pf[2 * n + hh]);
+      }
+    alignas(16) uint32_t pa[NP][4];
+#pragma unroll
+    for (int i = 0; i < NP; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) pa[i][e] = pf[e][i];
+    constexpr int VN = 4;   // products of eight elements at a time
+#pragma unroll
+    for (int n0 = 0; n0 < DHP / 8; n0 += VN) {
+      if (n0 * 8 >= dim) break;
+      uint32_t v[VN][2][NC];
+      float c[VN][4];
+#pragma unroll
+      for (int n = 0; n < VN; ++n) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const C* at = reinterpret_cast<const C*>(v_src + (8 * h + 2 * t) * v_pitch) + (n0 + n) * 8 + g;
+          const C* below = reinterpret_cast<const C*>(reinterpret_cast<const uint8_t*>(at) + v_pitch);
+          const bool live = (n0 + n) * 8 < dim;
+          split_bf16<NC>(live ? to_f<C>(*at) : 0.f, live ? to_f<C>(*below) : 0.f, v[n][h]);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c[n][e] = 0.f;
       }
 #pragma unroll
-    for (int n = 0; n < DHP / 8; ++n) {
-      if (n * 8 >= dim) break;
-      float c[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int j = NC - 1; j >= 0; --j)
 #pragma unroll
-      for (int kk = 0; kk < KEYS / 8; ++kk) {
-        const C* row0 = reinterpret_cast<const C*>(v_src + (kk * 8 + 2 * t) * pitch) + g;
-        const C* row1 = reinterpret_cast<const C*>(v_src + (kk * 8 + 2 * t + 1) * pitch) + g;
-        const float x0 = to_f<C>(row0[n * 8]), x1 = to_f<C>(row1[n * 8]);
-        const uint32_t h0 = tf32(x0), h1 = tf32(x1);
-        if (L::C_LO) mma1688(c, ph[kk], tf32(x0 - __uint_as_float(h0)), tf32(x1 - __uint_as_float(h1)));
-        if (L::P_LO) mma1688(c, pl[kk], h0, h1);
-        mma1688(c, ph[kk], h0, h1);
-      }
+        for (int i = NP - 1; i >= 0; --i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[n][e] = fmaf(o[n][e], keep[e >> 1], c[e]);
+          for (int n = 0; n < VN; ++n)
+            if (i + j <= LAST) mma16816<LBI_BF16>(c[n], pa[i], v[n][0][j], v[n][1][j]);
+#pragma unroll
+      for (int n = 0; n < VN; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[n0 + n][e] = fmaf(o[n0 + n][e], keep[e >> 1], c[n][e]);
     }
     __syncwarp();
   }
@@ -859,13 +906,15 @@ extern "C" lbi_attention_plan lbi_paged_attention_plan(const lbi_paged_batch* p,
     plan.split_keys = (int)std::max<int64_t>(128, ((longest + plan.splits - 1) / plan.splits + 127) / 128 * 128);
   } else {
     // Parts of equal length, so that a batch of uneven contexts is balanced by the order in which blocks finish: of about 2048 keys
-    // (the partial results are under 2 % of the bytes read), so many that the blocks fill whole rounds of two per SM, and not below
-    // 256 keys.
+    // (the partial results are under 2 % of the bytes read), so many that the blocks fill whole rounds of two per SM.  Not below 256
+    // keys, and 64, a tile per warp, for the kernel that splits its operands (2.6 us per tile; 7 sequences of up to 782 keys took 19.5 us
+    // in parts of 256).
+    const int64_t least = plan.kernel == 0 ? 64 : 256;
     if (plan.kernel == 1 && (int64_t)p->rows * group <= 8ll * p->batch) plan.rows = 8;
     const int64_t units = tile_bound(*p, group, plan.rows) * p->kv_heads, slots = 2 * sm_count;
     const int64_t rounds = std::max<int64_t>(1, (longest * units + slots * 2048 - 1) / (slots * 2048));
     const int64_t parts = std::max<int64_t>(1, rounds * slots / units);
-    const int64_t keys = std::max<int64_t>(256, ((longest + parts - 1) / parts + 63) / 64 * 64);
+    const int64_t keys = std::max<int64_t>(least, ((longest + parts - 1) / parts + 63) / 64 * 64);
     plan.splits = (int)std::max<int64_t>(1, (longest + keys - 1) / keys);
     plan.split_keys = (int)keys;
   }
