@@ -10,11 +10,18 @@
 #include "api_peer.h"
 #include "binding.h"
 
-// One word per device and thread that the kernels record wait time-outs and bad indices in.
+#include <mutex>
+
+// One word per device that the kernels record wait time-outs and bad indices in.  It is made by the first call that asks for it, which
+// should not be one that is being captured into a graph (the word would be zeroed by the replay only): ``make_status_word`` is the call
+// for that.
 torch::Tensor status_word(const torch::Tensor& like) {
-  static thread_local std::vector<torch::Tensor> words(16);
-  int dev = like.get_device();
-  if (!words[dev].defined()) words[dev] = torch::zeros({1}, like.options().dtype(at::kInt));
+  static std::mutex lock;
+  static std::vector<torch::Tensor>& words = *new std::vector<torch::Tensor>(64);   // outlives the runtime it would be freed with
+  const int dev = like.get_device();
+  TORCH_CHECK(dev >= 0 && dev < 64, "no status word for device ", dev);
+  std::lock_guard<std::mutex> guard(lock);
+  if (!words[dev].defined()) words[dev] = torch::zeros({1}, like.options().dtype(at::kInt).requires_grad(false));
   return words[dev];
 }
 
@@ -1309,6 +1316,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("dn_bf16"), py::arg("dv_out") = py::none());
   m.def("ssd_group_sum", &ssd_group_sum);
   m.def("kernel_status", &kernel_status);
+  m.def("make_status_word", [](const Tensor& like) { status_word(like); });
   m.def("set_peer_wait_limit_ms", &set_peer_wait_limit_ms);
   m.def("peer_barrier", &peer_barrier);
   m.def("peer_signal_all", &peer_signal_all);

@@ -163,6 +163,7 @@ Tensor paged_attention(const Tensor& q_in, const Tensor& k, const Tensor& v, con
   const int64_t heads = q_in.size(1);
   TORCH_CHECK_VALUE(heads > 0 && heads % p.kv_heads == 0 && q_in.size(2) == p.head_dim, "q has ", heads, " heads of ", q_in.size(2), ": pages have ",
                     p.kv_heads, " of ", p.head_dim);
+  TORCH_CHECK_VALUE(q_in.size(0) * heads < (1ll << 31), "2^31 rows times heads or more");
   const bool packed = q_in.stride(2) == 1 && (heads == 1 || q_in.stride(1) == p.head_dim);
   const Tensor q = aligned_rows(packed ? q_in : q_in.contiguous());
   Tensor o = output(out, q.sizes(), q, q.scalar_type(), p.batch == 0);

@@ -19,12 +19,12 @@ constexpr int COUNT_BYTES = 32768;
 constexpr int LOGIT_THREADS = 512;   // four blocks per SM: 2048 threads, 128 KB of counts
 
 template <int TYPE, typename COUNT>
-__global__ void __launch_bounds__(LOGIT_THREADS, 4) logits_kernel(const lbi_logit_rules p, int tile) {
+__global__ void __launch_bounds__(LOGIT_THREADS, 4) logits_kernel(const lbi_logit_rules p, int tile, unsigned tiles) {
   using T = typename Elem<TYPE>::T;
   constexpr bool WIDE = sizeof(COUNT) == 4;
   constexpr uint32_t PROMPT = WIDE ? 0x80000000u : 0x8000u;
   __shared__ alignas(16) COUNT count[COUNT_BYTES / sizeof(COUNT)];
-  const int b = blockIdx.y, v0 = blockIdx.x * tile, n = min(tile, p.vocab - v0);
+  const int b = blockIdx.x / tiles, v0 = (blockIdx.x % tiles) * tile, n = min(tile, p.vocab - v0);
   for (int i = threadIdx.x; i < tile * (int)sizeof(COUNT) / 16; i += LOGIT_THREADS) reinterpret_cast<uint4*>(count)[i] = make_uint4(0, 0, 0, 0);
   const int len = p.lengths ? min(max(p.lengths[b], 0), p.history) : p.history;
   const int prompt = p.prompt_lengths ? p.prompt_lengths[b] : 0;
@@ -84,20 +84,23 @@ __global__ void __launch_bounds__(LOGIT_THREADS, 4) logits_kernel(const lbi_logi
 }
 
 template <int TYPE>
-static void launch_logits(const lbi_logit_rules& p, int sm_count, cudaStream_t st) {
+static int launch_logits(const lbi_logit_rules& p, int sm_count, cudaStream_t st) {
   // As few tiles as the counts allow, then so many more as fit into the same number of rounds of four blocks per SM (192 x 128001: 9
   // instead of 8 per row), of 1024 tokens at least.
   const bool wide = p.history >= 32768;
   const int64_t most = COUNT_BYTES / (wide ? 4 : 2), slots = 4ll * sm_count;
   const int64_t fewest = (p.vocab + most - 1) / most, rounds = (fewest * p.batch + slots - 1) / slots;
-  const int64_t tiles = std::max(fewest, rounds * slots / p.batch);
-  const int tile = (int)std::min<int64_t>(most, std::max<int64_t>(1024, ((p.vocab + tiles - 1) / tiles + 31) / 32 * 32));
-  const dim3 grid((p.vocab + tile - 1) / tile, p.batch);
+  const int64_t wanted = std::max(fewest, rounds * slots / p.batch);
+  const int tile = (int)std::min<int64_t>(most, std::max<int64_t>(1024, ((p.vocab + wanted - 1) / wanted + 31) / 32 * 32));
+  const unsigned tiles = (unsigned)((p.vocab + tile - 1) / tile);
+  if ((int64_t)tiles * p.batch >= (1ll << 31)) return (int)cudaErrorInvalidValue;
+  const unsigned grid = tiles * p.batch;
   static lbi::PerDeviceOnce narrow_once, wide_once;
   narrow_once.all_shared(logits_kernel<TYPE, uint16_t>);
   wide_once.all_shared(logits_kernel<TYPE, uint32_t>);
-  if (wide) logits_kernel<TYPE, uint32_t><<<grid, LOGIT_THREADS, 0, st>>>(p, tile);
-  else logits_kernel<TYPE, uint16_t><<<grid, LOGIT_THREADS, 0, st>>>(p, tile);
+  if (wide) logits_kernel<TYPE, uint32_t><<<grid, LOGIT_THREADS, 0, st>>>(p, tile, tiles);
+  else logits_kernel<TYPE, uint16_t><<<grid, LOGIT_THREADS, 0, st>>>(p, tile, tiles);
+  return (int)cudaGetLastError();
 }
 
 }  // namespace paged
@@ -106,9 +109,7 @@ static void launch_logits(const lbi_logit_rules& p, int sm_count, cudaStream_t s
 extern "C" int lbi_adjust_logits(const lbi_logit_rules* p, int sm_count, cudaStream_t st) {
   using namespace lbi::paged;
   if (p->batch == 0 || p->vocab == 0) return 0;
-  if (p->batch > 65535 || p->type < 0 || p->type > LBI_F16) return (int)cudaErrorInvalidValue;
-  if (p->type == LBI_F32) launch_logits<LBI_F32>(*p, sm_count, st);
-  else if (p->type == LBI_BF16) launch_logits<LBI_BF16>(*p, sm_count, st);
-  else launch_logits<LBI_F16>(*p, sm_count, st);
-  return (int)cudaGetLastError();
+  if (p->type < 0 || p->type > LBI_F16) return (int)cudaErrorInvalidValue;
+  return p->type == LBI_F32 ? launch_logits<LBI_F32>(*p, sm_count, st)
+       : p->type == LBI_BF16 ? launch_logits<LBI_BF16>(*p, sm_count, st) : launch_logits<LBI_F16>(*p, sm_count, st);
 }

@@ -163,19 +163,20 @@ __global__ void __launch_bounds__(APPEND_THREADS, 8) append_kernel(const AppendA
 }
 
 template <int TYPE, bool E4M3>
-__global__ void __launch_bounds__(256) gather_kernel(const lbi_paged_batch p, void* k_out, void* v_out, int64_t max_len, int page_shift) {
+__global__ void __launch_bounds__(256) gather_kernel(const lbi_paged_batch p, void* k_out, void* v_out, int64_t max_len, int page_shift, unsigned blocks) {
   using T = typename Elem<TYPE>::T;
   using C = typename Elem<E4M3 ? LBI_E4M3 : TYPE>::T;
   const int dim = p.head_dim, parts = dim >> 4;   // 16 elements per thread
-  const int b = blockIdx.y / p.kv_heads, h = blockIdx.y % p.kv_heads;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t bh = blockIdx.x / blocks;
+  const int b = (int)(bh / p.kv_heads), h = (int)(bh % p.kv_heads);
+  const int64_t i = (int64_t)(blockIdx.x % blocks) * 256 + threadIdx.x;
   const int64_t pos = i / parts;
   if (pos >= max_len) return;
   const int d = (int)(i % parts) * 16;
   float x[16];
 #pragma unroll
   for (int e = 0; e < 16; ++e) x[e] = 0.f;
-  const bool is_k = blockIdx.z == 0;
+  const bool is_k = blockIdx.y == 0;
   if (pos < __ldg(p.context + b)) {
     const int page = page_of(p, b, (int)pos, page_shift);
     if (page >= 0) {
@@ -188,7 +189,7 @@ __global__ void __launch_bounds__(256) gather_kernel(const lbi_paged_batch p, vo
       }
     }
   }
-  T* out = (T*)(is_k ? k_out : v_out) + ((int64_t)blockIdx.y * max_len + pos) * dim + d;
+  T* out = (T*)(is_k ? k_out : v_out) + (bh * max_len + pos) * dim + d;
   store_f<T, 16>(out, x);
 }
 
@@ -223,10 +224,11 @@ extern "C" int lbi_kv_gather(const lbi_paged_batch* p, void* k_out, void* v_out,
   if (p->head_dim % 16 != 0 || p->head_dim > 256 || type < 0 || type > LBI_F16) return (int)cudaErrorInvalidValue;
   if (max_len <= 0 || p->batch == 0) return 0;
   const int64_t blocks = (max_len * (p->head_dim / 16) + 255) / 256;
-  if (blocks >= (1ll << 31) || (int64_t)p->batch * p->kv_heads > 65535) return (int)cudaErrorInvalidValue;
-  dim3 grid((unsigned)blocks, p->batch * p->kv_heads, 2);
+  const int64_t all = blocks * p->batch * p->kv_heads;
+  if (all >= (1ll << 31)) return (int)cudaErrorInvalidValue;
+  dim3 grid((unsigned)all, 2);
   const int shift = shift_of(p->page_size);
-#define LBI_GATHER(T, E) gather_kernel<T, E><<<grid, 256, 0, st>>>(*p, k_out, v_out, max_len, shift)
+#define LBI_GATHER(T, E) gather_kernel<T, E><<<grid, 256, 0, st>>>(*p, k_out, v_out, max_len, shift, (unsigned)blocks)
   LBI_BY_TYPE(type, p->cache_type == LBI_E4M3, LBI_GATHER);
 #undef LBI_GATHER
   return (int)cudaGetLastError();

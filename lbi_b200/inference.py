@@ -77,8 +77,8 @@ class _LogitRuleState:
                     raise ValueError("logit_bias maps token ids of the vocabulary to finite values")
                 dense[int(token)] = float(value)
             bias = dense
-        elif bias is not None and tuple(bias.shape) != (vocab,):
-            raise ValueError("logit_bias must have one entry per token of the vocabulary")
+        elif bias is not None and (tuple(bias.shape) != (vocab,) or not bool(torch.isfinite(bias).all())):
+            raise ValueError("logit_bias must have one finite entry per token of the vocabulary")
         self.bias = None if bias is None else bias.to(device=device, dtype=torch.float32).contiguous()
         allowed, self.grammar, self.mask = rules.allowed_tokens, None, None
         if callable(allowed):

@@ -54,7 +54,8 @@ def test_a_few_new_tokens(heads, kv_heads, dim, page, dtype, cache):
     check_attention(Batch([(3, 40), (3, 3), (3, 131)], heads, kv_heads, dim, page, dtype, cache, DEV), use_cu=False)
 
 
-@pytest.mark.parametrize("heads,kv_heads,dim,page", [(2, 2, 64, 16), (4, 1, 64, 32), (3, 1, 128, 8), (2, 1, 128, 128), (2, 1, 80, 64)])
+@pytest.mark.parametrize("heads,kv_heads,dim,page", [(2, 2, 64, 16), (4, 1, 64, 32), (3, 1, 128, 8), (2, 1, 128, 128), (2, 1, 80, 64), (2, 1, 64, 128),
+                                                       (1, 1, 64, 8)])
 @pytest.mark.parametrize("dtype,cache", [(BF16, "same"), (F16, "same"), (F32, "same"), (BF16, "e4m3"), (F16, "e4m3")])
 def test_chunks_of_new_tokens(heads, kv_heads, dim, page, dtype, cache):
     check_attention(Batch([(130, 130), (1, 50), (129, 400), (0, 3), (64, 64), (200, 100)], heads, kv_heads, dim, page, dtype, cache, DEV), tail=5)
@@ -70,6 +71,43 @@ def test_large_scores_and_uneven_values():
 def test_a_long_context(dtype, cache):
     check_attention(Batch([(1, 9000), (1, 37)], 2, 1, 64, 64, dtype, cache, DEV))
     check_attention(Batch([(2, 5000)], 2, 2, 128, 16, dtype, cache, DEV), max_context=100)   # a hint that is too short
+
+
+@pytest.mark.parametrize("dtype,cache", [(BF16, "same"), (BF16, "e4m3"), (F32, "same")])
+def test_many_sequences(dtype, cache):
+    """More sequences than a warp looks at in one step, empty ones among them; all heads of a token in several tiles."""
+    seqs = [(i % 3, 5 + 7 * i % 60) for i in range(41)]
+    check_attention(Batch(seqs, 4, 2, 64, 16, dtype, cache, DEV), tail=1)
+    check_append(seqs, 4, 2, 64, 16, dtype, cache, DEV, tail=1)
+    check_attention(Batch([(1, 40)] * 35, 2, 1, 64, 16, dtype, cache, DEV), use_cu=False)
+    check_attention(Batch([(2, 50), (1, 9)], 40, 1, 64, 16, dtype, cache, DEV))
+    check_attention(Batch([(1, 33), (3, 3)], 300, 1, 64, 16, dtype, cache, DEV))
+
+
+def test_batches_beyond_the_grid_limits_of_one_dimension():
+    pages = ops.kv_pages(2, 8, 8, 16, F32, DEV)
+    pages.k.normal_()
+    table = torch.arange(9000, device=DEV, dtype=torch.int32).remainder(2).view(9000, 1)
+    ctx = torch.arange(9000, device=DEV, dtype=torch.int32).remainder(9)
+    k, _ = ops.kv_gather(pages, table, ctx, 8)
+    want = pages.k[table[:, 0].long()] * (torch.arange(8, device=DEV) < ctx[:, None])[:, None, :, None]
+    assert torch.equal(k, want)
+    x = torch.randn(70000, 40, device=DEV)
+    tokens = torch.arange(70000, device=DEV).remainder(40).view(-1, 1)
+    got = ops.adjust_logits(x, tokens, presence=1.0)
+    assert torch.equal(got, x.scatter_add(1, tokens, torch.full((70000, 1), -1.0, device=DEV)))
+
+
+def test_nothing_in_the_table():
+    batch = Batch([(1, 0), (2, 1), (0, 0)], 2, 2, 64, 16, BF16, "same", DEV)   # contexts shorter than their new tokens
+    check_attention(batch)
+    empty = torch.zeros(3, 0, dtype=torch.int32, device=DEV)
+    q = batch.queries()
+    assert not bool(ops.paged_attention(q, batch.pages, empty, torch.zeros_like(batch.context), 0.1, cu_seqlens=batch.cu).any())
+    none = torch.zeros(0, dtype=torch.int32, device=DEV)
+    zero = torch.zeros(1, dtype=torch.int32, device=DEV)
+    assert not bool(ops.paged_attention(q, batch.pages, empty[:0], none, 0.1, cu_seqlens=zero).any())
+    assert ops.paged_attention(q[:0], batch.pages, empty[:0], none, 0.1).shape == (0, 2, 64)
 
 
 def test_given_outputs_keep_the_rows_behind_the_last_sequence():

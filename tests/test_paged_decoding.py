@@ -106,7 +106,7 @@ def test_rules_shape_what_is_generated():
     for bad in (dict(repetition_penalty=0.0), dict(presence_penalty=float("nan"))):
         with pytest.raises(ValueError):
             LogitRules(**bad)
-    for bad in (dict(logit_bias={VOCAB: 1.0}), dict(logit_bias=torch.zeros(3)), dict(allowed_tokens=[VOCAB]), dict(allowed_tokens=[]),
+    for bad in (dict(logit_bias={VOCAB: 1.0}), dict(logit_bias=torch.zeros(3)), dict(logit_bias=torch.full((VOCAB,), float("-inf"))), dict(allowed_tokens=[VOCAB]), dict(allowed_tokens=[]),
                 dict(allowed_tokens=torch.zeros(VOCAB, dtype=torch.bool)), dict(allowed_tokens=lambda t: torch.ones(3, dtype=torch.bool))):
         with pytest.raises(ValueError):
             generate(model, prompt, 2, rules=LogitRules(**bad))
