@@ -163,22 +163,20 @@ __global__ void __launch_bounds__(APPEND_THREADS, 8) append_kernel(const AppendA
 }
 
 template <int TYPE, bool E4M3>
-__global__ void __launch_bounds__(256) gather_kernel(const lbi_paged_batch p, void* k_out, void* v_out, int64_t max_len, int page_shift, unsigned blocks) {
+__global__ void __launch_bounds__(256) gather_kernel(const lbi_paged_batch p, void* k_out, void* v_out, int max_len, int page_shift, int bh0) {
   using T = typename Elem<TYPE>::T;
   using C = typename Elem<E4M3 ? LBI_E4M3 : TYPE>::T;
-  const int dim = p.head_dim, parts = dim >> 4;   // 16 elements per thread
-  const int64_t bh = blockIdx.x / blocks;
-  const int b = (int)(bh / p.kv_heads), h = (int)(bh % p.kv_heads);
-  const int64_t i = (int64_t)(blockIdx.x % blocks) * 256 + threadIdx.x;
-  const int64_t pos = i / parts;
+  const unsigned dim = p.head_dim, parts = dim >> 4;   // 16 elements per thread
+  const int bh = bh0 + blockIdx.y, b = bh / p.kv_heads, h = bh % p.kv_heads;
+  const unsigned i = blockIdx.x * 256 + threadIdx.x;
+  const int pos = (int)(i / parts), d = (int)(i % parts) * 16;
   if (pos >= max_len) return;
-  const int d = (int)(i % parts) * 16;
   float x[16];
 #pragma unroll
   for (int e = 0; e < 16; ++e) x[e] = 0.f;
-  const bool is_k = blockIdx.y == 0;
+  const bool is_k = blockIdx.z == 0;
   if (pos < __ldg(p.context + b)) {
-    const int page = page_of(p, b, (int)pos, page_shift);
+    const int page = page_of(p, b, pos, page_shift);
     if (page >= 0) {
       const int64_t slot = ((int64_t)page * p.kv_heads + h) * p.page_size + (pos & (p.page_size - 1));
       load_f<C, 16>((const C*)(is_k ? p.k : p.v) + slot * dim + d, x);
@@ -189,8 +187,7 @@ __global__ void __launch_bounds__(256) gather_kernel(const lbi_paged_batch p, vo
       }
     }
   }
-  T* out = (T*)(is_k ? k_out : v_out) + (bh * max_len + pos) * dim + d;
-  store_f<T, 16>(out, x);
+  store_f<T, 16>((T*)(is_k ? k_out : v_out) + ((int64_t)bh * max_len + pos) * dim + d, x);
 }
 
 }  // namespace paged
@@ -223,13 +220,14 @@ extern "C" int lbi_kv_gather(const lbi_paged_batch* p, void* k_out, void* v_out,
   using namespace lbi::paged;
   if (p->head_dim % 16 != 0 || p->head_dim > 256 || type < 0 || type > LBI_F16) return (int)cudaErrorInvalidValue;
   if (max_len <= 0 || p->batch == 0) return 0;
-  const int64_t blocks = (max_len * (p->head_dim / 16) + 255) / 256;
-  const int64_t all = blocks * p->batch * p->kv_heads;
-  if (all >= (1ll << 31)) return (int)cudaErrorInvalidValue;
-  dim3 grid((unsigned)all, 2);
+  const int64_t pairs = (int64_t)p->batch * p->kv_heads;
+  if (max_len * (p->head_dim / 16) >= (1ll << 31) || pairs >= (1ll << 31)) return (int)cudaErrorInvalidValue;
   const int shift = shift_of(p->page_size);
-#define LBI_GATHER(T, E) gather_kernel<T, E><<<grid, 256, 0, st>>>(*p, k_out, v_out, max_len, shift, (unsigned)blocks)
-  LBI_BY_TYPE(type, p->cache_type == LBI_E4M3, LBI_GATHER);
+  for (int64_t bh0 = 0; bh0 < pairs; bh0 += 65535) {   // what one grid holds in its second dimension
+    const dim3 grid((unsigned)((max_len * (p->head_dim / 16) + 255) / 256), (unsigned)(pairs - bh0 < 65535 ? pairs - bh0 : 65535), 2);
+#define LBI_GATHER(T, E) gather_kernel<T, E><<<grid, 256, 0, st>>>(*p, k_out, v_out, (int)max_len, shift, (int)bh0)
+    LBI_BY_TYPE(type, p->cache_type == LBI_E4M3, LBI_GATHER);
 #undef LBI_GATHER
+  }
   return (int)cudaGetLastError();
 }
