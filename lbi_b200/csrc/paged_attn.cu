@@ -3,7 +3,7 @@
 //   o_i = sum_j softmax_j(scale q_i . k_j) v_j   over the positions j <= context - new + i of the sequence; no position: o_i = 0.
 //
 // Kernels:
-//   attn_rows_kernel   16 query rows at a time (tokens x heads of a group) for 16-bit queries: decoding, a few new tokens.
+//   attn_rows_kernel   8 or 16 query rows at a time (tokens x heads of a group) for 16-bit queries: decoding, a few new tokens.
 //   attn_tiles_kernel  256 rows at a time on tcgen05 (paged_attn_tc.cu): chunks of a prompt.
 //   attn_any_kernel    16 rows at a time in (almost) full precision: fp32 queries, and head sizes that the other tiles do not cover.
 //   combine_kernel     joins the parts of a long context.
@@ -14,7 +14,7 @@
 namespace lbi {
 namespace paged {
 
-// ------------------------------------------------------------------------------------------------ 16-row tiles
+// ------------------------------------------------------------------------------------------------ tiles of 8 and 16 rows
 // Bound by reading the cache once: 2 head_dim sizeof(code) bytes per key and kv head.  All query heads of a group (and several new
 // tokens, if there are) share a tile of 8 or 16 rows, so that one read of a key serves them all, and mma.sync m16n8k16 does the
 // products with the keys (then the head's elements) as its 16 rows and the query rows as its 8 columns: S^T = K Q^T, O^T = V^T P^T.
@@ -28,6 +28,10 @@ namespace paged {
 // the value's scale and stay in (0, 1] (fp16 has no range for p * v_scale); the sum of exponentials takes 2^(u_j - max u) / v_scale_j.
 // P is rounded to the 16-bit type of the products before the second one (half a step of that type, as the result itself is rounded);
 // maximum, sum and output stay in fp32.
+//
+// Measured on a B200, 32 query heads on 8 of 128: 64 contexts of up to 8192 keys (ragged, 1.02 GB) 183 us, 5.6 TB/s, 0.85 of the copy
+// bandwidth; all 8192 long 0.94 of it.  e4m3: 2 contexts of 131072 keys (0.55 GB) 115 us, 4.8 TB/s, 0.73: the codes' way to fp16 takes
+// the issue slots (56 % busy) that the 16-bit pages leave free (26 %).
 
 constexpr int ROW_TILE = 16;   // rows of attn_any_kernel; attn_rows_kernel has tiles of 8, too
 constexpr int WARPS = 4;

@@ -9,6 +9,11 @@
 // thread's 16 elements are 8 of each half of the head (the two partners of 8 turns) or 16 neighbours when the pairs are
 // interleaved, so a turn needs no exchange between threads; a block owns one token, so a thread loads its 8 cosines and sines once
 // for all heads.
+//
+// Measured on a B200: 24617 tokens of 32 + 2 x 8 heads of 128, bf16, into e4m3 pages (559 MB) 130 us, 4.3 TB/s, 0.65 of the copy
+// bandwidth: the chain load - maximum over the head row - division - store and the issue slots (61 % busy) bound it, not DRAM (50 %).
+// 12 contexts of up to 16384 tokens from e4m3 (8 heads of 128, 1.05 GB) 178 us, 0.90 of the copy bandwidth.  One token per call: launch
+// and call, 7 us.
 #include "paged.cuh"
 
 namespace lbi {
