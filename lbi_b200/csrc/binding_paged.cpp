@@ -123,6 +123,7 @@ Tensor kv_append(const Tensor& qkv_in, const Tensor& k, const Tensor& v, const O
                     p.kv_heads, " heads of ", p.head_dim);
   const float *cp = nullptr, *sp = nullptr;
   int64_t rope_rows = 0;
+  TORCH_CHECK_VALUE(given(cos_tab) == given(sin_tab), "rope needs both tables");
   if (given(cos_tab)) {
     for (const Tensor& t : {*cos_tab, *sin_tab})
       TORCH_CHECK_VALUE(t.scalar_type() == at::kFloat && t.dim() == 2 && t.size(1) == p.head_dim / 2 && t.is_contiguous() && t.device() == k.device() &&

@@ -94,7 +94,7 @@ class _LogitRuleState:
             self.mask = ops.pack_token_mask(self._checked(mask).to(device))
 
     def _checked(self, mask: torch.Tensor) -> torch.Tensor:
-        if not torch.is_tensor(mask) or mask.dtype != torch.bool or mask.shape[-1] != self.vocab or mask.dim() > 2:
+        if not torch.is_tensor(mask) or mask.dtype != torch.bool or mask.dim() not in (1, 2) or mask.shape[-1] != self.vocab:
             raise ValueError("allowed_tokens must be (or return) a bool tensor [V] or [B, V]")
         if not bool(mask.any(dim=-1).all()):   # nothing to sample from
             raise ValueError("allowed_tokens allows no token")

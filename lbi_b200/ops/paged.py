@@ -107,7 +107,7 @@ def kv_append(qkv, pages, page_table, context_lens, n_heads, cu_seqlens=None, ro
     ``qkv`` [rows, (n_heads + 2 kv_heads) * head_dim] are packed projections; ``rope = (cos, sin, interleaved)`` (fp32 tables
     [positions, head_dim / 2]) turns q and k by their positions first.  Into e4m3 pages a head row goes as
     ``round(x / scale)`` with ``scale = max |x| / 448``.  Two sequences must not share a page that new tokens are written to."""
-    if qkv.requires_grad:
+    if qkv.requires_grad or pages[0].requires_grad or pages[1].requires_grad:
         _refuse_grad()
     cos, sin, interleaved = rope if rope is not None else (None, None, False)
     if _kernel_shape(qkv, pages[0].size(-1)):
@@ -119,6 +119,8 @@ def kv_append(qkv, pages, page_table, context_lens, n_heads, cu_seqlens=None, ro
     kv_heads, head_dim = pages.k.shape[1], pages.k.shape[3]
     if qkv.dim() != 2 or n_heads <= 0 or qkv.shape[1] != (n_heads + 2 * kv_heads) * head_dim:
         raise ValueError(f"qkv must be [rows, {(n_heads + 2 * kv_heads) * head_dim}]")
+    if (cos is None) != (sin is None):
+        raise ValueError("rope needs both tables")
     if cos is not None and (cos.dim() != 2 or cos.shape != sin.shape or 2 * cos.shape[1] != head_dim or cos.dtype != torch.float32 or sin.dtype != torch.float32):
         raise ValueError("rotary tables must be fp32 [positions, head_dim / 2] tensors")
     _check_rows(qkv, pages, out, (qkv.shape[0], n_heads, head_dim))
@@ -129,6 +131,8 @@ def kv_gather(pages, page_table, context_lens, max_len, dtype=None):
     """The cached keys and values as contiguous [B, kv_heads, max_len, head_dim] tensors, zero behind each context (the layout of
     ``CausalSelfAttention.step``).  ``dtype``: type of the result for e4m3 pages (default bf16); other pages keep theirs."""
     k = pages[0]
+    if k.requires_grad or pages[1].requires_grad:
+        _refuse_grad()
     dtype = dtype or (torch.bfloat16 if k.dtype == torch.float8_e4m3fn else k.dtype)
     if k.is_cuda and k.size(-1) % 16 == 0 and k.size(-1) <= 256 and native_available():
         KERNEL_LAUNCHES["count"] += 1
@@ -149,7 +153,7 @@ def paged_attention(q, pages, page_table, context_lens, scale, cu_seqlens=None, 
 
     ``max_context``: the longest context if the host knows it (a hint that sizes the launch, default: what the page table can
     hold); a longer context still gives right results.  ``out`` must not overlap ``q``."""
-    if q.requires_grad:
+    if q.requires_grad or pages[0].requires_grad or pages[1].requires_grad:
         _refuse_grad()
     if _kernel_shape(q, pages[0].size(-1)):
         KERNEL_LAUNCHES["count"] += 1
@@ -187,7 +191,7 @@ def adjust_logits(logits, tokens, lengths=None, prompt_lengths=None, *, repetiti
     * a token whose bit in ``allowed`` (``pack_token_mask``; [ceil(V / 32)] or one row each) is not set: -inf
 
     The three penalties are numbers or fp32 [B].  ``out`` may be ``logits`` itself when that is fp32."""
-    if logits.requires_grad or (bias is not None and bias.requires_grad):
+    if logits.requires_grad or any(torch.is_tensor(x) and x.requires_grad for x in (repetition, presence, frequency, bias)):
         _refuse_grad()
     if logits.is_cuda and logits.dtype in _TYPES and native_available():
         KERNEL_LAUNCHES["count"] += 1

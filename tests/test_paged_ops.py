@@ -98,6 +98,15 @@ def refusals(device):
     yield lambda: ops.adjust_logits(logits, tokens, bias=torch.zeros(39, device=device))
     yield lambda: ops.adjust_logits(logits, tokens, allowed=torch.zeros(2, 1, dtype=torch.int32, device=device))
     yield lambda: ops.adjust_logits(logits, tokens, out=torch.zeros(2, 39, device=device))
+    # one table of the two, and gradients that an operand other than the rows asks for
+    yield lambda: ops.kv_append(qkv, pages, table, ctx, 4, rope=(cos, None, False))
+    yield lambda: ops.kv_append(qkv, pages, table, ctx, 4, rope=(None, cos, False))
+    learned = pages._replace(v=pages.v.clone().requires_grad_())
+    yield lambda: ops.kv_append(qkv, learned, table, ctx, 4)
+    yield lambda: ops.paged_attention(q, learned, table, ctx, 1.0)
+    yield lambda: ops.kv_gather(learned, table, ctx, 4)
+    yield lambda: ops.adjust_logits(logits, tokens, frequency=torch.zeros(2, device=device, requires_grad=True))
+    yield lambda: ops.adjust_logits(logits, tokens, bias=torch.zeros(40, device=device, requires_grad=True))
 
 
 def test_refusals():
