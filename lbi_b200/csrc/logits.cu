@@ -9,9 +9,9 @@
 // that occurs in the prompt.  Every block of a row reads the row's history again, which stays in L2, so tiles are large: 16-bit counts,
 // two to a word, while the history is shorter than 2^15, else 32-bit counts of half as many tokens.
 //
-// Measured on a B200: 192 rows of 128001 fp32 logits, histories of up to 4096 tokens, bias and mask: 65 us against 32 us for reading and
+// Measured on a B200: 192 rows of 128001 fp32 logits, histories of up to 4096 tokens, bias and mask: 59 us against 32 us for reading and
 // writing the logits once (207 MB).  The rest is the blocks' start: counters to zero, a walk over the history (8 tiles read it), two
-// barriers; issue slots 59 % busy, DRAM 31 %.  A row of 32768: launch and call, 5.3 us.
+// barriers.  A row of 32768: launch and call, 5.3 us.
 #include <algorithm>
 
 #include "paged.cuh"
@@ -20,10 +20,12 @@ namespace lbi {
 namespace paged {
 
 constexpr int COUNT_BYTES = 32768;
-constexpr int LOGIT_THREADS = 512;   // four blocks per SM: 2048 threads, 128 KB of counts
+// Three blocks per SM leave registers for the loads of EACH elements at once.  Measured with 192 x 128001 (single calls): 62 us; four blocks 68 us, and 70 us
+// with 8 elements; three blocks with 2 or 8 elements 70 and 68 us; two blocks 76 us; blocks of 256 or 1024 threads 69 to 80 us.
+constexpr int LOGIT_THREADS = 512, LOGIT_BLOCKS = 3, EACH = 4;
 
 template <int TYPE, typename COUNT>
-__global__ void __launch_bounds__(LOGIT_THREADS, 4) logits_kernel(const lbi_logit_rules p, int tile, unsigned tiles) {
+__global__ void __launch_bounds__(LOGIT_THREADS, LOGIT_BLOCKS) logits_kernel(const lbi_logit_rules p, int tile, unsigned tiles) {
   using T = typename Elem<TYPE>::T;
   constexpr bool WIDE = sizeof(COUNT) == 4;
   constexpr uint32_t PROMPT = WIDE ? 0x80000000u : 0x8000u;
@@ -58,7 +60,6 @@ __global__ void __launch_bounds__(LOGIT_THREADS, 4) logits_kernel(const lbi_logi
   const int* allowed = p.allowed ? p.allowed + (int64_t)b * p.allowed_stride + (v0 >> 5) : nullptr;
   // Rows of odd vocabularies start anywhere, so an element per thread and access, several in flight; the tile's end is a case of its
   // own.  A tile starts at a multiple of 32, so a warp's 32 elements share a word of the mask.
-  constexpr int EACH = 8;
   auto rules = [&](int i, float f, float add, uint32_t bits) {
     const uint32_t c = count[i];
     if (c) {
@@ -89,10 +90,10 @@ __global__ void __launch_bounds__(LOGIT_THREADS, 4) logits_kernel(const lbi_logi
 
 template <int TYPE>
 static int launch_logits(const lbi_logit_rules& p, int sm_count, cudaStream_t st) {
-  // As few tiles as the counts allow, then so many more as fit into the same number of rounds of four blocks per SM (192 x 128001: 9
+  // As few tiles as the counts allow, then so many more as fit into the same number of rounds of blocks (192 x 128001: 9
   // instead of 8 per row), of 1024 tokens at least.
   const bool wide = p.history >= 32768;
-  const int64_t most = COUNT_BYTES / (wide ? 4 : 2), slots = 4ll * sm_count;
+  const int64_t most = COUNT_BYTES / (wide ? 4 : 2), slots = (int64_t)LOGIT_BLOCKS * sm_count;
   const int64_t fewest = (p.vocab + most - 1) / most, rounds = (fewest * p.batch + slots - 1) / slots;
   const int64_t wanted = std::max(fewest, rounds * slots / p.batch);
   const int tile = (int)std::min<int64_t>(most, std::max<int64_t>(1024, ((p.vocab + wanted - 1) / wanted + 31) / 32 * 32));

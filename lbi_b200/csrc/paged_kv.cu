@@ -10,8 +10,8 @@
 // interleaved, so a turn needs no exchange between threads; a block owns one token, so a thread loads its 8 cosines and sines once
 // for all heads.
 //
-// Measured on a B200: 24617 tokens of 32 + 2 x 8 heads of 128, bf16, into e4m3 pages (559 MB) 130 us, 4.3 TB/s, 0.65 of the copy
-// bandwidth: the chain load - maximum over the head row - division - store and the issue slots (61 % busy) bound it, not DRAM (50 %).
+// Measured on a B200: 24617 tokens of 32 + 2 x 8 heads of 128, bf16, into e4m3 pages (559 MB) 122 us, 4.6 TB/s, 0.70 of the copy
+// bandwidth: the chain load - maximum over the head row - division - store and the issue slots bound it, not DRAM.
 // 12 contexts of up to 16384 tokens from e4m3 (8 heads of 128, 1.05 GB) 178 us, 0.90 of the copy bandwidth.  One token per call: launch
 // and call, 7 us.
 #include "paged.cuh"
@@ -19,7 +19,9 @@
 namespace lbi {
 namespace paged {
 
-constexpr int APPEND_THREADS = 128;
+// A token's threads: 128 while blocks are few, for fewer passes over its heads (12 tokens of 48 heads 11.1 us, 64 threads 13.3; 240 tokens
+// 11.2 / 13.4), 64 from FEW_TOKENS on, for a block's start spread over more passes (1200 tokens 17.4 / 16.4 us, 24624 tokens 130 / 122).
+constexpr int APPEND_THREADS = 128, FEW_TOKENS = 600;
 
 struct AppendArgs {
   lbi_paged_batch b;
@@ -42,7 +44,7 @@ __global__ void __launch_bounds__(APPEND_THREADS, 8) append_kernel(const AppendA
   const int group = 1 << a.group_shift, lane = threadIdx.x & (group - 1);
   const int d0 = PAIRED ? lane * 16 : lane * 8, d1 = PAIRED ? d0 + 8 : d0 + half;   // two runs of 8 elements
   const bool active = lane * 16 < dim;
-  const int total = a.heads + 2 * p.kv_heads, per_pass = APPEND_THREADS >> a.group_shift, first = threadIdx.x >> a.group_shift;
+  const int total = a.heads + 2 * p.kv_heads, per_pass = blockDim.x >> a.group_shift, first = threadIdx.x >> a.group_shift;
   const T* src = (const T*)a.qkv + (int64_t)row * a.qkv_stride;
   T* q_out = (T*)a.q_out + (int64_t)row * a.heads * dim;
 
@@ -211,10 +213,11 @@ extern "C" int lbi_kv_append(const lbi_paged_batch* p, const void* qkv, int64_t 
   if (p->head_dim % 16 != 0 || p->head_dim > 256 || p->rows < 0 || type < 0 || type > LBI_F16) return (int)cudaErrorInvalidValue;
   if (p->rows == 0) return 0;
   AppendArgs a{*p, qkv, qkv_stride, q_out, heads, zero_tail, shift_of(p->page_size), shift_of(p->head_dim / 16), cos_tab, sin_tab, rope_rows};
+  const int threads = p->rows < FEW_TOKENS ? APPEND_THREADS : APPEND_THREADS / 2;
 #define LBI_APPEND(T, E)                                                             \
   do {                                                                                \
-    if (interleaved) append_kernel<T, E, true><<<p->rows, APPEND_THREADS, 0, st>>>(a); \
-    else append_kernel<T, E, false><<<p->rows, APPEND_THREADS, 0, st>>>(a);            \
+    if (interleaved) append_kernel<T, E, true><<<p->rows, threads, 0, st>>>(a); \
+    else append_kernel<T, E, false><<<p->rows, threads, 0, st>>>(a);            \
   } while (0)
   LBI_BY_TYPE(type, p->cache_type == LBI_E4M3, LBI_APPEND);
 #undef LBI_APPEND

@@ -42,6 +42,12 @@ def test_append_and_gather(heads, kv_heads, dim, page, dtype, cache):
 
 
 @pytest.mark.parametrize("heads,kv_heads,dim,page", SHAPES)
+@pytest.mark.parametrize("dtype,cache", [(BF16, "same"), (F32, "e4m3")])
+def test_append_of_many_tokens(heads, kv_heads, dim, page, dtype, cache):
+    check_append([(333, 401), (0, 5), (312, 312)], heads, kv_heads, dim, page, dtype, cache, DEV, tail=3)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,page", SHAPES)
 @pytest.mark.parametrize("dtype,cache", [(BF16, "same"), (F16, "same"), (F32, "same"), (BF16, "e4m3"), (F16, "e4m3"), (F32, "e4m3")])
 def test_single_tokens(heads, kv_heads, dim, page, dtype, cache):
     check_attention(Batch(STEPS, heads, kv_heads, dim, page, dtype, cache, DEV, extra_columns=1), tail=2)
