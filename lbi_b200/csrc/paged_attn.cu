@@ -887,20 +887,23 @@ extern "C" lbi_attention_plan lbi_paged_attention_plan(const lbi_paged_batch* p,
   const int group = heads / p->kv_heads;
   const int64_t capacity = (int64_t)p->table_width * p->page_size;
   const int64_t longest = max_context > 0 ? std::min(max_context, capacity) : capacity;
-  // Which tiles: by the rows (tokens x heads of a group) of an average sequence.  Measured with 32 / 8 heads of 128, 8 sequences over
-  // 4000 keys, 16-row against 256-row tiles: 16-bit pages 67 / 57 us at 32 rows, 91 / 80 us at 64, 170 / 81 us at 128; e4m3 46 / 74 us
-  // at 32, 90 / 104 us at 64, 145 / 94 us at 128.  The tcgen05 kernel takes its row maximum before the scale, so it needs a positive one.
+  // Which tiles: by the rows (tokens x heads of a group) of an average sequence.  The 16-row tiles read the cache once per 16 rows, the
+  // 256-row tiles cost the same up to 256.  Measured with 32 / 8 heads of 128, 8 sequences over 4000 keys (16 over 8000), 16-row / 256-row:
+  // 16-bit pages 73 / 62 us (175 / 171) around 30 rows; e4m3 64 / 83 us (206 / 249) at 48 rows, 93 / 83 (259 / 249) at 64, 114 / 83
+  // (363 / 249) at 92; e4m3 at head_dim 64 46 / 64 us (132 / 198) around 60 and equal at 96.  The tcgen05 kernel takes its row maximum before the scale, so it needs a positive one.
   const bool tiled = type != LBI_F32 && (p->head_dim == 32 || p->head_dim == 64 || p->head_dim == 128);
-  const int64_t enough = p->cache_type == LBI_E4M3 ? 96 : 32;
+  const int64_t enough = p->cache_type != LBI_E4M3 ? 32 : p->head_dim == 128 ? 64 : 96;
   plan.kernel = !tiled ? 0 : p->head_dim >= 64 && (int64_t)p->rows * group >= enough * p->batch && scale > 0.f ? 2 : 1;
   if (plan.kernel == 2) {
     // Parts of a context pay where there are too few units (256 rows x key head) for the slots: one block per SM, or two (head_dim 64,
     // 16-bit pages), of which the second adds less than the first.  Units of more than one round are left whole: those of a causal or a
     // ragged batch are uneven, the longest start first, and the others fill in behind them.  A part costs as much as 600 keys (its start,
-    // its partial result, the joining).  Over 87 batches of 1 to 16 sequences, 128 to 4096 new tokens behind 0 to 20000, 1 to 64 heads of 64
-    // or 128, this choice takes 1.033 times the best of 1 to 16 parts (geometric mean; 1.42 at worst); filling whole rounds of equal
-    // units took 1.085 (1.96), e.g. 130 us in two parts against 66 us whole for 16 prompts of 1024 tokens, 4 heads of 128.
-    const double mean_tiles = p->cu ? (double)p->rows * group / 256 + 0.5 * p->batch : (double)p->batch * ((p->rows / p->batch * group + 255) / 256);
+    // its partial result, the joining).  Over 174 batches of 1 to 32 sequences, 4 to 4096 new tokens behind 0 to 32000, 1 to 64 heads of 64
+    // or 128, this choice takes 1.03 times the best number of parts (geometric mean; 1.53 at worst); filling whole rounds of equal
+    // units took 1.085 (1.96) on half of them, e.g. 130 us in two parts against 66 us whole for 16 prompts of 1024 tokens, 4 heads of 128.
+    // Tiles, where the row offsets are on the device: half a tile's room per sequence, and a tile for each
+    const double mean_tiles = p->cu ? std::max((double)p->rows * group / 256 + 0.5 * p->batch, (double)std::min(p->batch, p->rows))
+                                    : (double)p->batch * ((p->rows / p->batch * group + 255) / 256);
     const double units = mean_tiles * p->kv_heads;
     const bool two = p->head_dim == 64 && p->cache_type != LBI_E4M3;
     const double slots = sm_count * (two ? 2 : 1);
@@ -908,7 +911,7 @@ extern "C" lbi_attention_plan lbi_paged_attention_plan(const lbi_paged_batch* p,
     for (int splits = 1; splits <= 16 && (splits == 1 || longest / splits >= 256); ++splits) {
       const double rounds = units * splits / slots;
       const double cost = (rounds >= 1 ? rounds : two ? 1 - std::min(0.3, 0.6 * (1 - rounds)) : 1) * ((double)longest / splits + 600);
-      if (splits == 1 || cost < 0.97 * best) {
+      if (splits == 1 || cost < 0.95 * best) {
         best = cost;
         plan.splits = splits;
       }
