@@ -889,8 +889,9 @@ extern "C" lbi_attention_plan lbi_paged_attention_plan(const lbi_paged_batch* p,
   const int64_t longest = max_context > 0 ? std::min(max_context, capacity) : capacity;
   // Which tiles: by the rows (tokens x heads of a group) of an average sequence.  The 16-row tiles read the cache once per 16 rows, the
   // 256-row tiles cost the same up to 256.  Measured with 32 / 8 heads of 128, 8 sequences over 4000 keys (16 over 8000), 16-row / 256-row:
-  // 16-bit pages 73 / 62 us (175 / 171) around 30 rows; e4m3 64 / 83 us (206 / 249) at 48 rows, 93 / 83 (259 / 249) at 64, 114 / 83
-  // (363 / 249) at 92; e4m3 at head_dim 64 46 / 64 us (132 / 198) around 60 and equal at 96.  The tcgen05 kernel takes its row maximum before the scale, so it needs a positive one.
+  // 16-bit pages 73 / 62 us (175 / 171) at 28 and 32 rows; e4m3 64 / 83 us (206 / 249) at 48 rows, 93 / 83 (259 / 249) at 64, 114 / 83
+  // (363 / 249) at 92; e4m3 at head_dim 64 46 / 64 us (132 / 198) at 60 and 64, equal at 96.  The tcgen05 kernel takes its row maximum
+  // before the scale, so it needs a positive one.
   const bool tiled = type != LBI_F32 && (p->head_dim == 32 || p->head_dim == 64 || p->head_dim == 128);
   const int64_t enough = p->cache_type != LBI_E4M3 ? 32 : p->head_dim == 128 ? 64 : 96;
   plan.kernel = !tiled ? 0 : p->head_dim >= 64 && (int64_t)p->rows * group >= enough * p->batch && scale > 0.f ? 2 : 1;
