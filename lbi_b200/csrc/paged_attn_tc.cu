@@ -382,6 +382,7 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
             }
             s.meta[j % META].there[lane] = there;
           }
+          __syncwarp();   // the words of all four lanes before lane 0's arrival, which the readers wait for
           const int at = lane * box - (i % COPIES) * COPY;   // row in the entry
           const bool here = good && at >= 0 && at < COPY;
           const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, here)) * (uint32_t)box * DH * (E4M3 ? 1 : 2);
