@@ -25,11 +25,21 @@ import torch
 CHUNK_TOKENS = 4096
 
 
-def _sample(logits: torch.Tensor, temperature: float, top_k: int | None, generator: torch.Generator | None) -> torch.Tensor:
-    """logits [B, V] -> token ids [B]: arg-max at temperature 0, else a draw from the (top-k) softmax."""
+# Penalties lie within this factor of 1 (repetition) or of 0: with 2^31 occurrences and any fp32 bias, logits of up to 1e10 stay
+# finite in fp32 (1e10 * 1e20 + 1e20 + 2^31 * 1e20 is below half a step of the largest fp32 number, 1e31).
+PENALTY_LIMIT = 1e20
+
+
+def _sample(logits: torch.Tensor, temperature: float, top_k: int | None, generator: torch.Generator | None,
+            wide: bool = False) -> torch.Tensor:
+    """logits [B, V] -> token ids [B]: arg-max at temperature 0, else a draw from the (top-k) softmax.  ``wide``: the logits may be
+    too large for a quotient by the temperature; the softmax of their differences to the largest is the same."""
     if temperature <= 0.0:
         return logits.argmax(dim=-1)
-    logits = logits.float() / temperature
+    logits = logits.float()
+    if wide:
+        logits = logits - logits.amax(dim=-1, keepdim=True)
+    logits = logits / temperature
     if top_k is not None and 0 < top_k < logits.shape[-1]:
         kth = torch.topk(logits, top_k, dim=-1).values[..., -1:]
         logits = logits.masked_fill(logits < kth, float("-inf"))
@@ -41,7 +51,8 @@ class LogitRules:
     """What ``generate`` does to the logits before it samples (``ops.adjust_logits``).
 
     ``logit_bias``: {token id: added value} or an fp32 tensor [V]; ``allowed_tokens``: bool tensor [V] (or token ids) of the tokens
-    that may be generated, or a grammar: a callable that takes the tokens so far [B, T] and returns a bool tensor [V] or [B, V]."""
+    that may be generated, or a grammar: a callable that takes the tokens so far [B, T] and returns a bool tensor [V] or [B, V].
+    The repetition penalty lies between 1e-20 and 1e20, the other two between -1e20 and 1e20, biases are finite in fp32."""
 
     repetition_penalty: float = 1.0
     presence_penalty: float = 0.0
@@ -50,10 +61,10 @@ class LogitRules:
     allowed_tokens: Any = None
 
     def __post_init__(self) -> None:
-        if not (self.repetition_penalty > 0.0 and math.isfinite(self.repetition_penalty)):
-            raise ValueError("repetition_penalty must be a positive number")
-        if not (math.isfinite(self.presence_penalty) and math.isfinite(self.frequency_penalty)):
-            raise ValueError("presence_penalty and frequency_penalty must be finite")
+        if not 1.0 / PENALTY_LIMIT <= self.repetition_penalty <= PENALTY_LIMIT:
+            raise ValueError(f"repetition_penalty must be a positive number between {1.0 / PENALTY_LIMIT:g} and {PENALTY_LIMIT:g}")
+        if not (abs(self.presence_penalty) <= PENALTY_LIMIT and abs(self.frequency_penalty) <= PENALTY_LIMIT):
+            raise ValueError(f"presence_penalty and frequency_penalty must lie between -{PENALTY_LIMIT:g} and {PENALTY_LIMIT:g}")
 
     @property
     def idle(self) -> bool:
@@ -73,13 +84,17 @@ class _LogitRuleState:
         if isinstance(bias, dict):
             dense = torch.zeros(vocab)
             for token, value in bias.items():
-                if not 0 <= int(token) < vocab or not math.isfinite(float(value)):
-                    raise ValueError("logit_bias maps token ids of the vocabulary to finite values")
+                if not 0 <= int(token) < vocab or not abs(float(value)) <= torch.finfo(torch.float32).max:
+                    raise ValueError("logit_bias maps token ids of the vocabulary to values that are finite in fp32")
                 dense[int(token)] = float(value)
             bias = dense
-        elif bias is not None and (tuple(bias.shape) != (vocab,) or not bool(torch.isfinite(bias).all())):
-            raise ValueError("logit_bias must have one finite entry per token of the vocabulary")
+        elif bias is not None:
+            if tuple(bias.shape) != (vocab,) or not bool(torch.isfinite(bias.float()).all()):
+                raise ValueError("logit_bias must have one entry per token of the vocabulary, finite in fp32")
         self.bias = None if bias is None else bias.to(device=device, dtype=torch.float32).contiguous()
+        # logits of a usual size stay far from fp32's limits with rules of a usual size (whatever the temperature)
+        self.wide = max(rules.repetition_penalty, 1.0 / rules.repetition_penalty, abs(rules.presence_penalty), abs(rules.frequency_penalty),
+                        0.0 if bias is None else float(bias.abs().max())) > 1e6
         allowed, self.grammar, self.mask = rules.allowed_tokens, None, None
         if callable(allowed):
             self.grammar = allowed
@@ -322,7 +337,7 @@ def generate(model: Any, input_ids: torch.Tensor, max_new_tokens: int, *, total_
             if adjust is None:
                 adjust = _LogitRuleState(rules, tokens.shape[0], input_ids.shape[1], logits.shape[-1], logits.device)
             logits = adjust(logits, tokens)
-        return _sample(logits, temperature, top_k, generator).unsqueeze(1)
+        return _sample(logits, temperature, top_k, generator, wide=adjust is not None and adjust.wide).unsqueeze(1)
 
     try:
         final_len = input_ids.shape[1] + int(max_new_tokens)

@@ -1,0 +1,52 @@
+"""Calls at the edges of what the serving paths document (CPU): what they answer and what they refuse."""
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+from lbi_b200.backbones import BackboneSpec
+from lbi_b200.inference import LogitRules, generate
+from lbi_b200.models import DenseLanguageModel
+from lbi_b200.serve import GenerationService
+
+VOCAB = 50
+
+
+def dense():
+    torch.manual_seed(0)
+    spec = BackboneSpec(name="transformer", dim=32, layers=2, n_heads=4, n_kv_heads=2, d_conv=0)
+    return DenseLanguageModel(vocab_size=VOCAB, backbone_spec=spec, tie_embeddings=True).eval()
+
+
+def service():
+    return GenerationService(dense(), SimpleNamespace(backbone="transformer", seq_len=32, vocab_size=VOCAB, data_mode="synthetic"))
+
+
+ASK = {"prompt_ids": [1, 2, 3], "max_new_tokens": 4, "temperature": 0.5}
+
+
+@pytest.mark.parametrize("bad", [{"presence_penalty": -1e39}, {"presence_penalty": 1e300}, {"frequency_penalty": 1e38},
+                                 {"repetition_penalty": 1e-38}, {"repetition_penalty": 1e-320}, {"repetition_penalty": 1e38},
+                                 {"logit_bias": {"3": 1e39}}, {"logit_bias": {"3": 1e300}}, {"logit_bias": {"3": float("nan")}}])
+def test_rules_that_leave_fp32_are_refused(bad):
+    """They would make the softmax of the sampler NaN, which on a GPU ends in a failed assert of the draw."""
+    with pytest.raises(ValueError):
+        service().handle({**ASK, **bad})
+
+
+def test_a_bias_tensor_outside_fp32_is_refused():
+    with pytest.raises(ValueError):
+        generate(dense(), torch.tensor([[1, 2]]), 2, rules=LogitRules(logit_bias=torch.full((VOCAB,), 1e300, dtype=torch.float64)))
+
+
+@pytest.mark.parametrize("temperature", [0.0, 1e-3, 0.5, 1.0, 1e3])
+def test_the_largest_rules_are_sampled_from(temperature):
+    top = torch.finfo(torch.float32).max
+    s = service()
+    ask = {**ASK, "temperature": temperature}
+    assert s.handle({**ask, "logit_bias": {"3": 3e38, "4": 2e38}})["new_ids"] == [3] * 4
+    assert s.handle({**ask, "logit_bias": {str(i): -top for i in range(VOCAB) if i != 7}})["new_ids"] == [7] * 4
+    allowed = [5, 9, 11, 12, 30]
+    for extra in ({"logit_bias": {"3": 3e38}}, {"presence_penalty": 1e20}, {"frequency_penalty": -1e20}, {"repetition_penalty": 1e-20},
+                  {"repetition_penalty": 1e20, "frequency_penalty": 1e20, "logit_bias": {str(i): -top for i in range(VOCAB)}}):
+        assert set(s.handle({**ask, **extra, "allowed_ids": allowed})["new_ids"]) <= set(allowed)
