@@ -37,9 +37,9 @@ def _sample(logits: torch.Tensor, temperature: float, top_k: int | None, generat
     if temperature <= 0.0:
         return logits.argmax(dim=-1)
     logits = logits.float()
-    if wide:
+    if wide or temperature < 1e-20:
         logits = logits - logits.amax(dim=-1, keepdim=True)
-    logits = logits / temperature
+    logits = logits / min(temperature, 1e30)   # masked logits stay -inf however hot it is
     if top_k is not None and 0 < top_k < logits.shape[-1]:
         kth = torch.topk(logits, top_k, dim=-1).values[..., -1:]
         logits = logits.masked_fill(logits < kth, float("-inf"))
@@ -327,6 +327,8 @@ def generate(model: Any, input_ids: torch.Tensor, max_new_tokens: int, *, total_
     caches.  ``rules``: penalties, biases and masks on the logits (``LogitRules``)."""
     if input_ids.dim() != 2 or input_ids.shape[1] == 0:
         raise ValueError("input_ids must be a non-empty [B, T] tensor")
+    if math.isnan(temperature) or 0.0 < temperature < 2.0 ** -126:   # its reciprocal is no fp32 number
+        raise ValueError("temperature must be 0 or at least 2^-126")
     was_training = model.training
     model.eval()
     adjust = None

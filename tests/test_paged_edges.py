@@ -50,3 +50,23 @@ def test_the_largest_rules_are_sampled_from(temperature):
     for extra in ({"logit_bias": {"3": 3e38}}, {"presence_penalty": 1e20}, {"frequency_penalty": -1e20}, {"repetition_penalty": 1e-20},
                   {"repetition_penalty": 1e20, "frequency_penalty": 1e20, "logit_bias": {str(i): -top for i in range(VOCAB)}}):
         assert set(s.handle({**ask, **extra, "allowed_ids": allowed})["new_ids"]) <= set(allowed)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), 1e-40, 5e-324])
+def test_temperatures_that_make_no_distribution_are_refused(bad):
+    with pytest.raises(ValueError):
+        service().handle({**ASK, "temperature": bad})
+    with pytest.raises(ValueError):
+        generate(dense(), torch.tensor([[1, 2]]), 2, temperature=bad)
+
+
+@pytest.mark.parametrize("temperature", [2.0 ** -126, 1e-37, 1e-30, 1e30, float("inf")])
+def test_extreme_temperatures_are_sampled_from(temperature):
+    """The coldest give the arg-max, the hottest any token that is allowed, beside masked ones, too."""
+    s = service()
+    ask = {**ASK, "temperature": temperature}
+    if temperature < 1:
+        for extra in ({}, {"logit_bias": {"3": 50.0, "4": 49.0}}):
+            assert s.handle({**ask, **extra})["new_ids"] == s.handle({**ASK, **extra, "temperature": 0.0})["new_ids"]
+    allowed = [5, 9, 11, 12, 30]
+    assert set(s.handle({**ask, "allowed_ids": allowed})["new_ids"]) <= set(allowed)
