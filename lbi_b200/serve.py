@@ -61,7 +61,8 @@ class GenerationService:
     def _rules(request: dict) -> LogitRules:
         try:
             bias = {int(k): float(v) for k, v in dict(request.get("logit_bias") or {}).items()} or None
-            allowed = [int(i) for i in request.get("allowed_ids") or []] or None
+            allowed = request.get("allowed_ids")
+            allowed = None if allowed is None else [int(i) for i in allowed]   # an empty list allows nothing and is refused
             return LogitRules(float(request.get("repetition_penalty", 1.0)), float(request.get("presence_penalty", 0.0)),
                               float(request.get("frequency_penalty", 0.0)), bias, allowed)
         except TypeError as exc:

@@ -70,3 +70,13 @@ def test_extreme_temperatures_are_sampled_from(temperature):
             assert s.handle({**ask, **extra})["new_ids"] == s.handle({**ASK, **extra, "temperature": 0.0})["new_ids"]
     allowed = [5, 9, 11, 12, 30]
     assert set(s.handle({**ask, "allowed_ids": allowed})["new_ids"]) <= set(allowed)
+
+
+def test_an_empty_list_of_allowed_ids_is_refused():
+    """It allows nothing; only a missing key (or null) allows everything."""
+    s = service()
+    with pytest.raises(ValueError):
+        s.handle({**ASK, "allowed_ids": []})
+    ask = {**ASK, "temperature": 0.0}
+    assert s.handle({**ask, "allowed_ids": None})["new_ids"] == s.handle(ask)["new_ids"]
+    assert s.handle({**ask, "logit_bias": {}})["new_ids"] == s.handle(ask)["new_ids"]
