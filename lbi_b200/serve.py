@@ -65,7 +65,7 @@ class GenerationService:
             allowed = None if allowed is None else [int(i) for i in allowed]   # an empty list allows nothing and is refused
             return LogitRules(float(request.get("repetition_penalty", 1.0)), float(request.get("presence_penalty", 0.0)),
                               float(request.get("frequency_penalty", 0.0)), bias, allowed)
-        except TypeError as exc:
+        except (TypeError, OverflowError) as exc:
             raise ValueError(f"malformed sampling rules: {exc}") from exc
 
     def handle(self, request: dict) -> dict:

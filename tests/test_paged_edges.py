@@ -80,3 +80,9 @@ def test_an_empty_list_of_allowed_ids_is_refused():
     ask = {**ASK, "temperature": 0.0}
     assert s.handle({**ask, "allowed_ids": None})["new_ids"] == s.handle(ask)["new_ids"]
     assert s.handle({**ask, "logit_bias": {}})["new_ids"] == s.handle(ask)["new_ids"]
+
+
+@pytest.mark.parametrize("bad", [{"allowed_ids": [float("inf")]}, {"logit_bias": {"3": 10 ** 400}}, {"presence_penalty": 10 ** 400}])
+def test_numbers_that_do_not_convert_are_malformed_rules(bad):
+    with pytest.raises(ValueError):
+        service().handle({**ASK, **bad})
