@@ -25,9 +25,11 @@ namespace paged {
 // are joined through shared memory at the end.  The page ids of a tile are loaded one tile ahead of its copies.
 //
 // e4m3 pages: codes become fp16 values exactly.  With u_j = scale s_j k_scale_j + log2 v_scale_j the weights 2^(u_j - max u) carry
-// the value's scale and stay in (0, 1] (fp16 has no range for p * v_scale); the sum of exponentials takes 2^(u_j - max u) / v_scale_j.
+// the value's scale (fp16 has no range for p * v_scale); the sum of exponentials takes 2^(u_j - max u) / v_scale_j.
 // P is rounded to the 16-bit type of the products before the second one (half a step of that type, as the result itself is rounded);
-// maximum, sum and output stay in fp32.
+// maximum, sum and output stay in fp32.  fp16 keeps that half step only down to 2^-14, and the keys of a long context may all weigh
+// less than that beside one heavy key: products in fp16 hold the weights times 2^15, so that the half step holds down to 2^-29 of
+// the heaviest key and what is lost below, 2^-40 of it per key, is nothing to the result.
 //
 // Measured on a B200, 32 query heads on 8 of 128: 64 contexts of up to 8192 keys (ragged, 1.02 GB) 183 us, 5.6 TB/s, 0.85 of the copy
 // bandwidth; all 8192 long 0.94 of it.  e4m3: 2 contexts of 131072 keys (0.55 GB) 115 us, 4.8 TB/s, 0.73: the codes' way to fp16 takes
@@ -117,8 +119,8 @@ __device__ __forceinline__ int key_slot(const AttnArgs& a, const RowsUnit& u, in
   if (p.status) atomicCAS(p.status, 0, 84);
   return -1;
 }
-// Joins the warps of a block and stores the result (or the part): `m`, `l` of rows g and g + 8 in every thread, the output row parts
-// behind ml in shared memory as [warp][row][dim + 4].
+// Joins the warps of a block and stores the result (or the part): references and sums of the warps' rows in `ml`, the output row parts
+// behind them as [warp][row][dim + 4].
 template <typename T, int ROWS>
 __device__ __forceinline__ void join_and_store(const AttnArgs& a, const RowsUnit& u, const float* ml, int dim) {
   const float* os = ml + 2 * WARPS * ROWS;
@@ -174,6 +176,10 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_rows_kernel(const Att
   using T = typename Elem<TYPE>::T;
   using L = RowsTile<E4M3, DH, KEYS, STAGES, NT>;
   constexpr int ROWS = L::ROWS, KT = KEYS / 16;
+  constexpr int MATH = E4M3 ? LBI_F16 : TYPE;             // of the products
+  constexpr float UP = MATH == LBI_F16 ? 15.f : 0.f;      // weights are held times 2^UP
+  // ... the sum of exponentials of e4m3 pages without the factor, which its range (1 / v_scale) has no room for
+  constexpr float DOWN = E4M3 ? 1.f / 32768.f : 1.f;
   extern __shared__ __align__(128) uint8_t smem[];
   const lbi_paged_batch& p = a.b;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -186,7 +192,6 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_rows_kernel(const Att
   // agree: natural for 16-bit pages (ldmatrix), 4 neighbours per thread for codes (one 32-bit load).
   // e4m3: the products run in fp16, which holds the codes and, behind a power of two per row that brings its largest element to
   // [2^14, 2^15), a bf16 query as well (29 binades below the largest to the normal range's end: nothing that an fp32 sum would notice).
-  constexpr int MATH = E4M3 ? LBI_F16 : TYPE;
   uint32_t qf[NT][DH / 16][2];
   int limit[NT][2];         // of the rows 8 n + 2 t and + 1, whose scores the thread has
   float row_scale[NT][2];
@@ -238,7 +243,7 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_rows_kernel(const Att
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[i][n][e] = 0.f;
-  float m[NT][2], l[NT][2];
+  float m[NT][2], l[NT][2];   // what the exponents are relative to: the running maximum less UP
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -327,7 +332,7 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_rows_kernel(const Att
           ks = __uint_as_float(lds32(vd + L::TILE + key * 4));
           const float vs = positive_scale(__uint_as_float(lds32(vd + L::TILE + (KEYS + key) * 4)));
           lv = lg2(vs);
-          inv_vs[kt][h] = rcp(vs);
+          inv_vs[kt][h] = rcp(vs) * DOWN;
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n)
@@ -360,7 +365,8 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_rows_kernel(const Att
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-        const float mn = fmaxf(m[n][e], top);
+        // rounded up: however large the scores, no weight is above 2^UP
+        const float mn = fmaxf(m[n][e], UP == 0.f ? top : __fadd_ru(top, -UP));
         ref[n][e] = mn == -INFINITY ? 0.f : mn;      // a row that has seen no key yet
         keep[n][e] = ex2(m[n][e] - ref[n][e]);
         m[n][e] = mn;
@@ -445,8 +451,8 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_rows_kernel(const Att
       float* to = os + (warp * ROWS + 8 * n + 2 * t + e) * (DH + 4);
 #pragma unroll
       for (int d = 0; d < DH / 16; ++d) {
-        to[E4M3 ? 32 * (d >> 1) + 4 * g + 2 * (d & 1) : 16 * d + g] = o[d][n][e];
-        to[E4M3 ? 32 * (d >> 1) + 4 * g + 2 * (d & 1) + 1 : 16 * d + g + 8] = o[d][n][2 + e];
+        to[E4M3 ? 32 * (d >> 1) + 4 * g + 2 * (d & 1) : 16 * d + g] = o[d][n][e] * DOWN;
+        to[E4M3 ? 32 * (d >> 1) + 4 * g + 2 * (d & 1) + 1 : 16 * d + g + 8] = o[d][n][2 + e] * DOWN;
       }
     }
   __syncthreads();

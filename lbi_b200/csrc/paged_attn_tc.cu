@@ -8,7 +8,9 @@
 //     O_g += P_g V_j         M 128 x N head_dim, accumulated in TMEM columns [2 KEYS + head_dim g, ..)
 // Products of a thread run in the order in which they are issued, so S_g of the next tile may be issued right behind the product that
 // still reads P_g, and the barrier that announces S_g(j + 1) also says that O_g holds tile j.  The running maximum follows the row only
-// when it has grown by more than 2^8: P stays in (0, 2^8], and O is rescaled (a read and a write of TMEM) in the first tiles only.
+// when it has grown by more than 2^8 (fp16: 2^4): P stays in (0, 2^8], and O is rescaled (a read and a write of TMEM) in the first tiles
+// only.  fp16 has half a step of 2^-11 only down to 2^-14, and the keys of a long context may all weigh less than that beside one heavy
+// key: there P is held times 2^11, up to 2^15, so that the half step holds down to 2^-25 of the heaviest key.
 // While one warpgroup computes exponentials the tensor core works for the other.
 //
 // What bounds it: the chain S -> maximum -> exponentials -> P -> products of a row tile, of which two (or, with 16-bit pages at head_dim
@@ -172,6 +174,16 @@ __device__ __forceinline__ float2 exp2_by_polynomial(float2 x) {
   return make_float2(__int_as_float(__float_as_int(r.x) + (__float_as_int(t.x) << 23)), __int_as_float(__float_as_int(r.y) + (__float_as_int(t.y) << 23)));
 }
 
+// Two weights as a word of P.  The largest is 2^15 or 2^8, but behind scores so large that their steps are whole binades the rounding of
+// score and maximum may add some: fp16 then takes its largest number, not infinity.
+template <int TYPE>
+__device__ __forceinline__ uint32_t pack_weights(float a, float b) {
+  if (TYPE != LBI_F16) return pack16<TYPE>(a, b);
+  uint32_t d;
+  asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(b), "f"(a));
+  return d;
+}
+
 template <int TYPE, bool E4M3, int DH>
 __global__ void __launch_bounds__(TcConfig<E4M3, DH>::THREADS, TcConfig<E4M3, DH>::BLOCKS)
 attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const AttnArgs a) {
@@ -179,6 +191,10 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   using C = TcConfig<E4M3, DH>;
   using Smem = TcSmem<E4M3, DH>;
   constexpr int KEYS = C::KEYS, SLOTS = C::SLOTS, META = C::META, RAW = C::RAW, PANELS = DH / 64;
+  constexpr float UP = TYPE == LBI_F16 ? 11.f : 0.f;        // P is held times 2^UP
+  constexpr float GROWTH = UP + (TYPE == LBI_F16 ? 4.f : 8.f);   // binary logarithm of the largest P
+  // ... the sum of exponentials of e4m3 pages without the factor, which its range (1 / v_scale) has no room for
+  constexpr float DOWN = E4M3 && TYPE == LBI_F16 ? 1.f / 2048.f : 1.f;
   constexpr int Q_BYTES = ROWS * DH * 2, Q_PANEL = ROWS * 128, KV_BYTES = KEYS * DH * 2, KV_PANEL = KEYS * 128;   // panels of 64 columns
   extern __shared__ uint8_t raw_smem[];
   Smem& s = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~uintptr_t(1023));
@@ -440,7 +456,7 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
           const uint32_t there = __ballot_sync(0xffffffffu, good[i]);
           meta.ks_lv[key >> 1][key & 1] = k_scale[i] * a.scale_log2;
           meta.ks_lv[key >> 1][2 + (key & 1)] = lg2(vs);
-          meta.iv[key] = __frcp_rn(vs);
+          meta.iv[key] = __frcp_rn(vs) * DOWN;
           if (lane == 0) meta.there[key >> 5] = there;
         }
         __syncwarp();
@@ -525,7 +541,8 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
       __syncwarp();
       if (lane == 0) mbar_arrive(&s.bar_p[g]);
     };
-    float m = -INFINITY, l = 0.f;                    // of the thread's row, in base-2 logarithms and relative to m
+    // of the thread's row: the point that exponents are relative to, in base-2 logarithms (UP below a maximum), and the sum
+    float m = -INFINITY, l = 0.f;
     bool ok = true;
     if constexpr (E4M3) {
       // Every column has its own scales.  A thread per row would read all of them from shared memory, 393 KB per 128 keys, which
@@ -591,13 +608,13 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
           top[k] = fmaxf(t0, t1);
           top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], 1));
           top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], 2));
-          grow = grow || top[k] > mr[k] + 8.f;
+          grow = grow || top[k] - mr[k] > GROWTH;
         }
         if (__any_sync(0xffffffffu, grow)) {
           float row_keep = 1.f;   // of row `lane`, for O
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const float m_new = top[k] > mr[k] + 8.f ? top[k] : mr[k];
+            const float m_new = top[k] - mr[k] > GROWTH ? (UP == 0.f ? top[k] : __fadd_ru(top[k], -UP)) : mr[k];
             const float keep = mr[k] == m_new ? 1.f : ex2(mr[k] - m_new);
             mr[k] = m_new;
             lr[k] *= keep;
@@ -624,7 +641,7 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
                 float2& u = x.f2[h][n0 + n][k];
                 u = add2(u, neg[2 * h + k]);
                 u = make_float2(ex2(u.x), ex2(u.y));
-                w[2 * n + k] = pack16<TYPE>(u.x, u.y);
+                w[2 * n + k] = pack_weights<TYPE>(u.x, u.y);
               }
             tmem_st_16x32(t_s + ((uint32_t)(16 * h) << 16) + n0 * 4, w);
           }
@@ -687,10 +704,10 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
 #pragma unroll
           for (int i = 0; i < 4; ++i) t4[i] = fmaxf(t4[i], fmaxf(x.f[e + i], x.f[e + 4 + i]));
         const float top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])) * a.scale_log2;   // positive, see the choice of the kernel
-        // the reference point follows only a growth by more than 2^8
-        const bool grow = top > m + 8.f;
+        // the reference point follows only a growth to more than 2^GROWTH
+        const bool grow = top - m > GROWTH;
         if (__any_sync(0xffffffffu, grow)) {
-          const float m_new = grow ? top : m;
+          const float m_new = grow ? (UP == 0.f ? top : __fadd_ru(top, -UP)) : m;
           const float keep = m == m_new ? 1.f : ex2(m - m_new);
           m = m_new;
           l2.x *= keep;
@@ -709,7 +726,7 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
               u = fma2(u, sc, neg);
               if (decltype(by_polynomial)::value && e % 8 < C::POLY) u = exp2_by_polynomial<TYPE>(u);
               else u = make_float2(ex2(u.x), ex2(u.y));
-              w[e] = pack16<TYPE>(u.x, u.y);
+              w[e] = pack_weights<TYPE>(u.x, u.y);
             }
             tmem_st_32x16(t_s + c * 16, w);
           }
@@ -728,7 +745,7 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     if (ok && mine > 0) ok = mbar_wait(&s.bar_o[g], 0, abortp, p.status, 46);
     if (ok) {
       fence_after_sync();
-      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const float inv = l == 0.f ? 0.f : DOWN / l;
       const int at = local + g * ROWS + row;
       const int64_t o_row = (int64_t)(r.x + at / a.group) * a.heads + kh * a.group + at % a.group;
 #pragma unroll
