@@ -26,13 +26,14 @@ typedef struct {
   int64_t table_stride;
   int num_pages, kv_heads, page_size, head_dim, cache_type;
   int table_width, batch;
-  int rows;     // new tokens (rows of qkv / q); rows behind the last sequence belong to nobody
+  int rows;     // new tokens (rows of qkv / q); rows in front of the first sequence and behind the last belong to nobody
   int* status;  // device int: 83 a position outside the rotary table, 84 a position or page outside the page table or the pool
 } lbi_paged_batch;
 
 // qkv [rows, (heads + 2 kv_heads) * head_dim] (rows qkv_stride elements apart, type `type`): rotates q and k by the rotary table
 // rows of their positions (cos / sin fp32 [rope_rows, head_dim / 2]; null: no turn), writes q_out [rows, heads * head_dim] and the
-// k / v rows into their pages.  Rows behind the last sequence: q_out is left as it is, or zeroed when zero_tail is set.
+// k / v rows into their pages.  Rows in front of the first sequence and behind the last: q_out is left as it is, or zeroed when
+// zero_tail is set.
 int lbi_kv_append(const lbi_paged_batch* p, const void* qkv, int64_t qkv_stride, void* q_out, int type, int heads, const float* cos_tab,
                   const float* sin_tab, int64_t rope_rows, int interleaved, int zero_tail, cudaStream_t stream);
 

@@ -110,8 +110,21 @@ __device__ __forceinline__ Place place_of_row(const lbi_paged_batch& p, int row)
   return {b, r.x, r.y, row >= r.x && row < r.y};
 }
 
-__device__ __forceinline__ int last_row(const lbi_paged_batch& p) {
-  return p.cu ? min(max(__ldg(p.cu + p.batch), 0), p.rows) : p.rows;
+// The rows [x, y) from the first sequence's to the last's; those in front and behind belong to nobody.
+__device__ __forceinline__ int2 owned_rows(const lbi_paged_batch& p) {
+  if (!p.cu) return make_int2(0, p.rows);
+  const int last = min(max(__ldg(p.cu + p.batch), 0), p.rows);
+  return make_int2(min(max(__ldg(p.cu), 0), last), last);
+}
+// Zeros in the rows of nobody of `out` [rows, width], shared among all blocks.
+template <typename T>
+__device__ __forceinline__ void zero_rows_of_nobody(const lbi_paged_batch& p, T* out, int width) {
+  const int2 own = owned_rows(p);
+  const int nobody = own.x + p.rows - own.y;
+  for (int64_t i = blockIdx.x; i < nobody; i += gridDim.x) {
+    const int64_t row = i < own.x ? i : i + own.y - own.x;
+    for (int e = threadIdx.x; e < width; e += blockDim.x) out[row * width + e] = from_f<T>(0.f);
+  }
 }
 
 // Page of position pos of sequence b, or -1 (recorded as status 84) where the table or the pool ends.

@@ -105,12 +105,6 @@ __device__ __forceinline__ RowsUnit rows_unit(const AttnArgs& a, int per_tile) {
   u.k1 = u.split == a.splits - 1 ? keys : min(keys, u.k0 + a.split_keys);
   return u;
 }
-template <typename T>
-__device__ __forceinline__ void zero_rows_of_nobody(const AttnArgs& a) {
-  if (a.zero_tail && !a.part_o)
-    for (int64_t row = (int64_t)last_row(a.b) + blockIdx.x; row < a.b.rows; row += gridDim.x)
-      for (int i = threadIdx.x; i < a.heads * a.b.head_dim; i += blockDim.x) ((T*)a.out)[row * a.heads * a.b.head_dim + i] = from_f<T>(0.f);
-}
 // Slot of key `lane` of a tile that starts at `base`, or -1 where there is no such key or page.
 __device__ __forceinline__ int key_slot(const AttnArgs& a, const RowsUnit& u, int pos, bool wanted, int page) {
   const lbi_paged_batch& p = a.b;
@@ -183,7 +177,7 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) attn_rows_kernel(const Att
   extern __shared__ __align__(128) uint8_t smem[];
   const lbi_paged_batch& p = a.b;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  zero_rows_of_nobody<T>(a);
+  if (a.zero_tail && !a.part_o) zero_rows_of_nobody(p, (T*)a.out, a.heads * DH);
   const RowsUnit u = rows_unit(a, ROWS);
   if (!u.any) return;
   const int kh = u.kh, k0 = u.k0, k1 = u.k1;
@@ -472,7 +466,8 @@ __global__ void __launch_bounds__(COMBINE_THREADS) combine_kernel(const AttnArgs
   const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES, share = group % SHARE, dim = p.head_dim;
   const int64_t at = (int64_t)blockIdx.x * ROWS + group / SHARE;
   const bool exists = at < (int64_t)p.rows * a.heads;
-  const bool owned = exists && at / a.heads < last_row(p);
+  const int2 own = owned_rows(p);
+  const bool owned = exists && at / a.heads >= own.x && at / a.heads < own.y;
   const float* lse = a.part_lse + at * a.splits;
   float top = -INFINITY;
   if (owned)
@@ -603,7 +598,7 @@ __global__ void __launch_bounds__(WARPS * 32) attn_any_kernel(const AttnArgs a) 
   extern __shared__ __align__(128) uint8_t smem[];
   const lbi_paged_batch& p = a.b;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, dim = p.head_dim;
-  zero_rows_of_nobody<T>(a);
+  if (a.zero_tail && !a.part_o) zero_rows_of_nobody(p, (T*)a.out, a.heads * dim);
   const RowsUnit u = rows_unit(a, ROW_TILE);
   if (!u.any) return;
 

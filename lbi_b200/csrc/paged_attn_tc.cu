@@ -201,9 +201,7 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   const lbi_paged_batch& p = a.b;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  if (a.zero_tail && !a.part_o)
-    for (int64_t row = (int64_t)last_row(p) + blockIdx.x; row < p.rows; row += gridDim.x)
-      for (int i = threadIdx.x; i < a.heads * DH; i += blockDim.x) ((T*)a.out)[row * a.heads * DH + i] = from_f<T>(0.f);
+  if (a.zero_tail && !a.part_o) zero_rows_of_nobody(p, (T*)a.out, a.heads * DH);
 
   // ------------------------------------------------------------------ the block's rows and keys
   const int64_t unit_block = (int64_t)gridDim.x - 1 - blockIdx.x;   // late tokens walk more keys: first

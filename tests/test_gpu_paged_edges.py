@@ -64,3 +64,37 @@ def test_one_key_far_above_thousands_of_others(new, group, dim, dtype, cache, bi
         return x
     # the short hint keeps the context in one part
     check_attention(Shaped(make, [(new, keys)], group, 1, dim, 64, dtype, cache, DEV), scale=1.0, max_context=64)
+
+
+# (new tokens, type, head_dim): every kernel, whole and in parts of a long context
+KERNELS = [(1, BF16, 64), (6, BF16, 64), (100, BF16, 64), (100, BF16, 128), (3, F32, 64), (2, BF16, 80)]
+
+
+@pytest.mark.parametrize("new,dtype,dim", KERNELS)
+@pytest.mark.parametrize("keys", [200, 3000])
+def test_rows_in_front_of_the_first_sequence_belong_to_nobody(new, dtype, dim, keys):
+    batch = Batch([(new, keys), (new, new)], 2, 1, dim, 16, dtype, "same", DEV)
+    front, behind, n = 5, 2, 2 * new
+    q = torch.ones(front + n + behind, 2, dim, device=DEV, dtype=dtype)
+    q[front : front + n] = batch.queries()
+    call = dict(q=q, pages=batch.pages, page_table=batch.table, context_lens=batch.context, scale=0.125, cu_seqlens=batch.cu + front)
+    want = ops.paged_attention(**{**call, "q": q[front : front + n], "cu_seqlens": batch.cu})
+    nan = [torch.full((2 ** i,), float("nan"), device=DEV) for i in range(8, 24)]   # what new memory holds
+    del nan
+    got = ops.paged_attention(**call)
+    assert torch.equal(got[front : front + n], want)
+    assert bool((got[:front] == 0).all()) and bool((got[front + n :] == 0).all())
+    out = torch.full_like(q, 7.0)
+    ops.paged_attention(**call, out=out)
+    assert torch.equal(out[front : front + n], want)
+    assert bool((out[:front] == 7).all()) and bool((out[front + n :] == 7).all())
+
+
+def test_append_leaves_rows_in_front_of_the_first_sequence_alone():
+    batch = Batch([(2, 20), (1, 5)], 4, 2, 64, 16, BF16, "same", DEV)
+    qkv = torch.randn(9, 8 * 64, device=DEV).bfloat16()
+    got = ops.kv_append(qkv, batch.pages, batch.table, batch.context, 4, cu_seqlens=batch.cu + 3)
+    assert torch.equal(got[3:6], qkv[3:6, : 4 * 64].view(3, 4, 64)) and not bool(got[:3].any()) and not bool(got[6:].any())
+    out = torch.full_like(got, 7.0)
+    ops.kv_append(qkv, batch.pages, batch.table, batch.context, 4, cu_seqlens=batch.cu + 3, out=out)
+    assert torch.equal(out[3:6], got[3:6]) and bool((out[:3] == 7).all()) and bool((out[6:] == 7).all())
