@@ -100,7 +100,9 @@ __device__ __forceinline__ RowsUnit rows_unit(const AttnArgs& a, int per_tile) {
   u.n_rows = min(per_tile, rows_b - u.local);
   u.first_pos = __ldg(p.context + u.b) - (r.y - r.x);              // position of the sequence's first new token
   const int64_t capacity = (int64_t)p.table_width << a.page_shift;
-  const int keys = (int)min((int64_t)u.first_pos + (u.local + u.n_rows - 1) / a.group + 1, capacity);
+  const int64_t seen = (int64_t)u.first_pos + (u.local + u.n_rows - 1) / a.group + 1;
+  const int keys = (int)min(seen, capacity);
+  if (u.any && seen > capacity && u.split == 0 && threadIdx.x == 0 && p.status) atomicCAS(p.status, 0, 84);   // the table ends before the context
   u.k0 = u.split * a.split_keys;
   u.k1 = u.split == a.splits - 1 ? keys : min(keys, u.k0 + a.split_keys);
   return u;

@@ -222,7 +222,9 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   auto key_tiles = [&](int g) {   // of row tile g
 
     const int last = min(n_rows, (g + 1) * ROWS) - 1;   // the tile's last row
-    const int keys = last < g * ROWS ? 0 : (int)min((int64_t)first_pos + (local + last) / a.group + 1, capacity);
+    const int64_t seen = last < g * ROWS ? 0 : (int64_t)first_pos + (local + last) / a.group + 1;
+    const int keys = (int)min(seen, capacity);
+    if (seen > capacity && split == 0 && threadIdx.x == 0 && p.status) atomicCAS(p.status, 0, 84);   // the table ends before the context
     const int k1 = split == a.splits - 1 ? keys : min(keys, k0 + a.split_keys);
     k_end = max(k_end, k1);
     return k1 > k0 ? (k1 - k0 + KEYS - 1) / KEYS : 0;

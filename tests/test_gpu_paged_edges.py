@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from lbi_b200 import ops
-from paged_oracle import Batch, check_attention
+from paged_oracle import Batch, attention_oracle, check_attention
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -98,3 +98,21 @@ def test_append_leaves_rows_in_front_of_the_first_sequence_alone():
     out = torch.full_like(got, 7.0)
     ops.kv_append(qkv, batch.pages, batch.table, batch.context, 4, cu_seqlens=batch.cu + 3, out=out)
     assert torch.equal(out[3:6], got[3:6]) and bool((out[:3] == 7).all()) and bool((out[6:] == 7).all())
+
+
+@pytest.mark.parametrize("new,dtype,dim", KERNELS)
+@pytest.mark.parametrize("keys", [200, 3000])
+def test_a_context_that_outruns_its_table_is_recorded(new, dtype, dim, keys):
+    """Positions behind the table are skipped: the result is that of the keys that have a page."""
+    batch = Batch([(new, keys)], 2, 1, dim, 8, dtype, "same", DEV)
+    q = batch.queries()
+    ops.paged_attention(q, batch.pages, batch.table, batch.context, 0.125)
+    assert ops.ext().kernel_status(q) == 0
+    columns = (keys - new) // 8 - 2                       # every new token sees all keys that are left
+    got = ops.paged_attention(q, batch.pages, batch.table[:, :columns].contiguous(), batch.context, 0.125)
+    assert ops.ext().kernel_status(q) == 84
+    left = Batch([(1, columns * 8)], 2, 1, dim, 8, dtype, "same", DEV)
+    left.k, left.v = ([x[0][:, : columns * 8]] for x in (batch.k, batch.v))
+    for i in range(new):
+        want, tol = attention_oracle(left, q[i : i + 1], 0.125)
+        assert bool(((got[i : i + 1].double().cpu() - want).abs() <= tol).all())
