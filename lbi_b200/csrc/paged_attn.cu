@@ -925,12 +925,15 @@ extern "C" lbi_attention_plan lbi_paged_attention_plan(const lbi_paged_batch* p,
     // Parts of equal length, so that a batch of uneven contexts is balanced by the order in which blocks finish: of about 2048 keys
     // (the partial results are under 2 % of the bytes read), so many that the blocks fill whole rounds of two per SM.  Not below 256
     // keys, and 64, a tile per warp, for the kernel that splits its operands (2.6 us per tile; 7 sequences of up to 782 keys took 19.5 us
-    // in parts of 256).
+    // in parts of 256).  Not more parts than 64 MB hold the results of: with so many rows those are seven rounds of blocks and more.
+    // Measured with and without this bound: 1024 new tokens, 16 heads of 256, over 16384 keys 7919 (3 parts) / 8118 us (8); 256 single
+    // tokens of 32 heads on 8 of 128 over 32768 keys, e4m3, 2749 (15) / 2770 us (16).
     const int64_t least = plan.kernel == 0 ? 64 : 256;
     if (plan.kernel == 1 && (int64_t)p->rows * group <= 8ll * p->batch) plan.rows = 8;
     const int64_t units = tile_bound(*p, group, plan.rows) * p->kv_heads, slots = 2 * sm_count;
     const int64_t rounds = std::max<int64_t>(1, (longest * units + slots * 2048 - 1) / (slots * 2048));
-    const int64_t parts = std::max<int64_t>(1, rounds * slots / units);
+    const int64_t room = (64ll << 20) / ((int64_t)p->rows * heads * (p->head_dim + 1) * 4);
+    const int64_t parts = std::max<int64_t>(1, std::min(room, rounds * slots / units));
     const int64_t keys = std::max<int64_t>(least, ((longest + parts - 1) / parts + 63) / 64 * 64);
     plan.splits = (int)std::max<int64_t>(1, (longest + keys - 1) / keys);
     plan.split_keys = (int)keys;

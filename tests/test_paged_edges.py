@@ -1,9 +1,11 @@
 """Calls at the edges of what the serving paths document (CPU): what they answer and what they refuse."""
+import ctypes
 from types import SimpleNamespace
 
 import pytest
 import torch
 
+from lbi_b200 import ops
 from lbi_b200.backbones import BackboneSpec
 from lbi_b200.inference import LogitRules, generate
 from lbi_b200.models import DenseLanguageModel
@@ -86,3 +88,37 @@ def test_an_empty_list_of_allowed_ids_is_refused():
 def test_numbers_that_do_not_convert_are_malformed_rules(bad):
     with pytest.raises(ValueError):
         service().handle({**ASK, **bad})
+
+
+class PagedBatch(ctypes.Structure):
+    """``lbi_paged_batch`` of api_paged.h."""
+
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k", "v", "k_scale", "v_scale", "table", "context", "cu")] + [("table_stride", ctypes.c_int64)] + \
+        [(n, ctypes.c_int) for n in ("num_pages", "kv_heads", "page_size", "head_dim", "cache_type", "table_width", "batch", "rows")] + \
+        [("status", ctypes.c_void_p)]
+
+
+class Plan(ctypes.Structure):
+    """``lbi_attention_plan`` of api_paged.h."""
+
+    _fields_ = [(n, ctypes.c_int) for n in ("kernel", "rows", "splits", "split_keys")]
+
+
+F32, BF16, E4M3 = 0, 1, 3
+
+
+# (sequences, rows, heads, kv heads, head_dim, keys, type, type of the pages): chunks in fp32 and at a head size without tiles of its own,
+# many single tokens, drafts of many sequences, a few rows over a long context
+@pytest.mark.skipif(not ops.native_available(), reason="the extension is not built")
+@pytest.mark.parametrize("batch,rows,heads,kv_heads,dim,keys,kind,cache", [
+    (8, 32768, 16, 16, 64, 32768, F32, F32), (1, 4096, 32, 32, 256, 131072, BF16, BF16), (1, 4096, 16, 16, 128, 32768, F32, E4M3),
+    (512, 512, 32, 8, 128, 131072, BF16, BF16), (32, 992, 32, 32, 128, 131072, BF16, E4M3), (1, 600, 32, 8, 80, 200000, BF16, BF16),
+    (64, 64, 32, 8, 128, 8192, BF16, BF16), (2, 2, 32, 8, 128, 131072, BF16, E4M3), (1, 1, 1, 1, 16, 1 << 30, F32, F32),
+    (4, 8192, 16, 16, 64, 10240, BF16, BF16), (1, 256, 2, 2, 64, 65536, BF16, E4M3), (1, 4096, 64, 8, 128, 1 << 20, BF16, BF16)])
+def test_the_workspace_of_the_parts_of_a_context_is_bounded(batch, rows, heads, kv_heads, dim, keys, kind, cache):
+    plan_of = ctypes.CDLL(ops.ext().__file__).lbi_paged_attention_plan
+    plan_of.restype = Plan
+    p = PagedBatch(cu=1, kv_heads=kv_heads, page_size=16, head_dim=dim, cache_type=cache, table_width=keys // 16, batch=batch, rows=rows)
+    plan = plan_of(ctypes.byref(p), kind, heads, ctypes.c_float(0.1), ctypes.c_int64(0), 148)
+    assert plan.splits >= 1 and plan.splits * plan.split_keys >= keys
+    assert plan.splits == 1 or rows * heads * plan.splits * (dim + 1) * 4 <= 80 * 2 ** 20
