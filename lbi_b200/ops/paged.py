@@ -57,6 +57,14 @@ def kv_pages(num_pages: int, page_size: int, n_kv_heads: int, head_dim: int, dty
     return KVPages(k, v, *(torch.zeros(shape[:3], dtype=torch.float32, device=device) for _ in range(2)))
 
 
+def _learned(x) -> bool:
+    return x is not None and x.requires_grad
+
+
+def _pages_learned(pages) -> bool:
+    return pages[0].requires_grad or pages[1].requires_grad or _learned(pages[2]) or _learned(pages[3])
+
+
 def _refuse_grad() -> None:
     if torch.is_grad_enabled():
         raise ValueError("the cache operators have no backward pass: call them under torch.no_grad()")
@@ -107,9 +115,9 @@ def kv_append(qkv, pages, page_table, context_lens, n_heads, cu_seqlens=None, ro
     ``qkv`` [rows, (n_heads + 2 kv_heads) * head_dim] are packed projections; ``rope = (cos, sin, interleaved)`` (fp32 tables
     [positions, head_dim / 2]) turns q and k by their positions first.  Into e4m3 pages a head row goes as
     ``round(x / scale)`` with ``scale = max |x| / 448``.  Two sequences must not share a page that new tokens are written to."""
-    if qkv.requires_grad or pages[0].requires_grad or pages[1].requires_grad:
-        _refuse_grad()
     cos, sin, interleaved = rope if rope is not None else (None, None, False)
+    if qkv.requires_grad or _pages_learned(pages) or _learned(cos) or _learned(sin) or _learned(out):
+        _refuse_grad()
     if _kernel_shape(qkv, pages[0].size(-1)):
         KERNEL_LAUNCHES["count"] += 1
         return ext().kv_append(qkv, *pages, page_table, context_lens, n_heads, cu_seqlens, cos, sin, interleaved, out)
@@ -131,7 +139,7 @@ def kv_gather(pages, page_table, context_lens, max_len, dtype=None):
     """The cached keys and values as contiguous [B, kv_heads, max_len, head_dim] tensors, zero behind each context (the layout of
     ``CausalSelfAttention.step``).  ``dtype``: type of the result for e4m3 pages (default bf16); other pages keep theirs."""
     k = pages[0]
-    if k.requires_grad or pages[1].requires_grad:
+    if _pages_learned(pages):
         _refuse_grad()
     dtype = dtype or (torch.bfloat16 if k.dtype == torch.float8_e4m3fn else k.dtype)
     if k.is_cuda and k.size(-1) % 16 == 0 and k.size(-1) <= 256 and native_available():
@@ -153,7 +161,7 @@ def paged_attention(q, pages, page_table, context_lens, scale, cu_seqlens=None, 
 
     ``max_context``: the longest context if the host knows it (a hint that sizes the launch, default: what the page table can
     hold); a longer context still gives right results.  ``out`` must not overlap ``q``."""
-    if q.requires_grad or pages[0].requires_grad or pages[1].requires_grad:
+    if q.requires_grad or _pages_learned(pages) or _learned(out):
         _refuse_grad()
     if _kernel_shape(q, pages[0].size(-1)):
         KERNEL_LAUNCHES["count"] += 1
@@ -191,7 +199,7 @@ def adjust_logits(logits, tokens, lengths=None, prompt_lengths=None, *, repetiti
     * a token whose bit in ``allowed`` (``pack_token_mask``; [ceil(V / 32)] or one row each) is not set: -inf
 
     The three penalties are numbers or fp32 [B].  ``out`` may be ``logits`` itself when that is fp32."""
-    if logits.requires_grad or any(torch.is_tensor(x) and x.requires_grad for x in (repetition, presence, frequency, bias)):
+    if logits.requires_grad or any(torch.is_tensor(x) and x.requires_grad for x in (repetition, presence, frequency, bias, out)):
         _refuse_grad()
     if logits.is_cuda and logits.dtype in _TYPES and native_available():
         KERNEL_LAUNCHES["count"] += 1

@@ -4,6 +4,7 @@ import torch
 
 from lbi_b200 import ops
 from paged_oracle import Batch, attention_oracle, check_attention
+from test_paged_edges import calls_that_ask_for_gradients
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -116,3 +117,12 @@ def test_a_context_that_outruns_its_table_is_recorded(new, dtype, dim, keys):
     for i in range(new):
         want, tol = attention_oracle(left, q[i : i + 1], 0.125)
         assert bool(((got[i : i + 1].double().cpu() - want).abs() <= tol).all())
+
+
+def test_every_operand_that_asks_for_a_gradient_is_refused():
+    for i, call in enumerate(calls_that_ask_for_gradients(DEV)):
+        with pytest.raises(ValueError):
+            call()
+            pytest.fail(f"call {i} was not refused")
+        with torch.no_grad():
+            call()

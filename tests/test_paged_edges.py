@@ -122,3 +122,29 @@ def test_the_workspace_of_the_parts_of_a_context_is_bounded(batch, rows, heads, 
     plan = plan_of(ctypes.byref(p), kind, heads, ctypes.c_float(0.1), ctypes.c_int64(0), 148)
     assert plan.splits >= 1 and plan.splits * plan.split_keys >= keys
     assert plan.splits == 1 or rows * heads * plan.splits * (dim + 1) * 4 <= 80 * 2 ** 20
+
+
+def calls_that_ask_for_gradients(device):
+    dtype = torch.bfloat16 if torch.device(device).type == "cuda" else torch.float32
+    pages = ops.kv_pages(4, 8, 2, 16, torch.float8_e4m3fn, device)
+    table, ctx = torch.zeros(2, 2, dtype=torch.int32, device=device), torch.tensor([3, 4], dtype=torch.int32, device=device)
+    qkv, q, cos = torch.zeros(2, 128, dtype=dtype, device=device), torch.zeros(2, 4, 16, dtype=dtype, device=device), torch.zeros(8, 8, device=device)
+    for learned in (pages._replace(k_scale=pages.k_scale.clone().requires_grad_()), pages._replace(v_scale=pages.v_scale.clone().requires_grad_())):
+        yield lambda p=learned: ops.kv_append(qkv, p, table, ctx, 4)
+        yield lambda p=learned: ops.kv_gather(p, table, ctx, 4, dtype=dtype)
+        yield lambda p=learned: ops.paged_attention(q, p, table, ctx, 1.0)
+    yield lambda: ops.kv_append(qkv, pages, table, ctx, 4, rope=(cos.clone().requires_grad_(), cos, False))
+    yield lambda: ops.kv_append(qkv, pages, table, ctx, 4, rope=(cos, cos.clone().requires_grad_(), False))
+    yield lambda: ops.kv_append(qkv, pages, table, ctx, 4, out=q.clone().requires_grad_())
+    yield lambda: ops.paged_attention(q, pages, table, ctx, 1.0, out=q.clone().requires_grad_())
+    x, tokens = torch.zeros(2, 40, device=device), torch.zeros(2, 3, dtype=torch.int64, device=device)
+    yield lambda: ops.adjust_logits(x, tokens, out=x.clone().requires_grad_())
+
+
+def test_every_operand_that_asks_for_a_gradient_is_refused():
+    for i, call in enumerate(calls_that_ask_for_gradients("cpu")):
+        with pytest.raises(ValueError):
+            call()
+            pytest.fail(f"call {i} was not refused")
+        with torch.no_grad():
+            call()
