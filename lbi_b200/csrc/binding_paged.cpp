@@ -223,7 +223,7 @@ Tensor adjust_logits(const Tensor& logits, const Tensor& tokens, const OptTensor
   penalty(frequency, logits, "frequency", &p.frequency_row, &p.frequency);
   TORCH_CHECK_VALUE(p.repetition_row || p.repetition > 0, "repetition must be positive");
   if (given(bias)) {
-    TORCH_CHECK_VALUE(bias->scalar_type() == at::kFloat && bias->device() == logits.device() && bias->size(-1) == vocab &&
+    TORCH_CHECK_VALUE(bias->scalar_type() == at::kFloat && bias->device() == logits.device() && bias->dim() >= 1 && bias->size(-1) == vocab &&
                           (bias->dim() == 1 || (bias->dim() == 2 && bias->size(0) == batch)) && (vocab <= 1 || bias->stride(-1) == 1),
                       "bias must be an fp32 tensor [vocab] or [batch, vocab]");
     p.bias = bias->data_ptr<float>();
@@ -231,7 +231,7 @@ Tensor adjust_logits(const Tensor& logits, const Tensor& tokens, const OptTensor
   }
   if (given(allowed)) {
     const int64_t words = (vocab + 31) / 32;
-    TORCH_CHECK_VALUE(allowed->scalar_type() == at::kInt && allowed->device() == logits.device() && allowed->size(-1) == words &&
+    TORCH_CHECK_VALUE(allowed->scalar_type() == at::kInt && allowed->device() == logits.device() && allowed->dim() >= 1 && allowed->size(-1) == words &&
                           (allowed->dim() == 1 || (allowed->dim() == 2 && allowed->size(0) == batch)) && (words <= 1 || allowed->stride(-1) == 1),
                       "allowed must be an int32 tensor [ceil(vocab / 32)] or [batch, ceil(vocab / 32)]");
     p.allowed = allowed->data_ptr<int>();

@@ -126,3 +126,10 @@ def test_every_operand_that_asks_for_a_gradient_is_refused():
             pytest.fail(f"call {i} was not refused")
         with torch.no_grad():
             call()
+
+
+def test_a_bias_or_a_mask_without_dimensions_is_refused():
+    x, tokens = torch.zeros(2, 40, device=DEV), torch.zeros(2, 3, dtype=torch.int64, device=DEV)
+    for bad in (dict(bias=torch.zeros((), device=DEV)), dict(allowed=torch.zeros((), dtype=torch.int32, device=DEV))):
+        with pytest.raises(ValueError):
+            ops.adjust_logits(x, tokens, **bad)
