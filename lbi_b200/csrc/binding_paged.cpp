@@ -201,8 +201,8 @@ Tensor adjust_logits(const Tensor& logits, const Tensor& tokens, const OptTensor
   const int64_t batch = logits.size(0), vocab = logits.size(1);
   TORCH_CHECK_VALUE(vocab < (1ll << 31) - 65536 && batch < (1ll << 31), "2^31 entries or rows or more");
   TORCH_CHECK_VALUE(tokens.scalar_type() == at::kLong && tokens.dim() == 2 && tokens.size(0) == batch && tokens.device() == logits.device() &&
-                        (tokens.size(1) <= 1 || tokens.stride(1) == 1) && tokens.size(1) < (1ll << 31),
-                    "tokens must be an int64 tensor [batch, history], contiguous along the history");
+                        (tokens.size(1) <= 1 || tokens.stride(1) == 1) && tokens.size(1) < (1ll << 31) - 65536,   // the kernel's steps stay whole numbers
+                    "tokens must be an int64 tensor [batch, history], contiguous along the history, of fewer than 2^31 - 65536 entries a row");
   lbi_logit_rules p{};
   p.type = type_of(logits, "logits");
   p.batch = (int)batch;

@@ -133,3 +133,8 @@ def test_a_bias_or_a_mask_without_dimensions_is_refused():
     for bad in (dict(bias=torch.zeros((), device=DEV)), dict(allowed=torch.zeros((), dtype=torch.int32, device=DEV))):
         with pytest.raises(ValueError):
             ops.adjust_logits(x, tokens, **bad)
+
+
+def test_histories_whose_steps_would_leave_32_bits_are_refused():
+    with pytest.raises(ValueError):
+        ops.adjust_logits(torch.zeros(1, 40, device=DEV), torch.empty(1, 2 ** 31 - 1000, dtype=torch.int64, device=DEV))
