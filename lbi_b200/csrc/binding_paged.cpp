@@ -65,7 +65,9 @@ lbi_paged_batch paged_batch(const Tensor& k, const Tensor& v, const OptTensor& k
   check_int32(context, k, 1, "context_lens");
   p.batch = (int)context.size(0);
   TORCH_CHECK_VALUE(table.size(0) == p.batch, "page_table has ", table.size(0), " rows for ", p.batch, " context lengths");
-  TORCH_CHECK_VALUE(table.size(1) * page < (1ll << 31) && rows < (1ll << 31), "2^31 positions or rows or more");
+  // room for a tile behind the last position: the kernels count positions in 32 bits
+  TORCH_CHECK_VALUE(table.size(1) * page < (1ll << 31) - 65536, "2^31 - 65536 positions in the page table or more");
+  TORCH_CHECK_VALUE(rows < (1ll << 31), "2^31 rows or more");
   if (given(cu)) {
     check_int32(*cu, k, 1, "cu_seqlens");
     TORCH_CHECK_VALUE(cu->size(0) == p.batch + 1, "cu_seqlens must have one entry more than context_lens");

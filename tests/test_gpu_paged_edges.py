@@ -138,3 +138,14 @@ def test_a_bias_or_a_mask_without_dimensions_is_refused():
 def test_histories_whose_steps_would_leave_32_bits_are_refused():
     with pytest.raises(ValueError):
         ops.adjust_logits(torch.zeros(1, 40, device=DEV), torch.empty(1, 2 ** 31 - 1000, dtype=torch.int64, device=DEV))
+
+
+def test_tables_whose_positions_would_leave_32_bits_are_refused():
+    pages = ops.kv_pages(2, 128, 1, 64, BF16, DEV)
+    table = torch.zeros(1, 2 ** 24 - 1, dtype=torch.int32, device=DEV)     # 2^31 - 128 positions
+    ctx = torch.ones(1, dtype=torch.int32, device=DEV)
+    qkv, q = torch.zeros(1, 3 * 64, device=DEV).bfloat16(), torch.zeros(1, 1, 64, device=DEV).bfloat16()
+    for call in (lambda: ops.kv_append(qkv, pages, table, ctx, 1), lambda: ops.kv_gather(pages, table, ctx, 4),
+                 lambda: ops.paged_attention(q, pages, table, ctx, 1.0)):
+        with pytest.raises(ValueError):
+            call()
