@@ -324,7 +324,8 @@ def generate(model: Any, input_ids: torch.Tensor, max_new_tokens: int, *, total_
     length; pass the training sequence length to decode under the cut the model was trained with).  Dense models decode with
     per-block caches over the whole sequence (``use_cache=False``: by re-running the forward); depth-axis LBI models always
     re-run their forward on the sequence so far.  ``kv_cache``: None, ``"paged"`` or ``"e4m3"``, for the models that decode with
-    caches.  ``rules``: penalties, biases and masks on the logits (``LogitRules``)."""
+    caches; what its kernels recorded (``utils.failure.check_kernel_status``) is raised at the end of the request.  ``rules``: penalties,
+    biases and masks on the logits (``LogitRules``)."""
     if input_ids.dim() != 2 or input_ids.shape[1] == 0:
         raise ValueError("input_ids must be a non-empty [B, T] tensor")
     if math.isnan(temperature) or 0.0 < temperature < 2.0 ** -126:   # its reciprocal is no fp32 number
@@ -341,6 +342,13 @@ def generate(model: Any, input_ids: torch.Tensor, max_new_tokens: int, *, total_
             logits = adjust(logits, tokens)
         return _sample(logits, temperature, top_k, generator, wide=adjust is not None and adjust.wide).unsqueeze(1)
 
+    def finished(tokens: torch.Tensor) -> torch.Tensor:
+        if kv_cache is not None and tokens.is_cuda:   # a page that was not there, a wait that ran out: not the model's tokens
+            from .utils.failure import check_kernel_status
+
+            check_kernel_status(tokens)
+        return tokens
+
     try:
         final_len = input_ids.shape[1] + int(max_new_tokens)
         tokens = input_ids
@@ -356,7 +364,7 @@ def generate(model: Any, input_ids: torch.Tensor, max_new_tokens: int, *, total_
                 tokens = torch.cat([tokens, nxt], dim=1)
                 if i + 1 < int(max_new_tokens):
                     logits = decoder.append(nxt)[:, -1]
-            return tokens
+            return finished(tokens)
         dense = None
         if use_cache is not False and hasattr(model, "backbone") and hasattr(model, "readout") and not hasattr(model, "interface"):
             try:
@@ -371,7 +379,7 @@ def generate(model: Any, input_ids: torch.Tensor, max_new_tokens: int, *, total_
                 tokens = torch.cat([tokens, nxt], dim=1)
                 if i + 1 < int(max_new_tokens):
                     logits = dense.append(nxt)[:, -1]
-            return tokens
+            return finished(tokens)
         if kv_cache is not None:
             raise ValueError("kv_cache needs a model that decodes with caches (dense, or cut along the sequence)")
         for _ in range(int(max_new_tokens)):

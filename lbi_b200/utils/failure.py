@@ -31,6 +31,10 @@ class KernelWaitTimeout(RuntimeError):
     """A bounded device-side wait ran out; the value is the site code the kernel recorded."""
 
 
+# what the paged cache operators record instead of a wait
+RECORDED = {83: "a position outside the rotary table", 84: "a position or page outside the page table or the pool"}
+
+
 class PeerFailure(RuntimeError):
     """A peer rank reported a failure or stopped publishing heartbeats."""
 
@@ -44,7 +48,7 @@ class InjectedFault(RuntimeError):
 
 
 def check_kernel_status(like: torch.Tensor | None = None) -> None:
-    """Raise if any kernel of the extension recorded a timed-out wait on this device (the word is reset)."""
+    """Raise if any kernel of the extension recorded a timed-out wait or a bad index on this device (the word is reset)."""
     from .. import ops
 
     if not torch.cuda.is_available() or not ops.native_available():
@@ -52,7 +56,8 @@ def check_kernel_status(like: torch.Tensor | None = None) -> None:
     ref = like if like is not None else torch.empty(0, device="cuda")
     code = int(ops.ext().kernel_status(ref))
     if code != 0:
-        raise KernelWaitTimeout(f"a bounded wait inside a kernel ran out (site {code})")
+        what = RECORDED.get(code)
+        raise KernelWaitTimeout(f"a bounded wait inside a kernel ran out (site {code})" if what is None else f"a kernel met {what} (site {code})")
 
 
 # ------------------------------------------------------------------------------------------------------ watchdog

@@ -3,6 +3,12 @@ import pytest
 import torch
 
 from lbi_b200 import ops
+from lbi_b200.backbones import BackboneSpec
+from lbi_b200.backbones.transformer.attention import CausalSelfAttention
+from lbi_b200.inference import generate
+from lbi_b200.interfaces import VectorMLPInterface
+from lbi_b200.models import DenseLanguageModel, LBILanguageModel
+from lbi_b200.utils.failure import KernelWaitTimeout
 from paged_oracle import Batch, attention_oracle, check_attention
 from test_paged_edges import calls_that_ask_for_gradients
 
@@ -149,3 +155,35 @@ def test_tables_whose_positions_would_leave_32_bits_are_refused():
                  lambda: ops.paged_attention(q, pages, table, ctx, 1.0)):
         with pytest.raises(ValueError):
             call()
+
+
+def dense_model(dtype=BF16):
+    torch.manual_seed(0)
+    spec = BackboneSpec(name="transformer", dim=128, layers=2, n_heads=4, n_kv_heads=2, d_conv=0)
+    return DenseLanguageModel(vocab_size=300, backbone_spec=spec, tie_embeddings=True).eval().to(dtype).to(DEV)
+
+
+def region_model(dtype=BF16):
+    torch.manual_seed(0)
+    spec = BackboneSpec(name="transformer", dim=128, layers=2, n_heads=4, n_kv_heads=2, d_conv=0)
+    interface = VectorMLPInterface(feature_dim=128, num_regions=2, interface_width=8, interface_map_hidden_dim=16)
+    return LBILanguageModel(vocab_size=300, layers_per_region=1, backbone_spec=spec, interface=interface, region_axis="sequence",
+                            num_sequence_regions=2, tie_embeddings=True).eval().to(dtype).to(DEV)
+
+
+@pytest.mark.parametrize("build", [dense_model, region_model])
+def test_generation_raises_what_the_kernels_recorded(build, monkeypatch):
+    model, prompt = build(), torch.randint(0, 300, (2, 40), device=DEV)
+    want = generate(model, prompt, 4, kv_cache="paged")
+    allocate = CausalSelfAttention.allocate_decode_state
+
+    def without_a_page(self, *args, **kw):
+        state = allocate(self, *args, **kw)
+        state["table"][1, 1] = 10 ** 6      # no such page: the operators skip it and record that
+        return state
+
+    monkeypatch.setattr(CausalSelfAttention, "allocate_decode_state", without_a_page)
+    with pytest.raises(KernelWaitTimeout, match="84"):
+        generate(model, prompt, 4, kv_cache="paged")
+    monkeypatch.undo()
+    assert torch.equal(generate(model, prompt, 4, kv_cache="paged"), want)
