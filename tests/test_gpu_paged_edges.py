@@ -187,3 +187,50 @@ def test_generation_raises_what_the_kernels_recorded(build, monkeypatch):
         generate(model, prompt, 4, kv_cache="paged")
     monkeypatch.undo()
     assert torch.equal(generate(model, prompt, 4, kv_cache="paged"), want)
+
+
+@pytest.mark.parametrize("dtype,cache", TYPES)
+@pytest.mark.parametrize("group,dim", [(1, 64), (4, 64), (1, 128), (4, 128)])
+def test_scores_that_grow_along_the_context(group, dim, dtype, cache):
+    """By 18 binades per 128 keys: the running maximum moves and the output is rescaled in every tile of every kernel."""
+    def make(name, n, gen):
+        x = 0.25 * torch.randn(group if name == "q" else 1, n, dim, generator=gen)
+        if name == "q":
+            x[..., 0] = 4.0
+        elif name == "k":
+            x[..., 0] = torch.arange(n) / 40.0
+        return x
+    for seqs in ([(130, 700), (100, 900)], [(1, 1500), (1, 300)], [(3, 700)]):
+        check_attention(Shaped(make, seqs, group, 1, dim, 16, dtype, cache, DEV), scale=1.0)
+
+
+@pytest.mark.parametrize("dtype,cache", [*TYPES, (F32, "e4m3")])
+@pytest.mark.parametrize("new,group,dim", ROW_FORMS + TILE_FORMS + [(100, 4, 128)])
+def test_values_whose_size_differs_from_token_to_token(new, group, dim, dtype, cache):
+    """By up to 2^10, and every fifth token's are 0: the weights of an 8-bit cache carry the scales of the values."""
+    def make(name, n, gen):
+        x = torch.randn(group if name == "q" else 1, n, dim, generator=gen)
+        if name == "v":
+            x = x * 2.0 ** torch.randint(-8, 3, (1, n, 1), generator=gen)
+            x[:, ::5] = 0.0
+        return x
+    check_attention(Shaped(make, [(new, 700), (new, new), (new, 1200)], group, 1, dim, 16, dtype, cache, DEV))
+
+
+@pytest.mark.parametrize("build", [dense_model, region_model])
+@pytest.mark.parametrize("kv_cache", ["paged", "e4m3"])
+def test_models_in_fp32_decode_as_on_the_host(build, kv_cache):
+    """The same weights through the kernels and through the statements.  Sums of at most 2700 terms follow one another, half a step of
+    fp32 each; in 8 bits a code near the middle of two may round the other way, an eighth of one of 2^17 elements: 64 of those are
+    2^-3 sqrt(64 / 2^17) of the norm."""
+    from lbi_b200.inference import IncrementalDenseDecoder, IncrementalLBIDecoder
+
+    model = build(F32)
+    ids = torch.randint(0, 300, (2, 230), generator=torch.Generator().manual_seed(1))
+    decoder = IncrementalDenseDecoder if build is dense_model else IncrementalLBIDecoder
+    rows = []
+    for device in (DEV, "cpu"):
+        d = decoder(model.to(device), 230, kv_cache=kv_cache)
+        x = ids.to(device)
+        rows.append(torch.cat([d.append(x[:, :200]), d.append(x[:, 200:201]), d.append(x[:, 201:])], dim=1).double().cpu())
+    assert float((rows[0] - rows[1]).norm() / rows[1].norm()) <= 2700 * 2.0 ** -24 + (2.0 ** -3 * (64 / 2 ** 17) ** 0.5 if kv_cache == "e4m3" else 0.0)
