@@ -9,9 +9,9 @@
 // that occurs in the prompt.  Every block of a row reads the row's history again, which stays in L2, so tiles are large: 16-bit counts,
 // two to a word, while the history is shorter than 2^15, else 32-bit counts of half as many tokens.
 //
-// Measured on a B200: 192 rows of 128001 fp32 logits, histories of up to 4096 tokens, bias and mask: 59 us against 32 us for reading and
-// writing the logits once (207 MB).  The rest is the blocks' start: counters to zero, a walk over the history (8 tiles read it), two
-// barriers.  A row of 32768: launch and call, 5.3 us.
+// Measured on a B200: 192 rows of 128001 fp32 logits, histories of up to 4096 tokens, bias and mask: 58 us against 32 us for reading and
+// writing the logits once (207 MB).  The rest is the blocks' start, during which no logit is loaded: counters to zero, a walk over the
+// history (9 tiles read it), two barriers; 65 % of the issue slots are busy, DRAM at 35 %.  A row of 32768: launch and call, 5.3 to 6.4 us.
 #include <algorithm>
 
 #include "paged.cuh"
@@ -20,8 +20,8 @@ namespace lbi {
 namespace paged {
 
 constexpr int COUNT_BYTES = 32768;
-// Three blocks per SM leave registers for the loads of EACH elements at once.  Measured with 192 x 128001 (single calls): 62 us; four blocks 68 us, and 70 us
-// with 8 elements; three blocks with 2 or 8 elements 70 and 68 us; two blocks 76 us; blocks of 256 or 1024 threads 69 to 80 us.
+// Three blocks per SM leave registers for the loads of EACH elements at once.  Measured with 192 x 128001: 58 us; four blocks 63 us; three
+// blocks with 2 or 8 elements 66 and 64 us; two blocks 71 us; six blocks of 256 threads 60 us, one of 1024 86 us.
 constexpr int LOGIT_THREADS = 512, LOGIT_BLOCKS = 3, EACH = 4;
 
 template <int TYPE, typename COUNT>

@@ -225,7 +225,7 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
 }
 
 // Scale of a value row: a row of zeros has scale 0, which has no logarithm and no reciprocal; its codes are 0, so any positive
-// scale serves.  A NaN stays.
+// scale serves.  A NaN stays.  A row whose largest element is below 4.5e-28 is read as one of up to that size.
 __device__ __forceinline__ float positive_scale(float s) { return s < 1e-30f ? 1e-30f : s; }
 
 __host__ __device__ __forceinline__ int shift_of(int page_size) {

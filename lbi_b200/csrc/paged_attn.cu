@@ -32,8 +32,8 @@ namespace paged {
 // the heaviest key and what is lost below, 2^-40 of it per key, is nothing to the result.
 //
 // Measured on a B200, 32 query heads on 8 of 128: 64 contexts of up to 8192 keys (ragged, 1.02 GB) 183 us, 5.6 TB/s, 0.85 of the copy
-// bandwidth; all 8192 long 0.94 of it.  e4m3: 2 contexts of 131072 keys (0.55 GB) 115 us, 4.8 TB/s, 0.73: the codes' way to fp16 takes
-// the issue slots (56 % busy) that the 16-bit pages leave free (26 %).
+// bandwidth; all 8192 long 0.94 of it.  e4m3: 2 contexts of 131072 keys (0.55 GB) 115 to 117 us, 4.8 TB/s, 0.73: the codes' way to
+// fp16 takes the issue slots (57 % busy) that the 16-bit pages leave free (26 %).
 
 constexpr int ROW_TILE = 16;   // rows of attn_any_kernel; attn_rows_kernel has tiles of 8, too
 constexpr int WARPS = 4;

@@ -16,10 +16,10 @@
 // What bounds it: the chain S -> maximum -> exponentials -> P -> products of a row tile, of which two (or, with 16-bit pages at head_dim
 // 64, four: two blocks per SM, 256 columns of TMEM each) run at a time.  The special-function unit would be the next bound (16
 // exponentials per clock and SM: 1024 cycles per 128 x 128 tile, as long as the products take at head_dim 128), so a part of the
-// exponentials is computed by a polynomial on the FMA units.  Measured on a B200 with 2368 new tokens over 8192 keys, 32 heads on 8:
-// head_dim 128 fp16 pages 231 us, 1170 TFLOP/s (0.71 of the measured bf16 product rate), e4m3 314 us, 866 TFLOP/s; head_dim 64 200 us,
-// 680 TFLOP/s, and 283 us.  Two warpgroups per row tile, each with half of the columns, were slower (261 us at head_dim 128): the
-// exchange of the maxima costs more than the shorter chain gives.
+// exponentials is computed by a polynomial on the FMA units.  Measured on a B200 with 2368 new tokens over 8192 keys, 32 heads on 8,
+// L2 flushed: head_dim 128 fp16 pages 250 us, 1090 TFLOP/s (0.66 of the measured bf16 product rate), bf16 246 us, e4m3 336 us, 810 TFLOP/s;
+// head_dim 64 209 us, 651 TFLOP/s, and 291 us.  Two warpgroups per row tile, each with half of the columns, were slower (261 against
+// 231 us at head_dim 128, side by side): the exchange of the maxima costs more than the shorter chain gives.
 //
 // Keys and values: 16-bit pages come by TMA, one box per page and 64 columns (128-byte swizzle), the ids of a tile's pages read one
 // tile ahead, a lane per page.  Slots behind the context and pages that do not exist are masked out of S, and their rows of V are

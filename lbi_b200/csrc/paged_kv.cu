@@ -10,17 +10,18 @@
 // interleaved, so a turn needs no exchange between threads; a block owns one token, so a thread loads its 8 cosines and sines once
 // for all heads.
 //
-// Measured on a B200: 24617 tokens of 32 + 2 x 8 heads of 128, bf16, into e4m3 pages (559 MB) 122 us, 4.6 TB/s, 0.70 of the copy
-// bandwidth: the chain load - maximum over the head row - division - store and the issue slots bound it, not DRAM.
-// 12 contexts of up to 16384 tokens from e4m3 (8 heads of 128, 1.05 GB) 178 us, 0.90 of the copy bandwidth.  One token per call: launch
-// and call, 7 us.
+// Measured on a B200: 24617 tokens of 32 + 2 x 8 heads of 128, bf16, into e4m3 pages (559 MB) 122 to 126 us, 4.5 TB/s, 0.69 of the
+// copy bandwidth: latency of the chain load - maximum over the head row - division - store (46 % of the warps resident, 60 % of the issue
+// slots busy, DRAM at 53 %).  12 contexts of up to 16384 tokens from e4m3 (8 heads of 128, 1.05 GB) 178 to 185 us, 0.87 to 0.90 of the copy
+// bandwidth.  One token per call: launch and call, 7 us.
 #include "paged.cuh"
 
 namespace lbi {
 namespace paged {
 
-// A token's threads: 128 while blocks are few, for fewer passes over its heads (12 tokens of 48 heads 11.1 us, 64 threads 13.3; 240 tokens
-// 11.2 / 13.4), 64 from FEW_TOKENS on, for a block's start spread over more passes (1200 tokens 17.4 / 16.4 us, 24624 tokens 130 / 122).
+// A token's threads: 128 while blocks are few, for fewer passes over its heads (12 tokens of 48 heads of 128 11.1 us, 64 threads 13.3; 240
+// tokens 11.2 / 13.4), 64 from FEW_TOKENS on, for a block's start spread over more passes (1200 tokens 17.4 / 16.4 us, 24624 tokens
+// 130 / 122).  Other shapes were not measured.
 constexpr int APPEND_THREADS = 128, FEW_TOKENS = 600;
 
 struct AppendArgs {

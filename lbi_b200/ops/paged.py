@@ -10,8 +10,8 @@ the pages of every sequence in order.  All operators take the batch the same way
 Token i of the q new tokens of a sequence stands at position ``context - q + i``; a negative position is padding (nothing is
 written for it, its output is zero).  Rows in front of the first sequence and behind the last belong to nobody: they are left as
 they are in a given ``out`` and are zero otherwise.  Lengths and page ids stay on the device: nothing synchronises.  A position without a page (the table or
-the pool ends) is skipped, recorded in the status word (84; 83 for a position behind the rotary table) and raised by
-``utils.failure.check_kernel_status``.  Keys and values inside a context have to be finite; whatever a page holds behind the
+the pool ends) is skipped, recorded by the kernels in the status word (84; 83 for a position behind the rotary table) and raised by
+``utils.failure.check_kernel_status``.  A table holds fewer than 2^31 - 65536 positions, a history as many tokens.  Keys and values inside a context have to be finite; whatever a page holds behind the
 context is never used.
 
 There is no backward pass: inputs that need a gradient are refused.
