@@ -12,16 +12,34 @@
 
 #include <mutex>
 
-// One word per device that the kernels record wait time-outs and bad indices in.  It is made by the first call that asks for it, which
-// should not be one that is being captured into a graph (the word would be zeroed by the replay only): ``make_status_word`` is the call
-// for that.
+// A zeroed word on the current device.  The call that asks for it may be one that is being captured into a graph, whose replays must not
+// zero the word again: it is allocated and zeroed on a stream of its own, in the capture mode that permits that.
+static int* zeroed_word() {
+  int* word = nullptr;
+  cudaStream_t own = nullptr;
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  C10_CUDA_CHECK(cudaThreadExchangeStreamCaptureMode(&mode));
+  cudaError_t e = cudaMalloc(&word, sizeof(int));
+  if (e == cudaSuccess) e = cudaStreamCreateWithFlags(&own, cudaStreamNonBlocking);
+  if (e == cudaSuccess) e = cudaMemsetAsync(word, 0, sizeof(int), own);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(own);
+  if (own) cudaStreamDestroy(own);
+  C10_CUDA_CHECK(cudaThreadExchangeStreamCaptureMode(&mode));
+  C10_CUDA_CHECK(e);
+  return word;
+}
+
+// One word per device that the kernels record wait time-outs and bad indices in, made by the first call that asks for it.
 torch::Tensor status_word(const torch::Tensor& like) {
   static std::mutex lock;
   static std::vector<torch::Tensor>& words = *new std::vector<torch::Tensor>(64);   // outlives the runtime it would be freed with
   const int dev = like.get_device();
   TORCH_CHECK(dev >= 0 && dev < 64, "no status word for device ", dev);
   std::lock_guard<std::mutex> guard(lock);
-  if (!words[dev].defined()) words[dev] = torch::zeros({1}, like.options().dtype(at::kInt).requires_grad(false));
+  if (!words[dev].defined()) {
+    c10::cuda::CUDAGuard device(like.device());
+    words[dev] = torch::from_blob(zeroed_word(), {1}, torch::TensorOptions().dtype(at::kInt).device(like.device()));
+  }
   return words[dev];
 }
 

@@ -51,7 +51,7 @@ def kv_pages(num_pages: int, page_size: int, n_kv_heads: int, head_dim: int, dty
     shape = (int(num_pages), int(n_kv_heads), int(page_size), int(head_dim))
     k, v = (torch.zeros(shape, dtype=dtype, device=device) for _ in range(2))
     if k.is_cuda and native_available():
-        ext().make_status_word(k)   # before any call is captured into a graph
+        ext().make_status_word(k)   # the allocation that a first call would make
     if dtype != torch.float8_e4m3fn:
         return KVPages(k, v)
     return KVPages(k, v, *(torch.zeros(shape[:3], dtype=torch.float32, device=device) for _ in range(2)))

@@ -234,3 +234,45 @@ def test_models_in_fp32_decode_as_on_the_host(build, kv_cache):
         x = ids.to(device)
         rows.append(torch.cat([d.append(x[:, :200]), d.append(x[:, 200:201]), d.append(x[:, 201:])], dim=1).double().cpu())
     assert float((rows[0] - rows[1]).norm() / rows[1].norm()) <= 2700 * 2.0 ** -24 + (2.0 ** -3 * (64 / 2 ** 17) ** 0.5 if kv_cache == "e4m3" else 0.0)
+
+
+FIRST_CALL_IN_A_CAPTURE = """
+import torch
+from lbi_b200 import ops
+
+dev, bf16 = "cuda", torch.bfloat16
+pages = ops.KVPages(*(torch.randn(2, 1, 8, 64, device=dev, dtype=bf16) for _ in range(2)))     # not from kv_pages
+table = torch.tensor([[0, 1]], dtype=torch.int32, device=dev)
+context = torch.tensor([10], dtype=torch.int32, device=dev)
+q = torch.randn(1, 1, 64, device=dev, dtype=bf16)
+junk = [torch.full((2 ** i,), 7, dtype=torch.int32, device=dev) for i in range(20)]
+del junk
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    out = ops.paged_attention(q, pages, table, context, 0.125)
+assert ops.ext().kernel_status(q) == 0, "before the first replay"
+graph.replay()
+assert ops.ext().kernel_status(q) == 0
+want = ops.paged_attention(q, pages, table, context, 0.125)
+assert torch.equal(out, want)
+table[0, 1] = 9
+graph.replay()
+table[0, 1] = 1
+graph.replay()
+assert ops.ext().kernel_status(q) == 84, "a record is kept until it is read"
+table[0, 1] = 9
+ops.paged_attention(q, pages, table, context, 0.125)
+table[0, 1] = 1
+graph.replay()
+assert ops.ext().kernel_status(q) == 84, "an eager call's, too"
+assert ops.ext().kernel_status(q) == 0
+"""
+
+
+def test_records_outlive_replays_when_the_first_call_was_captured():
+    import subprocess
+    import sys
+
+    done = subprocess.run([sys.executable, "-c", FIRST_CALL_IN_A_CAPTURE], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
