@@ -94,7 +94,7 @@ class _LogitRuleState:
         self.bias = None if bias is None else bias.to(device=device, dtype=torch.float32).contiguous()
         # logits of a usual size stay far from fp32's limits with rules of a usual size (whatever the temperature)
         self.wide = max(rules.repetition_penalty, 1.0 / rules.repetition_penalty, abs(rules.presence_penalty), abs(rules.frequency_penalty),
-                        0.0 if bias is None else float(bias.abs().max())) > 1e6
+                        0.0 if bias is None else float(self.bias.abs().max())) > 1e6
         allowed, self.grammar, self.mask = rules.allowed_tokens, None, None
         if callable(allowed):
             self.grammar = allowed

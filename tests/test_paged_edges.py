@@ -74,6 +74,14 @@ def test_extreme_temperatures_are_sampled_from(temperature):
     assert set(s.handle({**ask, "allowed_ids": allowed})["new_ids"]) <= set(allowed)
 
 
+@pytest.mark.parametrize("dtype", [torch.bool, torch.int32, torch.float16, torch.bfloat16, torch.float64])
+def test_a_bias_tensor_of_any_type(dtype):
+    bias = torch.zeros(VOCAB, dtype=dtype)
+    bias[7] = 1
+    prompt, same = torch.tensor([[1, 2]]), LogitRules(logit_bias=bias.float())
+    assert torch.equal(generate(dense(), prompt, 4, rules=LogitRules(logit_bias=bias)), generate(dense(), prompt, 4, rules=same))
+
+
 def test_an_empty_list_of_allowed_ids_is_refused():
     """It allows nothing; only a missing key (or null) allows everything."""
     s = service()
